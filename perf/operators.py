@@ -84,7 +84,7 @@ def draw(rng):
     if kind == "norm":
         rows = _spread(rng, 1, 262144)
         D = _spread(rng, 32, min(8192, max(32, 64_000_000 // rows)))
-        D += D % 8 if rng.random() < 0.5 else 0
+        D = -(-D // 8) * 8 if rng.random() < 0.6 else D
         gate, residual = rng.random() < 0.6, rng.random() < 0.5
         case = _norm(rng.choice(("serve", "train")), "", dtype, rows, D, gate, residual, residual and rng.random() < 0.6,
                      residual and rng.random() < 0.6)
