@@ -45,7 +45,7 @@ extern "C" {
 typedef enum PsigStatus {
     PSIG_OK = 0,
     PSIG_ERR_NULL = -1,        /* a required pointer is NULL */
-    PSIG_ERR_DTYPE = -2,       /* dtype is neither PSIG_F32 nor PSIG_F64 */
+    PSIG_ERR_DTYPE = -2,       /* dtype is not one the entry point takes (signatures: PSIG_F32, PSIG_F64) */
     PSIG_ERR_DEPTH = -3,       /* depth outside 1..12 */
     PSIG_ERR_SHAPE = -4,       /* B < 0, L < 2, d < 1, W < 0 or inconsistent level_sizes */
     PSIG_ERR_PACKING = -5,     /* d^depth does not fit a signed 64-bit word code */
@@ -55,7 +55,8 @@ typedef enum PsigStatus {
     PSIG_ERR_UNSUPPORTED = -9  /* configuration has no kernel */
 } PsigStatus;
 
-typedef enum PsigDtype { PSIG_F32 = 0, PSIG_F64 = 1 } PsigDtype;
+/* PSIG_BF16 and PSIG_F16 are types of the sequence operators (psig_attn_*, psig_norm_*) only. */
+typedef enum PsigDtype { PSIG_F32 = 0, PSIG_F64 = 1, PSIG_BF16 = 2, PSIG_F16 = 3 } PsigDtype;
 
 /* Algorithm selection for psig_sig_forward / psig_sig_backward (desc.algo). */
 typedef enum PsigAlgo {
@@ -248,6 +249,71 @@ int psig_chen_forward(const PsigChenDesc *desc, const void *a, const void *b, vo
  * uses no atomics: results are bit-reproducible from run to run. */
 int psig_chen_backward(const PsigChenDesc *desc, const void *a, const void *b, const void *grad_out,
                        void *grad_a, void *grad_b, void *stream);
+
+/* Decayed linear attention over the time axis; no counterpart in the reference.  Per sequence b and head h, with a
+ * state S of shape (dk, dv), S_{-1} = initial_state (or 0), for t = 0 .. n-1, n = lengths[b] (or L):
+ *     S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T          out_t = scale * S_t^T q_t
+ * and out_t = 0 for t >= n.  Query heads h share the key/value head h / (H / Hkv).  Nothing of rows t >= n is read.
+ *   q (B, L, H, dk), k (B, L, Hkv, dk), v (B, L, Hkv, dv): dtype; strides in elements for (b, t, head), the last
+ *     dimension has stride 1.
+ *   log_decay: element (b, t, h) at b*ds[0] + t*ds[1] + h*ds[2] (strides 0 where it does not vary); float32, or
+ *     float64 when dtype is PSIG_F64.  Meant to be <= 0; -inf forgets everything before the step.
+ *   initial_state, final_state and their gradients (B, H, dk, dv): contiguous, type of log_decay.
+ *   out, grad_out (B, L, H, dv), grad_q, grad_k, grad_v: contiguous, dtype.
+ * dk and dv are at most 256; sums and states are held in 32 bits (64 for PSIG_F64). */
+typedef struct PsigAttnDesc {
+    int32_t dtype;            /* PsigDtype */
+    int32_t dk, dv;           /* head sizes, 1..256 */
+    int32_t H, Hkv;           /* query heads; key/value heads, a divisor of H */
+    int32_t algo;             /* PSIG_ALGO_AUTO, or PSIG_ALGO_GENERIC: always the kernels that serve every size */
+    int64_t B, L;
+    int64_t q_strides[3], k_strides[3], v_strides[3], decay_strides[3];
+    double scale;
+    const int32_t *lengths;   /* device (B), clamped to [0, L], or NULL: every sequence has length L */
+} PsigAttnDesc;
+
+/* Scratch bytes of psig_attn_forward / psig_attn_backward (0: none), or a negative PsigStatus. */
+int64_t psig_attn_forward_workspace(const PsigAttnDesc *desc);
+int64_t psig_attn_backward_workspace(const PsigAttnDesc *desc);
+/* initial_state and final_state may be NULL.  `workspace`: 256-byte aligned, overwritten. */
+int psig_attn_forward(const PsigAttnDesc *desc, const void *q, const void *k, const void *v, const void *log_decay,
+                      const void *initial_state, void *out, void *final_state, void *workspace, int64_t workspace_bytes,
+                      void *stream);
+/* grad_state may be NULL (zero).  grad_log_decay (type of log_decay; may be NULL): (B, L, H), or (H) when decay_strides
+ * of b and t are both 0 (summed over them in a fixed order).  grad_initial_state may be NULL.  No atomics: the same
+ * bits on every run.  Rows t >= n of the gradients are zero. */
+int psig_attn_backward(const PsigAttnDesc *desc, const void *q, const void *k, const void *v, const void *log_decay,
+                       const void *initial_state, const void *grad_out, const void *grad_state, void *grad_q,
+                       void *grad_k, void *grad_v, void *grad_log_decay, void *grad_initial_state, void *workspace,
+                       int64_t workspace_bytes, void *stream);
+/* One time step for every sequence: state (B, H, dk, dv) is replaced by S_t and out (B, H, dv) is written.  Uses the
+ * description with L == 1; the time strides and lengths are ignored. */
+int psig_attn_step(const PsigAttnDesc *desc, const void *q, const void *k, const void *v, const void *log_decay,
+                   void *state, void *out, void *stream);
+
+/* Norm around a block, fused with the block's gate, the residual sum and the norm before the next block; no
+ * counterpart in the reference.  Per row of D features, rms(x) = x / sqrt(mean(x^2) + eps):
+ *     h = residual + residual_scale * (rms(x) * weight * act(gate)),      n = rms(h) * next_weight
+ * with h before it is rounded.  x, gate, residual, h, n (rows, D) contiguous in dtype; weight, residual_scale and
+ * next_weight (D) in float32 (float64 when dtype is PSIG_F64).  gate, residual, weight and residual_scale may be NULL
+ * (left out); n is computed when next_weight is given. */
+typedef struct PsigNormDesc {
+    int32_t dtype;        /* PsigDtype */
+    int32_t activation;   /* 0: act(g) = g * sigmoid(g); 1: act(g) = sigmoid(g) */
+    int64_t rows, D;
+    double eps;
+} PsigNormDesc;
+
+int psig_norm_forward(const PsigNormDesc *desc, const void *x, const void *weight, const void *gate, const void *residual,
+                      const void *residual_scale, const void *next_weight, void *h, void *n, void *stream);
+/* Scratch bytes of psig_norm_backward: one row of D sums per block and vector. */
+int64_t psig_norm_backward_workspace(const PsigNormDesc *desc);
+/* grad_h or grad_n may be NULL (zero; grad_n is used when next_weight is given).  Gradients of operands that are NULL,
+ * and those the caller does not want, are NULL.  No atomics: the same bits on every run. */
+int psig_norm_backward(const PsigNormDesc *desc, const void *x, const void *weight, const void *gate, const void *residual,
+                       const void *residual_scale, const void *next_weight, const void *grad_h, const void *grad_n,
+                       void *grad_x, void *grad_weight, void *grad_gate, void *grad_residual, void *grad_residual_scale,
+                       void *grad_next_weight, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -13,8 +13,10 @@ _ensure_loaded()
 from . import ops  # noqa: E402  (registers torch.ops.pathsig_b200.*)
 from .modules import LogSignature, Signature  # noqa: E402
 from .projections import projections  # noqa: E402
+from .sequence import gated_residual_norm, linear_attention, linear_attention_step  # noqa: E402
 
-__all__ = ["Signature", "LogSignature", "projections", "chen_product", "install_as_pathsig"]
+__all__ = ["Signature", "LogSignature", "projections", "chen_product", "linear_attention", "linear_attention_step",
+           "gated_residual_norm", "install_as_pathsig"]
 __version__ = "0.1.0"
 
 
@@ -44,7 +46,7 @@ def install_as_pathsig(register_ops: bool = True) -> None:
 
     module = sys.modules[__name__]
     sys.modules.setdefault("pathsig", module)
-    for sub in ("ops", "modules", "projections", "_load"):
+    for sub in ("ops", "modules", "projections", "sequence", "_load"):
         sys.modules.setdefault("pathsig." + sub, sys.modules[__name__ + "." + sub])
     if register_ops:
         import torch

@@ -19,7 +19,7 @@ BINDING_PATH = os.path.join(_HERE, BINDING_NAME)
 MAX_DEPTH = 12
 ABI_VERSION = 2
 
-PSIG_F32, PSIG_F64 = 0, 1
+PSIG_F32, PSIG_F64, PSIG_BF16, PSIG_F16 = 0, 1, 2, 3
 ALGO_AUTO, ALGO_GENERIC, ALGO_TILED, ALGO_CLOSURE = 0, 1, 2, 3
 FLAG_DETERMINISTIC = 1   # PSIG_FLAG_DETERMINISTIC of include/pathsig_b200.h
 
@@ -73,9 +73,41 @@ class ChenDesc(ctypes.Structure):
     ]
 
 
+class AttnDesc(ctypes.Structure):
+    """``PsigAttnDesc`` of include/pathsig_b200.h."""
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("dk", ctypes.c_int32),
+        ("dv", ctypes.c_int32),
+        ("H", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32),
+        ("algo", ctypes.c_int32),
+        ("B", ctypes.c_int64),
+        ("L", ctypes.c_int64),
+        ("q_strides", ctypes.c_int64 * 3),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+        ("decay_strides", ctypes.c_int64 * 3),
+        ("scale", ctypes.c_double),
+        ("lengths", ctypes.c_void_p),
+    ]
+
+
+class NormDesc(ctypes.Structure):
+    """``PsigNormDesc`` of include/pathsig_b200.h."""
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("rows", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("eps", ctypes.c_double),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/pathsig_b200.h declares.
 _vp, _i64, _int = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
 _SigP, _LogP, _ChenP = ctypes.POINTER(SigDesc), ctypes.POINTER(LogDesc), ctypes.POINTER(ChenDesc)
+_AttnP, _NormP = ctypes.POINTER(AttnDesc), ctypes.POINTER(NormDesc)
 EXPORTS = {
     "psig_abi_version": (_int, []),
     "psig_status_string": (ctypes.c_char_p, [_int]),
@@ -102,6 +134,14 @@ EXPORTS = {
     "psig_chen_size": (_i64, [_ChenP]),
     "psig_chen_forward": (_int, [_ChenP, _vp, _vp, _vp, _vp]),
     "psig_chen_backward": (_int, [_ChenP, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "psig_attn_forward_workspace": (_i64, [_AttnP]),
+    "psig_attn_backward_workspace": (_i64, [_AttnP]),
+    "psig_attn_forward": (_int, [_AttnP] + [_vp] * 8 + [_i64, _vp]),
+    "psig_attn_backward": (_int, [_AttnP] + [_vp] * 13 + [_i64, _vp]),
+    "psig_attn_step": (_int, [_AttnP] + [_vp] * 7),
+    "psig_norm_forward": (_int, [_NormP] + [_vp] * 9),
+    "psig_norm_backward_workspace": (_i64, [_NormP]),
+    "psig_norm_backward": (_int, [_NormP] + [_vp] * 15 + [_i64, _vp]),
 }
 
 

@@ -1,0 +1,551 @@
+// Decayed linear attention over the time axis: entry points, the kernels that serve every size and type, the
+// decay gradient, and the single time step.  Formulas: include/pathsig_b200.h; the sweep that the forward
+// pass and the three gradients share: sequence.cuh.
+//
+// Gradients.  With A_t = scale q_t go_t^T + exp(g_{t+1}) A_{t+1} (A behind the last step: grad_state),
+//     grad_q_t = scale S_t go_t,   grad_k_t = A_t v_t,   grad_v_t = A_t^T k_t,   grad_g_t = <A_t, exp(g_t) S_{t-1}>.
+// The first three are sweeps.  The last is the sum over all pairs s < t <= u of what the pair (s, u) adds to the
+// result; with x_t = q_t . grad_q_t (pairs that end at t) and y_s = k_s . grad_k_s (pairs that begin at s),
+//     grad_g_t = B_e + sum_{t <= i < e} (x_i - y_i),     B_e = <exp(g_e) A_e, S_{e-1}> (pairs across e)
+// for any e > t.  e is the end of t's segment of kSegment steps: B_e comes from the two states themselves, so that
+// the difference of the two sums never runs over more than a segment, however long the sequence is.
+#include "sequence.cuh"
+
+namespace psig {
+namespace {
+
+constexpr int kSweepThreads = 256;
+constexpr int kSweepSteps = 16;   // time steps staged at once
+constexpr int kSweepCols = 32;    // columns of the state per block
+
+__device__ __forceinline__ long long length_of(const int *lengths, long long b, long long L)
+{
+    if (lengths == nullptr) return L;
+    const long long n = lengths[b];
+    return n < 0 ? 0 : n > L ? L : n;
+}
+
+// The simplest sweep: one block per (sequence, head, 32 columns of the state), the state in registers (lane =
+// column, warp w holds rows w, w + 8, ...), one time step after another; each warp's share of the step's output
+// row goes to shared memory and is summed once per 16 steps.  Serves every type, size and alignment.
+template <typename T, int RPT>
+__global__ void __launch_bounds__(kSweepThreads) attn_sweep_rows(const Sweep a)
+{
+    using A = typename Acc<T>::type;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    A *r_s = reinterpret_cast<A *>(smem_raw);                // [steps][d1]
+    A *k_s = r_s + kSweepSteps * a.d1;                       // [steps][d1]
+    A *v_s = k_s + kSweepSteps * a.d1;                       // [steps][32]
+    A *part = v_s + kSweepSteps * kSweepCols;                // [8][steps][32]
+    A *w_s = part + 8 * kSweepSteps * kSweepCols;            // [steps]
+    __shared__ A dot_s[8];
+
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long bh = blockIdx.x;
+    const long long b = bh / a.H;
+    const int h = (int)(bh % a.H);
+    const int col0 = blockIdx.y * kSweepCols, col = col0 + lane;
+    const bool live = col < a.d2;
+    const long long n = length_of(a.lengths, b, a.L);
+    const T *r = static_cast<const T *>(a.r.data) + b * a.r.stride[0] + (h / a.r.share) * a.r.stride[2];
+    const T *k = static_cast<const T *>(a.k.data) + b * a.k.stride[0] + (h / a.k.share) * a.k.stride[2];
+    const T *v = static_cast<const T *>(a.v.data) + b * a.v.stride[0] + (h / a.v.share) * a.v.stride[2];
+    const A *g = static_cast<const A *>(a.decay) + b * a.decay_stride[0] + h * a.decay_stride[2];
+    const long long state0 = bh * a.d1 * a.d2;
+
+    A S[RPT];
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        const int row = warp + 8 * i;
+        S[i] = A(0);
+        if (a.init != nullptr && live && row < a.d1)
+            S[i] = static_cast<const A *>(a.init)[state0 + (a.init_transposed ? (long long)col * a.d1 + row
+                                                                              : (long long)row * a.d2 + col)];
+    }
+
+    const long long stages = (n + kSweepSteps - 1) / kSweepSteps;
+    const long long segments = (a.L + kSegment - 1) / kSegment;
+    for (long long st = 0; st < stages; ++st) {
+        const long long t0 = (a.reverse ? stages - 1 - st : st) * kSweepSteps;
+        const long long t1 = t0 + kSweepSteps < n ? t0 + kSweepSteps : n;
+        const int m = (int)(t1 - t0);
+        for (int e = threadIdx.x; e < m * a.d1; e += kSweepThreads) {
+            const int j = e / a.d1, d = e % a.d1;
+            const long long t = a.reverse ? t1 - 1 - j : t0 + j;
+            r_s[e] = to_acc<A>(r[t * a.r.stride[1] + d]);
+            k_s[e] = to_acc<A>(k[t * a.k.stride[1] + d]);
+        }
+        for (int e = threadIdx.x; e < m * kSweepCols; e += kSweepThreads) {
+            const int j = e / kSweepCols, c = col0 + e % kSweepCols;
+            const long long t = a.reverse ? t1 - 1 - j : t0 + j;
+            v_s[e] = c < a.d2 ? to_acc<A>(v[t * a.v.stride[1] + c]) * A(a.kv_scale) : A(0);
+        }
+        if (threadIdx.x < m) {
+            const long long t = a.reverse ? t1 - threadIdx.x : t0 + threadIdx.x;   // reverse: the step behind
+            w_s[threadIdx.x] = t < n ? exp_acc(g[t * a.decay_stride[1]]) : A(1);
+        }
+        __syncthreads();
+        const bool boundary = t1 == n || t1 % kSegment == 0;
+        const long long segment = (t1 - 1) / kSegment;
+        A first = w_s[0];
+        if (a.reverse && a.anchor_dots != nullptr && boundary) {
+            // the state just behind t1, decayed over t1, against the stored state of the steps before t1
+            const A *anchor = static_cast<const A *>(a.anchors) + (bh * segments + segment) * a.d1 * a.d2;
+            A dot = A(0);
+#pragma unroll
+            for (int i = 0; i < RPT; ++i) {
+                const int row = warp + 8 * i;
+                S[i] *= first;
+                if (live && row < a.d1) dot += S[i] * anchor[(long long)row * a.d2 + col];
+            }
+            first = A(1);
+            for (int s = 16; s >= 1; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
+            if (lane == 0) dot_s[warp] = dot;
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                A sum = A(0);
+                for (int i = 0; i < 8; ++i) sum += dot_s[i];
+                static_cast<A *>(a.anchor_dots)[(bh * segments + segment) * gridDim.y + blockIdx.y] = sum;
+            }
+        }
+        for (int j = 0; j < m; ++j) {
+            const A w = j == 0 ? first : w_s[j], vj = v_s[j * kSweepCols + lane];
+            A acc = A(0);
+#pragma unroll
+            for (int i = 0; i < RPT; ++i) {
+                const int row = warp + 8 * i;
+                if (row < a.d1) {
+                    S[i] = fma(k_s[j * a.d1 + row], vj, S[i] * w);
+                    acc = fma(r_s[j * a.d1 + row], S[i], acc);
+                }
+            }
+            part[(warp * kSweepSteps + j) * kSweepCols + lane] = acc;
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < m * kSweepCols; e += kSweepThreads) {
+            const int j = e / kSweepCols, c = col0 + e % kSweepCols;
+            if (c >= a.d2) continue;
+            A sum = A(0);
+            for (int i = 0; i < 8; ++i) sum += part[(i * kSweepSteps + j) * kSweepCols + e % kSweepCols];
+            sum *= A(a.out_scale);
+            const long long t = a.reverse ? t1 - 1 - j : t0 + j;
+            const long long at = ((b * a.L + t) * a.H + h) * a.d2 + c;
+            if (a.out_acc) static_cast<A *>(a.out)[at] = sum;
+            else static_cast<T *>(a.out)[at] = from_acc<T>(sum);
+        }
+        if (!a.reverse && a.anchors != nullptr && boundary) {
+            A *anchor = static_cast<A *>(a.anchors) + (bh * segments + segment) * a.d1 * a.d2;
+#pragma unroll
+            for (int i = 0; i < RPT; ++i) {
+                const int row = warp + 8 * i;
+                if (live && row < a.d1) anchor[(long long)row * a.d2 + col] = S[i];
+            }
+        }
+        __syncthreads();
+    }
+    for (long long e = threadIdx.x; e < (a.L - n) * kSweepCols; e += kSweepThreads) {
+        const long long t = n + e / kSweepCols;
+        const int c = col0 + (int)(e % kSweepCols);
+        const long long at = ((b * a.L + t) * a.H + h) * a.d2 + c;
+        if (c >= a.d2) continue;
+        if (a.out_acc) static_cast<A *>(a.out)[at] = A(0);
+        else static_cast<T *>(a.out)[at] = from_acc<T>(A(0));
+    }
+    if (a.final != nullptr) {
+        const A w = a.reverse && n > 0 ? exp_acc(g[0]) : A(1);
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+            const int row = warp + 8 * i;
+            if (live && row < a.d1)
+                static_cast<A *>(a.final)[state0 + (a.final_transposed ? (long long)col * a.d1 + row
+                                                                       : (long long)row * a.d2 + col)] = S[i] * w;
+        }
+    }
+}
+
+inline int column_tiles(int d2) { return (d2 + kSweepCols - 1) / kSweepCols; }
+
+template <typename T>
+int sweep_rows(const Sweep &a, cudaStream_t stream)
+{
+    using A = typename Acc<T>::type;
+    const dim3 grid((unsigned)(a.B * a.H), (unsigned)column_tiles(a.d2));
+    const size_t smem = sizeof(A) * (size_t)(2 * kSweepSteps * a.d1 + 9 * kSweepSteps * kSweepCols + kSweepSteps);
+    auto launch = [&](auto kernel) {
+        if (!prepare_kernel(kernel, smem, false)) return (int)PSIG_ERR_CUDA;
+        kernel<<<grid, kSweepThreads, smem, stream>>>(a);
+        return check_launch();
+    };
+    if (a.d1 <= 64) return launch(attn_sweep_rows<T, 8>);
+    if (a.d1 <= 128) return launch(attn_sweep_rows<T, 16>);
+    return launch(attn_sweep_rows<T, 32>);
+}
+
+// Sums of the query heads that share a key/value head, rounded once: (B*L, H, d) -> (B*L, Hkv, d).
+template <typename T>
+__global__ void attn_sum_heads(const typename Acc<T>::type *__restrict__ acc, T *__restrict__ out, long long total,
+                               int share, int d)
+{
+    using A = typename Acc<T>::type;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
+         i += (long long)gridDim.x * blockDim.x) {
+        const long long head = i / d;
+        const A *p = acc + head * share * d + i % d;
+        A sum = p[0];
+        for (int s = 1; s < share; ++s) sum += p[(long long)s * d];
+        out[i] = from_acc<T>(sum);
+    }
+}
+
+// x_t - y_t per (b, t, h), a warp each: q . grad_q - k . grad_k from the unrounded gradients.
+template <typename T>
+__global__ void attn_pair_difference(const SweepOperand q, const SweepOperand k,
+                                     const typename Acc<T>::type *__restrict__ gq,
+                                     const typename Acc<T>::type *__restrict__ gk, double *__restrict__ out,
+                                     long long rows, long long L, int H, int d)
+{
+    using A = typename Acc<T>::type;
+    const int lane = threadIdx.x & 31;
+    const long long warps = (long long)gridDim.x * (blockDim.x >> 5);
+    for (long long row = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); row < rows; row += warps) {
+        const int h = (int)(row % H);
+        const long long bt = row / H, b = bt / L, t = bt % L;
+        const T *qr = static_cast<const T *>(q.data) + b * q.stride[0] + t * q.stride[1] + (h / q.share) * q.stride[2];
+        const T *kr = static_cast<const T *>(k.data) + b * k.stride[0] + t * k.stride[1] + (h / k.share) * k.stride[2];
+        A sum = A(0);
+        for (int i = lane; i < d; i += 32) {
+            const A x = gq[row * d + i], y = gk[row * d + i];
+            // rows behind the last step hold zeros; what stands in q and k there is not looked at
+            if (x != A(0)) sum += to_acc<A>(qr[i]) * x;
+            if (y != A(0)) sum -= to_acc<A>(kr[i]) * y;
+        }
+        for (int s = 16; s >= 1; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+        if (lane == 0) out[row] = (double)sum;
+    }
+}
+
+// grad_g over one segment per block: B_e plus the sums of x - y from the segment's end, in 64 bits.  Writes
+// (B, L, H), or the segment's total for a decay per head.  A step whose decay underflows to 0 has gradient 0.
+template <typename A>
+__global__ void attn_decay_grad(const double *__restrict__ pairs, const A *__restrict__ dots, int tiles,
+                                const A *__restrict__ decay, long long s0, long long s1, long long s2,
+                                const int *__restrict__ lengths, long long L, int H, A *__restrict__ out,
+                                double *__restrict__ totals)
+{
+    __shared__ double carry_s[kSegment / 32], total_s[kSegment / 32];
+    const long long segments = gridDim.x;
+    const long long segment = blockIdx.x;
+    const int h = blockIdx.y % H;
+    const long long b = blockIdx.y / H, bh = blockIdx.y;
+    const long long n = length_of(lengths, b, L);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long end = (segment + 1) * kSegment < n ? (segment + 1) * kSegment : n;
+    // thread i takes step end - 1 - i, so that sums from the end are running sums over the threads
+    const long long t = end - 1 - threadIdx.x;
+    const bool live = t >= segment * kSegment && end > segment * kSegment;
+    double sum = live ? pairs[(b * L + t) * H + h] : 0.0;
+    for (int s = 1; s < 32; s <<= 1) {
+        const double up = __shfl_up_sync(0xffffffffu, sum, s);
+        if (lane >= s) sum += up;
+    }
+    if (lane == 31) carry_s[warp] = sum;
+    __syncthreads();
+    for (int i = 0; i < warp; ++i) sum += carry_s[i];
+    if (live)
+        for (int i = 0; i < tiles; ++i) sum += (double)dots[(bh * segments + segment) * tiles + i];
+    if (live && exp_acc(decay[b * s0 + t * s1 + h * s2]) == A(0)) sum = 0.0;
+    if (out != nullptr) {
+        if (live) out[(b * L + t) * H + h] = (A)sum;
+        const long long z = segment * kSegment + threadIdx.x;
+        if (z >= n && z < L) out[(b * L + z) * H + h] = A(0);
+    }
+    if (totals != nullptr) {
+        double all = live ? sum : 0.0;
+        for (int s = 16; s >= 1; s >>= 1) all += __shfl_xor_sync(0xffffffffu, all, s);
+        if (lane == 0) total_s[warp] = all;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            double v = 0.0;
+            for (int i = 0; i < kSegment / 32; ++i) v += total_s[i];
+            totals[bh * segments + segment] = v;
+        }
+    }
+}
+
+// One block per head: the segments' totals over all sequences, in a fixed order.
+template <typename A>
+__global__ void attn_decay_total(const double *__restrict__ totals, long long B, int H, long long segments,
+                                 A *__restrict__ out)
+{
+    __shared__ double part_s[8];
+    const int h = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    double sum = 0.0;
+    for (long long i = threadIdx.x; i < B * segments; i += blockDim.x)
+        sum += totals[(i / segments * H + h) * segments + i % segments];
+    for (int s = 16; s >= 1; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    if (lane == 0) part_s[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double v = 0.0;
+        for (int i = 0; i < 8; ++i) v += part_s[i];
+        out[h] = (A)v;
+    }
+}
+
+// One time step: a block takes 32 columns of one state, reads each entry once, writes it back decayed and with the
+// new product, and sums its columns of the output row.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_step_rows(const SweepOperand q, const SweepOperand k, const SweepOperand v,
+                                                      const typename Acc<T>::type *__restrict__ decay, long long s0,
+                                                      long long s2, typename Acc<T>::type *__restrict__ state,
+                                                      T *__restrict__ out, int H, int dk, int dv, double scale)
+{
+    using A = typename Acc<T>::type;
+    __shared__ A part[8][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long bh = blockIdx.x, b = bh / H;
+    const int h = (int)(bh % H), col = blockIdx.y * 32 + lane;
+    const T *qr = static_cast<const T *>(q.data) + b * q.stride[0] + (h / q.share) * q.stride[2];
+    const T *kr = static_cast<const T *>(k.data) + b * k.stride[0] + (h / k.share) * k.stride[2];
+    const T *vr = static_cast<const T *>(v.data) + b * v.stride[0] + (h / v.share) * v.stride[2];
+    const A w = exp_acc(decay[b * s0 + h * s2]);
+    A acc = A(0);
+    if (col < dv) {
+        const A vj = to_acc<A>(vr[col]);
+        A *s = state + bh * dk * dv + col;
+        for (int row = warp; row < dk; row += 8) {
+            const A next = fma(to_acc<A>(kr[row]), vj, s[(long long)row * dv] * w);
+            s[(long long)row * dv] = next;
+            acc = fma(to_acc<A>(qr[row]), next, acc);
+        }
+    }
+    part[warp][lane] = acc;
+    __syncthreads();
+    if (warp == 0 && col < dv) {
+        A sum = A(0);
+        for (int i = 0; i < 8; ++i) sum += part[i][lane];
+        out[bh * dv + col] = from_acc<T>(sum * A(scale));
+    }
+}
+
+// ------------------------------------------------------------------------------------------ host side
+
+int check_attn(const PsigAttnDesc *d)
+{
+    if (d == nullptr) return PSIG_ERR_NULL;
+    if (d->dtype < PSIG_F32 || d->dtype > PSIG_F16) return PSIG_ERR_DTYPE;
+    if (d->B < 0 || d->L < 0 || d->dk < 1 || d->dv < 1 || d->H < 1 || d->Hkv < 1 || d->H % d->Hkv != 0)
+        return PSIG_ERR_SHAPE;
+    if (d->dk > 256 || d->dv > 256) return PSIG_ERR_TOO_LARGE;
+    if (d->B * d->H > 0x7fffffffLL) return PSIG_ERR_TOO_LARGE;
+    return PSIG_OK;
+}
+
+SweepOperand operand(const void *data, const int64_t *strides, int share)
+{
+    return SweepOperand{data, {strides[0], strides[1], strides[2]}, share};
+}
+
+Sweep sweep_of(const PsigAttnDesc &d, const void *decay)
+{
+    Sweep s{};
+    s.decay = decay;
+    for (int i = 0; i < 3; ++i) s.decay_stride[i] = d.decay_strides[i];
+    s.lengths = d.lengths;
+    s.B = d.B;
+    s.L = d.L;
+    s.H = d.H;
+    s.out_scale = 1.0;
+    s.kv_scale = 1.0;
+    return s;
+}
+
+bool per_head(const PsigAttnDesc &d) { return d.decay_strides[0] == 0 && d.decay_strides[1] == 0; }
+
+// Scratch of the backward pass, in the order it is laid out (256-byte aligned pieces).
+struct BackwardScratch {
+    long long gq, gk, gv, pairs, anchors, dots, totals, bytes;
+};
+
+BackwardScratch backward_scratch(const PsigAttnDesc &d)
+{
+    const long long acc = d.dtype == PSIG_F64 ? 8 : 4, rows = d.B * d.L * d.H, bh = d.B * d.H, seg = segments_of(d.L);
+    BackwardScratch s{};
+    long long at = 0;
+    auto take = [&](long long bytes) {
+        const long long here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    s.gq = take(acc * rows * d.dk);
+    s.gk = take(acc * rows * d.dk);
+    s.gv = take(acc * rows * d.dv);
+    s.pairs = take(8 * rows);
+    s.anchors = take(acc * bh * seg * d.dk * d.dv);
+    s.dots = take(acc * bh * seg * column_tiles(d.dk));
+    s.totals = take(8 * bh * seg);
+    s.bytes = at;
+    return s;
+}
+
+template <typename T>
+int run_forward(const PsigAttnDesc &d, const void *q, const void *k, const void *v, const void *decay, const void *init,
+                void *out, void *final, cudaStream_t stream)
+{
+    Sweep s = sweep_of(d, decay);
+    s.r = operand(q, d.q_strides, 1);
+    s.k = operand(k, d.k_strides, d.H / d.Hkv);
+    s.v = operand(v, d.v_strides, d.H / d.Hkv);
+    s.d1 = d.dk;
+    s.d2 = d.dv;
+    s.out_scale = d.scale;
+    s.init = init;
+    s.final = final;
+    s.out = out;
+    return sweep_rows<T>(s, stream);
+}
+
+unsigned blocks_for(long long items, int per_block)
+{
+    const long long n = (items + per_block - 1) / per_block;
+    return (unsigned)(n < 1 ? 1 : n > 148 * 32 ? 148 * 32 : n);
+}
+
+template <typename T>
+int run_backward(const PsigAttnDesc &d, const void *q, const void *k, const void *v, const void *decay, const void *init,
+                 const void *go, const void *gs, void *grad_q, void *grad_k, void *grad_v, void *grad_decay,
+                 void *grad_init, char *ws, cudaStream_t stream)
+{
+    using A = typename Acc<T>::type;
+    const BackwardScratch at = backward_scratch(d);
+    const int share = d.H / d.Hkv;
+    const long long rows = d.B * d.L * d.H, kv_rows = d.B * d.L * d.Hkv, segments = segments_of(d.L);
+    A *gq = reinterpret_cast<A *>(ws + at.gq), *gk = reinterpret_cast<A *>(ws + at.gk);
+    A *gv = reinterpret_cast<A *>(ws + at.gv), *dots = reinterpret_cast<A *>(ws + at.dots);
+    double *pairs = reinterpret_cast<double *>(ws + at.pairs), *totals = reinterpret_cast<double *>(ws + at.totals);
+    const int64_t go_strides[3] = {d.L * d.H * d.dv, (int64_t)d.H * d.dv, d.dv};
+    const SweepOperand Q = operand(q, d.q_strides, 1), K = operand(k, d.k_strides, share),
+                       V = operand(v, d.v_strides, share), G = operand(go, go_strides, 1);
+    int rc;
+    Sweep s = sweep_of(d, decay);   // grad_q
+    s.r = G, s.k = V, s.v = K;
+    s.d1 = d.dv, s.d2 = d.dk;
+    s.out_scale = d.scale;
+    s.init = init, s.init_transposed = true;
+    s.out = gq, s.out_acc = true;
+    s.anchors = ws + at.anchors;
+    if ((rc = sweep_rows<T>(s, stream)) != PSIG_OK) return rc;
+    s = sweep_of(d, decay);         // grad_k
+    s.r = V, s.k = G, s.v = Q;
+    s.d1 = d.dv, s.d2 = d.dk;
+    s.reverse = true;
+    s.kv_scale = d.scale;
+    s.init = gs, s.init_transposed = true;
+    s.out = gk, s.out_acc = true;
+    s.anchors = ws + at.anchors, s.anchor_dots = dots;
+    if ((rc = sweep_rows<T>(s, stream)) != PSIG_OK) return rc;
+    s = sweep_of(d, decay);         // grad_v, and the gradient of the initial state
+    s.r = K, s.k = Q, s.v = G;
+    s.d1 = d.dk, s.d2 = d.dv;
+    s.reverse = true;
+    s.kv_scale = d.scale;
+    s.init = gs;
+    s.final = grad_init;
+    s.out = gv, s.out_acc = true;
+    if ((rc = sweep_rows<T>(s, stream)) != PSIG_OK) return rc;
+
+    attn_sum_heads<T><<<blocks_for(rows * d.dk, 256), 256, 0, stream>>>(gq, static_cast<T *>(grad_q), rows * d.dk, 1, d.dk);
+    if ((rc = check_launch()) != PSIG_OK) return rc;
+    attn_sum_heads<T><<<blocks_for(kv_rows * d.dk, 256), 256, 0, stream>>>(gk, static_cast<T *>(grad_k), kv_rows * d.dk, share, d.dk);
+    if ((rc = check_launch()) != PSIG_OK) return rc;
+    attn_sum_heads<T><<<blocks_for(kv_rows * d.dv, 256), 256, 0, stream>>>(gv, static_cast<T *>(grad_v), kv_rows * d.dv, share, d.dv);
+    if ((rc = check_launch()) != PSIG_OK) return rc;
+    if (grad_decay == nullptr) return PSIG_OK;
+    attn_pair_difference<T><<<blocks_for(rows, 8), 256, 0, stream>>>(Q, K, gq, gk, pairs, rows, d.L, d.H, d.dk);
+    if ((rc = check_launch()) != PSIG_OK) return rc;
+    const bool total = per_head(d);
+    // the grid's second dimension is limited to 65535
+    const long long per_launch = 65535 / d.H;
+    for (long long b0 = 0; b0 < d.B; b0 += per_launch) {
+        const long long nb = d.B - b0 < per_launch ? d.B - b0 : per_launch;
+        attn_decay_grad<A><<<dim3((unsigned)segments, (unsigned)(nb * d.H)), kSegment, 0, stream>>>(
+            pairs + b0 * d.L * d.H, dots + b0 * d.H * segments * column_tiles(d.dk), column_tiles(d.dk),
+            static_cast<const A *>(decay) + b0 * d.decay_strides[0], d.decay_strides[0], d.decay_strides[1],
+            d.decay_strides[2], d.lengths == nullptr ? nullptr : d.lengths + b0, d.L, d.H,
+            total ? nullptr : static_cast<A *>(grad_decay) + b0 * d.L * d.H, total ? totals + b0 * d.H * segments : nullptr);
+        if ((rc = check_launch()) != PSIG_OK) return rc;
+    }
+    if (total) {
+        attn_decay_total<A><<<(unsigned)d.H, 256, 0, stream>>>(totals, d.B, d.H, segments, static_cast<A *>(grad_decay));
+        if ((rc = check_launch()) != PSIG_OK) return rc;
+    }
+    return PSIG_OK;
+}
+
+}  // namespace
+}  // namespace psig
+
+using namespace psig;
+
+extern "C" int64_t psig_attn_forward_workspace(const PsigAttnDesc *desc) { return check_attn(desc); }
+
+extern "C" int64_t psig_attn_backward_workspace(const PsigAttnDesc *desc)
+{
+    const int rc = check_attn(desc);
+    return rc != PSIG_OK ? rc : backward_scratch(*desc).bytes;
+}
+
+extern "C" int psig_attn_forward(const PsigAttnDesc *desc, const void *q, const void *k, const void *v,
+                                 const void *log_decay, const void *initial_state, void *out, void *final_state,
+                                 void *workspace, int64_t workspace_bytes, void *stream)
+{
+    const int rc = check_attn(desc);
+    if (rc != PSIG_OK) return rc;
+    (void)workspace, (void)workspace_bytes;
+    if (desc->B == 0) return PSIG_OK;
+    if (desc->L > 0 && (!q || !k || !v || !log_decay || !out)) return PSIG_ERR_NULL;
+    if (desc->L == 0 && final_state == nullptr) return PSIG_OK;
+    return with_dtype(desc->dtype, [&](auto t) {
+        return run_forward<decltype(t)>(*desc, q, k, v, log_decay, initial_state, out, final_state,
+                                        static_cast<cudaStream_t>(stream));
+    });
+}
+
+extern "C" int psig_attn_backward(const PsigAttnDesc *desc, const void *q, const void *k, const void *v,
+                                  const void *log_decay, const void *initial_state, const void *grad_out,
+                                  const void *grad_state, void *grad_q, void *grad_k, void *grad_v,
+                                  void *grad_log_decay, void *grad_initial_state, void *workspace,
+                                  int64_t workspace_bytes, void *stream)
+{
+    const int rc = check_attn(desc);
+    if (rc != PSIG_OK) return rc;
+    if (desc->B == 0 || desc->L == 0) return PSIG_OK;   // nothing depends on the operands
+    if (!q || !k || !v || !log_decay || !grad_out || !grad_q || !grad_k || !grad_v) return PSIG_ERR_NULL;
+    const int64_t need = backward_scratch(*desc).bytes;
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return PSIG_ERR_WORKSPACE;
+    return with_dtype(desc->dtype, [&](auto t) {
+        return run_backward<decltype(t)>(*desc, q, k, v, log_decay, initial_state, grad_out, grad_state, grad_q, grad_k,
+                                         grad_v, grad_log_decay, grad_initial_state, static_cast<char *>(workspace),
+                                         static_cast<cudaStream_t>(stream));
+    });
+}
+
+extern "C" int psig_attn_step(const PsigAttnDesc *desc, const void *q, const void *k, const void *v,
+                              const void *log_decay, void *state, void *out, void *stream)
+{
+    const int rc = check_attn(desc);
+    if (rc != PSIG_OK) return rc;
+    if (desc->B == 0) return PSIG_OK;
+    if (!q || !k || !v || !log_decay || !state || !out) return PSIG_ERR_NULL;
+    const int share = desc->H / desc->Hkv;
+    const dim3 grid((unsigned)(desc->B * desc->H), (unsigned)column_tiles(desc->dv));
+    return with_dtype(desc->dtype, [&](auto t) {
+        using T = decltype(t);
+        using A = typename Acc<T>::type;
+        attn_step_rows<T><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
+            operand(q, desc->q_strides, 1), operand(k, desc->k_strides, share), operand(v, desc->v_strides, share),
+            static_cast<const A *>(log_decay), desc->decay_strides[0], desc->decay_strides[2], static_cast<A *>(state),
+            static_cast<T *>(out), desc->H, desc->dk, desc->dv, desc->scale);
+        return check_launch();
+    });
+}

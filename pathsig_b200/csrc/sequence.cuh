@@ -1,0 +1,81 @@
+// What the sequence operators (decayed linear attention, norm around a block) share: scalar types, the
+// description of one sweep over the time axis, and the checks of the C entry points (internal header).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace psig {
+
+// Type of sums, states and parameters next to a storage type: 32 bits, 64 for float64.
+template <typename T> struct Acc { using type = float; };
+template <> struct Acc<double> { using type = double; };
+
+template <typename A> __device__ __forceinline__ A to_acc(float v) { return (A)v; }
+template <typename A> __device__ __forceinline__ A to_acc(double v) { return (A)v; }
+template <typename A> __device__ __forceinline__ A to_acc(__nv_bfloat16 v) { return (A)__bfloat162float(v); }
+template <typename A> __device__ __forceinline__ A to_acc(__half v) { return (A)__half2float(v); }
+
+template <typename T> __device__ __forceinline__ T from_acc(float v) { return (T)v; }
+template <typename T> __device__ __forceinline__ T from_acc(double v) { return (T)v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_acc<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_acc<__half>(float v) { return __float2half_rn(v); }
+
+__device__ __forceinline__ float exp_acc(float v) { return expf(v); }
+__device__ __forceinline__ double exp_acc(double v) { return exp(v); }
+
+// Calls fn.template operator()<T>() with the storage type of a PsigDtype.
+template <typename Fn>
+int with_dtype(int dtype, Fn fn)
+{
+    switch (dtype) {
+        case PSIG_F32: return fn(float{});
+        case PSIG_F64: return fn(double{});
+        case PSIG_BF16: return fn(__nv_bfloat16{});
+        case PSIG_F16: return fn(__half{});
+        default: return PSIG_ERR_DTYPE;
+    }
+}
+
+// One sweep over the time axis, the shape that the forward pass and the three gradients share.  With weights
+// w(t, s) = exp(sum of the decays of the steps from s to t), S held per (sequence, head) with shape (d1, d2):
+//     out_t = out_scale * ( sum_{s before or at t} w(t, s) kv_scale (r_t . k_s) v_s + w(t, start) r_t^T init )
+// "before" is earlier, or later when `reverse` is set.
+//     forward:  r = q,  k = k,  v = v,  init = initial_state                  (d1, d2) = (dk, dv)
+//     grad_q:   r = go, k = v,  v = k,  init = initial_state^T                (d1, d2) = (dv, dk)
+//     grad_k:   r = v,  k = go, v = q,  init = grad_state^T, reverse          (d1, d2) = (dv, dk)
+//     grad_v:   r = k,  k = q,  v = go, init = grad_state,   reverse          (d1, d2) = (dk, dv)
+struct SweepOperand {
+    const void *data;
+    long long stride[3];  // elements, for (b, t, head)
+    int share;            // sweep heads per operand head
+};
+
+constexpr int kSegment = 512;  // time steps between two kept states of the decay gradient
+
+struct Sweep {
+    SweepOperand r, k, v;
+    const void *decay;
+    long long decay_stride[3];
+    const int *lengths;
+    long long B, L;
+    int H, d1, d2;
+    bool reverse;
+    double out_scale, kv_scale;
+    const void *init;     // (B, H, d1, d2), or (B, H, d2, d1) when transposed; NULL: zeros
+    bool init_transposed;
+    void *final;          // same, or NULL
+    bool final_transposed;
+    void *out;            // (B, L, H, d2): storage type, or the type of sums when out_acc is set
+    bool out_acc;
+    // Decay gradient (see attn_decay_grad): the grad_q sweep stores the state at the end of every kSegment steps,
+    // the grad_k sweep multiplies its own state into it and leaves one number per segment and column tile.
+    void *anchors;        // (B, H, segments, d1, d2)
+    void *anchor_dots;    // (B, H, segments, column tiles)
+};
+
+inline long long segments_of(long long L) { return (L + kSegment - 1) / kSegment; }
+
+}  // namespace psig

@@ -4,7 +4,8 @@
 // TORCH_LIBRARY_IMPL(pathsig, CUDA, ...) blocks of its launchers (src/pathsig/forward/sig_launch.cu:345-348,
 // src/pathsig/backward/sig_backward_launch.cu:468-471): the same four schemas, registered for the CUDA key
 // only, in the namespace `pathsig_b200` (so that a build of the reference can be loaded in the same
-// process), plus the operators the reference does not have (projected log-signature, Chen product).
+// process), plus the operators the reference does not have (projected log-signature, Chen product, decayed linear
+// attention, norm around a block).
 // Every implementation validates like the reference launchers (src/pathsig/forward/sig_launch.cu:84-121,
 // src/pathsig/backward/sig_backward_launch.cu:94-155), allocates its outputs with the caching allocator
 // and hands raw pointers plus the current stream to the C ABI of include/pathsig_b200.h.  torch is used
@@ -19,8 +20,10 @@
 #include <nvtx3/nvToolsExt.h>
 
 #include <atomic>
+#include <cmath>
 #include <list>
 #include <mutex>
+#include <optional>
 #include <tuple>
 #include <vector>
 
@@ -404,6 +407,303 @@ std::tuple<at::Tensor, at::Tensor> chen_product_backward(const at::Tensor &sig_a
     return std::make_tuple(ga, gb);
 }
 
+// ---- decayed linear attention and the norm around a block (no counterpart in the reference) ----
+
+int sequence_dtype(const at::Tensor &t, const char *name)
+{
+    switch (t.scalar_type()) {
+        case at::kFloat: return PSIG_F32;
+        case at::kDouble: return PSIG_F64;
+        case at::kBFloat16: return PSIG_BF16;
+        case at::kHalf: return PSIG_F16;
+        default: TORCH_CHECK(false, name, " must be float32, float64, bfloat16 or float16");
+    }
+}
+
+// Type of states, decays and parameters next to operands of this type.
+at::ScalarType sum_type(const at::Tensor &t) { return t.scalar_type() == at::kDouble ? at::kDouble : at::kFloat; }
+
+void check_operand(const at::Tensor &anchor, const at::Tensor &t, const char *name, at::ScalarType type)
+{
+    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(t.device() == anchor.device(), name, " must be on the same device as q or x (", name, " is on ",
+                t.device(), ", expected ", anchor.device(), ")");
+    TORCH_CHECK(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
+}
+
+// The kernels read operands through their strides; only the last dimension has to be dense.
+at::Tensor dense_last(const at::Tensor &t) { return t.size(-1) > 1 && t.stride(-1) != 1 ? t.contiguous() : t; }
+
+void set_strides(int64_t *to, const at::Tensor &t, bool has_time)
+{
+    to[0] = t.stride(0);
+    to[1] = has_time ? t.stride(1) : 0;
+    to[2] = t.stride(has_time ? 2 : 1);
+}
+
+// q (B, [L,] H, dk), k (B, [L,] Hkv, dk), v (B, [L,] Hkv, dv), log_decay (H) or (B, [L,] H)
+PsigAttnDesc attn_desc(at::Tensor &q, at::Tensor &k, at::Tensor &v, at::Tensor &log_decay, double scale, bool has_time)
+{
+    const int64_t dims = has_time ? 4 : 3;
+    const char *shape = has_time ? "(B, L, H, D)" : "(B, H, D)";
+    TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+    PsigAttnDesc desc{};
+    desc.dtype = sequence_dtype(q, "q");
+    check_operand(q, k, "k", q.scalar_type());
+    check_operand(q, v, "v", q.scalar_type());
+    check_operand(q, log_decay, "log_decay", sum_type(q));
+    TORCH_CHECK(q.dim() == dims && k.dim() == dims && v.dim() == dims, "q, k and v must have shape ", shape);
+    for (int64_t i = 0; i + 2 < dims; ++i)
+        TORCH_CHECK(k.size(i) == q.size(i) && v.size(i) == q.size(i), "q, k and v must agree in all but heads and head size");
+    TORCH_CHECK(k.size(-1) == q.size(-1), "k must have the head size of q");
+    TORCH_CHECK(k.size(-2) == v.size(-2), "k and v must have the same number of heads");
+    TORCH_CHECK(q.size(-2) >= 1 && k.size(-2) >= 1 && q.size(-2) % k.size(-2) == 0, "the number of heads of q (", q.size(-2),
+                ") must be a multiple of that of k and v (", k.size(-2), ")");
+    TORCH_CHECK(q.size(-1) >= 1 && q.size(-1) <= 256 && v.size(-1) >= 1 && v.size(-1) <= 256, "head sizes must be in [1,256]");
+    TORCH_CHECK(std::isfinite(scale), "scale must be finite");
+    desc.B = q.size(0);
+    desc.L = has_time ? q.size(1) : 1;
+    desc.H = (int32_t)q.size(-2);
+    desc.Hkv = (int32_t)k.size(-2);
+    desc.dk = (int32_t)q.size(-1);
+    desc.dv = (int32_t)v.size(-1);
+    desc.scale = scale;
+    desc.algo = g_algo.load() == PSIG_ALGO_GENERIC ? PSIG_ALGO_GENERIC : PSIG_ALGO_AUTO;
+    q = dense_last(q), k = dense_last(k), v = dense_last(v);
+    set_strides(desc.q_strides, q, has_time);
+    set_strides(desc.k_strides, k, has_time);
+    set_strides(desc.v_strides, v, has_time);
+    log_decay = log_decay.contiguous();
+    if (log_decay.dim() == 1) {
+        TORCH_CHECK(log_decay.size(0) == desc.H, "log_decay must have one entry per head of q");
+        desc.decay_strides[2] = 1;
+    } else {
+        TORCH_CHECK(log_decay.dim() == dims - 1 && log_decay.size(0) == desc.B && (!has_time || log_decay.size(1) == desc.L) &&
+                    log_decay.size(-1) == desc.H, "log_decay must have shape (H) or ", has_time ? "(B, L, H)" : "(B, H)");
+        desc.decay_strides[0] = desc.L * desc.H;
+        desc.decay_strides[1] = has_time ? desc.H : 0;
+        desc.decay_strides[2] = 1;
+    }
+    return desc;
+}
+
+void check_state(const PsigAttnDesc &desc, const at::Tensor &q, const at::Tensor &t, const char *name)
+{
+    check_operand(q, t, name, sum_type(q));
+    TORCH_CHECK(t.dim() == 4 && t.size(0) == desc.B && t.size(1) == desc.H && t.size(2) == desc.dk && t.size(3) == desc.dv, name,
+                " must have shape (B, H, Dk, Dv)");
+}
+
+at::Tensor sequence_lengths(const PsigAttnDesc &desc, const at::Tensor &q, const std::optional<at::Tensor> &lengths)
+{
+    if (!lengths.has_value()) return at::Tensor();
+    TORCH_CHECK(lengths->is_cuda() && lengths->device() == q.device(), "lengths must be on the same device as q");
+    TORCH_CHECK(lengths->scalar_type() == at::kInt || lengths->scalar_type() == at::kLong, "lengths must be int32 or int64");
+    TORCH_CHECK(lengths->dim() == 1 && lengths->size(0) == desc.B, "lengths must have shape (B)");
+    // clamped before the narrowing, so that no 64-bit value wraps into the valid range
+    return (lengths->scalar_type() == at::kLong ? lengths->clamp(0, desc.L).to(at::kInt) : *lengths).contiguous();
+}
+
+std::tuple<at::Tensor, at::Tensor> linear_attention(const at::Tensor &q_in, const at::Tensor &k_in, const at::Tensor &v_in,
+                                                    const at::Tensor &log_decay_in, const std::optional<at::Tensor> &initial_state,
+                                                    const std::optional<at::Tensor> &lengths_in, double scale, bool return_state)
+{
+    Range range("pathsig_b200::linear_attention");
+    TORCH_CHECK(q_in.is_cuda(), "q must be a CUDA tensor");
+    c10::cuda::CUDAGuard guard(q_in.device());
+    at::Tensor q = q_in, k = k_in, v = v_in, decay = log_decay_in;
+    PsigAttnDesc desc = attn_desc(q, k, v, decay, scale, true);
+    at::Tensor init;
+    if (initial_state.has_value()) {
+        check_state(desc, q, *initial_state, "initial_state");
+        init = initial_state->contiguous();
+    }
+    at::Tensor lengths = sequence_lengths(desc, q, lengths_in);
+    desc.lengths = lengths.defined() && lengths.numel() > 0 ? lengths.data_ptr<int32_t>() : nullptr;
+    at::Tensor out = at::empty({desc.B, desc.L, desc.H, desc.dv}, q.options());
+    at::Tensor final = return_state ? at::empty({desc.B, desc.H, desc.dk, desc.dv}, decay.options())
+                                    : at::empty({0}, decay.options());
+    if (desc.B == 0) return std::make_tuple(out, final);
+    if (desc.L == 0) {
+        if (return_state) init.defined() ? final.copy_(init) : final.zero_();
+        return std::make_tuple(out, final);
+    }
+    const int64_t ws_bytes = psig_attn_forward_workspace(&desc);
+    check(ws_bytes, "linear_attention");
+    at::Tensor ws = at::empty({ws_bytes}, q.options().dtype(at::kByte));
+    check(psig_attn_forward(&desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr(), init.defined() ? init.data_ptr() : nullptr,
+                            out.data_ptr(), return_state ? final.data_ptr() : nullptr, ws_bytes > 0 ? ws.data_ptr() : nullptr,
+                            ws_bytes, stream_of(q)),
+          "linear_attention");
+    return std::make_tuple(out, final);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_attention_backward(
+    const at::Tensor &q_in, const at::Tensor &k_in, const at::Tensor &v_in, const at::Tensor &log_decay_in,
+    const std::optional<at::Tensor> &initial_state, const std::optional<at::Tensor> &lengths_in,
+    const std::optional<at::Tensor> &grad_out, const std::optional<at::Tensor> &grad_state, double scale, bool decay_grad)
+{
+    Range range("pathsig_b200::linear_attention_backward");
+    TORCH_CHECK(q_in.is_cuda(), "q must be a CUDA tensor");
+    c10::cuda::CUDAGuard guard(q_in.device());
+    at::Tensor q = q_in, k = k_in, v = v_in, decay = log_decay_in;
+    PsigAttnDesc desc = attn_desc(q, k, v, decay, scale, true);
+    at::Tensor init, go, gs;
+    if (initial_state.has_value()) {
+        check_state(desc, q, *initial_state, "initial_state");
+        init = initial_state->contiguous();
+    }
+    if (grad_out.has_value()) {
+        check_operand(q, *grad_out, "grad_out", q.scalar_type());
+        TORCH_CHECK(grad_out->dim() == 4 && grad_out->size(0) == desc.B && grad_out->size(1) == desc.L &&
+                    grad_out->size(2) == desc.H && grad_out->size(3) == desc.dv, "grad_out must have the shape of the output");
+        go = grad_out->contiguous();
+    } else {
+        go = at::zeros({desc.B, desc.L, desc.H, desc.dv}, q.options());
+    }
+    if (grad_state.has_value()) {
+        check_state(desc, q, *grad_state, "grad_state");
+        gs = grad_state->contiguous();
+    }
+    at::Tensor lengths = sequence_lengths(desc, q, lengths_in);
+    desc.lengths = lengths.defined() && lengths.numel() > 0 ? lengths.data_ptr<int32_t>() : nullptr;
+    at::Tensor gq = at::empty(q.sizes(), q.options()), gk = at::empty(k.sizes(), q.options()), gv = at::empty(v.sizes(), q.options());
+    at::Tensor gd = decay_grad ? at::empty(decay.sizes(), decay.options()) : at::empty({0}, decay.options());
+    at::Tensor gi = init.defined() ? at::empty(init.sizes(), init.options()) : at::empty({0}, decay.options());
+    if (desc.B == 0 || desc.L == 0) {
+        gd.zero_();
+        if (init.defined()) gs.defined() ? gi.copy_(gs) : gi.zero_();
+        return std::make_tuple(gq, gk, gv, gd, gi);
+    }
+    const int64_t ws_bytes = psig_attn_backward_workspace(&desc);
+    check(ws_bytes, "linear_attention_backward");
+    at::Tensor ws = at::empty({ws_bytes}, q.options().dtype(at::kByte));
+    check(psig_attn_backward(&desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr(), init.defined() ? init.data_ptr() : nullptr,
+                             go.data_ptr(), gs.defined() ? gs.data_ptr() : nullptr, gq.data_ptr(), gk.data_ptr(), gv.data_ptr(),
+                             decay_grad ? gd.data_ptr() : nullptr, init.defined() ? gi.data_ptr() : nullptr,
+                             ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, stream_of(q)),
+          "linear_attention_backward");
+    return std::make_tuple(gq, gk, gv, gd, gi);
+}
+
+at::Tensor linear_attention_step(const at::Tensor &q_in, const at::Tensor &k_in, const at::Tensor &v_in,
+                                 const at::Tensor &log_decay_in, at::Tensor &state, double scale)
+{
+    Range range("pathsig_b200::linear_attention_step");
+    TORCH_CHECK(q_in.is_cuda(), "q must be a CUDA tensor");
+    c10::cuda::CUDAGuard guard(q_in.device());
+    at::Tensor q = q_in, k = k_in, v = v_in, decay = log_decay_in;
+    PsigAttnDesc desc = attn_desc(q, k, v, decay, scale, false);
+    check_state(desc, q, state, "state");
+    TORCH_CHECK(state.is_contiguous(), "state must be contiguous: it is updated in place");
+    for (const at::Tensor *t : {&q_in, &k_in, &v_in, &log_decay_in})
+        TORCH_CHECK(!t->is_alias_of(state), "state must not share memory with the other operands: it is updated in place");
+    at::Tensor out = at::empty({desc.B, desc.H, desc.dv}, q.options());
+    if (desc.B == 0) return out;
+    check(psig_attn_step(&desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr(), state.data_ptr(), out.data_ptr(),
+                         stream_of(q)),
+          "linear_attention_step");
+    return out;
+}
+
+// Operands of the norm, checked and contiguous; undefined where they are left out.
+struct NormOperands {
+    PsigNormDesc desc{};
+    at::Tensor x, weight, gate, residual, scale, next;
+};
+
+const void *data_or_null(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+NormOperands norm_operands(const at::Tensor &x, const std::optional<at::Tensor> &weight, const std::optional<at::Tensor> &gate,
+                           const std::optional<at::Tensor> &residual, const std::optional<at::Tensor> &residual_scale,
+                           const std::optional<at::Tensor> &next_weight, int64_t activation, double eps)
+{
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "x must have shape (..., D) with D >= 1");
+    TORCH_CHECK(activation == 0 || activation == 1, "activation must be 0 (silu) or 1 (sigmoid)");
+    TORCH_CHECK(std::isfinite(eps) && eps >= 0, "eps must be finite and not negative");
+    NormOperands n;
+    n.desc.dtype = sequence_dtype(x, "x");
+    n.desc.activation = (int32_t)activation;
+    n.desc.D = x.size(-1);
+    n.desc.rows = x.numel() / x.size(-1);
+    n.desc.eps = eps;
+    n.x = x.contiguous();
+    auto rows = [&](const std::optional<at::Tensor> &t, const char *name, at::Tensor *to) {
+        if (!t.has_value()) return;
+        check_operand(x, *t, name, x.scalar_type());
+        TORCH_CHECK(t->sizes() == x.sizes(), name, " must have the shape of x");
+        *to = t->contiguous();
+    };
+    auto vector = [&](const std::optional<at::Tensor> &t, const char *name, at::Tensor *to) {
+        if (!t.has_value()) return;
+        check_operand(x, *t, name, sum_type(x));
+        TORCH_CHECK(t->dim() == 1 && t->size(0) == n.desc.D, name, " must have shape (D)");
+        *to = t->contiguous();
+    };
+    rows(gate, "gate", &n.gate);
+    rows(residual, "residual", &n.residual);
+    vector(weight, "weight", &n.weight);
+    vector(residual_scale, "residual_scale", &n.scale);
+    vector(next_weight, "next_weight", &n.next);
+    return n;
+}
+
+std::tuple<at::Tensor, at::Tensor> gated_residual_norm(const at::Tensor &x, const std::optional<at::Tensor> &weight,
+                                                       const std::optional<at::Tensor> &gate, const std::optional<at::Tensor> &residual,
+                                                       const std::optional<at::Tensor> &residual_scale,
+                                                       const std::optional<at::Tensor> &next_weight, int64_t activation, double eps)
+{
+    Range range("pathsig_b200::gated_residual_norm");
+    TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    c10::cuda::CUDAGuard guard(x.device());
+    NormOperands o = norm_operands(x, weight, gate, residual, residual_scale, next_weight, activation, eps);
+    at::Tensor h = at::empty(x.sizes(), x.options());
+    at::Tensor n = o.next.defined() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+    if (o.desc.rows == 0) return std::make_tuple(h, n);
+    check(psig_norm_forward(&o.desc, o.x.data_ptr(), data_or_null(o.weight), data_or_null(o.gate), data_or_null(o.residual),
+                            data_or_null(o.scale), data_or_null(o.next), h.data_ptr(), o.next.defined() ? n.data_ptr() : nullptr,
+                            stream_of(x)),
+          "gated_residual_norm");
+    return std::make_tuple(h, n);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_residual_norm_backward(
+    const at::Tensor &x, const std::optional<at::Tensor> &weight, const std::optional<at::Tensor> &gate,
+    const std::optional<at::Tensor> &residual, const std::optional<at::Tensor> &residual_scale,
+    const std::optional<at::Tensor> &next_weight, const std::optional<at::Tensor> &grad_h_in,
+    const std::optional<at::Tensor> &grad_n_in, int64_t activation, double eps)
+{
+    Range range("pathsig_b200::gated_residual_norm_backward");
+    TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    c10::cuda::CUDAGuard guard(x.device());
+    NormOperands o = norm_operands(x, weight, gate, residual, residual_scale, next_weight, activation, eps);
+    at::Tensor grad_h, grad_n;
+    for (auto [t, name, to] : {std::make_tuple(&grad_h_in, "grad_h", &grad_h), std::make_tuple(&grad_n_in, "grad_n", &grad_n)}) {
+        if (!t->has_value()) continue;
+        check_operand(x, **t, name, x.scalar_type());
+        TORCH_CHECK((*t)->sizes() == x.sizes(), name, " must have the shape of x");
+        *to = (*t)->contiguous();
+    }
+    if (o.next.defined() && !grad_n.defined()) grad_n = at::zeros(x.sizes(), x.options());
+    auto like = [&](const at::Tensor &t) { return t.defined() ? at::empty(t.sizes(), t.options()) : at::empty({0}, x.options()); };
+    at::Tensor gx = at::empty(x.sizes(), x.options()), gw = like(o.weight), gg = like(o.gate), gr = like(o.residual),
+               gs = like(o.scale), gn = like(o.next);
+    if (o.desc.rows == 0) {
+        for (at::Tensor *t : {&gw, &gs, &gn}) t->zero_();
+        return std::make_tuple(gx, gw, gg, gr, gs, gn);
+    }
+    const int64_t ws_bytes = psig_norm_backward_workspace(&o.desc);
+    check(ws_bytes, "gated_residual_norm_backward");
+    at::Tensor ws = at::empty({ws_bytes}, x.options().dtype(at::kByte));
+    auto to = [](const at::Tensor &operand, at::Tensor &grad) { return operand.defined() ? grad.data_ptr() : nullptr; };
+    check(psig_norm_backward(&o.desc, o.x.data_ptr(), data_or_null(o.weight), data_or_null(o.gate), data_or_null(o.residual),
+                             data_or_null(o.scale), data_or_null(o.next), data_or_null(grad_h), data_or_null(grad_n), gx.data_ptr(),
+                             to(o.weight, gw), to(o.gate, gg), to(o.residual, gr), to(o.scale, gs), to(o.next, gn), ws.data_ptr(),
+                             ws_bytes, stream_of(x)),
+          "gated_residual_norm_backward");
+    return std::make_tuple(gx, gw, gg, gr, gs, gn);
+}
+
 }  // namespace
 
 // Kernel family used by the signature operators (PsigAlgo); tests flip it to compare families.
@@ -428,6 +728,16 @@ TORCH_LIBRARY(pathsig_b200, m)
           "int[] level_sizes, Tensor lower_columns) -> Tensor", {tag});
     m.def("chen_product(Tensor sig_a, Tensor sig_b, int depth, int d) -> Tensor", {tag});
     m.def("chen_product_backward(Tensor sig_a, Tensor sig_b, Tensor grad_out, int depth, int d) -> (Tensor, Tensor)", {tag});
+    m.def("linear_attention(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? initial_state, Tensor? lengths, "
+          "float scale, bool return_state) -> (Tensor, Tensor)", {tag});
+    m.def("linear_attention_backward(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? initial_state, Tensor? lengths, "
+          "Tensor? grad_out, Tensor? grad_state, float scale, bool decay_grad) -> (Tensor, Tensor, Tensor, Tensor, Tensor)", {tag});
+    m.def("linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor(a!) state, float scale) -> Tensor", {tag});
+    m.def("gated_residual_norm(Tensor x, Tensor? weight, Tensor? gate, Tensor? residual, Tensor? residual_scale, "
+          "Tensor? next_weight, int activation, float eps) -> (Tensor, Tensor)", {tag});
+    m.def("gated_residual_norm_backward(Tensor x, Tensor? weight, Tensor? gate, Tensor? residual, Tensor? residual_scale, "
+          "Tensor? next_weight, Tensor? grad_h, Tensor? grad_n, int activation, float eps) "
+          "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)", {tag});
 }
 
 TORCH_LIBRARY_IMPL(pathsig_b200, CUDA, m)
@@ -440,4 +750,9 @@ TORCH_LIBRARY_IMPL(pathsig_b200, CUDA, m)
     m.impl("logsig_projected_backward", &logsig_projected_backward);
     m.impl("chen_product", &chen_product);
     m.impl("chen_product_backward", &chen_product_backward);
+    m.impl("linear_attention", &linear_attention);
+    m.impl("linear_attention_backward", &linear_attention_backward);
+    m.impl("linear_attention_step", &linear_attention_step);
+    m.impl("gated_residual_norm", &gated_residual_norm);
+    m.impl("gated_residual_norm_backward", &gated_residual_norm_backward);
 }

@@ -3,8 +3,8 @@
 Host-side mirror of ``src/pathsig/ops.py`` of the reference: thin wrappers around the dispatcher
 entries, the same fake (meta) shape functions (``ops.py:59-84, 101-123, 152-179, 197-227``) and the
 same autograd wiring (``ops.py:231-297``).  The operators themselves -- the four schemas of
-``src/pathsig/bindings.cpp:9-63`` plus the projected log-signature and the Chen product, registered
-for the CUDA key only -- live in the compiled library ``libpathsig_b200_torch.so``
+``src/pathsig/bindings.cpp:9-63`` plus the projected log-signature, the Chen product, decayed linear
+attention and the norm around a block, registered for the CUDA key only -- live in the compiled library ``libpathsig_b200_torch.so``
 (``csrc/torch_binding.cpp``), which validates like the reference launchers, allocates outputs with
 torch's caching allocator and hands raw pointers plus the current stream to the C ABI
 (``include/pathsig_b200.h``).  torch is used for memory, streams and dispatch only.
@@ -18,7 +18,7 @@ the compiled ones.
 from __future__ import annotations
 
 import ctypes
-from typing import List, Sequence, Tuple
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
@@ -27,7 +27,9 @@ from . import _load
 
 __all__ = ["compute_signature", "sig_to_logsig", "signature_backward", "logsig_backward",
            "logsig_projected", "logsig_projected_backward", "logsig_projected_supported",
-           "chen_product", "chen_product_backward", "register_namespace", "NAMESPACE"]
+           "chen_product", "chen_product_backward", "linear_attention", "linear_attention_backward",
+           "linear_attention_step", "gated_residual_norm", "gated_residual_norm_backward", "register_namespace",
+           "NAMESPACE"]
 
 NAMESPACE = "pathsig_b200"
 
@@ -51,6 +53,18 @@ _SCHEMAS = {
     # not in the reference: Chen product of two dense truncated signatures and its adjoint
     "chen_product": "(Tensor sig_a, Tensor sig_b, int depth, int d) -> Tensor",
     "chen_product_backward": "(Tensor sig_a, Tensor sig_b, Tensor grad_out, int depth, int d) -> (Tensor, Tensor)",
+    # not in the reference: decayed linear attention over the time axis, and the norm around a block
+    "linear_attention": "(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? initial_state, Tensor? lengths, "
+                        "float scale, bool return_state) -> (Tensor, Tensor)",
+    "linear_attention_backward": "(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? initial_state, "
+                                 "Tensor? lengths, Tensor? grad_out, Tensor? grad_state, float scale, bool decay_grad) "
+                                 "-> (Tensor, Tensor, Tensor, Tensor, Tensor)",
+    "linear_attention_step": "(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor(a!) state, float scale) -> Tensor",
+    "gated_residual_norm": "(Tensor x, Tensor? weight, Tensor? gate, Tensor? residual, Tensor? residual_scale, "
+                           "Tensor? next_weight, int activation, float eps) -> (Tensor, Tensor)",
+    "gated_residual_norm_backward": "(Tensor x, Tensor? weight, Tensor? gate, Tensor? residual, Tensor? residual_scale, "
+                                    "Tensor? next_weight, Tensor? grad_h, Tensor? grad_n, int activation, float eps) "
+                                    "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)",
 }
 
 # Kernel family used by the signature operators: _load.ALGO_AUTO / ALGO_GENERIC / ALGO_TILED / ALGO_CLOSURE.
@@ -118,6 +132,14 @@ def logsig_projected_supported(dtype: torch.dtype, depth: int, d: int, level_siz
     desc.top_size = int(level_sizes[depth])
     desc.top_words = 1 if desc.top_size != int(d) ** int(depth) else None
     return lib.psig_logsig_cache_size(ctypes.byref(desc)) == 0
+
+
+_SEQUENCE_DTYPES = (torch.float32, torch.float64, torch.bfloat16, torch.float16)
+
+
+def _sum_dtype(t: Tensor) -> torch.dtype:
+    """Type of states, decays and parameters next to operands of this type."""
+    return torch.float64 if t.dtype == torch.float64 else torch.float32
 
 
 def _row_width(d: int, depth: int, alt: bool, level_sizes: Sequence[int]) -> int:
@@ -242,6 +264,45 @@ def _fake_chen_product_backward(sig_a, sig_b, grad_out, depth, d):
     return torch.empty_like(sig_a), torch.empty_like(sig_b)
 
 
+def _fake_attn_check(q, k, v, log_decay):
+    torch._check(q.dtype in _SEQUENCE_DTYPES, lambda: "q must be float32, float64, bfloat16 or float16")
+    torch._check(k.dtype == q.dtype and v.dtype == q.dtype, lambda: "q, k and v must have the same dtype")
+    torch._check(k.shape[-1] == q.shape[-1], lambda: "k must have the head size of q")
+    torch._check(log_decay.dtype == _sum_dtype(q), lambda: "log_decay must be float32 (float64 for float64 operands)")
+
+
+def _fake_linear_attention(q, k, v, log_decay, initial_state, lengths, scale, return_state):
+    _fake_attn_check(q, k, v, log_decay)
+    B, L, H, dk = q.shape
+    dv = v.shape[-1]
+    state = (B, H, dk, dv) if return_state else (0,)
+    return q.new_empty((B, L, H, dv)), log_decay.new_empty(state)
+
+
+def _fake_linear_attention_backward(q, k, v, log_decay, initial_state, lengths, grad_out, grad_state, scale, decay_grad):
+    _fake_attn_check(q, k, v, log_decay)
+    return (q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape),
+            log_decay.new_empty(log_decay.shape if decay_grad else (0,)),
+            log_decay.new_empty((0,) if initial_state is None else initial_state.shape))
+
+
+def _fake_linear_attention_step(q, k, v, log_decay, state, scale):
+    _fake_attn_check(q, k, v, log_decay)
+    return q.new_empty((q.shape[0], q.shape[1], v.shape[-1]))
+
+
+def _fake_gated_residual_norm(x, weight, gate, residual, residual_scale, next_weight, activation, eps):
+    torch._check(x.dtype in _SEQUENCE_DTYPES, lambda: "x must be float32, float64, bfloat16 or float16")
+    return x.new_empty(x.shape), x.new_empty((0,) if next_weight is None else x.shape)
+
+
+def _fake_gated_residual_norm_backward(x, weight, gate, residual, residual_scale, next_weight, grad_h, grad_n,
+                                       activation, eps):
+    def like(t):
+        return x.new_empty((0,)) if t is None else t.new_empty(t.shape)
+    return (x.new_empty(x.shape), like(weight), like(gate), like(residual), like(residual_scale), like(next_weight))
+
+
 # --------------------------------------------------------------------------------------
 # registration
 # --------------------------------------------------------------------------------------
@@ -255,6 +316,11 @@ _FAKES = {
     "logsig_projected_backward": _fake_logsig_projected_backward,
     "chen_product": _fake_chen_product,
     "chen_product_backward": _fake_chen_product_backward,
+    "linear_attention": _fake_linear_attention,
+    "linear_attention_backward": _fake_linear_attention_backward,
+    "linear_attention_step": _fake_linear_attention_step,
+    "gated_residual_norm": _fake_gated_residual_norm,
+    "gated_residual_norm_backward": _fake_gated_residual_norm_backward,
 }
 _libraries = {}  # namespace -> torch.library.Library or True (kept alive for the life of the process)
 
@@ -368,6 +434,38 @@ def register_namespace(ns: str) -> None:
             ga = op.chen_product_backward.default(zero, ggb, grad_out, ctx.depth, ctx.d)[0] - grad_out
         return ga, gb, gg, None, None
 
+    def setup_attn(ctx, inputs, output):
+        q, k, v, log_decay, initial_state, lengths, scale, return_state = inputs
+        ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths)
+        ctx.scale, ctx.return_state = scale, bool(return_state)
+        ctx.set_materialize_grads(False)
+
+    def backward_attn(ctx, grad_out, grad_state):
+        q, k, v, log_decay, initial_state, lengths = ctx.saved_tensors
+        if (grad_out is None and grad_state is None) or not any(ctx.needs_input_grad[:5]):
+            return (None,) * 8
+        grads = getattr(torch.ops, ns).linear_attention_backward.default(
+            q, k, v, log_decay, initial_state, lengths, grad_out, grad_state if ctx.return_state else None, ctx.scale,
+            ctx.needs_input_grad[3])
+        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad[:5])) + (None, None, None)
+
+    def setup_norm(ctx, inputs, output):
+        ctx.save_for_backward(*inputs[:6])
+        ctx.activation, ctx.eps = int(inputs[6]), float(inputs[7])
+        ctx.set_materialize_grads(False)
+
+    def backward_norm(ctx, grad_h, grad_n):
+        saved = ctx.saved_tensors
+        if saved[5] is None:
+            grad_n = None
+        if (grad_h is None and grad_n is None) or not any(ctx.needs_input_grad[:6]):
+            return (None,) * 8
+        grads = getattr(torch.ops, ns).gated_residual_norm_backward.default(*saved, grad_h, grad_n, ctx.activation,
+                                                                            ctx.eps)
+        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad[:6])) + (None, None)
+
+    torch.library.register_autograd(f"{ns}::linear_attention", backward_attn, setup_context=setup_attn, lib=lib)
+    torch.library.register_autograd(f"{ns}::gated_residual_norm", backward_norm, setup_context=setup_norm, lib=lib)
     torch.library.register_autograd(f"{ns}::chen_product", backward_chen, setup_context=setup_chen, lib=lib)
     torch.library.register_autograd(f"{ns}::chen_product_backward", backward_chen_bwd,
                                     setup_context=setup_chen_bwd, lib=lib)
@@ -426,6 +524,44 @@ def chen_product(sig_a: Tensor, sig_b: Tensor, depth: int, d: int) -> Tensor:
 def chen_product_backward(sig_a: Tensor, sig_b: Tensor, grad_out: Tensor, depth: int, d: int) -> Tuple[Tensor, Tensor]:
     """(dL/dsig_a, dL/dsig_b) from dL/d(chen_product)."""
     return _ops.chen_product_backward.default(sig_a, sig_b, grad_out, depth, d)
+
+
+def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, initial_state: Optional[Tensor],
+                     lengths: Optional[Tensor], scale: float, return_state: bool) -> Tuple[Tensor, Tensor]:
+    """(out, final state) of decayed linear attention over the time axis; the state has no elements unless
+    ``return_state``.  Differentiable wrt q, k, v, log_decay and initial_state.  Not an operator of the reference."""
+    return _ops.linear_attention.default(q, k, v, log_decay, initial_state, lengths, scale, return_state)
+
+
+def linear_attention_backward(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, initial_state: Optional[Tensor],
+                              lengths: Optional[Tensor], grad_out: Optional[Tensor], grad_state: Optional[Tensor],
+                              scale: float, decay_grad: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """Gradients of :func:`linear_attention` wrt q, k, v, log_decay (no elements unless ``decay_grad``) and
+    initial_state (no elements without one)."""
+    return _ops.linear_attention_backward.default(q, k, v, log_decay, initial_state, lengths, grad_out, grad_state,
+                                                  scale, decay_grad)
+
+
+def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, scale: float) -> Tensor:
+    """One time step of :func:`linear_attention` for every sequence; ``state`` is updated in place."""
+    return _ops.linear_attention_step.default(q, k, v, log_decay, state, scale)
+
+
+def gated_residual_norm(x: Tensor, weight: Optional[Tensor], gate: Optional[Tensor], residual: Optional[Tensor],
+                        residual_scale: Optional[Tensor], next_weight: Optional[Tensor], activation: int,
+                        eps: float) -> Tuple[Tensor, Tensor]:
+    """(h, n) of the norm around a block; n has no elements without ``next_weight``.  Differentiable wrt all
+    tensors.  Not an operator of the reference."""
+    return _ops.gated_residual_norm.default(x, weight, gate, residual, residual_scale, next_weight, activation, eps)
+
+
+def gated_residual_norm_backward(x: Tensor, weight: Optional[Tensor], gate: Optional[Tensor], residual: Optional[Tensor],
+                                 residual_scale: Optional[Tensor], next_weight: Optional[Tensor],
+                                 grad_h: Optional[Tensor], grad_n: Optional[Tensor], activation: int,
+                                 eps: float) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """Gradients of :func:`gated_residual_norm` wrt its six tensors (no elements for those left out)."""
+    return _ops.gated_residual_norm_backward.default(x, weight, gate, residual, residual_scale, next_weight, grad_h,
+                                                     grad_n, activation, eps)
 
 
 def logsig_backward(signature: Tensor, P_arr: Tensor, grad_logsig: Tensor, depth: int,

@@ -1,0 +1,252 @@
+"""The norm around a block (gate, residual, next norm) on the GPU against 64-bit formulas and their autograd gradients."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from . import sequence_oracle as so
+from . import util
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TYPES = [torch.float64, torch.float32, torch.bfloat16, torch.float16]
+NAMES = ("x", "weight", "gate", "residual", "residual_scale", "next_weight")
+FORMS = [  # weight, gate, activation, residual, residual_scale, next_weight
+    (False, None, False, False, False),
+    (True, None, False, False, False),
+    (True, "silu", False, False, False),
+    (True, "sigmoid", True, False, True),
+    (True, "silu", True, True, True),
+    (False, None, True, True, True),
+    (True, None, False, True, True),
+]
+
+
+@pytest.fixture(scope="module")
+def ps():
+    import pathsig_b200
+    return pathsig_b200
+
+
+def _make(seed, rows, D, dtype, form, eps=1e-6):
+    gen = torch.Generator().manual_seed(seed)
+    sums = torch.float64 if dtype == torch.float64 else torch.float32
+
+    def normal(*shape, to=dtype, std=1.0, mean=0.0):
+        return (mean + std * torch.randn(*shape, generator=gen, dtype=torch.float64)).to(to).double()
+
+    weight, act, residual, scale, after = form
+    return {"x": normal(rows, D, std=2.0), "weight": normal(D, to=sums, std=0.2, mean=1.0) if weight else None,
+            "gate": normal(rows, D) if act else None, "residual": normal(rows, D, std=3.0) if residual else None,
+            "residual_scale": normal(D, to=sums, std=0.5) if scale else None,
+            "next_weight": normal(D, to=sums, std=0.2, mean=1.0) if after else None,
+            "grad_h": normal(rows, D), "grad_n": normal(rows, D) if after else None, "activation": act or "silu", "eps": eps}
+
+
+def _gpu(c, dtype):
+    sums = torch.float64 if dtype == torch.float64 else torch.float32
+    wide = ("weight", "residual_scale", "next_weight")
+    return {n: t.to(sums if n in wide else dtype).to(DEV) if isinstance(t, torch.Tensor) else t for n, t in c.items()}
+
+
+def _run(f, c):
+    leaves = {n: c[n].detach().requires_grad_(True) if c[n] is not None else None for n in NAMES}
+    h, n = f(leaves)
+    heads, grads = [h], [c["grad_h"]]
+    if n is not None:
+        heads.append(n)
+        grads.append(c["grad_n"])
+    wanted = {k: t for k, t in leaves.items() if t is not None}
+    got = {"grad_" + k: g for k, g in zip(wanted, torch.autograd.grad(heads, list(wanted.values()), grads))}
+    return got | {"h": h.detach()} | ({"n": n.detach()} if n is not None else {})
+
+
+def _ours(ps, eps):
+    def f(leaves):
+        activation = leaves.get("activation", "silu")
+        got = ps.gated_residual_norm(leaves["x"], leaves["weight"], gate=leaves["gate"], residual=leaves["residual"],
+                                     residual_scale=leaves["residual_scale"], next_weight=leaves["next_weight"],
+                                     activation=activation, eps=eps)
+        return got if leaves["next_weight"] is not None else (got, None)
+    return f
+
+
+def _check(ps, c, dtype):
+    ours = _run(lambda t: _ours(ps, c["eps"])(dict(t, activation=c["activation"])), _gpu(c, dtype))
+    exact, bounds = so.norm_bounds(c, dtype)
+    assert set(ours) == set(exact)
+    for name, want in exact.items():
+        assert ours[name].shape == want.shape, name
+        off = (ours[name].double().cpu() - want).abs()
+        bad = ~(off <= bounds[name])
+        assert not bad.any(), (name, int(bad.sum()), float(off[bad].max()), float((off / bounds[name].clamp_min(1e-300)).max()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("rows,D", [(1, 1), (3, 2), (5, 7), (33, 32), (64, 64), (7, 100), (130, 128), (9, 340), (40, 1024),
+                                    (3, 1001), (2, 4680), (2, 4096)])
+def test_outputs_and_gradients(ps, rows, D, form, dtype):
+    c = _make(rows + D, rows, D, dtype, form)
+    _check(ps, c, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,D", [(2, 8192), (2, 9001), (3, 16384), (1, 30000), (2, 69904)])
+def test_wide_rows(ps, rows, D, dtype):
+    """The widest: depth-4 signatures of 16 channels."""
+    c = _make(D, rows, D, dtype, FORMS[4])
+    _check(ps, c, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,D", [(20000, 16), (3001, 128), (2500, 1000), (1500, 2048)])
+def test_many_rows(ps, rows, D, dtype):
+    c = _make(D, rows, D, dtype, FORMS[4])
+    _check(ps, c, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_zero_rows_and_large_values(ps, dtype):
+    """A row of zeros (eps alone under the root), rows of large and of tiny values, gates far out on both sides."""
+    c = _make(1, 4, 64, dtype, FORMS[2], eps=1e-5)
+    c["x"][0] = 0
+    c["x"][1] = (c["x"][1] * 1000).to(dtype).double()      # the operands of both sides are of the type
+    c["x"][2] = (c["x"][2] * 2.0 ** -7).to(dtype).double()
+    c["gate"][3, :8] = torch.tensor([-300.0, 300.0, -90.0, 90.0, 0.0, -20.0, 20.0, -5.0], dtype=torch.float64).to(dtype).double()
+    _check(ps, c, dtype)
+
+
+def test_gradients_against_differences(ps):
+    c = _gpu(_make(4, 3, 5, torch.float64, FORMS[4]), torch.float64)
+    leaves = [c[n].requires_grad_(True) for n in NAMES]
+    for activation in ("silu", "sigmoid"):
+        assert torch.autograd.gradcheck(
+            lambda x, w, g, r, s, n: ps.gated_residual_norm(x, w, gate=g, residual=r, residual_scale=s, next_weight=n,
+                                                            activation=activation), leaves, eps=1e-6, atol=1e-8)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_shapes_strides_and_16_bit_parameters(ps, dtype):
+    x = torch.randn(2, 3, 5, 64, device=DEV).to(dtype)
+    w = torch.rand(64, device=DEV).to(dtype).requires_grad_(True)
+    want = ps.gated_residual_norm(x, w.detach().float())
+    assert want.shape == x.shape and want.dtype == dtype
+    got = ps.gated_residual_norm(x.transpose(0, 1).contiguous().transpose(0, 1), w)
+    assert torch.equal(got, want)
+    odd = torch.nn.functional.pad(x.reshape(-1), (1, 0))[1:].view_as(x)      # rows that start off a 16-byte boundary
+    assert util.rel_error(ps.gated_residual_norm(odd, w), want) < so.half_step(dtype)
+    got.float().sum().backward()
+    assert w.grad.dtype == dtype and w.grad.shape == (64,)
+    assert ps.gated_residual_norm(x[0, 0, 0]).shape == (64,)
+    assert ps.gated_residual_norm(x[:0]).shape == (0, 3, 5, 64)
+
+
+def test_only_the_next_norm_is_used(ps):
+    c = _gpu(_make(8, 6, 96, torch.float32, FORMS[4]), torch.float32)
+    r = c["residual"].requires_grad_(True)
+    _, n = ps.gated_residual_norm(c["x"], c["weight"], gate=c["gate"], residual=r, residual_scale=c["residual_scale"],
+                                  next_weight=c["next_weight"])
+    got, = torch.autograd.grad(n, r, c["grad_n"])
+    wide = {k: t.detach().double().cpu() if isinstance(t, torch.Tensor) else t for k, t in c.items()}
+    wide["residual"].requires_grad_(True)
+    want, = torch.autograd.grad(so.norm(wide)[1], wide["residual"], wide["grad_n"])
+    assert util.rel_error(got, want) < 200 * so.half_step(torch.float32)
+
+
+def test_empty_rows_have_zero_parameter_gradients(ps):
+    x = torch.zeros(0, 16, device=DEV)
+    w = torch.ones(16, device=DEV, requires_grad=True)
+    ps.gated_residual_norm(x, w).sum().backward()
+    assert torch.equal(w.grad, torch.zeros_like(w))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_same_bits_every_run_on_streams_and_in_graphs(ps, dtype):
+    c = _gpu(_make(5, 700, 1024, dtype, FORMS[4]), dtype)
+    first = _run(_ours(ps, 1e-6), c)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = _run(_ours(ps, 1e-6), c)
+    torch.cuda.current_stream().wait_stream(side)
+    args = [c[n] for n in NAMES]
+    with torch.cuda.stream(side):
+        torch.ops.pathsig_b200.gated_residual_norm_backward(*args, c["grad_h"], c["grad_n"], 0, 1e-6)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h, n = torch.ops.pathsig_b200.gated_residual_norm(*args, 0, 1e-6)
+        grads = torch.ops.pathsig_b200.gated_residual_norm_backward(*args, c["grad_h"], c["grad_n"], 0, 1e-6)
+    graph.replay()
+    graph.replay()
+    torch.cuda.synchronize()
+    third = {"h": h, "n": n, **{"grad_" + name: g for name, g in zip(NAMES, grads)}}
+    for name in first:
+        assert torch.equal(first[name], second[name]) and torch.equal(first[name], third[name]), name
+
+
+def test_a_mixing_block_on_window_signatures(ps):
+    """The operators as they are used together: window signatures, norm before the block, projections, decayed
+    attention, norm of each head with its gate, projection, norm after the block with the scaled residual and the norm
+    before the next block; outputs and the gradients of all parameters and of the paths, in 64 bits."""
+    B, d, depth, E, H = 3, 3, 3, 24, 2
+    x = util.brownian_path(B, 65, d, seed=2, dtype=torch.float64)
+    win = torch.tensor([[8 * i, 8 * i + 16] for i in range(7)], dtype=torch.int32, device=DEV)
+    gen = torch.Generator().manual_seed(5)
+    width = d + d ** 2 + d ** 3
+
+    def weight(*shape):
+        return torch.randn(*shape, generator=gen, dtype=torch.float64) / shape[0] ** 0.5
+
+    p = {"win": weight(width, E), "wqkvg": weight(E, 4 * E), "wo": weight(E, E), "n1": 1 + 0.1 * weight(width),
+         "nh": 1 + 0.1 * weight(E // H), "n2": 1 + 0.1 * weight(E), "n3": 1 + 0.1 * weight(E), "s": 0.3 * weight(E),
+         "decay": -torch.rand(H, generator=gen, dtype=torch.float64)}
+    sig_gpu = ps.Signature(depth=depth, windows=win)
+
+    def block(sig, p, norm, attention):
+        t = norm(sig, p["n1"]) @ p["win"]
+        q, k, v, g = (norm(t, None) @ p["wqkvg"]).unflatten(-1, (4, H, E // H)).unbind(-3)
+        o = norm(attention(q, k, v, p["decay"]), p["nh"], gate=g).flatten(-2) @ p["wo"]
+        h, n = norm(o, p["n2"], residual=t, residual_scale=p["s"], next_weight=p["n3"])
+        return h, n
+
+    def plain_norm(x, w, gate=None, residual=None, residual_scale=None, next_weight=None):
+        h, n = so.norm({"x": x, "weight": w, "gate": gate, "residual": residual, "residual_scale": residual_scale,
+                        "next_weight": next_weight, "activation": "silu", "eps": 1e-6})
+        return h if next_weight is None else (h, n)
+
+    def plain_attention(q, k, v, decay):
+        S, outs = torch.zeros(B, H, E // H, E // H, dtype=torch.float64), []
+        for t in range(q.shape[1]):
+            S = S * decay.exp()[:, None, None] + k[:, t, :, :, None] * v[:, t, :, None, :]
+            outs.append((q[:, t, :, None, :] @ S)[..., 0, :] * (E // H) ** -0.5)
+        return torch.stack(outs, 1)
+
+    xg = x.to(DEV).requires_grad_(True)
+    pg = {n: t.to(DEV).requires_grad_(True) for n, t in p.items()}
+    sig = sig_gpu(xg)
+    h, n = block(sig, pg, ps.gated_residual_norm, ps.linear_attention)
+    (h.square().sum() + n.sin().sum()).backward()
+    sig_cpu = sig.detach().cpu().requires_grad_(True)
+    pc = {n: t.clone().requires_grad_(True) for n, t in p.items()}
+    h2, n2 = block(sig_cpu, pc, plain_norm, plain_attention)
+    (h2.square().sum() + n2.sin().sum()).backward()
+    assert util.rel_error(h, h2) < 1e-12 and util.rel_error(n, n2) < 1e-12
+    for name in p:
+        assert util.rel_error(pg[name].grad, pc[name].grad) < 1e-11, name
+    want, = torch.autograd.grad(sig_gpu(xg), xg, sig_cpu.grad.to(DEV))
+    assert util.rel_error(xg.grad, want) < 1e-11
+
+
+def test_refusals_on_the_gpu(ps):
+    x = torch.zeros(4, 8, device=DEV)
+    for more, error in [(dict(weight=torch.ones(7, device=DEV)), "weight"), (dict(gate=torch.zeros(4, 7, device=DEV)), "gate"),
+                        (dict(gate=torch.zeros(4, 8, device=DEV, dtype=torch.bfloat16)), "gate"), (dict(residual=torch.zeros(8, device=DEV)), "residual"),
+                        (dict(next_weight=torch.ones(8, device=DEV, dtype=torch.float64)), "next_weight"), (dict(weight=torch.ones(8)), "weight")]:
+        with pytest.raises(RuntimeError, match=error):
+            ps.gated_residual_norm(x, **more)
+    with pytest.raises(RuntimeError, match="float32"):
+        ps.gated_residual_norm(x.int())
+    with pytest.raises(RuntimeError, match="D >= 1"):
+        ps.gated_residual_norm(torch.zeros(3, 0, device=DEV))

@@ -1,0 +1,116 @@
+"""CPU tests of the sequence operators' host side: entry points' checks without a GPU, shapes of fake tensors,
+refusals, and the oracle against automatic differentiation."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import pathsig_b200 as ps
+from pathsig_b200 import _load
+
+from . import sequence_oracle as so
+
+
+def _attn(**change):
+    d = _load.AttnDesc()
+    d.dtype, d.dk, d.dv, d.H, d.Hkv, d.B, d.L, d.scale = 0, 8, 8, 4, 2, 2, 5, 1.0
+    for n, v in change.items():
+        setattr(d, n, v)
+    return d
+
+
+@pytest.mark.parametrize("change,status", [(dict(dtype=4), -2), (dict(dtype=-1), -2), (dict(Hkv=3), -4), (dict(H=0), -4), (dict(B=-1), -4),
+                                           (dict(dk=257), -8), (dict(dv=0), -4), (dict(B=2 ** 30), -8)])
+def test_attention_descriptions_are_checked(change, status):
+    lib = _load.ensure_loaded()
+    d = ctypes.byref(_attn(**change))
+    assert lib.psig_attn_forward_workspace(d) == status
+    assert lib.psig_attn_backward_workspace(d) == status
+    assert lib.psig_attn_forward(d, *[None] * 8, 0, None) == status
+    assert lib.psig_attn_backward(d, *[None] * 13, 0, None) == status
+    assert lib.psig_attn_step(d, *[None] * 7) == status
+
+
+def test_missing_pointers_and_workspaces_are_refused():
+    lib = _load.ensure_loaded()
+    d = ctypes.byref(_attn())
+    one = ctypes.c_void_p(256)     # never dereferenced: every call below is refused on the host
+    assert lib.psig_attn_forward(d, *[None] * 8, 0, None) == -1
+    assert lib.psig_attn_step(d, *[None] * 7) == -1
+    assert lib.psig_attn_backward(d, *[None] * 13, 0, None) == -1
+    need = lib.psig_attn_backward_workspace(d)
+    assert need > 0
+    assert lib.psig_attn_backward(d, *[one] * 12, None, need, None) == -6
+    assert lib.psig_attn_backward(d, *[one] * 12, one, need - 1, None) == -6
+    assert lib.psig_attn_forward(None, *[None] * 8, 0, None) == -1
+    n = _load.NormDesc()
+    n.dtype, n.rows, n.D, n.eps = 0, 3, 8, 1e-6
+    assert lib.psig_norm_forward(ctypes.byref(n), *[None] * 9) == -1
+    need = lib.psig_norm_backward_workspace(ctypes.byref(n))
+    assert need > 0
+    assert lib.psig_norm_backward(ctypes.byref(n), one, None, None, None, None, None, one, None, *[None] * 6, one, need - 1, None) == -6
+    n.activation = 2
+    assert lib.psig_norm_forward(ctypes.byref(n), *[None] * 9) == -4
+    n.activation, n.dtype = 0, 9
+    assert lib.psig_norm_backward_workspace(ctypes.byref(n)) == -2
+
+
+def test_nothing_to_do_is_no_error():
+    lib = _load.ensure_loaded()
+    d = ctypes.byref(_attn(B=0))
+    assert lib.psig_attn_forward(d, *[None] * 8, 0, None) == 0
+    assert lib.psig_attn_step(d, *[None] * 7) == 0
+    assert lib.psig_attn_backward(d, *[None] * 13, 0, None) == 0
+
+
+def test_fake_tensors_give_the_shapes():
+    with FakeTensorMode():
+        op = torch.ops.pathsig_b200
+        q, k, v = (torch.empty(2, 9, h, d, device="cuda", dtype=torch.bfloat16) for h, d in ((4, 16), (2, 16), (2, 24)))
+        decay = torch.empty(2, 9, 4, device="cuda")
+        out, state = ps.linear_attention(q, k, v, decay, return_state=True)
+        assert out.shape == (2, 9, 4, 24) and out.dtype == torch.bfloat16
+        assert state.shape == (2, 4, 16, 24) and state.dtype == torch.float32
+        grads = op.linear_attention_backward(q, k, v, decay, state, None, out, None, 1.0, True)
+        assert [g.shape for g in grads] == [t.shape for t in (q, k, v, decay, state)]
+        assert ps.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], decay[:, 0], state).shape == (2, 4, 24)
+        x = torch.empty(3, 5, 32, device="cuda")
+        w = torch.empty(32, device="cuda")
+        h, n = ps.gated_residual_norm(x, w, gate=x, next_weight=w)
+        assert h.shape == n.shape == x.shape
+        assert ps.gated_residual_norm(x).shape == x.shape
+        grads = op.gated_residual_norm_backward(x, w, None, x, None, w, h, n, 0, 1e-6)
+        assert [g.shape for g in grads] == [x.shape, w.shape, (0,), x.shape, (0,), w.shape]
+
+
+def test_refusals_without_a_gpu():
+    z = torch.zeros
+    with pytest.raises(NotImplementedError):
+        ps.linear_attention(z(1, 2, 1, 4), z(1, 2, 1, 4), z(1, 2, 1, 4), z(1))
+    with pytest.raises(NotImplementedError):
+        ps.gated_residual_norm(z(2, 4))
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        ps.linear_attention_step(z(1, 1, 4, requires_grad=True), z(1, 1, 4), z(1, 1, 4), z(1), z(1, 1, 4, 4))
+    with pytest.raises(ValueError, match="activation"):
+        ps.gated_residual_norm(z(2, 4), activation="relu")
+    for eps in (-1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="eps"):
+            ps.gated_residual_norm(z(2, 4), eps=eps)
+    for scale in (float("inf"), float("nan"), z(1)):
+        with pytest.raises(ValueError, match="scale"):
+            ps.linear_attention(z(1, 2, 1, 4), z(1, 2, 1, 4), z(1, 2, 1, 4), z(1), scale=scale)
+
+
+@pytest.mark.parametrize("decay", ["step", "head"])
+def test_oracle_gradients_against_automatic_differentiation(decay):
+    c = so.make(3, 2, 12, 4, 2, 3, 5, torch.float64, decay=decay, state=True, lengths=torch.tensor([12, 7]))
+    names = ("q", "k", "v", "log_decay", "initial_state")
+    leaves = {n: c[n].clone().requires_grad_(True) for n in names}
+    got = so.attention({**c, **leaves})
+    want = torch.autograd.grad((got["out"] * c["grad_out"]).sum() + (got["state"] * c["grad_state"]).sum(), list(leaves.values()))
+    plain = so.attention(c)
+    for n, w in zip(names, want):
+        assert torch.allclose(plain["grad_" + n], w, rtol=1e-11, atol=1e-12), n
