@@ -226,8 +226,13 @@ __global__ void attn_pair_difference(const SweepOperand q, const SweepOperand k,
 
 // grad_g over one segment per block: B_e plus the sums of x - y from the segment's end, in 64 bits.  Writes
 // (B, L, H), or the segment's total for a decay per head.  A step whose decay underflows to 0 has gradient 0.
-template <typename A>
-__global__ void attn_decay_grad(const double *__restrict__ pairs, const A *__restrict__ dots, int tiles,
+struct PairSums {      // x - y of a step: the sum over `plus` arrays minus the sum over `minus` arrays, `step` apart
+    const void *plus, *minus;
+    int n_plus, n_minus;
+    long long step;
+};
+template <typename A, typename P>
+__global__ void attn_decay_grad(const PairSums pairs, const A *__restrict__ dots, int tiles,
                                 const A *__restrict__ decay, long long s0, long long s1, long long s2,
                                 const int *__restrict__ lengths, long long L, int H, A *__restrict__ out,
                                 double *__restrict__ totals)
@@ -243,7 +248,13 @@ __global__ void attn_decay_grad(const double *__restrict__ pairs, const A *__res
     // thread i takes step end - 1 - i, so that sums from the end are running sums over the threads
     const long long t = end - 1 - threadIdx.x;
     const bool live = t >= segment * kSegment && end > segment * kSegment;
-    double sum = live ? pairs[(b * L + t) * H + h] : 0.0;
+    double sum = 0.0;
+    if (live) {
+        const P *x = static_cast<const P *>(pairs.plus) + (b * L + t) * H + h;
+        const P *y = static_cast<const P *>(pairs.minus) + (b * L + t) * H + h;
+        for (int i = 0; i < pairs.n_plus; ++i) sum += (double)x[i * pairs.step];
+        for (int i = 0; i < pairs.n_minus; ++i) sum -= (double)y[i * pairs.step];
+    }
     for (int s = 1; s < 32; s <<= 1) {
         const double up = __shfl_up_sync(0xffffffffu, sum, s);
         if (lane >= s) sum += up;
@@ -362,10 +373,75 @@ Sweep sweep_of(const PsigAttnDesc &d, const void *decay)
 
 bool per_head(const PsigAttnDesc &d) { return d.decay_strides[0] == 0 && d.decay_strides[1] == 0; }
 
-// Scratch of the backward pass, in the order it is laid out (256-byte aligned pieces).
+// The operands of the sweeps of a call, and whether the tensor-core form serves them.
+struct Call {
+    const PsigAttnDesc &d;
+    const void *decay;
+    SweepOperand q, k, v, go;
+    int share;
+
+    Call(const PsigAttnDesc &desc, const void *q_, const void *k_, const void *v_, const void *decay_, const void *go_)
+        : d(desc), decay(decay_), share(desc.H / desc.Hkv)
+    {
+        const int64_t go_strides[3] = {d.L * d.H * d.dv, (int64_t)d.H * d.dv, d.dv};
+        q = operand(q_, d.q_strides, 1);
+        k = operand(k_, d.k_strides, share);
+        v = operand(v_, d.v_strides, share);
+        go = operand(go_, go_strides, 1);
+    }
+    Sweep forward() const
+    {
+        Sweep s = sweep_of(d, decay);
+        s.r = q, s.k = k, s.v = v;
+        s.d1 = d.dk, s.d2 = d.dv;
+        s.out_scale = d.scale;
+        return s;
+    }
+    Sweep grad_q() const
+    {
+        Sweep s = sweep_of(d, decay);
+        s.r = go, s.k = v, s.v = k;
+        s.d1 = d.dv, s.d2 = d.dk;
+        s.out_scale = d.scale;
+        s.init_transposed = true;
+        return s;
+    }
+    Sweep grad_k() const
+    {
+        Sweep s = sweep_of(d, decay);
+        s.r = v, s.k = go, s.v = q;
+        s.d1 = d.dv, s.d2 = d.dk;
+        s.reverse = true;
+        s.kv_scale = d.scale;
+        s.init_transposed = true;
+        return s;
+    }
+    Sweep grad_v() const
+    {
+        Sweep s = sweep_of(d, decay);
+        s.r = k, s.k = q, s.v = go;
+        s.d1 = d.dk, s.d2 = d.dv;
+        s.reverse = true;
+        s.kv_scale = d.scale;
+        return s;
+    }
+    bool tiles() const
+    {
+        return d.algo != PSIG_ALGO_GENERIC && attn_tiles_supported(forward(), d.dtype);
+    }
+};
+
+// Scratch of the backward pass, in the order it is laid out (256-byte aligned pieces).  It does not depend on which
+// form of the sweeps serves the call, which the operands' addresses decide too.
 struct BackwardScratch {
     long long gq, gk, gv, pairs, anchors, dots, totals, bytes;
 };
+
+int anchor_parts(const PsigAttnDesc &d)
+{
+    const int rows = column_tiles(d.dk), tiles = kTileDots * tile_columns(d.dk);
+    return rows > tiles ? rows : tiles;
+}
 
 BackwardScratch backward_scratch(const PsigAttnDesc &d)
 {
@@ -380,29 +456,23 @@ BackwardScratch backward_scratch(const PsigAttnDesc &d)
     s.gq = take(acc * rows * d.dk);
     s.gk = take(acc * rows * d.dk);
     s.gv = take(acc * rows * d.dv);
-    s.pairs = take(8 * rows);
+    const long long pair_bytes = 4 * 4 * tile_columns(d.dk);   // the tiles' two sets of two float arrays per column tile
+    s.pairs = take((pair_bytes > 8 ? pair_bytes : 8) * rows);
     s.anchors = take(acc * bh * seg * d.dk * d.dv);
-    s.dots = take(acc * bh * seg * column_tiles(d.dk));
+    s.dots = take(acc * bh * seg * anchor_parts(d));
     s.totals = take(8 * bh * seg);
     s.bytes = at;
     return s;
 }
 
 template <typename T>
-int run_forward(const PsigAttnDesc &d, const void *q, const void *k, const void *v, const void *decay, const void *init,
-                void *out, void *final, cudaStream_t stream)
+int run_forward(const Call &c, const void *init, void *out, void *final, cudaStream_t stream)
 {
-    Sweep s = sweep_of(d, decay);
-    s.r = operand(q, d.q_strides, 1);
-    s.k = operand(k, d.k_strides, d.H / d.Hkv);
-    s.v = operand(v, d.v_strides, d.H / d.Hkv);
-    s.d1 = d.dk;
-    s.d2 = d.dv;
-    s.out_scale = d.scale;
+    Sweep s = c.forward();
     s.init = init;
     s.final = final;
     s.out = out;
-    return sweep_rows<T>(s, stream);
+    return c.tiles() ? attn_sweep_on_tiles(s, false, c.d.dtype, stream) : sweep_rows<T>(s, stream);
 }
 
 unsigned blocks_for(long long items, int per_block)
@@ -411,66 +481,25 @@ unsigned blocks_for(long long items, int per_block)
     return (unsigned)(n < 1 ? 1 : n > 148 * 32 ? 148 * 32 : n);
 }
 
-template <typename T>
-int run_backward(const PsigAttnDesc &d, const void *q, const void *k, const void *v, const void *decay, const void *init,
-                 const void *go, const void *gs, void *grad_q, void *grad_k, void *grad_v, void *grad_decay,
-                 void *grad_init, char *ws, cudaStream_t stream)
+template <typename T, typename P>
+int decay_gradient(const Call &c, PairSums pairs, const typename Acc<T>::type *dots, int parts, void *grad_decay,
+                   double *totals, cudaStream_t stream)
 {
     using A = typename Acc<T>::type;
-    const BackwardScratch at = backward_scratch(d);
-    const int share = d.H / d.Hkv;
-    const long long rows = d.B * d.L * d.H, kv_rows = d.B * d.L * d.Hkv, segments = segments_of(d.L);
-    A *gq = reinterpret_cast<A *>(ws + at.gq), *gk = reinterpret_cast<A *>(ws + at.gk);
-    A *gv = reinterpret_cast<A *>(ws + at.gv), *dots = reinterpret_cast<A *>(ws + at.dots);
-    double *pairs = reinterpret_cast<double *>(ws + at.pairs), *totals = reinterpret_cast<double *>(ws + at.totals);
-    const int64_t go_strides[3] = {d.L * d.H * d.dv, (int64_t)d.H * d.dv, d.dv};
-    const SweepOperand Q = operand(q, d.q_strides, 1), K = operand(k, d.k_strides, share),
-                       V = operand(v, d.v_strides, share), G = operand(go, go_strides, 1);
-    int rc;
-    Sweep s = sweep_of(d, decay);   // grad_q
-    s.r = G, s.k = V, s.v = K;
-    s.d1 = d.dv, s.d2 = d.dk;
-    s.out_scale = d.scale;
-    s.init = init, s.init_transposed = true;
-    s.out = gq, s.out_acc = true;
-    s.anchors = ws + at.anchors;
-    if ((rc = sweep_rows<T>(s, stream)) != PSIG_OK) return rc;
-    s = sweep_of(d, decay);         // grad_k
-    s.r = V, s.k = G, s.v = Q;
-    s.d1 = d.dv, s.d2 = d.dk;
-    s.reverse = true;
-    s.kv_scale = d.scale;
-    s.init = gs, s.init_transposed = true;
-    s.out = gk, s.out_acc = true;
-    s.anchors = ws + at.anchors, s.anchor_dots = dots;
-    if ((rc = sweep_rows<T>(s, stream)) != PSIG_OK) return rc;
-    s = sweep_of(d, decay);         // grad_v, and the gradient of the initial state
-    s.r = K, s.k = Q, s.v = G;
-    s.d1 = d.dk, s.d2 = d.dv;
-    s.reverse = true;
-    s.kv_scale = d.scale;
-    s.init = gs;
-    s.final = grad_init;
-    s.out = gv, s.out_acc = true;
-    if ((rc = sweep_rows<T>(s, stream)) != PSIG_OK) return rc;
-
-    attn_sum_heads<T><<<blocks_for(rows * d.dk, 256), 256, 0, stream>>>(gq, static_cast<T *>(grad_q), rows * d.dk, 1, d.dk);
-    if ((rc = check_launch()) != PSIG_OK) return rc;
-    attn_sum_heads<T><<<blocks_for(kv_rows * d.dk, 256), 256, 0, stream>>>(gk, static_cast<T *>(grad_k), kv_rows * d.dk, share, d.dk);
-    if ((rc = check_launch()) != PSIG_OK) return rc;
-    attn_sum_heads<T><<<blocks_for(kv_rows * d.dv, 256), 256, 0, stream>>>(gv, static_cast<T *>(grad_v), kv_rows * d.dv, share, d.dv);
-    if ((rc = check_launch()) != PSIG_OK) return rc;
-    if (grad_decay == nullptr) return PSIG_OK;
-    attn_pair_difference<T><<<blocks_for(rows, 8), 256, 0, stream>>>(Q, K, gq, gk, pairs, rows, d.L, d.H, d.dk);
-    if ((rc = check_launch()) != PSIG_OK) return rc;
+    const PsigAttnDesc &d = c.d;
+    const long long segments = segments_of(d.L);
     const bool total = per_head(d);
+    int rc;
     // the grid's second dimension is limited to 65535
-    const long long per_launch = 65535 / d.H;
+    const long long per_launch = 65535 / d.H > 0 ? 65535 / d.H : 1;
     for (long long b0 = 0; b0 < d.B; b0 += per_launch) {
         const long long nb = d.B - b0 < per_launch ? d.B - b0 : per_launch;
-        attn_decay_grad<A><<<dim3((unsigned)segments, (unsigned)(nb * d.H)), kSegment, 0, stream>>>(
-            pairs + b0 * d.L * d.H, dots + b0 * d.H * segments * column_tiles(d.dk), column_tiles(d.dk),
-            static_cast<const A *>(decay) + b0 * d.decay_strides[0], d.decay_strides[0], d.decay_strides[1],
+        PairSums p = pairs;
+        p.plus = static_cast<const P *>(pairs.plus) + b0 * d.L * d.H;
+        p.minus = static_cast<const P *>(pairs.minus) + b0 * d.L * d.H;
+        attn_decay_grad<A, P><<<dim3((unsigned)segments, (unsigned)(nb * d.H)), kSegment, 0, stream>>>(
+            p, dots + b0 * d.H * segments * parts, parts,
+            static_cast<const A *>(c.decay) + b0 * d.decay_strides[0], d.decay_strides[0], d.decay_strides[1],
             d.decay_strides[2], d.lengths == nullptr ? nullptr : d.lengths + b0, d.L, d.H,
             total ? nullptr : static_cast<A *>(grad_decay) + b0 * d.L * d.H, total ? totals + b0 * d.H * segments : nullptr);
         if ((rc = check_launch()) != PSIG_OK) return rc;
@@ -480,6 +509,91 @@ int run_backward(const PsigAttnDesc &d, const void *q, const void *k, const void
         if ((rc = check_launch()) != PSIG_OK) return rc;
     }
     return PSIG_OK;
+}
+
+template <typename T>
+int sum_heads(const void *acc, void *out, long long rows, int share, int d, cudaStream_t stream)
+{
+    using A = typename Acc<T>::type;
+    attn_sum_heads<T><<<blocks_for(rows * d, 256), 256, 0, stream>>>(static_cast<const A *>(acc), static_cast<T *>(out),
+                                                                     rows * d, share, d);
+    return check_launch();
+}
+
+// Three sweeps on the tensor cores.  Gradients go straight to their place, in 32 bits to scratch where heads share
+// a key/value head.  With a decay gradient the sweeps of grad_q and grad_k are the exact ones.
+template <typename T>
+int run_backward_tiles(const Call &c, const void *init, const void *gs, void *grad_q, void *grad_k, void *grad_v,
+                       void *grad_decay, void *grad_init, char *ws, cudaStream_t stream)
+{
+    const PsigAttnDesc &d = c.d;
+    const BackwardScratch at = backward_scratch(d);
+    const long long rows = d.B * d.L * d.H, kv_rows = d.B * d.L * d.Hkv;
+    const int tiles = tile_columns(d.dk);
+    const bool shared = c.share > 1;
+    float *x = reinterpret_cast<float *>(ws + at.pairs), *y = x + 2 * tiles * rows;
+    int rc;
+    Sweep s = c.grad_q();
+    s.init = init;
+    s.out = grad_q;
+    if (grad_decay != nullptr) s.anchors = ws + at.anchors, s.dot = c.q, s.dots = x;
+    if ((rc = attn_sweep_on_tiles(s, grad_decay != nullptr, d.dtype, stream)) != PSIG_OK) return rc;
+    s = c.grad_k();
+    s.init = gs;
+    s.out = shared ? ws + at.gk : grad_k, s.out_acc = shared;
+    if (grad_decay != nullptr) s.anchors = ws + at.anchors, s.anchor_dots = ws + at.dots, s.dot = c.k, s.dots = y;
+    if ((rc = attn_sweep_on_tiles(s, grad_decay != nullptr, d.dtype, stream)) != PSIG_OK) return rc;
+    s = c.grad_v();
+    s.init = gs;
+    s.final = grad_init;
+    s.out = shared ? ws + at.gv : grad_v, s.out_acc = shared;
+    if ((rc = attn_sweep_on_tiles(s, false, d.dtype, stream)) != PSIG_OK) return rc;
+    if (shared) {
+        if ((rc = sum_heads<T>(ws + at.gk, grad_k, kv_rows, c.share, d.dk, stream)) != PSIG_OK) return rc;
+        if ((rc = sum_heads<T>(ws + at.gv, grad_v, kv_rows, c.share, d.dv, stream)) != PSIG_OK) return rc;
+    }
+    if (grad_decay == nullptr) return PSIG_OK;
+    const PairSums pairs{x, y, 2 * tiles, 2 * tiles, rows};
+    return decay_gradient<T, float>(c, pairs, reinterpret_cast<const typename Acc<T>::type *>(ws + at.dots), kTileDots * tiles,
+                                    grad_decay, reinterpret_cast<double *>(ws + at.totals), stream);
+}
+
+template <typename T>
+int run_backward(const Call &c, const void *init, const void *gs, void *grad_q, void *grad_k, void *grad_v,
+                 void *grad_decay, void *grad_init, char *ws, cudaStream_t stream)
+{
+    using A = typename Acc<T>::type;
+    if (c.tiles() && attn_tiles_supported(c.grad_q(), c.d.dtype))
+        return run_backward_tiles<T>(c, init, gs, grad_q, grad_k, grad_v, grad_decay, grad_init, ws, stream);
+    const PsigAttnDesc &d = c.d;
+    const BackwardScratch at = backward_scratch(d);
+    const long long rows = d.B * d.L * d.H, kv_rows = d.B * d.L * d.Hkv;
+    A *gq = reinterpret_cast<A *>(ws + at.gq), *gk = reinterpret_cast<A *>(ws + at.gk);
+    double *pairs = reinterpret_cast<double *>(ws + at.pairs);
+    int rc;
+    Sweep s = c.grad_q();
+    s.init = init;
+    s.out = gq, s.out_acc = true;
+    s.anchors = ws + at.anchors;
+    if ((rc = sweep_rows<T>(s, stream)) != PSIG_OK) return rc;
+    s = c.grad_k();
+    s.init = gs;
+    s.out = gk, s.out_acc = true;
+    s.anchors = ws + at.anchors, s.anchor_dots = ws + at.dots;
+    if ((rc = sweep_rows<T>(s, stream)) != PSIG_OK) return rc;
+    s = c.grad_v();
+    s.init = gs;
+    s.final = grad_init;
+    s.out = ws + at.gv, s.out_acc = true;
+    if ((rc = sweep_rows<T>(s, stream)) != PSIG_OK) return rc;
+    if ((rc = sum_heads<T>(gq, grad_q, rows, 1, d.dk, stream)) != PSIG_OK) return rc;
+    if ((rc = sum_heads<T>(gk, grad_k, kv_rows, c.share, d.dk, stream)) != PSIG_OK) return rc;
+    if ((rc = sum_heads<T>(ws + at.gv, grad_v, kv_rows, c.share, d.dv, stream)) != PSIG_OK) return rc;
+    if (grad_decay == nullptr) return PSIG_OK;
+    attn_pair_difference<T><<<blocks_for(rows, 8), 256, 0, stream>>>(c.q, c.k, gq, gk, pairs, rows, d.L, d.H, d.dk);
+    if ((rc = check_launch()) != PSIG_OK) return rc;
+    return decay_gradient<T, double>(c, PairSums{pairs, pairs, 1, 0, 0}, reinterpret_cast<const A *>(ws + at.dots),
+                                     column_tiles(d.dk), grad_decay, reinterpret_cast<double *>(ws + at.totals), stream);
 }
 
 }  // namespace
@@ -506,7 +620,7 @@ extern "C" int psig_attn_forward(const PsigAttnDesc *desc, const void *q, const 
     if (desc->L > 0 && (!q || !k || !v || !log_decay || !out)) return PSIG_ERR_NULL;
     if (desc->L == 0 && final_state == nullptr) return PSIG_OK;
     return with_dtype(desc->dtype, [&](auto t) {
-        return run_forward<decltype(t)>(*desc, q, k, v, log_decay, initial_state, out, final_state,
+        return run_forward<decltype(t)>(Call(*desc, q, k, v, log_decay, nullptr), initial_state, out, final_state,
                                         static_cast<cudaStream_t>(stream));
     });
 }
@@ -524,11 +638,13 @@ extern "C" int psig_attn_backward(const PsigAttnDesc *desc, const void *q, const
     const int64_t need = backward_scratch(*desc).bytes;
     if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return PSIG_ERR_WORKSPACE;
     return with_dtype(desc->dtype, [&](auto t) {
-        return run_backward<decltype(t)>(*desc, q, k, v, log_decay, initial_state, grad_out, grad_state, grad_q, grad_k,
+        return run_backward<decltype(t)>(Call(*desc, q, k, v, log_decay, grad_out), initial_state, grad_state, grad_q, grad_k,
                                          grad_v, grad_log_decay, grad_initial_state, static_cast<char *>(workspace),
                                          static_cast<cudaStream_t>(stream));
     });
 }
+
+extern "C" int64_t psig_attn_wait_timeouts(void) { return attn_tile_timeouts(); }
 
 extern "C" int psig_attn_step(const PsigAttnDesc *desc, const void *q, const void *k, const void *v,
                               const void *log_decay, void *state, void *out, void *stream)

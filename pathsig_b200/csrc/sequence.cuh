@@ -73,9 +73,21 @@ struct Sweep {
     // Decay gradient (see attn_decay_grad): the grad_q sweep stores the state at the end of every kSegment steps,
     // the grad_k sweep multiplies its own state into it and leaves one number per segment and column tile.
     void *anchors;        // (B, H, segments, d1, d2)
-    void *anchor_dots;    // (B, H, segments, column tiles)
+    void *anchor_dots;    // (B, H, segments, parts of the sum)
+    // Tensor-core sweeps only: the unrounded output row times the row of a third operand, summed over each block's and
+    // each warp's columns: (2 * column tiles of 64, B, L, H).
+    SweepOperand dot;
+    float *dots;
 };
 
 inline long long segments_of(long long L) { return (L + kSegment - 1) / kSegment; }
+
+// Tensor-core form of the sweep (linear_attention_tiles.cu).  `exact`: results are good to 32 bits, not only to the
+// storage type.
+bool attn_tiles_supported(const Sweep &a, int dtype);
+int attn_sweep_on_tiles(const Sweep &a, bool exact, int dtype, cudaStream_t stream);
+long long attn_tile_timeouts();
+constexpr int kTileDots = 8;   // parts of an anchor's sum per column tile of 64
+inline int tile_columns(int d2) { return (d2 + 63) / 64; }
 
 }  // namespace psig
