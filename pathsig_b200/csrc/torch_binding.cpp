@@ -10,12 +10,13 @@
 // src/pathsig/backward/sig_backward_launch.cu:94-155), allocates its outputs with the caching allocator
 // and hands raw pointers plus the current stream to the C ABI of include/pathsig_b200.h.  torch is used
 // for memory, streams and dispatch only; fake (meta) implementations and autograd formulas are registered
-// from Python (pathsig_b200/ops.py).
+// from Python (pathsig_b200/ops.py), but for the autograd formulas of the sequence operators, which are below.
 #include <ATen/ATen.h>
 #include <ATen/Context.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 #include <nvtx3/nvToolsExt.h>
 
@@ -704,6 +705,126 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
     return std::make_tuple(gx, gw, gg, gr, gs, gn);
 }
 
+// ---- autograd of the sequence operators ----
+//
+// In C++ because their small calls (one row, one window) are bound by the host: the formulas registered from Python
+// cost 150-250 us for a forward and backward pass (8 us here is a whole step of a kept state).
+
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+using OptionalTensor = std::optional<at::Tensor>;
+
+OptionalTensor given(const Variable &t) { return t.defined() ? OptionalTensor(t) : std::nullopt; }
+Variable plain(const OptionalTensor &t) { return t.has_value() ? *t : Variable(); }
+bool tracked(const OptionalTensor &t) { return t.has_value() && t->defined() && t->requires_grad(); }
+
+template <typename Fn>
+c10::TypedOperatorHandle<Fn> handle(const char *name)
+{
+    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Fn>();
+}
+
+std::tuple<at::Tensor, at::Tensor> attention_below(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
+                                                   const at::Tensor &decay, const OptionalTensor &init,
+                                                   const OptionalTensor &lengths, double scale, bool return_state)
+{
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = handle<decltype(linear_attention)>("pathsig_b200::linear_attention");
+    return op.call(q, k, v, decay, init, lengths, scale, return_state);
+}
+
+struct AttentionFunction : torch::autograd::Function<AttentionFunction> {
+    static variable_list forward(AutogradContext *ctx, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
+                                 const at::Tensor &decay, const OptionalTensor &init, const OptionalTensor &lengths, double scale,
+                                 bool return_state)
+    {
+        auto [out, state] = attention_below(q, k, v, decay, init, lengths, scale, return_state);
+        ctx->save_for_backward({q, k, v, decay, plain(init), plain(lengths)});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["state"] = return_state;
+        ctx->saved_data["decay"] = decay.requires_grad();
+        ctx->set_materialize_grads(false);
+        return {out, state};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        variable_list none(8);
+        if (!ctx->saved_data["state"].toBool()) grads[1] = Variable();
+        if (!grads[0].defined() && !grads[1].defined()) return none;
+        const variable_list s = ctx->get_saved_variables();
+        static const auto op = handle<decltype(linear_attention_backward)>("pathsig_b200::linear_attention_backward");
+        const bool decay_grad = ctx->saved_data["decay"].toBool();
+        auto [gq, gk, gv, gd, gi] = op.call(s[0], s[1], s[2], s[3], given(s[4]), given(s[5]), given(grads[0]), given(grads[1]),
+                                            ctx->saved_data["scale"].toDouble(), decay_grad);
+        none[0] = gq, none[1] = gk, none[2] = gv;
+        if (decay_grad) none[3] = gd;
+        if (s[4].defined()) none[4] = gi;
+        return none;
+    }
+};
+
+std::tuple<at::Tensor, at::Tensor> linear_attention_autograd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
+                                                             const at::Tensor &decay, const OptionalTensor &init,
+                                                             const OptionalTensor &lengths, double scale, bool return_state)
+{
+    if (!at::GradMode::is_enabled() ||
+        !(q.requires_grad() || k.requires_grad() || v.requires_grad() || decay.requires_grad() || tracked(init)))
+        return attention_below(q, k, v, decay, init, lengths, scale, return_state);
+    variable_list got = AttentionFunction::apply(q, k, v, decay, init, lengths, scale, return_state);
+    return std::make_tuple(got[0], got[1]);
+}
+
+std::tuple<at::Tensor, at::Tensor> norm_below(const at::Tensor &x, const OptionalTensor &weight, const OptionalTensor &gate,
+                                              const OptionalTensor &residual, const OptionalTensor &residual_scale,
+                                              const OptionalTensor &next_weight, int64_t activation, double eps)
+{
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = handle<decltype(gated_residual_norm)>("pathsig_b200::gated_residual_norm");
+    return op.call(x, weight, gate, residual, residual_scale, next_weight, activation, eps);
+}
+
+struct NormFunction : torch::autograd::Function<NormFunction> {
+    static variable_list forward(AutogradContext *ctx, const at::Tensor &x, const OptionalTensor &weight, const OptionalTensor &gate,
+                                 const OptionalTensor &residual, const OptionalTensor &residual_scale,
+                                 const OptionalTensor &next_weight, int64_t activation, double eps)
+    {
+        auto [h, n] = norm_below(x, weight, gate, residual, residual_scale, next_weight, activation, eps);
+        ctx->save_for_backward({x, plain(weight), plain(gate), plain(residual), plain(residual_scale), plain(next_weight)});
+        ctx->saved_data["activation"] = activation;
+        ctx->saved_data["eps"] = eps;
+        ctx->set_materialize_grads(false);
+        return {h, n};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        variable_list none(8);
+        const variable_list s = ctx->get_saved_variables();
+        if (!s[5].defined()) grads[1] = Variable();
+        if (!grads[0].defined() && !grads[1].defined()) return none;
+        static const auto op = handle<decltype(gated_residual_norm_backward)>("pathsig_b200::gated_residual_norm_backward");
+        auto [gx, gw, gg, gr, gs, gn] =
+            op.call(s[0], given(s[1]), given(s[2]), given(s[3]), given(s[4]), given(s[5]), given(grads[0]), given(grads[1]),
+                    ctx->saved_data["activation"].toInt(), ctx->saved_data["eps"].toDouble());
+        const at::Tensor *got[6] = {&gx, &gw, &gg, &gr, &gs, &gn};
+        for (int i = 0; i < 6; ++i)
+            if (s[i].defined()) none[i] = *got[i];
+        return none;
+    }
+};
+
+std::tuple<at::Tensor, at::Tensor> gated_residual_norm_autograd(const at::Tensor &x, const OptionalTensor &weight,
+                                                                const OptionalTensor &gate, const OptionalTensor &residual,
+                                                                const OptionalTensor &residual_scale, const OptionalTensor &next_weight,
+                                                                int64_t activation, double eps)
+{
+    if (!at::GradMode::is_enabled() || !(x.requires_grad() || tracked(weight) || tracked(gate) || tracked(residual) ||
+                                         tracked(residual_scale) || tracked(next_weight)))
+        return norm_below(x, weight, gate, residual, residual_scale, next_weight, activation, eps);
+    variable_list got = NormFunction::apply(x, weight, gate, residual, residual_scale, next_weight, activation, eps);
+    return std::make_tuple(got[0], got[1]);
+}
+
 }  // namespace
 
 // Kernel family used by the signature operators (PsigAlgo); tests flip it to compare families.
@@ -755,4 +876,10 @@ TORCH_LIBRARY_IMPL(pathsig_b200, CUDA, m)
     m.impl("linear_attention_step", &linear_attention_step);
     m.impl("gated_residual_norm", &gated_residual_norm);
     m.impl("gated_residual_norm_backward", &gated_residual_norm_backward);
+}
+
+TORCH_LIBRARY_IMPL(pathsig_b200, Autograd, m)
+{
+    m.impl("linear_attention", &linear_attention_autograd);
+    m.impl("gated_residual_norm", &gated_residual_norm_autograd);
 }

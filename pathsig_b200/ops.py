@@ -464,8 +464,9 @@ def register_namespace(ns: str) -> None:
                                                                             ctx.eps)
         return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad[:6])) + (None, None)
 
-    torch.library.register_autograd(f"{ns}::linear_attention", backward_attn, setup_context=setup_attn, lib=lib)
-    torch.library.register_autograd(f"{ns}::gated_residual_norm", backward_norm, setup_context=setup_norm, lib=lib)
+    if lib is not None:   # those of this package's own namespace are part of the compiled library
+        torch.library.register_autograd(f"{ns}::linear_attention", backward_attn, setup_context=setup_attn, lib=lib)
+        torch.library.register_autograd(f"{ns}::gated_residual_norm", backward_norm, setup_context=setup_norm, lib=lib)
     torch.library.register_autograd(f"{ns}::chen_product", backward_chen, setup_context=setup_chen, lib=lib)
     torch.library.register_autograd(f"{ns}::chen_product_backward", backward_chen_bwd,
                                     setup_context=setup_chen_bwd, lib=lib)
