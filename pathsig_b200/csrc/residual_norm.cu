@@ -7,12 +7,20 @@
 //     dx = r (w dz) - x r^3 mean(w dz x)
 // h is recomputed from the operands (the residual is read where a saved h would have been), so that nothing of
 // the forward pass is kept and h is not rounded in between.  Sums are in 32 bits (64 for float64).
+//
+// What bounds it: memory, each operand once.  A row is held in registers by a team of threads (part of a warp for short rows,
+// a whole block else), 8 or 16 values to a thread, in accesses of 16 bytes where the rows allow it; sums over the row
+// are the only exchange, by shuffles and, between warps, one barrier each.  Rows too wide for that are walked in
+// pieces and read again, mostly from L2.
 #include "sequence.cuh"
 
 namespace psig {
 namespace {
 
-constexpr int kNormThreads = 256;
+constexpr int kTeamMax = 512;                  // threads of a block that holds one row
+constexpr int kNormWidest = kTeamMax * 16;     // widest row held in registers
+constexpr int kShortThreads = 256;             // block size for rows of at most one warp
+constexpr int kWideThreads = 512;              // block size for rows that are walked
 
 struct NormArgs {
     const void *x, *gate, *residual, *grad_h, *grad_n;
@@ -25,139 +33,13 @@ struct NormArgs {
     int activation;
 };
 
-template <typename A>
-__device__ __forceinline__ A block_sum(A v, A *shared)
-{
-    for (int s = 16; s >= 1; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
-    __syncthreads();
-    A sum = A(0);
-    for (int i = 0; i < kNormThreads / 32; ++i) sum += shared[i];
-    return sum;
-}
-
-// act(g) and its derivative
-template <typename A>
-__device__ __forceinline__ A gate_value(A g, int activation, A *slope)
-{
-    const A s = A(1) / (A(1) + exp_acc(-g));
-    *slope = activation == 0 ? s * (A(1) + g * (A(1) - s)) : s * (A(1) - s);
-    return activation == 0 ? g * s : s;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kNormThreads) norm_forward_rows(const NormArgs a)
-{
-    using A = typename Acc<T>::type;
-    __shared__ A shared[kNormThreads / 32];
-    const A *w = static_cast<const A *>(a.weight), *c = static_cast<const A *>(a.scale);
-    const A *w2 = static_cast<const A *>(a.next_weight);
-    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const T *x = static_cast<const T *>(a.x) + row * a.D;
-        const T *gate = a.gate ? static_cast<const T *>(a.gate) + row * a.D : nullptr;
-        const T *res = a.residual ? static_cast<const T *>(a.residual) + row * a.D : nullptr;
-        T *h = static_cast<T *>(a.h) + row * a.D;
-        A sum = A(0);
-        for (long long i = threadIdx.x; i < a.D; i += kNormThreads) { const A v = to_acc<A>(x[i]); sum += v * v; }
-        const A r = A(1) / sqrt(block_sum(sum, shared) / A(a.D) + A(a.eps));
-        auto value = [&](long long i) {
-            A v = to_acc<A>(x[i]) * r, slope;
-            if (w) v *= w[i];
-            if (gate) v *= gate_value(to_acc<A>(gate[i]), a.activation, &slope);
-            if (c) v *= c[i];
-            return res ? to_acc<A>(res[i]) + v : v;
-        };
-        sum = A(0);
-        for (long long i = threadIdx.x; i < a.D; i += kNormThreads) {
-            const A v = value(i);
-            sum += v * v;
-            h[i] = from_acc<T>(v);
-        }
-        if (w2 == nullptr) continue;
-        const A r2 = A(1) / sqrt(block_sum(sum, shared) / A(a.D) + A(a.eps));
-        for (long long i = threadIdx.x; i < a.D; i += kNormThreads)
-            static_cast<T *>(a.n)[row * a.D + i] = from_acc<T>(value(i) * r2 * w2[i]);
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kNormThreads) norm_backward_rows(const NormArgs a)
-{
-    using A = typename Acc<T>::type;
-    __shared__ A shared[kNormThreads / 32];
-    const A *w = static_cast<const A *>(a.weight), *c = static_cast<const A *>(a.scale);
-    const A *w2 = static_cast<const A *>(a.next_weight);
-    A *part = static_cast<A *>(a.partial) + (long long)blockIdx.x * 3 * a.D;
-    for (long long i = threadIdx.x; i < 3 * a.D; i += kNormThreads) part[i] = A(0);
-    __syncthreads();
-    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const T *x = static_cast<const T *>(a.x) + row * a.D;
-        const T *gate = a.gate ? static_cast<const T *>(a.gate) + row * a.D : nullptr;
-        const T *res = a.residual ? static_cast<const T *>(a.residual) + row * a.D : nullptr;
-        const T *gh = a.grad_h ? static_cast<const T *>(a.grad_h) + row * a.D : nullptr;
-        const T *gn = w2 ? static_cast<const T *>(a.grad_n) + row * a.D : nullptr;
-        A sum = A(0);
-        for (long long i = threadIdx.x; i < a.D; i += kNormThreads) { const A v = to_acc<A>(x[i]); sum += v * v; }
-        const A r = A(1) / sqrt(block_sum(sum, shared) / A(a.D) + A(a.eps));
-        A r2 = A(0), m2 = A(0);
-        auto value = [&](long long i) {
-            A v = to_acc<A>(x[i]) * r, slope;
-            if (w) v *= w[i];
-            if (gate) v *= gate_value(to_acc<A>(gate[i]), a.activation, &slope);
-            if (c) v *= c[i];
-            return res ? to_acc<A>(res[i]) + v : v;
-        };
-        if (w2) {
-            A hh = A(0), nh = A(0);
-            for (long long i = threadIdx.x; i < a.D; i += kNormThreads) {
-                const A v = value(i);
-                hh += v * v;
-                nh += w2[i] * to_acc<A>(gn[i]) * v;
-            }
-            r2 = A(1) / sqrt(block_sum(hh, shared) / A(a.D) + A(a.eps));
-            m2 = block_sum(nh, shared) / A(a.D) * r2 * r2 * r2;
-        }
-        auto total = [&](long long i) {   // gradient of h
-            A v = gh ? to_acc<A>(gh[i]) : A(0);
-            if (w2) v += w2[i] * to_acc<A>(gn[i]) * r2 - value(i) * m2;
-            return v;
-        };
-        sum = A(0);
-        for (long long i = threadIdx.x; i < a.D; i += kNormThreads) {
-            const A dh = total(i), xv = to_acc<A>(x[i]), ci = c ? c[i] : A(1), wi = w ? w[i] : A(1);
-            A slope = A(0), act = A(1);
-            if (gate) act = gate_value(to_acc<A>(gate[i]), a.activation, &slope);
-            const A z = xv * r * wi, dz = dh * ci * act;
-            if (w2) part[2 * a.D + i] += to_acc<A>(gn[i]) * value(i) * r2;
-            part[a.D + i] += dh * z * act;
-            part[i] += dz * xv * r;
-            if (a.grad_residual) static_cast<T *>(a.grad_residual)[row * a.D + i] = from_acc<T>(dh);
-            if (a.grad_gate) static_cast<T *>(a.grad_gate)[row * a.D + i] = from_acc<T>(dh * ci * z * slope);
-            sum += wi * dz * xv;
-        }
-        const A m = block_sum(sum, shared) / A(a.D) * r * r * r;
-        if (a.grad_x)
-            for (long long i = threadIdx.x; i < a.D; i += kNormThreads) {
-                const A dh = total(i), ci = c ? c[i] : A(1), wi = w ? w[i] : A(1);
-                A slope, act = A(1);
-                if (gate) act = gate_value(to_acc<A>(gate[i]), a.activation, &slope);
-                static_cast<T *>(a.grad_x)[row * a.D + i] = from_acc<T>(r * wi * dh * ci * act - to_acc<A>(x[i]) * m);
-            }
-    }
-}
-
-// ---- rows held in registers (up to kNormWidest features) ----
-//
-// A team of 2^k threads takes a row, E values to an access and NV accesses to a thread, so that every operand is read
-// once and the sums over a row are the only exchange: shuffles inside a warp, one barrier for teams of several warps.
-
 template <int BYTES> struct Raw;
 template <> struct Raw<16> { using type = uint4; };
 template <> struct Raw<8> { using type = uint2; };
 template <> struct Raw<4> { using type = uint32_t; };
 template <> struct Raw<2> { using type = uint16_t; };
 
+// E neighbouring values as one access.
 template <typename T, int E>
 struct Pack {
     using raw = typename Raw<(int)sizeof(T) * E>::type;
@@ -170,7 +52,44 @@ struct Pack {
     __device__ __forceinline__ void store(void *p, long long at) const { *reinterpret_cast<raw *>(static_cast<T *>(p) + at) = bits; }
 };
 
-// E values of a parameter vector (type of sums); 1 where there is none.
+// The E values of an access in the type of sums, and back (16-bit types two at a time).
+template <typename T, int E>
+__device__ __forceinline__ void widen(const Pack<T, E> &p, typename Acc<T>::type (&x)[E])
+{
+    if constexpr (std::is_same<T, __nv_bfloat16>::value && E > 1) {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(&p.bits);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            x[e] = __uint_as_float(w[e / 2] << 16);
+            x[e + 1] = __uint_as_float(w[e / 2] & 0xFFFF0000u);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = to_acc<typename Acc<T>::type>(p.v[e]);
+    }
+}
+template <typename T, int E>
+__device__ __forceinline__ void narrow(const typename Acc<T>::type (&x)[E], Pack<T, E> &p)
+{
+    if constexpr (sizeof(T) == 2 && E > 1) {
+        uint32_t *w = reinterpret_cast<uint32_t *>(&p.bits);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                const __nv_bfloat162 two = __floats2bfloat162_rn(x[e], x[e + 1]);
+                w[e / 2] = *reinterpret_cast<const uint32_t *>(&two);
+            } else {
+                const __half2 two = __floats2half2_rn(x[e], x[e + 1]);
+                w[e / 2] = *reinterpret_cast<const uint32_t *>(&two);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) p.v[e] = from_acc<T>(x[e]);
+    }
+}
+
+// E values of a parameter vector (type of sums; 16-byte aligned where E > 1); 1 where there is none.
 template <typename A, int E>
 __device__ __forceinline__ void load_vector(const void *p, long long at, A (&v)[E])
 {
@@ -179,7 +98,7 @@ __device__ __forceinline__ void load_vector(const void *p, long long at, A (&v)[
         for (int e = 0; e < E; ++e) v[e] = A(1);
         return;
     }
-    constexpr int W = 16 / (int)sizeof(A) < E ? 16 / (int)sizeof(A) : E;   // vectors start on 16 bytes where E > 1
+    constexpr int W = 16 / (int)sizeof(A) < E ? 16 / (int)sizeof(A) : E;
 #pragma unroll
     for (int e = 0; e < E; e += W) {
         Pack<A, W> w;
@@ -189,263 +108,664 @@ __device__ __forceinline__ void load_vector(const void *p, long long at, A (&v)[
     }
 }
 
-constexpr int kTeamMax = 512;
-constexpr int kNormWidest = kTeamMax * 16;
-
-// Sums N values over the team.  `round` alternates between two sets of partial sums, so that one barrier is enough.
-template <typename A, int N>
-__device__ __forceinline__ void team_sum(A (&v)[N], int team_log2, A *shared, int round)
+// 1 / (1 + exp(-g)).  In 32 bits with the hardware's exponential and reciprocal (a few units of 2^-24 together): the
+// library's cost more instructions than all the rest of the row's arithmetic.
+__device__ __forceinline__ float sigmoid(float g)
 {
-    const int inside = team_log2 < 5 ? team_log2 : 5;
-    for (int s = 0; s < inside; ++s)
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 1 << s);
-    if (team_log2 <= 5) return;
-    A *mine = shared + (round & 1) * 2 * (kTeamMax / 32);
-    const int warp = threadIdx.x >> 5, warps = 1 << (team_log2 - 5);
-    if ((threadIdx.x & 31) == 0)
-#pragma unroll
-        for (int i = 0; i < N; ++i) mine[warp * 2 + i] = v[i];
-    __syncthreads();
-    const int first = warp & ~(warps - 1);
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = A(0);
-    for (int w = 0; w < warps; ++w)
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += mine[(first + w) * 2 + i];
+    float e, s;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+    return s;
+}
+__device__ __forceinline__ double sigmoid(double g) { return 1.0 / (1.0 + exp(-g)); }
+
+template <typename A>
+__device__ __forceinline__ A gate_value(A g, int activation)
+{
+    const A s = sigmoid(g);
+    return activation == 0 ? g * s : s;
+}
+template <typename A>
+__device__ __forceinline__ A gate_slope(A g, int activation)
+{
+    const A s = sigmoid(g);
+    return activation == 0 ? s * (A(1) + g * (A(1) - s)) : s * (A(1) - s);
 }
 
 __device__ __forceinline__ float inverse_root(float v) { return rsqrtf(v); }
 __device__ __forceinline__ double inverse_root(double v) { return rsqrt(v); }
 
-template <typename T, int E, int NV>
-__global__ void __launch_bounds__(kTeamMax) norm_forward_team(const NormArgs a, int team_log2)
+// Sums N values over the team: 2^team_log2 neighbouring lanes, or the whole block when team_log2 is 5.  Partial sums
+// of the warps go to one of two sets in turn (`round`), so that one barrier is enough.
+template <typename A, int N>
+__device__ __forceinline__ void team_sum(A (&v)[N], int team_log2, A *shared, int round)
+{
+    for (int s = 0; s < team_log2; ++s)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 1 << s);
+    if (team_log2 < 5 || blockDim.x == 32) return;
+    A *mine = shared + (round & 1) * 2 * (kTeamMax / 32);
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+        for (int i = 0; i < N; ++i) mine[(threadIdx.x >> 5) * 2 + i] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = A(0);
+    for (int w = 0; w < blockDim.x >> 5; ++w)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += mine[w * 2 + i];
+}
+
+// ---- rows held by a team ----
+//
+// RING: the rows of one block are streamed into shared memory ahead of their use (one thread, cp.async.bulk, an mbarrier
+// for each of the stages), so that the memory system is busy while a row waits at its barriers; every pass
+// reads its operands from there.  Needs rows that are whole 16-byte pieces.  Otherwise a thread loads its part of a row itself.
+
+__device__ __forceinline__ uint32_t norm_shared(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+constexpr int kNormOperands = 5;
+constexpr unsigned kNormPolls = 1u << 22;
+__device__ unsigned long long g_norm_timeouts;
+
+struct Ring {
+    int stages;
+    int row_bytes;                       // of one operand
+    int count;                           // operands per stage
+    const void *data[kNormOperands];     // in the order of their slots
+};
+
+struct RingState {
+    unsigned char *buffer;
+    uint32_t bars;
+    const Ring &ring;
+    __device__ __forceinline__ uint32_t bar(int stage) const { return bars + 8 * stage; }
+    __device__ __forceinline__ void init() const
+    {
+        for (int i = 0; i < ring.stages; ++i)
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar(i)) : "memory");
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // one thread: row `row` into stage `stage`
+    __device__ __forceinline__ void load(int stage, long long row) const
+    {
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar(stage)), "r"(ring.count * ring.row_bytes) : "memory");
+        for (int i = 0; i < ring.count; ++i)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                         ::"r"(norm_shared(buffer + (long long)(stage * ring.count + i) * ring.row_bytes)),
+                           "l"(static_cast<const unsigned char *>(ring.data[i]) + row * ring.row_bytes), "r"(ring.row_bytes), "r"(bar(stage))
+                         : "memory");
+    }
+    __device__ __forceinline__ bool wait(int stage, uint32_t parity) const
+    {
+        for (unsigned i = 0; i < kNormPolls; ++i) {
+            uint32_t ok;
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+                         : "=r"(ok) : "r"(bar(stage)), "r"(parity) : "memory");
+            if (ok) return true;
+        }
+        atomicAdd(&g_norm_timeouts, 1ull);
+        return false;
+    }
+};
+
+template <typename T, int E, int NV, bool NEXT, bool RING>
+__global__ void __launch_bounds__(kTeamMax) norm_forward_team(const NormArgs a, int team_log2, int threads, const Ring ring)
 {
     using A = typename Acc<T>::type;
     __shared__ A shared[4 * (kTeamMax / 32)];
-    const int team = threadIdx.x >> team_log2, j = threadIdx.x & ((1 << team_log2) - 1);
-    const long long row = (long long)blockIdx.x * (blockDim.x >> team_log2) + team;
-    const long long base = row * a.D;
-    Pack<T, E> x[NV], g[NV], res[NV];
-    bool live[NV];
-    int col[NV];
-    A sum[1] = {A(0)};
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        col[v] = (j + (v << team_log2)) * E;
-        live[v] = row < a.rows && col[v] < a.D;
-        if (live[v]) {
-            x[v].load(a.x, base + col[v]);
-            if (a.gate) g[v].load(a.gate, base + col[v]);
-            if (a.residual) res[v].load(a.residual, base + col[v]);
+    extern __shared__ __align__(128) unsigned char dynamic[];
+    const int teams = team_log2 < 5 ? blockDim.x >> team_log2 : 1;
+    const int team = team_log2 < 5 ? threadIdx.x >> team_log2 : 0, j = team_log2 < 5 ? threadIdx.x & (threads - 1) : threadIdx.x;
+    const A mean = A(1) / A((int)a.D), eps = (A)a.eps;
+    const long long step = (long long)gridDim.x * teams;
+    const RingState rs{dynamic + 128, norm_shared(dynamic), ring};
+    if (RING) {
+        if (threadIdx.x == 0) {
+            rs.init();
+            for (int i = 0; i < ring.stages; ++i)
+                if (blockIdx.x + i * step < a.rows) rs.load(i, blockIdx.x + i * step);
         }
+        __syncthreads();
     }
+    int round = 0, stage = 0;
+    uint32_t phase = 0;
+    for (long long first = (long long)blockIdx.x * teams; first < a.rows; first += step) {
+        const long long row = first + team, base = row * a.D;
+        const int D = row < a.rows ? (int)a.D : 0;
+        Pack<T, E> x[NV], g[NV], res[NV];
+        const unsigned char *here = rs.buffer + (long long)stage * ring.count * ring.row_bytes;
+        if (RING) rs.wait(stage, phase);
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int e = 0; e < E; ++e) { const A t = to_acc<A>(x[v].v[e]); sum[0] += t * t; }
-    team_sum(sum, team_log2, shared, 0);
-    const A r = inverse_root(sum[0] / A(a.D) + A(a.eps));
-    A h[NV * E];
-    sum[0] = A(0);
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        if (!live[v]) continue;
-        A w[E], c[E];
-        load_vector<A, E>(a.weight, col[v], w);
-        load_vector<A, E>(a.scale, col[v], c);
-        Pack<T, E> out;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            A slope, t = to_acc<A>(x[v].v[e]) * r * w[e];
-            if (a.gate) t *= gate_value(to_acc<A>(g[v].v[e]), a.activation, &slope);
-            t *= c[e];
-            if (a.residual) t += to_acc<A>(res[v].v[e]);
-            h[v * E + e] = t;
-            sum[0] += t * t;
-            out.v[e] = from_acc<T>(t);
+        for (int v = 0; v < NV; ++v) {
+            const int col = (j + v * threads) * E;
+            if (col >= D) continue;
+            if (RING) {
+                x[v].load(here, col);
+            } else {
+                x[v].load(a.x, base + col);
+                if (a.gate) g[v].load(a.gate, base + col);
+                if (a.residual) res[v].load(a.residual, base + col);
+            }
         }
-        out.store(a.h, base + col[v]);
-    }
-    if (a.next_weight == nullptr) return;
-    team_sum(sum, team_log2, shared, 1);
-    const A r2 = inverse_root(sum[0] / A(a.D) + A(a.eps));
+        A sum[1] = {A(0)};
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        if (!live[v]) continue;
-        A w[E];
-        load_vector<A, E>(a.next_weight, col[v], w);
-        Pack<T, E> out;
+        for (int v = 0; v < NV; ++v) {
+            A t[E];
+            widen(x[v], t);
 #pragma unroll
-        for (int e = 0; e < E; ++e) out.v[e] = from_acc<T>(h[v * E + e] * r2 * w[e]);
-        out.store(a.n, base + col[v]);
+            for (int e = 0; e < E; ++e) sum[0] += t[e] * t[e];
+        }
+        team_sum(sum, team_log2, shared, round++);
+        const A r = inverse_root(sum[0] * mean + eps);
+        A h[NEXT ? NV * E : 1];
+        sum[0] = A(0);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int col = (j + v * threads) * E;
+            if (col >= D) continue;
+            if (RING) {
+                if (a.gate) g[v].load(here + ring.row_bytes, col);
+                if (a.residual) res[v].load(here + (a.gate ? 2 : 1) * ring.row_bytes, col);
+            }
+            A f[E];
+            load_vector<A, E>(a.weight, col, f);
+            if (a.scale) {
+                A c[E];
+                load_vector<A, E>(a.scale, col, c);
+#pragma unroll
+                for (int e = 0; e < E; ++e) f[e] *= c[e];
+            }
+            A t[E];
+            if (a.gate) {
+                widen(g[v], t);
+#pragma unroll
+                for (int e = 0; e < E; ++e) f[e] *= sigmoid(t[e]);
+                if (a.activation == 0)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) f[e] *= t[e];
+            }
+            widen(x[v], t);
+#pragma unroll
+            for (int e = 0; e < E; ++e) f[e] *= t[e] * r;
+            if (a.residual) {
+                widen(res[v], t);
+#pragma unroll
+                for (int e = 0; e < E; ++e) f[e] += t[e];
+            }
+            if (NEXT)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    h[NEXT ? v * E + e : 0] = f[e];
+                    sum[0] += f[e] * f[e];
+                }
+            Pack<T, E> out;
+            narrow(f, out);
+            out.store(a.h, base + col);
+        }
+        if (NEXT || RING) team_sum(sum, team_log2, shared, round++);   // RING: also tells that the stage has been read
+        if (RING) {
+            if (threadIdx.x == 0 && first + ring.stages * step < a.rows) rs.load(stage, first + ring.stages * step);
+            if (++stage == ring.stages) stage = 0, phase ^= 1;
+        }
+        if (!NEXT) continue;
+        const A r2 = inverse_root(sum[0] * mean + eps);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int col = (j + v * threads) * E;
+            if (col >= D) continue;
+            A w[E];
+            load_vector<A, E>(a.next_weight, col, w);
+            Pack<T, E> out;
+#pragma unroll
+            for (int e = 0; e < E; ++e) w[e] *= h[NEXT ? v * E + e : 0] * r2;
+            narrow(w, out);
+            out.store(a.n, base + col);
+        }
     }
 }
 
-// Blocks walk the rows; a thread keeps the sums over rows for its own columns in registers.  NEXT: with the norm before
-// the next block (three exchanges a row instead of one).
-template <typename T, int E, int NV, bool NEXT>
-__global__ void __launch_bounds__(kTeamMax) norm_backward_team(const NormArgs a, int team_log2)
+// Blocks walk the rows; a thread keeps the sums over rows for its own columns in registers: q = sum dh act x r, which
+// is the gradient of weight but for the factor residual_scale of the column, and the other way round, and sum dn h r2.
+// NEXT: with the norm before the next block (three exchanges a row instead of one).
+template <typename T, int E, int NV, bool NEXT, bool RING>
+__global__ void __launch_bounds__(kTeamMax) norm_backward_team(const NormArgs a, int team_log2, int threads, const Ring ring)
 {
     using A = typename Acc<T>::type;
     __shared__ A shared[4 * (kTeamMax / 32)];
-    extern __shared__ __align__(16) unsigned char fold_raw[];
-    A *fold = reinterpret_cast<A *>(fold_raw);
-    const int team = threadIdx.x >> team_log2, j = threadIdx.x & ((1 << team_log2) - 1), teams = blockDim.x >> team_log2;
-    A sum_w[NV * E], sum_c[NV * E], sum_n[NEXT ? NV * E : 1];
+    extern __shared__ __align__(128) unsigned char dynamic[];
+    const int teams = team_log2 < 5 ? blockDim.x >> team_log2 : 1;
+    const int team = team_log2 < 5 ? threadIdx.x >> team_log2 : 0, j = team_log2 < 5 ? threadIdx.x & (threads - 1) : threadIdx.x;
+    constexpr bool KEEP = NV * E == 8;       // column constants and the next row fit in registers
+    constexpr bool PREFETCH = KEEP && !RING;
+    const A mean = A(1) / A((int)a.D), eps = (A)a.eps;
+    const int D = (int)a.D;
+    const long long step = (long long)gridDim.x * teams;
+    A q[NV * E], qn[NEXT ? NV * E : 1], wc_kept[KEEP ? NV * E : 1], w2_kept[KEEP && NEXT ? NV * E : 1];
+    auto product = [&](int col, A (&f)[E]) {   // weight times residual_scale
+        load_vector<A, E>(a.weight, col, f);
+        if (a.scale) {
+            A c[E];
+            load_vector<A, E>(a.scale, col, c);
 #pragma unroll
-    for (int i = 0; i < NV * E; ++i) {
-        sum_w[i] = sum_c[i] = A(0);
-        if (NEXT) sum_n[i] = A(0);
+            for (int e = 0; e < E; ++e) f[e] *= c[e];
+        }
+    };
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const int col = (j + v * threads) * E;
+        A f[E], w[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] = w[e] = A(0);
+        if (KEEP && col < D) {
+            product(col, f);
+            if (NEXT) load_vector<A, E>(a.next_weight, col, w);
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            q[v * E + e] = A(0);
+            if (NEXT) qn[NEXT ? v * E + e : 0] = A(0);
+            if (KEEP) wc_kept[KEEP ? v * E + e : 0] = f[e];
+            if (KEEP && NEXT) w2_kept[KEEP && NEXT ? v * E + e : 0] = w[e];
+        }
     }
-    const bool want_c = a.scale != nullptr, want_w = a.weight != nullptr;
-    const A mean = A(1) / A(a.D);
-    int round = 0;
-    for (long long first = (long long)blockIdx.x * teams; first < a.rows; first += (long long)gridDim.x * teams) {
+    struct Operands { Pack<T, E> x, g, res, gh, gn; };
+    Operands now[RING ? 1 : NV];
+    auto fetch = [&](auto &o, long long row) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int col = (j + v * threads) * E;
+            if (row < a.rows && col < D) {
+                const long long at = row * a.D + col;
+                o[v].x.load(a.x, at);
+                if (a.gate) o[v].g.load(a.gate, at);
+                if (NEXT && a.residual) o[v].res.load(a.residual, at);
+                if (a.grad_h) o[v].gh.load(a.grad_h, at);
+                if (NEXT) o[v].gn.load(a.grad_n, at);
+            }
+        }
+    };
+    const RingState rs{dynamic + 128, norm_shared(dynamic), ring};
+    if (RING) {
+        if (threadIdx.x == 0) {
+            rs.init();
+            for (int i = 0; i < ring.stages; ++i)
+                if (blockIdx.x + i * step < a.rows) rs.load(i, blockIdx.x + i * step);
+        }
+        __syncthreads();
+    } else if (PREFETCH) {
+        fetch(now, (long long)blockIdx.x * teams + team);
+    }
+    int round = 0, stage = 0;
+    uint32_t phase = 0;
+    for (long long first = (long long)blockIdx.x * teams; first < a.rows; first += step) {
         const long long row = first + team, base = row * a.D;
-        Pack<T, E> x[NV], g[NV], res[NV], gh[NV], gn[NV];
-        bool live[NV];
-        int col[NV];
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            col[v] = (j + (v << team_log2)) * E;
-            live[v] = row < a.rows && col[v] < a.D;
-            if (live[v]) {
-                x[v].load(a.x, base + col[v]);
-                if (a.gate) g[v].load(a.gate, base + col[v]);
-                if (NEXT && a.residual) res[v].load(a.residual, base + col[v]);
-                if (a.grad_h) gh[v].load(a.grad_h, base + col[v]);
-                if (NEXT) gn[v].load(a.grad_n, base + col[v]);
-            }
-        }
+        const bool live_row = row < a.rows;
+        Operands next[PREFETCH ? NV : 1];
+        const unsigned char *here = rs.buffer + (long long)stage * ring.count * ring.row_bytes;
+        if (RING) rs.wait(stage, phase);
+        else if constexpr (PREFETCH) fetch(next, row + step);
+        else fetch(now, row);
+        // operand number `slot` of the stage: x, then gate, residual, grad_h, grad_n as far as they are there
+        int slot = 1;
+        const unsigned char *at_g = here + (a.gate ? slot++ : 0) * ring.row_bytes, *at_res = here + (NEXT && a.residual ? slot++ : 0) * ring.row_bytes;
+        const unsigned char *at_gh = here + (a.grad_h ? slot++ : 0) * ring.row_bytes, *at_gn = here + (NEXT ? slot++ : 0) * ring.row_bytes;
+        auto get = [&](int v, const unsigned char *at, bool given, const Pack<T, E> &held) {
+            Pack<T, E> p;
+            if (!RING) return held;
+            const int col = (j + v * threads) * E;
+            if (given && col < D) p.load(at, col);
+            return p;
+        };
+#define PSIG_OPERAND(v, at, given, name) get(v, at, given, now[RING ? 0 : v].name)
         A r, r2 = A(0), m2 = A(0), m;
-        A xx[2] = {A(0), A(0)};
-        if (!NEXT) {   // the gradient of h is there: both sums in one exchange
-#pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                if (!live[v]) continue;
-                A w[E], c[E];
-                load_vector<A, E>(a.weight, col[v], w);
-                load_vector<A, E>(a.scale, col[v], c);
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    A act = A(1), slope, t = to_acc<A>(x[v].v[e]);
-                    if (a.gate) act = gate_value(to_acc<A>(g[v].v[e]), a.activation, &slope);
-                    xx[0] += t * t;
-                    xx[1] += w[e] * (to_acc<A>(gh[v].v[e]) * c[e] * act) * t;
-                }
-            }
-            team_sum(xx, team_log2, shared, round++);
-            r = inverse_root(xx[0] * mean + A(a.eps));
-            m = xx[1] * mean * r * r * r;
-        } else {
-            A sx[1] = {A(0)};
-#pragma unroll
-            for (int v = 0; v < NV; ++v)
-#pragma unroll
-                for (int e = 0; e < E; ++e) { const A t = to_acc<A>(x[v].v[e]); sx[0] += t * t; }
-            team_sum(sx, team_log2, shared, round++);
-            r = inverse_root(sx[0] * mean + A(a.eps));
-#pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                if (!live[v]) continue;
-                A w[E], c[E], w2[E];
-                load_vector<A, E>(a.weight, col[v], w);
-                load_vector<A, E>(a.scale, col[v], c);
-                load_vector<A, E>(a.next_weight, col[v], w2);
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    A slope, t = to_acc<A>(x[v].v[e]) * r * w[e];
-                    if (a.gate) t *= gate_value(to_acc<A>(g[v].v[e]), a.activation, &slope);
-                    t *= c[e];
-                    if (a.residual) t += to_acc<A>(res[v].v[e]);
-                    xx[0] += t * t;
-                    xx[1] += w2[e] * to_acc<A>(gn[v].v[e]) * t;
-                }
-            }
-            team_sum(xx, team_log2, shared, round++);
-            r2 = inverse_root(xx[0] * mean + A(a.eps));
-            m2 = xx[1] * mean * r2 * r2 * r2;
-            sx[0] = A(0);
-#pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                if (!live[v]) continue;
-                A w[E], c[E], w2[E];
-                load_vector<A, E>(a.weight, col[v], w);
-                load_vector<A, E>(a.scale, col[v], c);
-                load_vector<A, E>(a.next_weight, col[v], w2);
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const A t = to_acc<A>(x[v].v[e]);
-                    A act = A(1), slope;
-                    if (a.gate) act = gate_value(to_acc<A>(g[v].v[e]), a.activation, &slope);
-                    A h = t * r * w[e] * act * c[e];
-                    if (a.residual) h += to_acc<A>(res[v].v[e]);
-                    const A dh = to_acc<A>(gh[v].v[e]) + w2[e] * to_acc<A>(gn[v].v[e]) * r2 - h * m2;
-                    sx[0] += w[e] * dh * c[e] * act * t;
-                }
-            }
-            team_sum(sx, team_log2, shared, round++);
-            m = sx[0] * mean * r * r * r;
-        }
+        A dh[NV * E], f[NV * E], sig[NV * E];   // gradient of h; factor of x in u, without r; sigmoid of the gate
+        A two[2] = {A(0), A(0)}, one[1] = {A(0)};
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            if (!live[v]) continue;
-            A w[E], c[E], w2[E];
-            load_vector<A, E>(a.weight, col[v], w);
-            load_vector<A, E>(a.scale, col[v], c);
-            if (NEXT) load_vector<A, E>(a.next_weight, col[v], w2);
-            Pack<T, E> out_x, out_g, out_r;
+            const int col = (j + v * threads) * E;
+            const Pack<T, E> x = PSIG_OPERAND(v, here, true, x), gh = PSIG_OPERAND(v, at_gh, a.grad_h != nullptr, gh);
+            A fv[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) fv[e] = KEEP ? wc_kept[KEEP ? v * E + e : 0] : A(0);
+            if (!KEEP && col < D) product(col, fv);
+            A t[E], d[E];
+            if (a.gate) {
+                widen(PSIG_OPERAND(v, at_g, true, g), t);
+#pragma unroll
+                for (int e = 0; e < E; ++e) fv[e] *= sig[v * E + e] = sigmoid(t[e]);
+                if (a.activation == 0)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) fv[e] *= t[e];
+            }
+            widen(x, t);
+            widen(gh, d);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const A t = to_acc<A>(x[v].v[e]);
-                A act = A(1), slope = A(0);
-                if (a.gate) act = gate_value(to_acc<A>(g[v].v[e]), a.activation, &slope);
-                const A z = t * r * w[e];
-                A dh = to_acc<A>(gh[v].v[e]);
-                if (NEXT) {
-                    A h = z * act * c[e];
-                    if (a.residual) h += to_acc<A>(res[v].v[e]);
-                    const A dn = to_acc<A>(gn[v].v[e]);
-                    dh += w2[e] * dn * r2 - h * m2;
-                    sum_n[v * E + e] += dn * h * r2;
-                }
-                const A dz = dh * c[e] * act;
-                sum_c[v * E + e] += dh * z * act;
-                sum_w[v * E + e] += dz * t * r;
-                out_r.v[e] = from_acc<T>(dh);
-                out_g.v[e] = from_acc<T>(dh * c[e] * z * slope);
-                out_x.v[e] = from_acc<T>(r * w[e] * dz - t * m);
+                f[v * E + e] = fv[e];
+                dh[v * E + e] = d[e];
+                two[0] += t[e] * t[e];
+                if (!NEXT) two[1] += d[e] * fv[e] * t[e];
             }
-            if (a.grad_residual) out_r.store(a.grad_residual, base + col[v]);
-            if (a.grad_gate) out_g.store(a.grad_gate, base + col[v]);
-            if (a.grad_x) out_x.store(a.grad_x, base + col[v]);
         }
+        if (!NEXT) {   // the gradient of h is there: both sums in one exchange
+            team_sum(two, team_log2, shared, round++);
+            r = inverse_root(two[0] * mean + eps);
+            m = two[1] * mean * r * r * r;
+        } else {
+            one[0] = two[0];
+            team_sum(one, team_log2, shared, round++);
+            r = inverse_root(one[0] * mean + eps);
+            two[0] = two[1] = A(0);
+            A h[NV * E];
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const int col = (j + v * threads) * E;
+                const Pack<T, E> x = PSIG_OPERAND(v, here, true, x), gn = PSIG_OPERAND(v, at_gn, true, gn);
+                const Pack<T, E> res = PSIG_OPERAND(v, at_res, a.residual != nullptr, res);
+                A w2[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) w2[e] = KEEP ? w2_kept[KEEP && NEXT ? v * E + e : 0] : A(0);
+                if (!KEEP && col < D) load_vector<A, E>(a.next_weight, col, w2);
+                A t[E], u[E], d[E];
+                widen(x, t);
+                widen(res, u);
+                widen(gn, d);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const int i = v * E + e;
+                    h[i] = t[e] * r * f[i] + u[e];
+                    two[0] += h[i] * h[i];
+                    two[1] += w2[e] * d[e] * h[i];
+                }
+            }
+            team_sum(two, team_log2, shared, round++);
+            r2 = inverse_root(two[0] * mean + eps);
+            m2 = two[1] * mean * r2 * r2 * r2;
+            one[0] = A(0);
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const int col = (j + v * threads) * E;
+                const Pack<T, E> x = PSIG_OPERAND(v, here, true, x), gn = PSIG_OPERAND(v, at_gn, true, gn);
+                A w2[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) w2[e] = KEEP ? w2_kept[KEEP && NEXT ? v * E + e : 0] : A(0);
+                if (!KEEP && col < D) load_vector<A, E>(a.next_weight, col, w2);
+                A t[E], d[E];
+                widen(x, t);
+                widen(gn, d);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const int i = v * E + e;
+                    const A dn = d[e] * r2;
+                    dh[i] += w2[e] * dn - h[i] * m2;
+                    qn[NEXT ? i : 0] += dn * h[i];
+                    one[0] += dh[i] * f[i] * t[e];
+                }
+            }
+            team_sum(one, team_log2, shared, round++);
+            m = one[0] * mean * r * r * r;
         }
-    // the block's teams hold the same columns: fold them in order, one vector after the other
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int col = (j + v * threads) * E;
+            if (!live_row || col >= D) continue;
+            A t[E], o[E];
+            widen(PSIG_OPERAND(v, here, true, x), t);
+            Pack<T, E> out;
+            if (a.grad_residual) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = dh[v * E + e];
+                narrow(o, out);
+                out.store(a.grad_residual, base + col);
+            }
+            if (a.grad_x) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = r * f[v * E + e] * dh[v * E + e] - t[e] * m;
+                narrow(o, out);
+                out.store(a.grad_x, base + col);
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) t[e] *= dh[v * E + e] * r;
+            if (a.gate) {
+                A g[E], fv[E];
+                widen(PSIG_OPERAND(v, at_g, true, g), g);
+#pragma unroll
+                for (int e = 0; e < E; ++e) fv[e] = KEEP ? wc_kept[KEEP ? v * E + e : 0] : A(0);
+                if (!KEEP) product(col, fv);
+                if (a.activation == 0) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const A s1 = sig[v * E + e], act = g[e] * s1;
+                        o[e] = t[e] * fv[e] * (s1 + act * (A(1) - s1));
+                        q[v * E + e] += t[e] * act;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const A s1 = sig[v * E + e];
+                        o[e] = t[e] * fv[e] * (s1 * (A(1) - s1));
+                        q[v * E + e] += t[e] * s1;
+                    }
+                }
+                narrow(o, out);
+                if (a.grad_gate) out.store(a.grad_gate, base + col);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) q[v * E + e] += t[e];
+            }
+        }
+#undef PSIG_OPERAND
+        if (RING) {
+            __syncthreads();   // the stage has been read
+            if (threadIdx.x == 0 && first + ring.stages * step < a.rows) rs.load(stage, first + ring.stages * step);
+            if (++stage == ring.stages) stage = 0, phase ^= 1;
+        }
+        if constexpr (PREFETCH)
+#pragma unroll
+            for (int v = 0; v < NV; ++v) now[v] = next[v];
+    }
+    // the block's teams hold the same columns: fold them in order
+    A *fold = reinterpret_cast<A *>(dynamic);
     A *part = static_cast<A *>(a.partial) + (long long)blockIdx.x * 3 * a.D;
 #pragma unroll
-    for (int which = 0; which < (NEXT ? 3 : 2); ++which) {
-        if (which == 0 ? !want_w : which == 1 ? !want_c : false) continue;
+    for (int which = 0; which < (NEXT ? 2 : 1); ++which) {
+        if (which == 0 && a.weight == nullptr && a.scale == nullptr) continue;
         if (teams > 1) {
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < NV * E; ++i)
-                fold[i * blockDim.x + threadIdx.x] = which == 0 ? sum_w[i] : which == 1 ? sum_c[i] : sum_n[NEXT ? i : 0];
+            for (int i = 0; i < NV * E; ++i) fold[i * blockDim.x + threadIdx.x] = which == 0 ? q[i] : qn[NEXT ? i : 0];
             __syncthreads();
         }
-        if (team == 0)
+        if (team != 0) continue;
 #pragma unroll
-            for (int v = 0; v < NV; ++v)
+        for (int v = 0; v < NV; ++v) {
+            const int col = (j + v * threads) * E;
+            if (col >= D) continue;
+            A w[E], c[E];
+            load_vector<A, E>(a.weight, col, w);
+            load_vector<A, E>(a.scale, col, c);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int i = v * E + e;
+                A s = which == 0 ? q[i] : qn[NEXT ? i : 0];
+                for (int k = 1; k < teams; ++k) s += fold[i * blockDim.x + (k << team_log2) + j];
+                if (which == 1) part[2 * a.D + col + e] = s;
+                else if (a.weight) part[col + e] = s * c[e];
+                if (which == 0 && a.scale) part[a.D + col + e] = s * w[e];
+            }
+        }
+    }
+}
+
+// ---- rows wider than a block holds: walked in accesses of E values, read again for each sum ----
+
+template <typename T, int E>
+__device__ __forceinline__ void wide_values(const NormArgs &a, long long base, long long col,
+                                            typename Acc<T>::type r, typename Acc<T>::type (&x)[E], typename Acc<T>::type (&f)[E],
+                                            typename Acc<T>::type (&h)[E])
+{
+    using A = typename Acc<T>::type;
+    Pack<T, E> p, g, res;
+    p.load(a.x, base + col);
+    if (a.gate) g.load(a.gate, base + col);
+    if (a.residual) res.load(a.residual, base + col);
+    load_vector<A, E>(a.weight, col, f);
+    if (a.scale) {
+        A c[E];
+        load_vector<A, E>(a.scale, col, c);
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] *= c[e];
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if (a.gate) f[e] *= gate_value(to_acc<A>(g.v[e]), a.activation);
+        x[e] = to_acc<A>(p.v[e]);
+        h[e] = x[e] * r * f[e] + to_acc<A>(res.v[e]);
+    }
+}
+
+template <typename T, int E>
+__global__ void __launch_bounds__(kWideThreads) norm_forward_wide(const NormArgs a)
+{
+    using A = typename Acc<T>::type;
+    __shared__ A shared[4 * (kTeamMax / 32)];
+    const A mean = A(1) / A(a.D), eps = (A)a.eps;
+    int round = 0;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const long long base = row * a.D;
+        A sum[1] = {A(0)};
+#pragma unroll 4
+        for (long long col = threadIdx.x * E; col < a.D; col += kWideThreads * E) {
+            Pack<T, E> p;
+            p.load(a.x, base + col);
+#pragma unroll
+            for (int e = 0; e < E; ++e) { const A t = to_acc<A>(p.v[e]); sum[0] += t * t; }
+        }
+        team_sum(sum, 5, shared, round++);
+        const A r = inverse_root(sum[0] * mean + eps);
+        sum[0] = A(0);
+        for (long long col = threadIdx.x * E; col < a.D; col += kWideThreads * E) {
+            A x[E], f[E], h[E];
+            wide_values<T, E>(a, base, col, r, x, f, h);
+            Pack<T, E> out;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                out.v[e] = from_acc<T>(h[e]);
+                sum[0] += h[e] * h[e];
+            }
+            out.store(a.h, base + col);
+        }
+        if (a.next_weight == nullptr) continue;
+        team_sum(sum, 5, shared, round++);
+        const A r2 = inverse_root(sum[0] * mean + eps);
+        for (long long col = threadIdx.x * E; col < a.D; col += kWideThreads * E) {
+            A x[E], f[E], h[E], w[E];
+            wide_values<T, E>(a, base, col, r, x, f, h);
+            load_vector<A, E>(a.next_weight, col, w);
+            Pack<T, E> out;
+#pragma unroll
+            for (int e = 0; e < E; ++e) out.v[e] = from_acc<T>(h[e] * r2 * w[e]);
+            out.store(a.n, base + col);
+        }
+    }
+}
+
+// The block's sums over its rows are kept in its part of the workspace, each entry by the thread that owns the column.
+template <typename T, int E>
+__global__ void __launch_bounds__(kWideThreads) norm_backward_wide(const NormArgs a)
+{
+    using A = typename Acc<T>::type;
+    __shared__ A shared[4 * (kTeamMax / 32)];
+    const A mean = A(1) / A(a.D), eps = (A)a.eps;
+    A *part = static_cast<A *>(a.partial) + (long long)blockIdx.x * 3 * a.D;
+    int round = 0;
+    bool fresh = true;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const long long base = row * a.D;
+        A one[1] = {A(0)}, two[2] = {A(0), A(0)};
+#pragma unroll 4
+        for (long long col = threadIdx.x * E; col < a.D; col += kWideThreads * E) {
+            Pack<T, E> p;
+            p.load(a.x, base + col);
+#pragma unroll
+            for (int e = 0; e < E; ++e) { const A t = to_acc<A>(p.v[e]); one[0] += t * t; }
+        }
+        team_sum(one, 5, shared, round++);
+        const A r = inverse_root(one[0] * mean + eps);
+        A r2 = A(0), m2 = A(0);
+        if (a.next_weight != nullptr) {
+            for (long long col = threadIdx.x * E; col < a.D; col += kWideThreads * E) {
+                A x[E], f[E], h[E], w2[E];
+                Pack<T, E> gn;
+                wide_values<T, E>(a, base, col, r, x, f, h);
+                load_vector<A, E>(a.next_weight, col, w2);
+                gn.load(a.grad_n, base + col);
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const int c = (j + (v << team_log2)) * E + e, i = v * E + e;
-                    if (c >= a.D) continue;
-                    A s = which == 0 ? sum_w[i] : which == 1 ? sum_c[i] : sum_n[NEXT ? i : 0];
-                    if (teams > 1)
-                        for (int k = 1; k < teams; ++k) s += fold[i * blockDim.x + (k << team_log2) + j];
-                    part[which * a.D + c] = s;
+                    two[0] += h[e] * h[e];
+                    two[1] += w2[e] * to_acc<A>(gn.v[e]) * h[e];
                 }
+            }
+            team_sum(two, 5, shared, round++);
+            r2 = inverse_root(two[0] * mean + eps);
+            m2 = two[1] * mean * r2 * r2 * r2;
+        }
+        auto gradient = [&](long long col, const A (&h)[E], A (&dh)[E], A (&dn)[E]) {
+            Pack<T, E> gh;
+            if (a.grad_h) gh.load(a.grad_h, base + col);
+#pragma unroll
+            for (int e = 0; e < E; ++e) dh[e] = to_acc<A>(gh.v[e]), dn[e] = A(0);
+            if (a.next_weight != nullptr) {
+                A w2[E];
+                Pack<T, E> gn;
+                load_vector<A, E>(a.next_weight, col, w2);
+                gn.load(a.grad_n, base + col);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    dn[e] = to_acc<A>(gn.v[e]);
+                    dh[e] += w2[e] * dn[e] * r2 - h[e] * m2;
+                }
+            }
+        };
+        one[0] = A(0);
+        for (long long col = threadIdx.x * E; col < a.D; col += kWideThreads * E) {
+            A x[E], f[E], h[E], dh[E], dn[E];
+            wide_values<T, E>(a, base, col, r, x, f, h);
+            gradient(col, h, dh, dn);
+#pragma unroll
+            for (int e = 0; e < E; ++e) one[0] += dh[e] * f[e] * x[e];
+        }
+        team_sum(one, 5, shared, round++);
+        const A m = one[0] * mean * r * r * r;
+        for (long long col = threadIdx.x * E; col < a.D; col += kWideThreads * E) {
+            A x[E], f[E], h[E], dh[E], dn[E], w[E], c[E];
+            wide_values<T, E>(a, base, col, r, x, f, h);
+            gradient(col, h, dh, dn);
+            load_vector<A, E>(a.weight, col, w);
+            load_vector<A, E>(a.scale, col, c);
+            Pack<T, E> out_x, out_g, out_r, g;
+            if (a.gate) g.load(a.gate, base + col);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                A act = A(1), slope = A(0);
+                if (a.gate) {
+                    act = gate_value(to_acc<A>(g.v[e]), a.activation);
+                    slope = gate_slope(to_acc<A>(g.v[e]), a.activation);
+                }
+                const A t = dh[e] * act * x[e] * r;
+                if (a.weight) part[col + e] = (fresh ? A(0) : part[col + e]) + t * c[e];
+                if (a.scale) part[a.D + col + e] = (fresh ? A(0) : part[a.D + col + e]) + t * w[e];
+                if (a.next_weight) part[2 * a.D + col + e] = (fresh ? A(0) : part[2 * a.D + col + e]) + dn[e] * h[e] * r2;
+                out_r.v[e] = from_acc<T>(dh[e]);
+                out_g.v[e] = from_acc<T>(dh[e] * c[e] * w[e] * x[e] * r * slope);
+                out_x.v[e] = from_acc<T>(r * f[e] * dh[e] - x[e] * m);
+            }
+            if (a.grad_residual) out_r.store(a.grad_residual, base + col);
+            if (a.grad_gate) out_g.store(a.grad_gate, base + col);
+            if (a.grad_x) out_x.store(a.grad_x, base + col);
+        }
+        fresh = false;
     }
 }
 
@@ -479,28 +799,56 @@ int check_norm(const PsigNormDesc *d)
     return PSIG_OK;
 }
 
-// How a row is dealt to threads: 8 values to a thread while the team has at most kTeamMax threads then 16.
+// How a row is dealt to threads: 8 values to a thread, 16 where the row would need more than 256 threads (a block with
+// more of them waits longer at its barriers than the larger number of values costs: 4680 values, see norm_forward_team).
 struct TeamPlan {
-    int team_log2, values, threads;   // values per thread; threads per block
+    int team_log2, threads, block;   // log2 of the team inside a warp (5: the block is the team); threads per row; block size
+    int values;                      // per thread
+    int teams() const { return team_log2 < 5 ? block >> team_log2 : 1; }
 };
 
 TeamPlan team_plan(long long D)
 {
-    TeamPlan p{0, 8, 256};
-    while ((8LL << p.team_log2) < D && (1 << p.team_log2) < kTeamMax) ++p.team_log2;
-    while ((long long)p.values << p.team_log2 < D) p.values *= 2;
-    if (1 << p.team_log2 > p.threads) p.threads = 1 << p.team_log2;
+    TeamPlan p{0, 1, kShortThreads, 8};
+    if (D <= 128) {
+        while ((8LL << p.team_log2) < D) ++p.team_log2;
+        p.threads = 1 << p.team_log2;
+        return p;
+    }
+    if (D > 256 * 8) p.values = 16;
+    p.team_log2 = 5;
+    p.threads = p.block = (int)((D + p.values - 1) / p.values + 31) / 32 * 32;
     return p;
 }
 
-// Resident blocks are enough: each keeps its column sums over all its rows.
+// Blocks of the backward pass: about as many as are resident together (each keeps its column sums over all its rows).
 int backward_blocks(const PsigNormDesc &d)
 {
-    if (d.D > kNormWidest) return (int)(d.rows < 148 * 4 ? d.rows : 148 * 4);
+    if (d.D > kNormWidest) return (int)(d.rows < 148 * 2 ? d.rows : 148 * 2);
     const TeamPlan p = team_plan(d.D);
-    const long long teams = p.threads >> p.team_log2, need = (d.rows + teams - 1) / teams;
-    const long long most = 148LL * (p.threads > 256 ? 2 : 4);
-    return (int)(need < most ? need : most);
+    const long long need = (d.rows + p.teams() - 1) / p.teams(), per_sm = p.block <= 128 ? 8 : p.block <= 256 ? 4 : p.block <= 320 ? 3 : 2;
+    return (int)(need < 148 * per_sm ? need : 148 * per_sm);
+}
+
+// Shared memory of a block's ring, with `per_sm` blocks on an SM: as many stages (2 to 4) as fit; none when rows are no whole
+// 16-byte pieces, or too short for a block of their own.
+template <typename T>
+int plan_ring(const NormArgs &a, const TeamPlan &p, bool backward, bool next, int per_sm, Ring *ring)
+{
+    *ring = Ring{};
+    const void *operands[] = {a.x, a.gate, backward && !next ? nullptr : a.residual, backward ? a.grad_h : nullptr,
+                              backward && next ? a.grad_n : nullptr};
+    for (const void *o : operands) {
+        if (o == nullptr) continue;
+        if (reinterpret_cast<uintptr_t>(o) % 16 != 0) return 0;
+        ring->data[ring->count++] = o;
+    }
+    const long long bytes = a.D * (long long)sizeof(T);
+    if (p.team_log2 < 5 || bytes % 16 != 0 || sizeof(T) == 8) return 0;
+    ring->row_bytes = (int)bytes;
+    const long long room = 220 * 1024 / per_sm - 1024 - 128, stage = bytes * ring->count;
+    ring->stages = (int)(room / stage < 4 ? room / stage : 4);
+    return ring->stages < 2 ? 0 : 128 + (int)(stage * ring->stages);
 }
 
 // Largest number of values that one access of every operand can hold (all rows start on such a boundary).
@@ -519,20 +867,24 @@ int access_width(const NormArgs &a)
     return width;
 }
 
-// Calls fn with (values per access, accesses per thread) as compile-time numbers.
+// Calls fn with the values per access, or with them and the accesses per thread, as compile-time numbers.
+template <typename T, typename Fn>
+int with_width(int width, Fn fn)
+{
+    constexpr int full = sizeof(T) == 8 ? 1 : 16 / (int)sizeof(T);
+    if (width >= full) return fn(std::integral_constant<int, full>{});
+    if constexpr (full == 8)
+        if (width >= 2) return fn(std::integral_constant<int, 2>{});
+    return fn(std::integral_constant<int, 1>{});
+}
 template <typename T, typename Fn>
 int with_shape(int width, int values, Fn fn)
 {
-    constexpr int full = sizeof(T) == 8 ? 1 : 16 / (int)sizeof(T);
-    auto by_values = [&](auto w) {
-        constexpr int E = decltype(w)::value;
-        if (values == 8) return fn(w, std::integral_constant<int, 8 / E>{});
-        return fn(w, std::integral_constant<int, 16 / E>{});
-    };
-    if (width >= full) return by_values(std::integral_constant<int, full>{});
-    if constexpr (full == 8)
-        if (width >= 2) return by_values(std::integral_constant<int, 2>{});
-    return by_values(std::integral_constant<int, 1>{});
+    return with_width<T>(width, [&](auto e) {
+        constexpr int E = decltype(e)::value;
+        if (values == 8) return fn(e, std::integral_constant<int, 8 / E>{});
+        return fn(e, std::integral_constant<int, 16 / E>{});
+    });
 }
 
 }  // namespace
@@ -556,16 +908,32 @@ extern "C" int psig_norm_forward(const PsigNormDesc *desc, const void *x, const 
     return with_dtype(desc->dtype, [&](auto t) {
         using T = decltype(t);
         if (a.D > kNormWidest) {
-            const unsigned grid = (unsigned)(a.rows < 148 * 16 ? a.rows : 148 * 16);
-            norm_forward_rows<T><<<grid, kNormThreads, 0, s>>>(a);
-            return check_launch();
+            const unsigned grid = (unsigned)(a.rows < 148 * 4 ? a.rows : 148 * 4);
+            return with_width<T>(access_width<T>(a), [&](auto e) {
+                norm_forward_wide<T, decltype(e)::value><<<grid, kWideThreads, 0, s>>>(a);
+                return check_launch();
+            });
         }
         const TeamPlan p = team_plan(a.D);
-        const long long teams = p.threads >> p.team_log2, blocks = (a.rows + teams - 1) / teams;
+        const long long blocks = (a.rows + p.teams() - 1) / p.teams();
         if (blocks > 0x7fffffffLL) return (int)PSIG_ERR_TOO_LARGE;
+        const int per_sm = p.block <= 128 ? 12 : p.block <= 256 ? 6 : 4;
+        Ring ring;
+        // a ring pays when a block walks several rows
+        const int smem = a.rows >= 148LL * per_sm * 4 ? plan_ring<T>(a, p, false, a.next_weight != nullptr, per_sm, &ring) : 0;
         return with_shape<T>(access_width<T>(a), p.values, [&](auto e, auto nv) {
-            norm_forward_team<T, decltype(e)::value, decltype(nv)::value><<<(unsigned)blocks, p.threads, 0, s>>>(a, p.team_log2);
-            return check_launch();
+            constexpr int E = decltype(e)::value, NV = decltype(nv)::value;
+            auto launch = [&](auto kernel, unsigned grid, int bytes) {
+                if (!prepare_kernel(kernel, bytes, false)) return (int)PSIG_ERR_CUDA;
+                kernel<<<grid, p.block, bytes, s>>>(a, p.team_log2, p.threads, ring);
+                return check_launch();
+            };
+            if constexpr (E * sizeof(T) == 16)
+                if (smem > 0)
+                    return a.next_weight ? launch(norm_forward_team<T, E, NV, true, true>, 148 * per_sm, smem)
+                                         : launch(norm_forward_team<T, E, NV, false, true>, 148 * per_sm, smem);
+            return a.next_weight ? launch(norm_forward_team<T, E, NV, true, false>, (unsigned)blocks, 0)
+                                 : launch(norm_forward_team<T, E, NV, false, false>, (unsigned)blocks, 0);
         });
     });
 }
@@ -601,16 +969,29 @@ extern "C" int psig_norm_backward(const PsigNormDesc *desc, const void *x, const
         using A = typename Acc<T>::type;
         int status;
         if (a.D > kNormWidest) {
-            norm_backward_rows<T><<<blocks, kNormThreads, 0, s>>>(a);
-            status = check_launch();
+            status = with_width<T>(access_width<T>(a), [&](auto e) {
+                norm_backward_wide<T, decltype(e)::value><<<blocks, kWideThreads, 0, s>>>(a);
+                return check_launch();
+            });
         } else {
             const TeamPlan p = team_plan(a.D);
+            Ring ring;
+            const int per_sm = (blocks + 147) / 148;
+            const int smem = a.rows >= blocks * 4LL ? plan_ring<T>(a, p, true, a.next_weight != nullptr, per_sm, &ring) : 0;
             status = with_shape<T>(access_width<T>(a), p.values, [&](auto e, auto nv) {
                 constexpr int E = decltype(e)::value, NV = decltype(nv)::value;
-                const size_t fold = (p.threads >> p.team_log2) > 1 ? sizeof(A) * E * NV * p.threads : 0;
-                if (a.next_weight) norm_backward_team<T, E, NV, true><<<blocks, p.threads, fold, s>>>(a, p.team_log2);
-                else norm_backward_team<T, E, NV, false><<<blocks, p.threads, fold, s>>>(a, p.team_log2);
-                return check_launch();
+                auto launch = [&](auto kernel, int bytes) {
+                    if (!prepare_kernel(kernel, bytes, false)) return (int)PSIG_ERR_CUDA;
+                    kernel<<<blocks, p.block, bytes, s>>>(a, p.team_log2, p.threads, ring);
+                    return check_launch();
+                };
+                if constexpr (E * sizeof(T) == 16)
+                    if (smem > 0)
+                        return a.next_weight ? launch(norm_backward_team<T, E, NV, true, true>, smem)
+                                             : launch(norm_backward_team<T, E, NV, false, true>, smem);
+                const int fold = p.teams() > 1 ? (int)sizeof(A) * E * NV * p.block : 0;
+                return a.next_weight ? launch(norm_backward_team<T, E, NV, true, false>, fold)
+                                     : launch(norm_backward_team<T, E, NV, false, false>, fold);
             });
         }
         if (status != PSIG_OK || (!grad_weight && !grad_residual_scale && !grad_next_weight)) return status;
