@@ -291,10 +291,10 @@ int psig_attn_backward(const PsigAttnDesc *desc, const void *q, const void *k, c
 int psig_attn_step(const PsigAttnDesc *desc, const void *q, const void *k, const void *v, const void *log_decay,
                    void *state, void *out, void *stream);
 
-/* Diagnostic: waits inside the tensor-core kernels of psig_attn_* that ran out on the current device since the last call
+/* Diagnostic: waits inside the kernels of psig_attn_* and psig_norm_* that ran out on the current device since the last call
  * (read and cleared; synchronises).  Every wait for a copy, a matrix product or another warp is bounded; one that runs
  * out ends its block early, and the call's results are then not valid.  0 in normal operation. */
-int64_t psig_attn_wait_timeouts(void);
+int64_t psig_sequence_wait_timeouts(void);
 
 /* Norm around a block, fused with the block's gate, the residual sum and the norm before the next block; no
  * counterpart in the reference.  Per row of D features, rms(x) = x / sqrt(mean(x^2) + eps):

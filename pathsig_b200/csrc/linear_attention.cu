@@ -425,8 +425,10 @@ struct Call {
         s.kv_scale = d.scale;
         return s;
     }
-    bool tiles() const
+    bool tiles(const void *o1, const void *o2 = nullptr, const void *o3 = nullptr) const
     {
+        for (const void *o : {o1, o2, o3})
+            if (reinterpret_cast<uintptr_t>(o) % 16 != 0) return false;
         return d.algo != PSIG_ALGO_GENERIC && attn_tiles_supported(forward(), d.dtype);
     }
 };
@@ -472,7 +474,7 @@ int run_forward(const Call &c, const void *init, void *out, void *final, cudaStr
     s.init = init;
     s.final = final;
     s.out = out;
-    return c.tiles() ? attn_sweep_on_tiles(s, false, c.d.dtype, stream) : sweep_rows<T>(s, stream);
+    return c.tiles(out) ? attn_sweep_on_tiles(s, false, c.d.dtype, stream) : sweep_rows<T>(s, stream);
 }
 
 unsigned blocks_for(long long items, int per_block)
@@ -563,7 +565,7 @@ int run_backward(const Call &c, const void *init, const void *gs, void *grad_q, 
                  void *grad_decay, void *grad_init, char *ws, cudaStream_t stream)
 {
     using A = typename Acc<T>::type;
-    if (c.tiles() && attn_tiles_supported(c.grad_q(), c.d.dtype))
+    if (c.tiles(grad_q, grad_k, grad_v) && attn_tiles_supported(c.grad_q(), c.d.dtype))
         return run_backward_tiles<T>(c, init, gs, grad_q, grad_k, grad_v, grad_decay, grad_init, ws, stream);
     const PsigAttnDesc &d = c.d;
     const BackwardScratch at = backward_scratch(d);
@@ -644,7 +646,7 @@ extern "C" int psig_attn_backward(const PsigAttnDesc *desc, const void *q, const
     });
 }
 
-extern "C" int64_t psig_attn_wait_timeouts(void) { return attn_tile_timeouts(); }
+extern "C" int64_t psig_sequence_wait_timeouts(void) { return attn_tile_timeouts() + attn_split_timeouts() + norm_timeouts(); }
 
 extern "C" int psig_attn_step(const PsigAttnDesc *desc, const void *q, const void *k, const void *v,
                               const void *log_decay, void *state, void *out, void *stream)

@@ -888,6 +888,15 @@ int with_shape(int width, int values, Fn fn)
 }
 
 }  // namespace
+
+long long norm_timeouts()
+{
+    unsigned long long count = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&count, g_norm_timeouts, sizeof(count)) != cudaSuccess) return -1;
+    if (count != 0) cudaMemcpyToSymbol(g_norm_timeouts, &zero, sizeof(zero));
+    return (long long)count;
+}
+
 }  // namespace psig
 
 using namespace psig;

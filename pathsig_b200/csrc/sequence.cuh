@@ -86,7 +86,10 @@ inline long long segments_of(long long L) { return (L + kSegment - 1) / kSegment
 // storage type.
 bool attn_tiles_supported(const Sweep &a, int dtype);
 int attn_sweep_on_tiles(const Sweep &a, bool exact, int dtype, cudaStream_t stream);
+int attn_sweep_split(const Sweep &a, bool exact, int dtype, cudaStream_t stream);   // float16 and float32
 long long attn_tile_timeouts();
+long long attn_split_timeouts();
+long long norm_timeouts();
 constexpr int kTileDots = 8;   // parts of an anchor's sum per column tile of 64
 inline int tile_columns(int d2) { return (d2 + 63) / 64; }
 

@@ -1,0 +1,252 @@
+// Building blocks of the tensor-core sweeps (linear_attention_tiles.cu, linear_attention_split.cu): tensor memory,
+// matrix instructions, TMA, bounded waits, and the decay tables of a piece (internal header).
+#pragma once
+
+#include "sequence.cuh"
+
+#include <cuda.h>
+
+#include <type_traits>
+
+namespace psig {
+
+namespace {
+
+__device__ unsigned long long g_tile_timeouts;   // of the translation unit
+
+// Read and clear.
+[[maybe_unused]] long long take_timeouts()
+{
+    unsigned long long count = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&count, g_tile_timeouts, sizeof(count)) != cudaSuccess) return -1;
+    if (count != 0) cudaMemcpyToSymbol(g_tile_timeouts, &zero, sizeof(zero));
+    return (long long)count;
+}
+
+constexpr int kPiece = 128;
+constexpr int kCompute = 256;                 // compute threads
+constexpr int kTileThreads = kCompute + 64;   // + issuing warp + decay warp
+constexpr int kTileBytes = kPiece * 128;      // 128 rows of 64 16-bit values
+constexpr unsigned kWaitPolls = 1u << 22;     // each poll blocks for a hardware-defined time at most
+
+struct DecayTables {       // of one piece; all exponents are of 2
+    double a[kPiece];      // a_t
+    float la[kPiece];      // a_s - (a at the low end of s's block of 32)
+    float cf[kPiece];      // 2^-la
+    float tail[kPiece];    // 2^(a_end - a_s)
+    float head[kPiece];    // 2^a_t
+    float keep;            // 2^a_end, what is left of the state
+    float pad[3];
+};
+
+__device__ __forceinline__ uint32_t shared_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count)
+{
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Waits for the phase of this parity; false when the bound ran out here or in another thread of the block.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *failed)
+{
+    for (unsigned i = 0; i < kWaitPolls; ++i) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+        if (*failed) return false;
+    }
+    if (atomicExch(const_cast<int *>(failed), 1) == 0) atomicAdd(&g_tile_timeouts, 1ull);
+    return false;
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int head, int t, int b)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(head), "r"(t), "r"(b) : "memory");
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle.  Rows of 128 bytes, eight rows (1024 bytes) to a swizzle
+// atom; `lead` is the distance of neighbouring 64-element blocks where the row runs along M or N.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lead)
+{
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t instr_desc(int n, bool a_rows_along_m, bool b_rows_along_n)
+{
+    const uint32_t type = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    return (1u << 4) | (type << 7) | (type << 10) | ((a_rows_along_m ? 1u : 0u) << 15) | ((b_rows_along_n ? 1u : 0u) << 16) |
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_load16(uint32_t addr, float (&x)[16])
+{
+    uint32_t *r = reinterpret_cast<uint32_t *>(x);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+__device__ __forceinline__ void tmem_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float exp_two(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Two values as 16-bit pair (low half first), and back.
+__device__ __forceinline__ uint32_t pack(float x, float y, __nv_bfloat16) { __nv_bfloat162 p = __floats2bfloat162_rn(x, y); return *reinterpret_cast<uint32_t *>(&p); }
+__device__ __forceinline__ uint32_t pack(float x, float y, __half) { __half2 p = __floats2half2_rn(x, y); return *reinterpret_cast<uint32_t *>(&p); }
+__device__ __forceinline__ float2 unpack(uint32_t v, __nv_bfloat16) { return float2{__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)}; }
+__device__ __forceinline__ float2 unpack(uint32_t v, __half) { return __half22float2(*reinterpret_cast<__half2 *>(&v)); }
+
+// The next 16-bit term of a pair; leaves what the rounding left.
+template <typename T>
+__device__ __forceinline__ uint32_t next_term(float &x, float &y, bool last)
+{
+    const uint32_t p = pack(x, y, T{});
+    if (!last) {
+        const float2 back = unpack(p, T{});
+        x -= back.x;
+        y -= back.y;
+    }
+    return p;
+}
+
+__device__ __forceinline__ uint32_t swizzled(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
+
+// One warp: the decay tables of the sweep's pieces, one piece ahead of their use, in two buffers in turn.
+template <bool REV>
+__device__ __forceinline__ void sum_decays(const float *g, long long stride, long long n, int pieces, DecayTables *tables,
+                                           uint32_t full0, uint32_t free0, volatile int *failed)
+{
+    const int lane = threadIdx.x & 31;
+    for (int i = 0; i < pieces; ++i) {
+        const long long t0 = (long long)(REV ? pieces - 1 - i : i) * kPiece;
+        const int m = (int)(n - t0 < kPiece ? n - t0 : kPiece);
+        double c[4];
+        double sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int t = lane * 4 + j;
+            float x = t < m ? g[(t0 + t) * stride] : 0.f;
+            x = x < -100.f ? -100.f : x;   // exp(-100) is 0 in 32 bits already; keeps sums finite, lets a NaN through
+            sum += (double)x * 1.4426950408889634;
+            c[j] = sum;
+        }
+        double before = sum;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const double up = __shfl_up_sync(0xffffffffu, before, s);
+            if (lane >= s) before += up;
+        }
+        const double end = __shfl_sync(0xffffffffu, before, 31);
+        before -= sum;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[j] = REV ? end - (before + c[j]) : before + c[j];
+        // the low end of each block of 32 steps: its last step, or, in reverse, its first
+        const double low = __shfl_sync(0xffffffffu, REV ? c[0] : c[3], REV ? (lane & ~7) : (lane | 7));
+        bool ok = i < 2 || bar_wait(free0 + 8 * (i & 1), ((i >> 1) & 1) ^ 1, failed);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        DecayTables &d = tables[i & 1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int t = lane * 4 + j;
+            const float la = (float)(c[j] - low);
+            d.a[t] = c[j];
+            d.la[t] = la;
+            d.cf[t] = exp2f(-la);
+            d.tail[t] = exp2f((float)(end - c[j]));
+            d.head[t] = exp2f((float)c[j]);
+        }
+        if (lane == 0) d.keep = exp2f((float)end);
+        __syncwarp();
+        if (lane == 0) bar_arrive(full0 + 8 * (i & 1));
+    }
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiled encoder()
+{
+    static const EncodeTiled fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult st;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &st) != cudaSuccess ||
+            st != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return fn;
+}
+
+// (d, heads, L, B) of values of a type; a box is one row of 128 bytes of one head at 128 time steps.
+inline bool encode(CUtensorMap *map, const SweepOperand &o, const Sweep &a, int d, int dtype)
+{
+    const int size = dtype == PSIG_F32 ? 4 : 2;
+    const long long heads = a.H / o.share;
+    const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)a.L, (cuuint64_t)a.B};
+    // the stride of a dimension of one element is never used, but has to be a valid one
+    auto bytes = [&](long long stride, long long n) { return (cuuint64_t)(n > 1 ? stride * size : (d * size + 15) / 16 * 16); };
+    const cuuint64_t strides[3] = {bytes(o.stride[2], heads), bytes(o.stride[1], a.L), bytes(o.stride[0], a.B)};
+    const cuuint32_t box[4] = {(cuuint32_t)(128 / size), 1, kPiece, 1}, unit[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType type = dtype == PSIG_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                     : dtype == PSIG_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    auto call = [&] {
+        return encoder()(map, type, 4, const_cast<void *>(o.data), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    if (call() == CUDA_SUCCESS) return true;
+    // a thread that has made no runtime call yet (autograd's) has no current context, which the driver call wants
+    int device = 0;
+    return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess && call() == CUDA_SUCCESS;
+}
+
+bool operand_fits(const SweepOperand &o, const Sweep &a, int d, int size)
+{
+    const int unit = 16 / size;   // TMA wants 16-byte addresses, strides and rows
+    if (d % unit != 0 || (reinterpret_cast<uintptr_t>(o.data) & 15) != 0) return false;
+    const long long sizes[3] = {a.B, a.L, a.H / o.share};
+    for (int i = 0; i < 3; ++i)
+        if (sizes[i] > 1 && (o.stride[i] <= 0 || o.stride[i] % unit != 0 || o.stride[i] >= (1LL << 37))) return false;
+    return true;
+}
+
+}  // namespace
+}  // namespace psig
