@@ -555,7 +555,8 @@ int run_backward_tiles(const Call &c, const void *init, const void *gs, void *gr
         if ((rc = sum_heads<T>(ws + at.gv, grad_v, kv_rows, c.share, d.dv, stream)) != PSIG_OK) return rc;
     }
     if (grad_decay == nullptr) return PSIG_OK;
-    const PairSums pairs{x, y, 2 * tiles, 2 * tiles, rows};
+    const int arrays = attn_tile_dots(d.dtype) * tiles;
+    const PairSums pairs{x, y, arrays, arrays, rows};
     return decay_gradient<T, float>(c, pairs, reinterpret_cast<const typename Acc<T>::type *>(ws + at.dots), kTileDots * tiles,
                                     grad_decay, reinterpret_cast<double *>(ws + at.totals), stream);
 }

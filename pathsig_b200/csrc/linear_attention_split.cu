@@ -19,6 +19,9 @@ enum Barrier { kRaw, kRawV, kReady, kScores, kInc, kP, kO1, kEpi, kDecFull0, kDe
 
 using bf16 = __nv_bfloat16;
 
+constexpr int kCompute = 256;                 // compute threads
+constexpr int kTileThreads = kCompute + 64;   // + issuing warp + decay warp
+
 template <int NI, int PANELS, int LEVEL>
 struct SplitLayout {
     static constexpr int NP = LEVEL + 1, NS = LEVEL + 1, NV = 3;
@@ -127,17 +130,17 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
     if (tid == 0) {
         bar_init(bar(kRaw), 1);
         bar_init(bar(kRawV), 1);
-        bar_init(bar(kReady), kCompute);
+        bar_init(bar(kReady), kCompute / 32);
         bar_init(bar(kScores), 1);
         bar_init(bar(kInc), 1);
-        bar_init(bar(kP), kCompute);
+        bar_init(bar(kP), kCompute / 32);
         bar_init(bar(kO1), 1);
-        bar_init(bar(kEpi), kCompute);
+        bar_init(bar(kEpi), kCompute / 32);
         bar_init(bar(kDecFull0), 1);
         bar_init(bar(kDecFull1), 1);
-        bar_init(bar(kDecFree0), kCompute);
-        bar_init(bar(kDecFree1), kCompute);
-        bar_init(bar(kSwap), kCompute);
+        bar_init(bar(kDecFree0), kCompute / 32);
+        bar_init(bar(kDecFree1), kCompute / 32);
+        bar_init(bar(kSwap), kCompute / 32);
         *failed = 0;
         failed[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -153,12 +156,14 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
 
     if (warp == 8) {
         // ------------------------------------------------------------------ TMA and MMA, one thread
-        if (lane == 0 && pieces > 0) {
+        if (pieces > 0) {
+            const uint32_t lead = lane == 0, base16 = base >> 4;
             const int rh = h / a.r.share, kh = h / a.k.share, vh = h / a.v.share;
             const int halves = pieces * PANELS;
             auto start = [&](int piece) { return (REV ? pieces - 1 - piece : piece) * kPiece; };
             constexpr int per_box = 128 / (int)sizeof(T);
             auto load_rk = [&](int idx) {
+                if (!lead) return;
                 const int t0 = start(idx / PANELS), x0 = idx % PANELS * 64;
                 bar_expect(bar(kRaw), 2 * RAW_BOXES * kTileBytes);
 #pragma unroll
@@ -168,6 +173,7 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                 }
             };
             auto load_v = [&](int piece) {
+                if (!lead) return;
                 bar_expect(bar(kRawV), RAW_BOXES * kTileBytes);
 #pragma unroll
                 for (int p = 0; p < RAW_BOXES; ++p)
@@ -181,8 +187,8 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                 const uint32_t ph = i & 1;
                 for (int p = 0; p < PANELS && ok; ++p) {
                     const int idx = i * PANELS + p;
-                    ok = bar_wait(bar(kReady), idx & 1, failed);
-                    if (ok && p == 0 && i > 0) ok = bar_wait(bar(kO1), ph ^ 1, failed) && bar_wait(bar(kEpi), ph ^ 1, failed);
+                    ok = warp_wait(bar(kReady), idx & 1, failed);
+                    if (ok && p == 0 && i > 0) ok = warp_wait(bar(kO1), ph ^ 1, failed) && warp_wait(bar(kEpi), ph ^ 1, failed);
                     if (!ok) break;
                     fence_after();
                     bool add = p > 0;
@@ -191,17 +197,17 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                         if (const int x = pair_first(NI, NI, pair), y = pair_second(NI, NI, pair); x + y <= LEVEL)
 #pragma unroll
                             for (int j = 0; j < 4; ++j, add = true)
-                                mma_ss(tmem, tile_desc(base + Lay::r + x * kTileBytes + j * 32, 16),
-                                       tile_desc(base + Lay::k + y * kTileBytes + j * 32, 16), instr_desc<bf16>(128, false, false), add);
-                    if (p == PANELS - 1) mma_commit(bar(kScores));
+                                mma_ss(tmem, tile_desc(base16 + ((Lay::r + x * kTileBytes + j * 32) >> 4), 16),
+                                       tile_desc(base16 + ((Lay::k + y * kTileBytes + j * 32) >> 4), 16), instr_desc<bf16>(128, false, false), add, lead);
+                    if (p == PANELS - 1) mma_commit(bar(kScores), lead);
                     add = p > 0;
 #pragma unroll
                     for (int pair = 0; pair < NI * Lay::NS; ++pair)
                         if (const int x = pair_first(NI, Lay::NS, pair), y = pair_second(NI, Lay::NS, pair); x + y <= LEVEL)
 #pragma unroll
                             for (int j = 0; j < 4; ++j, add = true)
-                                mma_ss(tmem + Lay::c_o2, tile_desc(base + Lay::r + x * kTileBytes + j * 32, 16),
-                                       tile_desc(base + Lay::s + y * 8192 + j * 2048, kTileBytes), instr_desc<bf16>(64, false, true), add);
+                                mma_ss(tmem + Lay::c_o2, tile_desc(base16 + ((Lay::r + x * kTileBytes + j * 32) >> 4), 16),
+                                       tile_desc(base16 + ((Lay::s + y * 8192 + j * 2048) >> 4), kTileBytes), instr_desc<bf16>(64, false, true), add, lead);
                     add = false;
                     // the state's 64 rows twice (the distance of the second block is 0), so that all lanes hold some
 #pragma unroll
@@ -209,16 +215,16 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                         if (const int x = pair_first(NI, Lay::NV, pair), y = pair_second(NI, Lay::NV, pair); x + y <= 2)
 #pragma unroll
                             for (int j = 0; j < kPiece / 16; ++j, add = true)
-                                mma_ss(tmem + Lay::c_i + p * 64, tile_desc(base + Lay::k + x * kTileBytes + j * 2048, 0),
-                                       tile_desc(base + Lay::vw + y * kTileBytes + j * 2048, kTileBytes), instr_desc<bf16>(64, true, true), add);
-                    mma_commit(bar(kInc));
-                    ok = bar_wait(bar(kInc), idx & 1, failed);
+                                mma_ss(tmem + Lay::c_i + p * 64, tile_desc(base16 + ((Lay::k + x * kTileBytes + j * 2048) >> 4), 0),
+                                       tile_desc(base16 + ((Lay::vw + y * kTileBytes + j * 2048) >> 4), kTileBytes), instr_desc<bf16>(64, true, true), add, lead);
+                    mma_commit(bar(kInc), lead);
+                    ok = warp_wait(bar(kInc), idx & 1, failed);
                     if (ok && idx + 1 < halves) {
                         load_rk(idx + 1);
                         ++loaded;
                     }
                 }
-                ok = ok && bar_wait(bar(kP), ph, failed);
+                ok = ok && warp_wait(bar(kP), ph, failed);
                 if (!ok) break;
                 fence_after();
                 bool add = false;
@@ -228,12 +234,12 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
 #pragma unroll
                         for (int j = 0; j < kPiece / 16; ++j, add = true) {
                             const int col = x == 0 ? (j / 4) * 64 + (j % 4) * 8 : Lay::c_p + (x - 1) * 64 + j * 8;
-                            mma_ts(tmem + Lay::c_i, tmem + col, tile_desc(base + Lay::v + y * kTileBytes + j * 2048, kTileBytes),
-                                   instr_desc<bf16>(64, false, true), add);
+                            mma_ts(tmem + Lay::c_i, tmem + col, tile_desc(base16 + ((Lay::v + y * kTileBytes + j * 2048) >> 4), kTileBytes),
+                                   instr_desc<bf16>(64, false, true), add, lead);
                         }
-                mma_commit(bar(kO1));
+                mma_commit(bar(kO1), lead);
                 if (i + 1 < pieces) {
-                    ok = bar_wait(bar(kO1), ph, failed);
+                    ok = warp_wait(bar(kO1), ph, failed);
                     if (!ok) break;
                     load_v(i + 1);
                     ++loaded_v;
@@ -241,8 +247,8 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
             }
             if (*failed) {
                 // let what is in flight land before the block gives its memory back
-                bar_wait(bar(kRaw), (loaded - 1) & 1, failed + 1);
-                bar_wait(bar(kRawV), (loaded_v - 1) & 1, failed + 1);
+                warp_wait(bar(kRaw), (loaded - 1) & 1, failed + 1);
+                warp_wait(bar(kRawV), (loaded_v - 1) & 1, failed + 1);
             }
         }
         __syncwarp();
@@ -289,8 +295,8 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
         // float32: the terms of a row's one half overwrite the raw values of its other half, which another thread holds
         auto swap = [&]() {
             if constexpr (sizeof(T) != 4) return true;
-            bar_arrive(bar(kSwap));
-            return bar_wait(bar(kSwap), swaps++ & 1, failed);
+            warp_arrive(bar(kSwap));
+            return warp_wait(bar(kSwap), swaps++ & 1, failed);
         };
         bool ok = true;
         for (int i = 0; i < pieces; ++i) {
@@ -308,13 +314,13 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                 if (lane == 0) static_cast<float *>(a.anchor_dots)[((bh * segments + segment) * tiles + vt) * 8 + warp] = dot;
             }
             const DecayTables &d = tables[i & 1];
-            ok = bar_wait(bar(kDecFull0 + (i & 1)), (i >> 1) & 1, failed);
+            ok = warp_wait(bar(kDecFull0 + (i & 1)), (i >> 1) & 1, failed);
 #pragma unroll
             for (int p = 0; p < PANELS; ++p) {
                 const int idx = i * PANELS + p;
-                ok = ok && bar_wait(bar(kRaw), idx & 1, failed);   // all products of the half before are done, too
-                if (p == 0) ok = ok && bar_wait(bar(kRawV), ph, failed);
-                if (!__all_sync(0xffffffffu, ok)) break;
+                ok = ok && warp_wait(bar(kRaw), idx & 1, failed);   // all products of the half before are done, too
+                if (p == 0) ok = ok && warp_wait(bar(kRawV), ph, failed);
+                if (!ok) break;
                 {   // the state's half as an operand
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
@@ -336,7 +342,7 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                 read_raw<T>(smem + Lay::r, row, half, row < m, x);
                 read_raw<T>(smem + Lay::k, row, half, row < m, y);
                 ok = swap();
-                if (!__all_sync(0xffffffffu, ok)) break;
+                if (!ok) break;
                 write_terms<NI>(smem + Lay::r, kTileBytes, row, half * 4, x);
                 write_terms<NI>(smem + Lay::k, kTileBytes, row, half * 4, y);
                 if (p == 0) {
@@ -345,17 +351,17 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
 #pragma unroll
                     for (int j = 0; j < 32; ++j) y[j] = x[j] * w;
                     ok = swap();
-                    if (!__all_sync(0xffffffffu, ok)) break;
+                    if (!ok) break;
                     write_terms<NI>(smem + Lay::v, kTileBytes, row, half * 4, x);
                     write_terms<Lay::NV>(smem + Lay::vw, kTileBytes, row, half * 4, y);
                 }
                 fence_async();
-                bar_arrive(bar(kReady));
+                warp_arrive(bar(kReady));
             }
-            if (!__all_sync(0xffffffffu, ok)) break;
+            if (!ok) break;
             // P = scores, weighted
-            ok = bar_wait(bar(kScores), ph, failed);
-            if (!__all_sync(0xffffffffu, ok)) break;
+            ok = warp_wait(bar(kScores), ph, failed);
+            if (!ok) break;
             fence_after();
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -395,8 +401,8 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
             }
             tmem_stored();
             // the state behind the piece
-            ok = bar_wait(bar(kInc), (i * PANELS + PANELS - 1) & 1, failed);
-            if (!__all_sync(0xffffffffu, ok)) break;
+            ok = warp_wait(bar(kInc), (i * PANELS + PANELS - 1) & 1, failed);
+            if (!ok) break;
             fence_after();
 #pragma unroll
             for (int p = 0; p < PANELS; ++p) {
@@ -407,15 +413,15 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                 for (int j = 0; j < 16; ++j) S[p][j] = fmaf(S[p][j], d.keep, x[j] * kv_scale);
             }
             fence_before();
-            bar_arrive(bar(kP));
+            warp_arrive(bar(kP));
             if (!REV && a.anchors != nullptr && boundary) {
                 float *anchor = static_cast<float *>(a.anchors) + (bh * segments + (end - 1) / kSegment) * a.d1 * a.d2;
                 all_state([&](float v, long long at, long long) { anchor[at] = v; });
             }
             // out
             const float head = d.head[row];
-            ok = bar_wait(bar(kO1), ph, failed);
-            if (!__all_sync(0xffffffffu, ok)) break;
+            ok = warp_wait(bar(kO1), ph, failed);
+            if (!ok) break;
             fence_after();
             const long long t = t0 + row;
             float dot = 0.f;
@@ -463,8 +469,8 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                 }
             }
             fence_before();
-            bar_arrive(bar(kEpi));
-            bar_arrive(bar(kDecFree0 + (i & 1)));
+            warp_arrive(bar(kEpi));
+            warp_arrive(bar(kDecFree0 + (i & 1)));
             if (dot_row != nullptr && t < a.L) a.dots[((long long)(vt * 2 + half) * a.B * a.L + b * a.L + t) * a.H + h] = dot;
         }
         // rows behind the last piece, and the last state

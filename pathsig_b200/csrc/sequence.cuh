@@ -75,7 +75,7 @@ struct Sweep {
     void *anchors;        // (B, H, segments, d1, d2)
     void *anchor_dots;    // (B, H, segments, parts of the sum)
     // Tensor-core sweeps only: the unrounded output row times the row of a third operand, summed over each block's and
-    // each warp's columns: (2 * column tiles of 64, B, L, H).
+    // each warp's columns: (attn_tile_dots * column tiles of 64, B, L, H).
     SweepOperand dot;
     float *dots;
 };
@@ -90,6 +90,7 @@ int attn_sweep_split(const Sweep &a, bool exact, int dtype, cudaStream_t stream)
 long long attn_tile_timeouts();
 long long attn_split_timeouts();
 long long norm_timeouts();
+inline int attn_tile_dots(int dtype) { return dtype == PSIG_BF16 ? 1 : 2; }   // at most 2
 constexpr int kTileDots = 8;   // parts of an anchor's sum per column tile of 64
 inline int tile_columns(int d2) { return (d2 + 63) / 64; }
 

@@ -24,10 +24,9 @@ __device__ unsigned long long g_tile_timeouts;   // of the translation unit
 }
 
 constexpr int kPiece = 128;
-constexpr int kCompute = 256;                 // compute threads
-constexpr int kTileThreads = kCompute + 64;   // + issuing warp + decay warp
 constexpr int kTileBytes = kPiece * 128;      // 128 rows of 64 16-bit values
-constexpr unsigned kWaitPolls = 1u << 22;     // each poll blocks for a hardware-defined time at most
+constexpr unsigned kWaitPolls = 1u << 22;     // of at most kPollTime each: two to three seconds
+constexpr unsigned kPollTime = 10000;         // ns a poll may sleep; warps that spin take issue slots and instruction cache from others
 
 struct DecayTables {       // of one piece; all exponents are of 2
     double a[kPiece];      // a_t
@@ -55,6 +54,7 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes)
 // Waits for the phase of this parity; false when the bound ran out here or in another thread of the block.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *failed)
 {
+#pragma unroll 1
     for (unsigned i = 0; i < kWaitPolls; ++i) {
         uint32_t ok;
         asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
@@ -64,6 +64,17 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     }
     if (atomicExch(const_cast<int *>(failed), 1) == 0) atomicAdd(&g_tile_timeouts, 1ull);
     return false;
+}
+// For a whole warp: one lane polls, and one arrives (all lanes' work before it).  An mbarrier operation of 32 lanes
+// is 32 operations on one word, one after the other: a wait for a phase long past took 250 cycles that way.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *failed)
+{
+    return __all_sync(0xffffffffu, bar_wait(bar, parity, failed));
+}
+__device__ __forceinline__ void warp_arrive(uint32_t bar)
+{
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) bar_arrive(bar);
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -75,35 +86,40 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, u
                  ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(head), "r"(t), "r"(b) : "memory");
 }
 
-// Shared-memory matrix descriptor, 128-byte swizzle.  Rows of 128 bytes, eight rows (1024 bytes) to a swizzle
-// atom; `lead` is the distance of neighbouring 64-element blocks where the row runs along M or N.
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lead)
+// Shared-memory matrix descriptor, 128-byte swizzle, from an address in units of 16 bytes.  Rows of 128 bytes, eight
+// rows (1024 bytes) to a swizzle atom; `lead` (bytes) is the distance of neighbouring 64-element blocks where the row
+// runs along M or N.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr16, uint32_t lead)
 {
-    return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(addr16 | (lead >> 4) << 16), "r"((1024u >> 4) | 1u << 14 | 2u << 29));
+    return d;
 }
 template <typename T>
 __device__ __forceinline__ constexpr uint32_t instr_desc(int n, bool a_rows_along_m, bool b_rows_along_n)
 {
-    const uint32_t type = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     return (1u << 4) | (type << 7) | (type << 10) | ((a_rows_along_m ? 1u : 0u) << 15) | ((b_rows_along_n ? 1u : 0u) << 16) |
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
+// Matrix instructions run in the one thread of the warp with `lead` set, but the warp stays together: the operands are then
+// uniform, and issuing one takes a handful of cycles (from a branch of a single thread it took 55 to 65).
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add, uint32_t lead)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(lead) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add, uint32_t lead)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(lead) : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint32_t bar)
+__device__ __forceinline__ void mma_commit(uint32_t bar, uint32_t lead)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead) : "memory");
 }
 __device__ __forceinline__ void tmem_load16(uint32_t addr, float (&x)[16])
 {
@@ -112,6 +128,12 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, float (&x)[16])
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
                    "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(addr));
+}
+__device__ __forceinline__ void tmem_load8(uint32_t addr, float (&x)[8])
+{
+    uint32_t *r = reinterpret_cast<uint32_t *>(x);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(addr));
 }
 __device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t (&r)[8])
 {
@@ -147,6 +169,15 @@ __device__ __forceinline__ uint32_t next_term(float &x, float &y, bool last)
     return p;
 }
 
+__device__ __forceinline__ void tma_store(uint32_t src, const CUtensorMap *map, int x, int head, int t, int b)
+{
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+                 ::"l"(map), "r"(src), "r"(x), "r"(head), "r"(t), "r"(b) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void tma_store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 __device__ __forceinline__ uint32_t swizzled(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
 
 // One warp: the decay tables of the sweep's pieces, one piece ahead of their use, in two buffers in turn.
@@ -155,6 +186,7 @@ __device__ __forceinline__ void sum_decays(const float *g, long long stride, lon
                                            uint32_t full0, uint32_t free0, volatile int *failed)
 {
     const int lane = threadIdx.x & 31;
+#pragma unroll 1
     for (int i = 0; i < pieces; ++i) {
         const long long t0 = (long long)(REV ? pieces - 1 - i : i) * kPiece;
         const int m = (int)(n - t0 < kPiece ? n - t0 : kPiece);
@@ -180,8 +212,7 @@ __device__ __forceinline__ void sum_decays(const float *g, long long stride, lon
         for (int j = 0; j < 4; ++j) c[j] = REV ? end - (before + c[j]) : before + c[j];
         // the low end of each block of 32 steps: its last step, or, in reverse, its first
         const double low = __shfl_sync(0xffffffffu, REV ? c[0] : c[3], REV ? (lane & ~7) : (lane | 7));
-        bool ok = i < 2 || bar_wait(free0 + 8 * (i & 1), ((i >> 1) & 1) ^ 1, failed);
-        if (!__all_sync(0xffffffffu, ok)) break;
+        if (i >= 2 && !warp_wait(free0 + 8 * (i & 1), ((i >> 1) & 1) ^ 1, failed)) break;
         DecayTables &d = tables[i & 1];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -189,13 +220,12 @@ __device__ __forceinline__ void sum_decays(const float *g, long long stride, lon
             const float la = (float)(c[j] - low);
             d.a[t] = c[j];
             d.la[t] = la;
-            d.cf[t] = exp2f(-la);
-            d.tail[t] = exp2f((float)(end - c[j]));
-            d.head[t] = exp2f((float)c[j]);
+            d.cf[t] = exp_two(-la);
+            d.tail[t] = exp_two((float)(end - c[j]));
+            d.head[t] = exp_two((float)c[j]);
         }
-        if (lane == 0) d.keep = exp2f((float)end);
-        __syncwarp();
-        if (lane == 0) bar_arrive(full0 + 8 * (i & 1));
+        if (lane == 0) d.keep = exp_two((float)end);
+            warp_arrive(full0 + 8 * (i & 1));
     }
 }
 
