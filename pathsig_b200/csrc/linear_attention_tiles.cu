@@ -31,7 +31,7 @@ constexpr int kStateThreads = 256, kScoreThreads = 256, kOutThreads = 128;
 constexpr int kTileThreads = kStateThreads + kScoreThreads + kOutThreads + 96;
 
 enum Barrier {
-    kFullRK, kFullV0, kFullV1, kVReady, kScores, kInc, kP, kO1, kEpi, kFix, kOutFull, kOutFree,
+    kFullRK, kFullV0, kFullV1, kVReady, kScores, kInc, kP, kO1, kEpi, kFix, kOutFull, kOutFree, kDot,
     kDecFull0, kDecFull1, kDecFree0, kDecFree1, kBarriers
 };
 
@@ -60,7 +60,8 @@ struct TileLayout {
 template <typename T, int KP, int NP, int NS, int NV, bool REV>
 __global__ void __launch_bounds__(kTileThreads, 1)
 attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_k,
-                 const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_out, const Sweep a)
+                 const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_out,
+                 const __grid_constant__ CUtensorMap map_dot, const Sweep a)
 {
     using Lay = TileLayout<KP, NP, NS, NV>;
     extern __shared__ __align__(1024) unsigned char smem[];   // the swizzle atoms start on 1024-byte boundaries
@@ -97,6 +98,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
         bar_init(bar(kFix), kStateThreads / 32);
         bar_init(bar(kOutFull), kOutThreads / 32);
         bar_init(bar(kOutFree), 1);
+        bar_init(bar(kDot), 1);
         for (int i = 0; i < 2; ++i) {
             bar_init(bar(kDecFull0 + i), 1);
             bar_init(bar(kDecFree0 + i), (kStateThreads + kScoreThreads + kOutThreads) / 32);
@@ -187,8 +189,8 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                 warp_arrive(bar(kFix));
             }
             const float w = d.tail[row], keep = d.keep;
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {   // not unrolled, like the loops below: the roles' code has to stay in the instruction cache
+#pragma unroll 2
+            for (int c = 0; c < 4; ++c) {   // not wholly unrolled, like the loop over the scores: the roles' code has to stay in the instruction cache
                 const uint32_t at = swizzled(row, half * 4 + c);
                 const uint4 in = *reinterpret_cast<const uint4 *>(v_tile + at);
                 float2 x[4] = {unpack(in.x, T{}), unpack(in.y, T{}), unpack(in.z, T{}), unpack(in.w, T{})};
@@ -292,12 +294,18 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
         }
     } else if (warp < 20) {
         // ------------------------------------------------------------------ out
+        // The third operand of the decay gradient comes by TMA into the tile that the output leaves by: a thread reads its 16
+        // bytes there and writes its output over them.
         T *out_t = static_cast<T *>(a.out);
         float *out_f = static_cast<float *>(a.out);
-        const T *dot_row = static_cast<const T *>(a.dot.data);
-        if (dot_row != nullptr) dot_row += b * a.dot.stride[0] + (h / a.dot.share) * a.dot.stride[2];
-        const bool writer = tid == kStateThreads + kScoreThreads;   // starts the copies of the output tiles
+        const bool with_dot = a.dot.data != nullptr, staged = !a.out_acc;
+        const bool writer = tid == kStateThreads + kScoreThreads;   // starts the copies of these tiles
         const int col0 = vt * 64;
+        auto load_dot = [&](int i) {
+            bar_expect(bar(kDot), kTileBytes);
+            tma_load(base + Lay::out, &map_dot, bar(kDot), col0, h / a.dot.share, (int)piece_start(i), (int)b);
+        };
+        if (writer && with_dot && pieces > 0) load_dot(0);
 #pragma unroll 1
         for (int i = 0; i < pieces; ++i) {
             const long long t0 = piece_start(i), t = t0 + row;
@@ -305,57 +313,61 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
             if (!warp_wait(bar(kDecFull0 + (i & 1)), (i >> 1) & 1, failed)) break;
             const float f1 = (float)(a.out_scale * a.kv_scale), f2 = (float)a.out_scale * tables[i & 1].head[row];
             warp_arrive(bar(kDecFree0 + (i & 1)));
-            if (!a.out_acc && i > 0) {
-                if (writer) {
-                    tma_store_read();
-                    bar_arrive(bar(kOutFree));
-                }
-                if (!warp_wait(bar(kOutFree), (i - 1) & 1, failed)) break;
-            }
+            if (staged && !with_dot && i > 0 && !warp_wait(bar(kOutFree), (i - 1) & 1, failed)) break;
+            if (with_dot && !warp_wait(bar(kDot), i & 1, failed)) break;   // loaded behind the last store's reads
             if (!warp_wait(bar(kO1), i & 1, failed)) break;
             fence_after();
             float dot = 0.f;
 #pragma unroll 1
-            for (int c = 0; c < 8; ++c) {   // 8 columns each
-                const int col = col0 + c * 8;
-                uint4 w = {0, 0, 0, 0};
-                if (dot_row != nullptr && row < m && col < a.d2) w = *reinterpret_cast<const uint4 *>(dot_row + t * a.dot.stride[1] + col);
-                float x[8], y[8];
-                tmem_load8(tmem + lanes + Lay::c_o1 + c * 8, x);
-                tmem_load8(tmem + lanes + Lay::c_o2 + c * 8, y);
+            for (int c = 0; c < 4; ++c) {   // 16 columns each
+                float u[16], w[16];
+                tmem_load16(tmem + lanes + Lay::c_o1 + c * 16, u);
+                tmem_load16(tmem + lanes + Lay::c_o2 + c * 16, w);
                 tmem_loaded();
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = row < m ? fmaf(x[j], f1, y[j] * f2) : 0.f;
-                if (!a.out_acc) {
-                    uint4 o;
-                    o.x = pack(x[0], x[1], T{});
-                    o.y = pack(x[2], x[3], T{});
-                    o.z = pack(x[4], x[5], T{});
-                    o.w = pack(x[6], x[7], T{});
-                    *reinterpret_cast<uint4 *>(smem + Lay::out + swizzled(row, c)) = o;
-                } else if (t < a.L && col < a.d2) {
-                    float *at = out_f + ((b * a.L + t) * a.H + h) * a.d2 + col;
-                    *reinterpret_cast<float4 *>(at) = make_float4(x[0], x[1], x[2], x[3]);
-                    *reinterpret_cast<float4 *>(at + 4) = make_float4(x[4], x[5], x[6], x[7]);
-                }
-                if (dot_row != nullptr) {
-                    const float2 two[4] = {unpack(w.x, T{}), unpack(w.y, T{}), unpack(w.z, T{}), unpack(w.w, T{})};
+                for (int j = 0; j < 16; ++j) u[j] = row < m ? fmaf(u[j], f1, w[j] * f2) : 0.f;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) dot += x[2 * j] * two[j].x + x[2 * j + 1] * two[j].y;
+                for (int e = 0; e < 16; e += 8) {
+                    uint4 *tile = reinterpret_cast<uint4 *>(smem + Lay::out + swizzled(row, c * 2 + e / 8));
+                    if (with_dot && row < m) {
+                        const uint4 p = *tile;
+                        const float2 two[4] = {unpack(p.x, T{}), unpack(p.y, T{}), unpack(p.z, T{}), unpack(p.w, T{})};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) dot += u[e + 2 * j] * two[j].x + u[e + 2 * j + 1] * two[j].y;
+                    }
+                    const int col = col0 + c * 16 + e;
+                    if (staged) {
+                        uint4 o;
+                        o.x = pack(u[e], u[e + 1], T{});
+                        o.y = pack(u[e + 2], u[e + 3], T{});
+                        o.z = pack(u[e + 4], u[e + 5], T{});
+                        o.w = pack(u[e + 6], u[e + 7], T{});
+                        *tile = o;
+                    } else if (t < a.L && col < a.d2) {
+                        float *at = out_f + ((b * a.L + t) * a.H + h) * a.d2 + col;
+                        *reinterpret_cast<float4 *>(at) = make_float4(u[e], u[e + 1], u[e + 2], u[e + 3]);
+                        *reinterpret_cast<float4 *>(at + 4) = make_float4(u[e + 4], u[e + 5], u[e + 6], u[e + 7]);
+                    }
                 }
             }
             fence_before();
             warp_arrive(bar(kEpi));
-            if (!a.out_acc) {
-                fence_async();
-                warp_arrive(bar(kOutFull));
-                if (writer) {
-                    // steps behind the tensor's end and columns behind its rows are not written
-                    if (bar_wait(bar(kOutFull), i & 1, failed)) tma_store(base + Lay::out, &map_out, col0, h, (int)t0, (int)b);
+            fence_async();
+            warp_arrive(bar(kOutFull));
+            if (writer && bar_wait(bar(kOutFull), i & 1, failed)) {
+                // steps behind the tensor's end and columns behind its rows are not written
+                if (staged) {
+                    tma_store(base + Lay::out, &map_out, col0, h, (int)t0, (int)b);
+                    tma_store_read();
                 }
-                __syncwarp();
+                if (with_dot) {
+                    if (i + 1 < pieces) load_dot(i + 1);
+                } else {
+                    bar_arrive(bar(kOutFree));
+                }
             }
-            if (dot_row != nullptr && t < a.L) a.dots[((long long)vt * a.B * a.L + b * a.L + t) * a.H + h] = dot;
+            __syncwarp();
+            if (with_dot && t < a.L) a.dots[((long long)vt * a.B * a.L + b * a.L + t) * a.H + h] = dot;
         }
         // rows behind the last piece
         const long long first = (long long)pieces * kPiece;
@@ -368,10 +380,11 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
             *reinterpret_cast<uint4 *>(a.out_acc ? (void *)(out_f + at) : (void *)(out_t + at)) = zero;
             if (a.out_acc) *reinterpret_cast<uint4 *>(out_f + at + 4) = zero;
         }
-        if (dot_row != nullptr)
+        if (with_dot)
             for (long long t = first + tid - (kStateThreads + kScoreThreads); t < a.L; t += kOutThreads)
                 a.dots[((long long)vt * a.B * a.L + b * a.L + t) * a.H + h] = 0.f;
         if (writer) tma_store_done();
+        if (writer && with_dot && *failed) bar_wait(bar(kDot), (pieces - 1) & 1, failed + 1);
     } else if (warp == 20) {
         // ------------------------------------------------------------------ TMA and MMA
         if (pieces > 0) {
@@ -487,15 +500,16 @@ template <typename T, int KP, int NP, int NS, int NV, bool REV>
 int launch_tiles(const Sweep &a, int dtype, cudaStream_t stream)
 {
     using Lay = TileLayout<KP, NP, NS, NV>;
-    CUtensorMap r, k, v, out;
+    CUtensorMap r, k, v, out, dot;
     const SweepOperand o{a.out, {a.L * a.H * a.d2, (long long)a.H * a.d2, a.d2}, 1};
     if (encoder() == nullptr || !encode(&r, a.r, a, a.d1, dtype) || !encode(&k, a.k, a, a.d1, dtype) ||
-        !encode(&v, a.v, a, a.d2, dtype) || !encode(&out, o, a, a.d2, dtype))
+        !encode(&v, a.v, a, a.d2, dtype) || !encode(&out, o, a, a.d2, dtype) ||
+        !encode(&dot, a.dot.data ? a.dot : o, a, a.d2, dtype))
         return PSIG_ERR_CUDA;
     auto kernel = attn_sweep_tiles<T, KP, NP, NS, NV, REV>;
     if (!prepare_kernel(kernel, Lay::alloc, true)) return PSIG_ERR_CUDA;
     const long long blocks = a.B * a.H * ((a.d2 + 63) / 64);
-    kernel<<<(unsigned)blocks, kTileThreads, Lay::alloc, stream>>>(r, k, v, out, a);
+    kernel<<<(unsigned)blocks, kTileThreads, Lay::alloc, stream>>>(r, k, v, out, dot, a);
     return check_launch();
 }
 
