@@ -460,7 +460,8 @@ BackwardScratch backward_scratch(const PsigAttnDesc &d)
     s.gv = take(acc * rows * d.dv);
     const long long pair_bytes = 4 * 4 * tile_columns(d.dk);   // the tiles' two sets of two float arrays per column tile
     s.pairs = take((pair_bytes > 8 ? pair_bytes : 8) * rows);
-    s.anchors = take(acc * bh * seg * d.dk * d.dv);
+    // the tensor-core sweeps store whole tiles of 64 by 64
+    s.anchors = take(acc * bh * seg * ((d.dk + 63) / 64 * 64) * ((d.dv + 63) / 64 * 64));
     s.dots = take(acc * bh * seg * anchor_parts(d));
     s.totals = take(8 * bh * seg);
     s.bytes = at;

@@ -307,9 +307,12 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
             const bool boundary = end == n || end % kSegment == 0;
             if (REV && a.anchor_dots != nullptr && boundary) {
                 const long long segment = (end - 1) / kSegment;
-                const float *anchor = static_cast<const float *>(a.anchors) + (bh * segments + segment) * a.d1 * a.d2;
+                const float *anchor = static_cast<const float *>(a.anchors) + ((bh * segments + segment) * tiles + vt) * PANELS * 4096 + tid;
                 float dot = 0.f;
-                all_state([&](float v, long long at, long long) { dot += v * anchor[at]; });
+#pragma unroll
+                for (int p = 0; p < PANELS; ++p)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) dot = fmaf(S[p][j], anchor[(p * 16 + j) * kCompute], dot);
                 for (int s = 16; s >= 1; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
                 if (lane == 0) static_cast<float *>(a.anchor_dots)[((bh * segments + segment) * tiles + vt) * 8 + warp] = dot;
             }
@@ -415,8 +418,12 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
             fence_before();
             warp_arrive(bar(kP));
             if (!REV && a.anchors != nullptr && boundary) {
-                float *anchor = static_cast<float *>(a.anchors) + (bh * segments + (end - 1) / kSegment) * a.d1 * a.d2;
-                all_state([&](float v, long long at, long long) { anchor[at] = v; });
+                // in the threads' own order: the sweep that reads them has the same threads
+                float *anchor = static_cast<float *>(a.anchors) + ((bh * segments + (end - 1) / kSegment) * tiles + vt) * PANELS * 4096 + tid;
+#pragma unroll
+                for (int p = 0; p < PANELS; ++p)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) anchor[(p * 16 + j) * kCompute] = S[p][j];
             }
             // out
             const float head = d.head[row];

@@ -8,11 +8,17 @@
 // All run as tcgen05.mma with M = 128 and fp32 accumulators in tensor memory; R, K, V come by TMA into 128-byte
 // swizzled tiles, in which K and V serve both as they are and transposed (the descriptor's major bit).
 //
-// Rounding.  The products take 16-bit operands, exact for R, K and V.  P, S and V' are computed in 32 bits and
-// enter as a sum of NP, NS and NV 16-bit terms (the value, what its rounding left, what that left): one term where
-// only a 16-bit output depends on it, three (24 bits) where a 32-bit result does: the state itself, and the decay
+// Rounding.  The products take 16-bit operands, exact for R, K and V.  P, S and V' are computed in 32 bits.  P enters
+// rounded once: only the 16-bit output depends on it.  S and V' enter as a sum of NS and NV 16-bit terms (the value, what
+// its rounding left, what that left): three (24 bits) where a 32-bit result depends on them, the state itself or the decay
 // gradient.  The state lives in registers in 32 bits and is never rounded but for its copy as an operand.  Sums of
 // decays are in 64 bits, so that a weight exp(a_t - a_s) does not lose the difference of two long sums.
+//
+// DOT: the sweep also gives x_t = out_t . y_t for the rows y of a third operand, to 32 bits (the decay gradient needs
+// q . grad_q and k . grad_k).  The part of the piece's own pairs is sum_s exp(a_t - a_s) (r_t . k_s) (y_t . v_s), the
+// weighted scores times a second product Y V^T, entry by entry before anything is rounded; the state's part is
+// exp(a_t) (r_t^T S) . y_t.  (With the output row itself, P would have to enter as three terms: 380 us against
+// the time in launch_tiles.)
 //
 // Warps, so that a piece's stages overlap with the neighbouring pieces': 8 hold the state and weigh V (thread = state
 // row, and = time step), 8 weigh the scores, 4 write the output, one each issues the products, starts the copies, and sums the next piece's decays.
@@ -31,39 +37,42 @@ constexpr int kStateThreads = 256, kScoreThreads = 256, kOutThreads = 128;
 constexpr int kTileThreads = kStateThreads + kScoreThreads + kOutThreads + 96;
 
 enum Barrier {
-    kFullRK, kFullV0, kFullV1, kVReady, kScores, kInc, kP, kO1, kEpi, kFix, kOutFull, kOutFree, kDot,
+    kFullRK, kFullV0, kFullV1, kVReady, kScores, kInc, kP, kO1, kEpi, kFix, kOutFull, kOutFree, kDot, kDotFree,
     kDecFull0, kDecFull1, kDecFree0, kDecFree1, kBarriers
 };
 
-template <int KP, int NP, int NS, int NV>
+template <int KP, int NS, int NV, bool DOT>
 struct TileLayout {
     static constexpr int panels = KP / 64;
+    static constexpr int VS = DOT ? 1 : 2;                  // pieces of V in turn (shared memory is full with DOT)
     static constexpr int r = 0;
     static constexpr int k = r + panels * kTileBytes;
-    static constexpr int v = k + panels * kTileBytes;       // two pieces in turn
-    static constexpr int vw = v + 2 * kTileBytes;           // V' terms
+    static constexpr int v = k + panels * kTileBytes;
+    static constexpr int vw = v + VS * kTileBytes;          // V' terms
     static constexpr int s = vw + NV * kTileBytes;          // state terms, KP rows of 128 bytes
     static constexpr int out = s + NS * KP * 128;           // the output tile on its way out
-    static constexpr int decay = out + kTileBytes;
-    static constexpr int bars = decay + 2 * (int)sizeof(DecayTables);
+    static constexpr int dot = out + kTileBytes;            // the third operand's tile
+    static constexpr int decay = dot + (DOT ? kTileBytes : 0);
+    static constexpr int sums = decay + 2 * (int)sizeof(DecayTables);   // [2 pieces][2 halves][128] sums of pairs
+    static constexpr int bars = sums + (DOT ? 4 * kPiece * 4 : 0);
     static constexpr int tmem = bars + kBarriers * 8;
     static constexpr int alloc = tmem + 16;
-    // tensor memory columns: scores (P's first term takes the columns its own thread has read), the further terms
-    // of P, O2, I and O1
-    static constexpr int c_p = 128;
-    static constexpr int c_o2 = 128 + (NP - 1) * 64;
+    // tensor memory columns: scores (P takes the columns its own thread has read), the second scores, O2, I and O1
+    static constexpr int c_two = 128;
+    static constexpr int c_o2 = DOT ? 256 : 128;
     static constexpr int c_i = c_o2 + 64;
     static constexpr int c_o1 = c_i + 64;
     static constexpr int columns = 512;
 };
 
-template <typename T, int KP, int NP, int NS, int NV, bool REV>
+template <typename T, int KP, int NS, int NV, bool DOT, bool REV>
 __global__ void __launch_bounds__(kTileThreads, 1)
 attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_out,
                  const __grid_constant__ CUtensorMap map_dot, const Sweep a)
 {
-    using Lay = TileLayout<KP, NP, NS, NV>;
+    using Lay = TileLayout<KP, NS, NV, DOT>;
+    constexpr int VS = Lay::VS;
     extern __shared__ __align__(1024) unsigned char smem[];   // the swizzle atoms start on 1024-byte boundaries
     const uint32_t base = shared_addr(smem);
     DecayTables *tables = reinterpret_cast<DecayTables *>(smem + Lay::decay);
@@ -99,6 +108,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
         bar_init(bar(kOutFull), kOutThreads / 32);
         bar_init(bar(kOutFree), 1);
         bar_init(bar(kDot), 1);
+        bar_init(bar(kDotFree), kOutThreads / 32);
         for (int i = 0; i < 2; ++i) {
             bar_init(bar(kDecFull0 + i), 1);
             bar_init(bar(kDecFree0 + i), (kStateThreads + kScoreThreads + kOutThreads) / 32);
@@ -116,6 +126,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
     // All columns are ours, so they start at 0: as a constant it costs the issuing warp no register moves per product.
     constexpr uint32_t tmem = 0;
     if (tid == 0 && (*tmem_slot != 0 || (base & 1023) != 0)) *failed = 1, atomicAdd(&g_tile_timeouts, 1ull);
+    float *sums = reinterpret_cast<float *>(smem + Lay::sums);
     const int quarter = warp & 3, half = (warp >> 2) & 1;
     const int row = quarter * 32 + lane;                 // time step in the piece, or lane of tensor memory
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
@@ -169,9 +180,9 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
             const bool boundary = end == n || end % kSegment == 0;
             const DecayTables &d = tables[i & 1];
             if (!warp_wait(bar(kDecFull0 + (i & 1)), (i >> 1) & 1, failed)) break;
-            if (!warp_wait(bar(kFullV0 + (i & 1)), (i >> 1) & 1, failed)) break;
+            if (!warp_wait(bar(kFullV0 + i % VS), (i / VS) & 1, failed)) break;
             const bool fix = a.lengths != nullptr && m < kPiece;
-            unsigned char *v_tile = smem + Lay::v + (i & 1) * kTileBytes;
+            unsigned char *v_tile = smem + Lay::v + (i % VS) * kTileBytes;
             if (fix) {
                 if (!warp_wait(bar(kFullRK), ph, failed)) break;
                 if (row >= m) {
@@ -212,9 +223,10 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
             if (REV && a.anchor_dots != nullptr && boundary) {
                 // the state behind this piece against the stored state of the steps up to here
                 const long long segment = (end - 1) / kSegment;
+                const float *anchor = static_cast<const float *>(a.anchors) + ((bh * segments + segment) * tiles + vt) * KP * 64 + tid;
                 float dot = 0.f;
-                all_state(false, (bh * segments + segment) * a.d1 * a.d2,
-                          [&](float &v, long long at) { dot += v * static_cast<const float *>(a.anchors)[at]; });
+#pragma unroll
+                for (int j = 0; j < SC; ++j) dot = fmaf(S[j], anchor[j * kStateThreads], dot);
                 for (int s = 16; s >= 1; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
                 if (lane == 0) static_cast<float *>(a.anchor_dots)[((bh * segments + segment) * tiles + vt) * 8 + warp] = dot;
             }
@@ -227,9 +239,12 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
 #pragma unroll
             for (int j = 0; j < SC; ++j) S[j] = fmaf(S[j], keep, x[j / 16][j % 16] * kv_scale);
             store_terms();
-            if (!REV && a.anchors != nullptr && boundary)
-                all_state(false, (bh * segments + (end - 1) / kSegment) * a.d1 * a.d2,
-                          [&](float &v, long long at) { static_cast<float *>(a.anchors)[at] = v; });
+            if (!REV && a.anchors != nullptr && boundary) {
+                // in the threads' own order: the sweep that reads them has the same threads
+                float *anchor = static_cast<float *>(a.anchors) + ((bh * segments + (end - 1) / kSegment) * tiles + vt) * KP * 64 + tid;
+#pragma unroll
+                for (int j = 0; j < SC; ++j) anchor[j * kStateThreads] = S[j];
+            }
         }
         if (a.final != nullptr)
             all_state(a.final_transposed, state0, [&](float &v, long long at) { static_cast<float *>(a.final)[at] = v; });
@@ -246,12 +261,15 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
             for (int q = 0; q < 2; ++q) f[q] = exp_two((float)(d.a[row] - d.a[(half * 2 + q) * 32 + (REV ? 0 : 31)]));
             if (!warp_wait(bar(kScores), i & 1, failed)) break;
             fence_after();
+            float sum = 0.f;
 #pragma unroll 1
             for (int q = 0; q < 4; ++q) {   // 16 columns each
                 const int block = half * 2 + q / 2, s0 = half * 64 + q * 16;
-                float x[16];
+                uint32_t p[8];
                 if (REV ? block >= quarter : block <= quarter) {
+                    float x[16], y[16];
                     tmem_load16(own + q * 16, x);
+                    if (DOT) tmem_load16(own + Lay::c_two + q * 16, y);
                     const float4 *table = reinterpret_cast<const float4 *>((block == quarter ? d.la : d.cf) + s0);
                     float t[16];
 #pragma unroll
@@ -271,22 +289,19 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                     tmem_loaded();
                     // (weight 0 against a score that is not finite: only in rows behind the end, which nobody reads)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) x[j] *= t[j];
+                    for (int j = 0; j < 16; ++j) {
+                        x[j] *= t[j];
+                        if (DOT) sum = fmaf(x[j], y[j], sum);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) p[j] = pack(x[2 * j], x[2 * j + 1], T{});
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) x[j] = 0.f;
+                    for (int j = 0; j < 8; ++j) p[j] = 0;
                 }
-                uint32_t p0[8], p1[8], p2[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    p0[j] = next_term<T>(x[2 * j], x[2 * j + 1], NP == 1);
-                    if (NP > 1) p1[j] = next_term<T>(x[2 * j], x[2 * j + 1], NP == 2);
-                    if (NP > 2) p2[j] = next_term<T>(x[2 * j], x[2 * j + 1], NP == 3);
-                }
-                tmem_store8(own + q * 8, p0);
-                if (NP > 1) tmem_store8(tmem + lanes + Lay::c_p + half * 32 + q * 8, p1);
-                if (NP > 2) tmem_store8(tmem + lanes + Lay::c_p + 64 + half * 32 + q * 8, p2);
+                tmem_store8(own + q * 8, p);
             }
+            if (DOT) sums[((i & 1) * 2 + half) * kPiece + row] = sum;
             tmem_stored();
             fence_before();
             warp_arrive(bar(kP));
@@ -294,18 +309,11 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
         }
     } else if (warp < 20) {
         // ------------------------------------------------------------------ out
-        // The third operand of the decay gradient comes by TMA into the tile that the output leaves by: a thread reads its 16
-        // bytes there and writes its output over them.
         T *out_t = static_cast<T *>(a.out);
         float *out_f = static_cast<float *>(a.out);
-        const bool with_dot = a.dot.data != nullptr, staged = !a.out_acc;
-        const bool writer = tid == kStateThreads + kScoreThreads;   // starts the copies of these tiles
+        const bool staged = !a.out_acc;
+        const bool writer = tid == kStateThreads + kScoreThreads;   // starts the copies of the output tiles
         const int col0 = vt * 64;
-        auto load_dot = [&](int i) {
-            bar_expect(bar(kDot), kTileBytes);
-            tma_load(base + Lay::out, &map_dot, bar(kDot), col0, h / a.dot.share, (int)piece_start(i), (int)b);
-        };
-        if (writer && with_dot && pieces > 0) load_dot(0);
 #pragma unroll 1
         for (int i = 0; i < pieces; ++i) {
             const long long t0 = piece_start(i), t = t0 + row;
@@ -313,28 +321,37 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
             if (!warp_wait(bar(kDecFull0 + (i & 1)), (i >> 1) & 1, failed)) break;
             const float f1 = (float)(a.out_scale * a.kv_scale), f2 = (float)a.out_scale * tables[i & 1].head[row];
             warp_arrive(bar(kDecFree0 + (i & 1)));
-            if (staged && !with_dot && i > 0 && !warp_wait(bar(kOutFree), (i - 1) & 1, failed)) break;
-            if (with_dot && !warp_wait(bar(kDot), i & 1, failed)) break;   // loaded behind the last store's reads
+            uint4 y[DOT ? 8 : 1];
+            if (DOT) {
+                if (!warp_wait(bar(kDot), i & 1, failed)) break;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) y[DOT ? c : 0] = *reinterpret_cast<const uint4 *>(smem + Lay::dot + swizzled(row, c));
+                warp_arrive(bar(kDotFree));
+            }
+            if (staged && i > 0 && !warp_wait(bar(kOutFree), (i - 1) & 1, failed)) break;
             if (!warp_wait(bar(kO1), i & 1, failed)) break;
             fence_after();
             float dot = 0.f;
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {   // 16 columns each
+            auto columns = [&](int c, const uint4 &p0, const uint4 &p1) {   // 16 of them
                 float u[16], w[16];
                 tmem_load16(tmem + lanes + Lay::c_o1 + c * 16, u);
                 tmem_load16(tmem + lanes + Lay::c_o2 + c * 16, w);
                 tmem_loaded();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) u[j] = row < m ? fmaf(u[j], f1, w[j] * f2) : 0.f;
+                for (int j = 0; j < 16; ++j) {
+                    w[j] = row < m ? w[j] * f2 : 0.f;
+                    u[j] = row < m ? fmaf(u[j], f1, w[j]) : 0.f;
+                }
+                if (DOT) {
+                    const uint32_t words[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float2 two = unpack(words[j], T{});
+                        dot = fmaf(w[2 * j], two.x, fmaf(w[2 * j + 1], two.y, dot));
+                    }
+                }
 #pragma unroll
                 for (int e = 0; e < 16; e += 8) {
-                    uint4 *tile = reinterpret_cast<uint4 *>(smem + Lay::out + swizzled(row, c * 2 + e / 8));
-                    if (with_dot && row < m) {
-                        const uint4 p = *tile;
-                        const float2 two[4] = {unpack(p.x, T{}), unpack(p.y, T{}), unpack(p.z, T{}), unpack(p.w, T{})};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) dot += u[e + 2 * j] * two[j].x + u[e + 2 * j + 1] * two[j].y;
-                    }
                     const int col = col0 + c * 16 + e;
                     if (staged) {
                         uint4 o;
@@ -342,32 +359,38 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                         o.y = pack(u[e + 2], u[e + 3], T{});
                         o.z = pack(u[e + 4], u[e + 5], T{});
                         o.w = pack(u[e + 6], u[e + 7], T{});
-                        *tile = o;
+                        *reinterpret_cast<uint4 *>(smem + Lay::out + swizzled(row, c * 2 + e / 8)) = o;
                     } else if (t < a.L && col < a.d2) {
                         float *at = out_f + ((b * a.L + t) * a.H + h) * a.d2 + col;
                         *reinterpret_cast<float4 *>(at) = make_float4(u[e], u[e + 1], u[e + 2], u[e + 3]);
                         *reinterpret_cast<float4 *>(at + 4) = make_float4(u[e + 4], u[e + 5], u[e + 6], u[e + 7]);
                     }
                 }
+            };
+            if constexpr (DOT) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) columns(c, y[2 * c], y[2 * c + 1]);
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) columns(c, y[0], y[0]);
+            }
+            if (DOT && t < a.L) {
+                const float pairs = sums[((i & 1) * 2) * kPiece + row] + sums[((i & 1) * 2 + 1) * kPiece + row];
+                a.dots[((long long)vt * a.B * a.L + b * a.L + t) * a.H + h] = row < m ? fmaf(pairs, f1, dot) : 0.f;
             }
             fence_before();
             warp_arrive(bar(kEpi));
-            fence_async();
-            warp_arrive(bar(kOutFull));
-            if (writer && bar_wait(bar(kOutFull), i & 1, failed)) {
-                // steps behind the tensor's end and columns behind its rows are not written
-                if (staged) {
+            if (staged) {
+                fence_async();
+                warp_arrive(bar(kOutFull));
+                if (writer && bar_wait(bar(kOutFull), i & 1, failed)) {
+                    // steps behind the tensor's end and columns behind its rows are not written
                     tma_store(base + Lay::out, &map_out, col0, h, (int)t0, (int)b);
                     tma_store_read();
-                }
-                if (with_dot) {
-                    if (i + 1 < pieces) load_dot(i + 1);
-                } else {
                     bar_arrive(bar(kOutFree));
                 }
+                __syncwarp();
             }
-            __syncwarp();
-            if (with_dot && t < a.L) a.dots[((long long)vt * a.B * a.L + b * a.L + t) * a.H + h] = dot;
         }
         // rows behind the last piece
         const long long first = (long long)pieces * kPiece;
@@ -380,11 +403,10 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
             *reinterpret_cast<uint4 *>(a.out_acc ? (void *)(out_f + at) : (void *)(out_t + at)) = zero;
             if (a.out_acc) *reinterpret_cast<uint4 *>(out_f + at + 4) = zero;
         }
-        if (with_dot)
+        if (DOT)
             for (long long t = first + tid - (kStateThreads + kScoreThreads); t < a.L; t += kOutThreads)
                 a.dots[((long long)vt * a.B * a.L + b * a.L + t) * a.H + h] = 0.f;
         if (writer) tma_store_done();
-        if (writer && with_dot && *failed) bar_wait(bar(kDot), (pieces - 1) & 1, failed + 1);
     } else if (warp == 20) {
         // ------------------------------------------------------------------ TMA and MMA
         if (pieces > 0) {
@@ -395,6 +417,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                 if (!warp_wait(bar(kFullRK), ph, failed)) break;
                 if (a.lengths != nullptr && n - piece_start(i) < kPiece && !warp_wait(bar(kFix), 0, failed)) break;
                 if (i > 0 && !warp_wait(bar(kO1), ph ^ 1, failed)) break;   // P of the piece before has been used
+                if (DOT && !(warp_wait(bar(kDot), ph, failed) && warp_wait(bar(kFullV0), ph, failed))) break;
                 fence_after();
                 // scores = R K^T
 #pragma unroll
@@ -403,6 +426,11 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                     mma_ss(tmem, tile_desc(base16 + ((Lay::r + off) >> 4), 16), tile_desc(base16 + ((Lay::k + off) >> 4), 16),
                            instr_desc<T>(128, false, false), j > 0, lead);
                 }
+                if (DOT)   // Y V^T
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        mma_ss(tmem + Lay::c_two, tile_desc(base16 + ((Lay::dot + j * 32) >> 4), 16), tile_desc(base16 + ((Lay::v + j * 32) >> 4), 16),
+                               instr_desc<T>(128, false, false), j > 0, lead);
                 mma_commit(bar(kScores), lead);
                 // O2 = R S, when O2 of the piece before has been read and the state's operand is there (it was written before
                 // V').  Small terms first here and below: the accumulator drops what does not fit its 24 bits at every step,
@@ -427,17 +455,13 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                                term < NV - 1 || j > 0, lead);
                 mma_commit(bar(kInc), lead);
                 // O1 = P V
-                const uint32_t v16 = base16 + (Lay::v >> 4) + ph * (kTileBytes >> 4);
+                const uint32_t v16 = base16 + (Lay::v >> 4) + (VS == 2 ? ph * (kTileBytes >> 4) : 0);
                 if (!warp_wait(bar(kP), ph, failed)) break;
                 fence_after();
 #pragma unroll
-                for (int term = NP - 1; term >= 0; --term)
-#pragma unroll
-                    for (int j = 0; j < kPiece / 16; ++j) {
-                        const int col = term == 0 ? (j / 4) * 64 + (j % 4) * 8 : Lay::c_p + (term - 1) * 64 + j * 8;
-                        mma_ts(tmem + Lay::c_o1, tmem + col, tile_desc(v16 + (j * 2048 >> 4), kTileBytes),
-                               instr_desc<T>(64, false, true), term < NP - 1 || j > 0, lead);
-                    }
+                for (int j = 0; j < kPiece / 16; ++j)
+                    mma_ts(tmem + Lay::c_o1, tmem + (j / 4) * 64 + (j % 4) * 8, tile_desc(v16 + (j * 2048 >> 4), kTileBytes),
+                           instr_desc<T>(64, false, true), j > 0, lead);
                 mma_commit(bar(kO1), lead);
             }
         }
@@ -458,28 +482,39 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
             };
             auto load_v = [&](int i) {
                 if (!lead) return;
-                bar_expect(bar(kFullV0 + (i & 1)), kTileBytes);
-                tma_load(base + Lay::v + (i & 1) * kTileBytes, &map_v, bar(kFullV0 + (i & 1)), vt * 64, vh, (int)piece_start(i), (int)b);
+                bar_expect(bar(kFullV0 + i % VS), kTileBytes);
+                tma_load(base + Lay::v + (i % VS) * kTileBytes, &map_v, bar(kFullV0 + i % VS), vt * 64, vh, (int)piece_start(i), (int)b);
+            };
+            auto load_dot = [&](int i) {
+                if (!lead) return;
+                bar_expect(bar(kDot), kTileBytes);
+                tma_load(base + Lay::dot, &map_dot, bar(kDot), vt * 64, h / a.dot.share, (int)piece_start(i), (int)b);
             };
             load_rk(0);
             load_v(0);
-            if (pieces > 1) load_v(1);
-            int loaded_rk = 1, loaded_v = pieces > 1 ? 2 : 1;
+            if (DOT) load_dot(0);
+            if (VS == 2 && pieces > 1) load_v(1);
+            int loaded_rk = 1, loaded_dot = 1, loaded_v = VS == 2 && pieces > 1 ? 2 : 1;
 #pragma unroll 1
             for (int i = 0; i + 1 < pieces; ++i) {
+                if (DOT) {
+                    if (!warp_wait(bar(kScores), i & 1, failed) || !warp_wait(bar(kDotFree), i & 1, failed)) break;
+                    load_dot(i + 1);
+                    ++loaded_dot;
+                }
                 if (!warp_wait(bar(kInc), i & 1, failed)) break;    // the last product that reads R and K
                 load_rk(i + 1);
                 ++loaded_rk;
-                if (i + 2 >= pieces) continue;
+                if (loaded_v == pieces) continue;
                 if (!warp_wait(bar(kO1), i & 1, failed)) break;     // the last product that reads V
-                load_v(i + 2);
-                ++loaded_v;
+                load_v(loaded_v++);
             }
             if (*failed) {
                 // let what is in flight land before the block gives its memory back
                 warp_wait(bar(kFullRK), (loaded_rk - 1) & 1, failed + 1);
-                for (int i = loaded_v > 1 ? loaded_v - 2 : 0; i < loaded_v; ++i)
-                    warp_wait(bar(kFullV0 + (i & 1)), (i >> 1) & 1, failed + 1);
+                if (DOT) warp_wait(bar(kDot), (loaded_dot - 1) & 1, failed + 1);
+                for (int i = loaded_v > VS ? loaded_v - VS : 0; i < loaded_v; ++i)
+                    warp_wait(bar(kFullV0 + i % VS), (i / VS) & 1, failed + 1);
             }
         }
     } else {
@@ -496,17 +531,17 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
 
 // ------------------------------------------------------------------------------------------ host side
 
-template <typename T, int KP, int NP, int NS, int NV, bool REV>
+template <typename T, int KP, int NS, int NV, bool DOT, bool REV>
 int launch_tiles(const Sweep &a, int dtype, cudaStream_t stream)
 {
-    using Lay = TileLayout<KP, NP, NS, NV>;
+    using Lay = TileLayout<KP, NS, NV, DOT>;
     CUtensorMap r, k, v, out, dot;
     const SweepOperand o{a.out, {a.L * a.H * a.d2, (long long)a.H * a.d2, a.d2}, 1};
     if (encoder() == nullptr || !encode(&r, a.r, a, a.d1, dtype) || !encode(&k, a.k, a, a.d1, dtype) ||
         !encode(&v, a.v, a, a.d2, dtype) || !encode(&out, o, a, a.d2, dtype) ||
         !encode(&dot, a.dot.data ? a.dot : o, a, a.d2, dtype))
         return PSIG_ERR_CUDA;
-    auto kernel = attn_sweep_tiles<T, KP, NP, NS, NV, REV>;
+    auto kernel = attn_sweep_tiles<T, KP, NS, NV, DOT, REV>;
     if (!prepare_kernel(kernel, Lay::alloc, true)) return PSIG_ERR_CUDA;
     const long long blocks = a.B * a.H * ((a.d2 + 63) / 64);
     kernel<<<(unsigned)blocks, kTileThreads, Lay::alloc, stream>>>(r, k, v, out, dot, a);
@@ -514,11 +549,14 @@ int launch_tiles(const Sweep &a, int dtype, cudaStream_t stream)
 }
 
 template <typename T, bool REV>
-int select_tiles(const Sweep &a, bool exact, int dtype, cudaStream_t stream)
+int select_tiles(const Sweep &a, int dtype, cudaStream_t stream)
 {
-    if (exact)
-        return a.d1 <= 64 ? launch_tiles<T, 64, 3, 3, 3, REV>(a, dtype, stream) : launch_tiles<T, 128, 3, 3, 3, REV>(a, dtype, stream);
-    return a.d1 <= 64 ? launch_tiles<T, 64, 1, 1, 3, REV>(a, dtype, stream) : launch_tiles<T, 128, 1, 1, 3, REV>(a, dtype, stream);
+    if (a.dot.data != nullptr)
+        return a.d1 <= 64 ? launch_tiles<T, 64, 3, 3, true, REV>(a, dtype, stream) : launch_tiles<T, 128, 3, 3, true, REV>(a, dtype, stream);
+    // two terms of V' (16 bits) are plenty for a state that nobody sees but through a 16-bit output
+    if (a.final == nullptr)
+        return a.d1 <= 64 ? launch_tiles<T, 64, 1, 2, false, REV>(a, dtype, stream) : launch_tiles<T, 128, 1, 2, false, REV>(a, dtype, stream);
+    return a.d1 <= 64 ? launch_tiles<T, 64, 1, 3, false, REV>(a, dtype, stream) : launch_tiles<T, 128, 1, 3, false, REV>(a, dtype, stream);
 }
 
 }  // namespace
@@ -535,8 +573,7 @@ bool attn_tiles_supported(const Sweep &a, int dtype)
 int attn_sweep_on_tiles(const Sweep &a, bool exact, int dtype, cudaStream_t stream)
 {
     if (dtype != PSIG_BF16) return attn_sweep_split(a, exact, dtype, stream);
-    return a.reverse ? select_tiles<__nv_bfloat16, true>(a, exact, dtype, stream)
-                     : select_tiles<__nv_bfloat16, false>(a, exact, dtype, stream);
+    return a.reverse ? select_tiles<__nv_bfloat16, true>(a, dtype, stream) : select_tiles<__nv_bfloat16, false>(a, dtype, stream);
 }
 
 long long attn_tile_timeouts() { return take_timeouts(); }

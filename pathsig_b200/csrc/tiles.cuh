@@ -100,9 +100,7 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, u
 // runs along M or N.
 __device__ __forceinline__ uint64_t tile_desc(uint32_t addr16, uint32_t lead)
 {
-    uint64_t d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(addr16 | (lead >> 4) << 16), "r"((1024u >> 4) | 1u << 14 | 2u << 29));
-    return d;
+    return (uint64_t)(addr16 | (lead >> 4) << 16) | (uint64_t)((1024u >> 4) | 1u << 14 | 2u << 29) << 32;
 }
 template <typename T>
 __device__ __forceinline__ constexpr uint32_t instr_desc(int n, bool a_rows_along_m, bool b_rows_along_n)
