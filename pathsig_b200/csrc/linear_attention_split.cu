@@ -33,28 +33,33 @@ struct SplitLayout {
     static constexpr int decay = s + NS * 64 * 128;
     static constexpr int bars = decay + 2 * (int)sizeof(DecayTables);
     static constexpr int tmem = bars + kBarriers * 8;
-    static constexpr int alloc = tmem + 16 + 1024;
+    static constexpr int alloc = tmem + 16;
     static constexpr int c_p = 128;                          // further terms of P
     static constexpr int c_o2 = 128 + (NP - 1) * 64;
     static constexpr int c_i = c_o2 + 64;                    // one I per half; O1 takes the first's columns
     static constexpr int columns = c_i + PANELS * 64 <= 256 ? 256 : 512;
 };
 
-// Pair number i of nx by ny terms, the smallest products (largest x + y) first: the accumulator drops what does not fit its 24
-// bits at every step, towards zero, so the steps that come while it is still small cost nothing (float32 outputs
-// of a 128-step piece: 1.8e-6 with the large products first, see select_split).
-__host__ __device__ constexpr int pair_at(int nx, int ny, int i, bool second)
+// The pairs (x, y) of nx by ny terms with x + y <= level, the smallest products (largest x + y) first: the accumulator drops
+// what does not fit its 24 bits at every step, towards zero, so the steps that come while it is still small cost nothing
+// (error of float32 outputs over a 128-step piece: 1.7e-7, with the large products first 1.8e-6).  As numbers of
+// four bits, x in the lower two.
+__host__ __device__ constexpr int pair_count(int nx, int ny, int level)
 {
-    for (int sum = nx + ny - 2; sum >= 0; --sum)
-        for (int x = 0; x < nx; ++x) {
-            const int y = sum - x;
-            if (y < 0 || y >= ny) continue;
-            if (i-- == 0) return second ? y : x;
-        }
-    return 0;
+    int n = 0;
+    for (int x = 0; x < nx; ++x)
+        for (int y = 0; y < ny; ++y) n += x + y <= level;
+    return n;
 }
-__host__ __device__ constexpr int pair_first(int nx, int ny, int i) { return pair_at(nx, ny, i, false); }
-__host__ __device__ constexpr int pair_second(int nx, int ny, int i) { return pair_at(nx, ny, i, true); }
+__host__ __device__ constexpr unsigned long long pair_list(int nx, int ny, int level)
+{
+    unsigned long long list = 0;
+    int n = 0;
+    for (int sum = level; sum >= 0; --sum)
+        for (int x = 0; x < nx; ++x)
+            if (sum - x >= 0 && sum - x < ny) list |= (unsigned long long)(x | (sum - x) << 2) << (4 * n++);
+    return list;
+}
 
 // 32 neighbouring values of a row of a raw tile (columns 32 half .. ), and their terms into the tiles.
 template <typename T>
@@ -106,8 +111,7 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
     constexpr int NI = sizeof(T) == 4 ? 3 : 2;
     using Lay = SplitLayout<NI, PANELS, LEVEL>;
     constexpr int RAW_BOXES = sizeof(T) == 4 ? 2 : 1;   // boxes of 128 bytes to a half row of 64 values
-    extern __shared__ unsigned char smem_raw[];
-    unsigned char *smem = smem_raw + ((1024 - (shared_addr(smem_raw) & 1023)) & 1023);
+    extern __shared__ __align__(1024) unsigned char smem[];   // the swizzle atoms start on 1024-byte boundaries
     const uint32_t base = shared_addr(smem);
     DecayTables *tables = reinterpret_cast<DecayTables *>(smem + Lay::decay);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Lay::tmem);
@@ -192,27 +196,27 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                     if (!ok) break;
                     fence_after();
                     bool add = p > 0;
-#pragma unroll
-                    for (int pair = 0; pair < NI * NI; ++pair)
-                        if (const int x = pair_first(NI, NI, pair), y = pair_second(NI, NI, pair); x + y <= LEVEL)
+#pragma unroll 1
+                    for (int pair = 0; pair < pair_count(NI, NI, LEVEL); ++pair)
+                        if (const int x = (int)(pair_list(NI, NI, LEVEL) >> (4 * pair)) & 3, y = (int)(pair_list(NI, NI, LEVEL) >> (4 * pair + 2)) & 3; true)
 #pragma unroll
                             for (int j = 0; j < 4; ++j, add = true)
                                 mma_ss(tmem, tile_desc(base16 + ((Lay::r + x * kTileBytes + j * 32) >> 4), 16),
                                        tile_desc(base16 + ((Lay::k + y * kTileBytes + j * 32) >> 4), 16), instr_desc<bf16>(128, false, false), add, lead);
                     if (p == PANELS - 1) mma_commit(bar(kScores), lead);
                     add = p > 0;
-#pragma unroll
-                    for (int pair = 0; pair < NI * Lay::NS; ++pair)
-                        if (const int x = pair_first(NI, Lay::NS, pair), y = pair_second(NI, Lay::NS, pair); x + y <= LEVEL)
+#pragma unroll 1
+                    for (int pair = 0; pair < pair_count(NI, Lay::NS, LEVEL); ++pair)
+                        if (const int x = (int)(pair_list(NI, Lay::NS, LEVEL) >> (4 * pair)) & 3, y = (int)(pair_list(NI, Lay::NS, LEVEL) >> (4 * pair + 2)) & 3; true)
 #pragma unroll
                             for (int j = 0; j < 4; ++j, add = true)
                                 mma_ss(tmem + Lay::c_o2, tile_desc(base16 + ((Lay::r + x * kTileBytes + j * 32) >> 4), 16),
                                        tile_desc(base16 + ((Lay::s + y * 8192 + j * 2048) >> 4), kTileBytes), instr_desc<bf16>(64, false, true), add, lead);
                     add = false;
                     // the state's 64 rows twice (the distance of the second block is 0), so that all lanes hold some
-#pragma unroll
-                    for (int pair = 0; pair < NI * Lay::NV; ++pair)
-                        if (const int x = pair_first(NI, Lay::NV, pair), y = pair_second(NI, Lay::NV, pair); x + y <= 2)
+#pragma unroll 1
+                    for (int pair = 0; pair < pair_count(NI, Lay::NV, 2); ++pair)
+                        if (const int x = (int)(pair_list(NI, Lay::NV, 2) >> (4 * pair)) & 3, y = (int)(pair_list(NI, Lay::NV, 2) >> (4 * pair + 2)) & 3; true)
 #pragma unroll
                             for (int j = 0; j < kPiece / 16; ++j, add = true)
                                 mma_ss(tmem + Lay::c_i + p * 64, tile_desc(base16 + ((Lay::k + x * kTileBytes + j * 2048) >> 4), 0),
@@ -228,9 +232,9 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                 if (!ok) break;
                 fence_after();
                 bool add = false;
-#pragma unroll
-                for (int pair = 0; pair < Lay::NP * NI; ++pair)
-                    if (const int x = pair_first(Lay::NP, NI, pair), y = pair_second(Lay::NP, NI, pair); x + y <= LEVEL)
+#pragma unroll 1
+                for (int pair = 0; pair < pair_count(Lay::NP, NI, LEVEL); ++pair)
+                    if (const int x = (int)(pair_list(Lay::NP, NI, LEVEL) >> (4 * pair)) & 3, y = (int)(pair_list(Lay::NP, NI, LEVEL) >> (4 * pair + 2)) & 3; true)
 #pragma unroll
                         for (int j = 0; j < kPiece / 16; ++j, add = true) {
                             const int col = x == 0 ? (j / 4) * 64 + (j % 4) * 8 : Lay::c_p + (x - 1) * 64 + j * 8;
@@ -341,23 +345,24 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                         }
                     }
                 }
-                float x[32], y[32];
-                read_raw<T>(smem + Lay::r, row, half, row < m, x);
-                read_raw<T>(smem + Lay::k, row, half, row < m, y);
-                ok = swap();
-                if (!ok) break;
-                write_terms<NI>(smem + Lay::r, kTileBytes, row, half * 4, x);
-                write_terms<NI>(smem + Lay::k, kTileBytes, row, half * 4, y);
-                if (p == 0) {
-                    read_raw<T>(smem + Lay::v, row, half, row < m, x);
-                    const float w = d.tail[row];
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) y[j] = x[j] * w;
+                // R, K and, with the first half, V and V'.  One loop for all: the code has to stay in the instruction cache
+#pragma unroll 1
+                for (int tile = 0; tile < (p == 0 ? 3 : 2); ++tile) {
+                    unsigned char *at = smem + tile * NI * kTileBytes;   // R, K, V stand one behind the other
+                    float x[32];
+                    read_raw<T>(at, row, half, row < m, x);
                     ok = swap();
                     if (!ok) break;
-                    write_terms<NI>(smem + Lay::v, kTileBytes, row, half * 4, x);
-                    write_terms<Lay::NV>(smem + Lay::vw, kTileBytes, row, half * 4, y);
+                    if (tile == 2) {
+                        float y[32];
+                        const float w = d.tail[row];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) y[j] = x[j] * w;
+                        write_terms<Lay::NV>(smem + Lay::vw, kTileBytes, row, half * 4, y);
+                    }
+                    write_terms<NI>(at, kTileBytes, row, half * 4, x);
                 }
+                if (!ok) break;
                 fence_async();
                 warp_arrive(bar(kReady));
             }
