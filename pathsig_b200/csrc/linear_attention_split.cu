@@ -6,21 +6,29 @@
 // float16 result needs) or 2 (24 bits).  So float32 calls keep float32's precision at six bfloat16 products instead
 // of fused multiply-adds, which have a thirtieth of the rate; and float16 scores, weights and states cannot overflow.
 //
-// TMA brings the raw rows; the compute threads turn them into terms in place (the raw tile of a float16 operand is as
-// large as its first term, that of a float32 operand as its first two), clearing rows behind the sequence's end on
-// the way.  Rows of more than 64 values are taken in two halves, one after the other through the same buffers: the
-// scores add up, and each half of the state is its own product.
+// Where the second operand's terms stand one behind the other in shared memory, the terms that belong with one term of the
+// first are one product: P_x [V_0 V_1 ..], with the columns for x + y = 0, 1, 2 side by side in tensor memory (added up on
+// the way out), reads P_x once.  A product of 64 columns is bound by reading its operands from shared memory.
+//
+// TMA brings the raw rows; eight warps turn them into terms in place (the raw tile of a float16 operand is as large as its
+// first term, that of a float32 operand as its first two), clearing rows behind the sequence's end on the way, and hold
+// the state; eight more weigh the scores and write the output, so that one piece's conversion overlaps with the piece
+// before.  Rows of more than 64 values are taken in two halves, one after the other through the same buffers: the scores
+// add up, and each half of the state is its own product.
+//
+// Measured, 8 x 2047 steps of 8 heads of 64 in float32: 20000 cycles a piece when eight warps did all stages (4200
+// conversion, 11000 products, 3400 output) and each pair of terms was its own product; see launch_split for this form.
 #include "tiles.cuh"
 
 namespace psig {
 namespace {
 
-enum Barrier { kRaw, kRawV, kReady, kScores, kInc, kP, kO1, kEpi, kDecFull0, kDecFull1, kDecFree0, kDecFree1, kSwap, kBarriers };
+enum Barrier { kRaw, kRawV, kReady, kReadyV, kScores, kInc, kIncRead, kP, kO1, kEpi, kDecFull0, kDecFull1, kDecFree0, kDecFree1, kSwap, kBarriers };
 
 using bf16 = __nv_bfloat16;
 
-constexpr int kCompute = 256;                 // compute threads
-constexpr int kTileThreads = kCompute + 64;   // + issuing warp + decay warp
+constexpr int kStateThreads = 256, kOutThreads = 256;
+constexpr int kSplitThreads = kStateThreads + kOutThreads + 96;   // + products, copies, decays
 
 template <int NI, int PANELS, int LEVEL>
 struct SplitLayout {
@@ -34,10 +42,13 @@ struct SplitLayout {
     static constexpr int bars = decay + 2 * (int)sizeof(DecayTables);
     static constexpr int tmem = bars + kBarriers * 8;
     static constexpr int alloc = tmem + 16;
-    static constexpr int c_p = 128;                          // further terms of P
-    static constexpr int c_o2 = 128 + (NP - 1) * 64;
-    static constexpr int c_i = c_o2 + 64;                    // one I per half; O1 takes the first's columns
-    static constexpr int columns = c_i + PANELS * 64 <= 256 ? 256 : 512;
+    // tensor memory columns: scores (P's first term takes the columns its own thread has read), the further terms of P,
+    // O2, and I, whose place O1 takes: both by the order x + y of their terms
+    static constexpr int c_p = 128;
+    static constexpr int c_o2 = 256;
+    static constexpr int c_i = 320;
+    static constexpr int orders = 3;
+    static constexpr int columns = 512;
 };
 
 // The pairs (x, y) of nx by ny terms with x + y <= level, the smallest products (largest x + y) first: the accumulator drops
@@ -104,7 +115,7 @@ __device__ __forceinline__ void write_terms(unsigned char *tile, int stride, int
 }
 
 template <typename T, int PANELS, int LEVEL, bool REV>
-__global__ void __launch_bounds__(kTileThreads, 1)
+__global__ void __launch_bounds__(kSplitThreads, 1)
 attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const Sweep a)
 {
@@ -130,170 +141,65 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
     }
     const int pieces = (int)((n + kPiece - 1) / kPiece);
     const long long segments = (a.L + kSegment - 1) / kSegment;
+    auto piece_start = [&](int i) { return (long long)(REV ? pieces - 1 - i : i) * kPiece; };
 
     if (tid == 0) {
+        const int warps_state = kStateThreads / 32, warps_out = kOutThreads / 32;
         bar_init(bar(kRaw), 1);
         bar_init(bar(kRawV), 1);
-        bar_init(bar(kReady), kCompute / 32);
+        bar_init(bar(kReady), warps_state);
+        bar_init(bar(kReadyV), warps_state);
         bar_init(bar(kScores), 1);
         bar_init(bar(kInc), 1);
-        bar_init(bar(kP), kCompute / 32);
+        bar_init(bar(kIncRead), warps_state);
+        bar_init(bar(kP), warps_out);
         bar_init(bar(kO1), 1);
-        bar_init(bar(kEpi), kCompute / 32);
-        bar_init(bar(kDecFull0), 1);
-        bar_init(bar(kDecFull1), 1);
-        bar_init(bar(kDecFree0), kCompute / 32);
-        bar_init(bar(kDecFree1), kCompute / 32);
-        bar_init(bar(kSwap), kCompute / 32);
-        *failed = 0;
-        failed[1] = 0;
+        bar_init(bar(kEpi), warps_out);
+        bar_init(bar(kSwap), warps_state);
+        for (int i = 0; i < 2; ++i) {
+            bar_init(bar(kDecFull0 + i), 1);
+            bar_init(bar(kDecFree0 + i), warps_state + warps_out);
+        }
+        failed[0] = failed[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_addr(tmem_slot)), "n"(Lay::columns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = *tmem_slot;
+    constexpr uint32_t tmem = 0;   // all columns are ours, so they start at 0
+    if (tid == 0 && (*tmem_slot != 0 || (base & 1023) != 0)) *failed = 1, atomicAdd(&g_tile_timeouts, 1ull);
+    const int quarter = warp & 3, half = (warp >> 2) & 1;
+    const int row = quarter * 32 + lane;                       // time step in the piece
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
 
-    if (warp == 8) {
-        // ------------------------------------------------------------------ TMA and MMA, one thread
-        if (pieces > 0) {
-            const uint32_t lead = lane == 0, base16 = base >> 4;
-            const int rh = h / a.r.share, kh = h / a.k.share, vh = h / a.v.share;
-            const int halves = pieces * PANELS;
-            auto start = [&](int piece) { return (REV ? pieces - 1 - piece : piece) * kPiece; };
-            constexpr int per_box = 128 / (int)sizeof(T);
-            auto load_rk = [&](int idx) {
-                if (!lead) return;
-                const int t0 = start(idx / PANELS), x0 = idx % PANELS * 64;
-                bar_expect(bar(kRaw), 2 * RAW_BOXES * kTileBytes);
-#pragma unroll
-                for (int p = 0; p < RAW_BOXES; ++p) {
-                    tma_load(base + Lay::r + p * kTileBytes, &map_r, bar(kRaw), x0 + p * per_box, rh, t0, (int)b);
-                    tma_load(base + Lay::k + p * kTileBytes, &map_k, bar(kRaw), x0 + p * per_box, kh, t0, (int)b);
-                }
-            };
-            auto load_v = [&](int piece) {
-                if (!lead) return;
-                bar_expect(bar(kRawV), RAW_BOXES * kTileBytes);
-#pragma unroll
-                for (int p = 0; p < RAW_BOXES; ++p)
-                    tma_load(base + Lay::v + p * kTileBytes, &map_v, bar(kRawV), vt * 64 + p * per_box, vh, start(piece), (int)b);
-            };
-            load_rk(0);
-            load_v(0);
-            int loaded = 1, loaded_v = 1;
-            bool ok = true;
-            for (int i = 0; i < pieces && ok; ++i) {
-                const uint32_t ph = i & 1;
-                for (int p = 0; p < PANELS && ok; ++p) {
-                    const int idx = i * PANELS + p;
-                    ok = warp_wait(bar(kReady), idx & 1, failed);
-                    if (ok && p == 0 && i > 0) ok = warp_wait(bar(kO1), ph ^ 1, failed) && warp_wait(bar(kEpi), ph ^ 1, failed);
-                    if (!ok) break;
-                    fence_after();
-                    bool add = p > 0;
-#pragma unroll 1
-                    for (int pair = 0; pair < pair_count(NI, NI, LEVEL); ++pair)
-                        if (const int x = (int)(pair_list(NI, NI, LEVEL) >> (4 * pair)) & 3, y = (int)(pair_list(NI, NI, LEVEL) >> (4 * pair + 2)) & 3; true)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j, add = true)
-                                mma_ss(tmem, tile_desc(base16 + ((Lay::r + x * kTileBytes + j * 32) >> 4), 16),
-                                       tile_desc(base16 + ((Lay::k + y * kTileBytes + j * 32) >> 4), 16), instr_desc<bf16>(128, false, false), add, lead);
-                    if (p == PANELS - 1) mma_commit(bar(kScores), lead);
-                    add = p > 0;
-#pragma unroll 1
-                    for (int pair = 0; pair < pair_count(NI, Lay::NS, LEVEL); ++pair)
-                        if (const int x = (int)(pair_list(NI, Lay::NS, LEVEL) >> (4 * pair)) & 3, y = (int)(pair_list(NI, Lay::NS, LEVEL) >> (4 * pair + 2)) & 3; true)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j, add = true)
-                                mma_ss(tmem + Lay::c_o2, tile_desc(base16 + ((Lay::r + x * kTileBytes + j * 32) >> 4), 16),
-                                       tile_desc(base16 + ((Lay::s + y * 8192 + j * 2048) >> 4), kTileBytes), instr_desc<bf16>(64, false, true), add, lead);
-                    add = false;
-                    // the state's 64 rows twice (the distance of the second block is 0), so that all lanes hold some
-#pragma unroll 1
-                    for (int pair = 0; pair < pair_count(NI, Lay::NV, 2); ++pair)
-                        if (const int x = (int)(pair_list(NI, Lay::NV, 2) >> (4 * pair)) & 3, y = (int)(pair_list(NI, Lay::NV, 2) >> (4 * pair + 2)) & 3; true)
-#pragma unroll
-                            for (int j = 0; j < kPiece / 16; ++j, add = true)
-                                mma_ss(tmem + Lay::c_i + p * 64, tile_desc(base16 + ((Lay::k + x * kTileBytes + j * 2048) >> 4), 0),
-                                       tile_desc(base16 + ((Lay::vw + y * kTileBytes + j * 2048) >> 4), kTileBytes), instr_desc<bf16>(64, true, true), add, lead);
-                    mma_commit(bar(kInc), lead);
-                    ok = warp_wait(bar(kInc), idx & 1, failed);
-                    if (ok && idx + 1 < halves) {
-                        load_rk(idx + 1);
-                        ++loaded;
-                    }
-                }
-                ok = ok && warp_wait(bar(kP), ph, failed);
-                if (!ok) break;
-                fence_after();
-                bool add = false;
-#pragma unroll 1
-                for (int pair = 0; pair < pair_count(Lay::NP, NI, LEVEL); ++pair)
-                    if (const int x = (int)(pair_list(Lay::NP, NI, LEVEL) >> (4 * pair)) & 3, y = (int)(pair_list(Lay::NP, NI, LEVEL) >> (4 * pair + 2)) & 3; true)
-#pragma unroll
-                        for (int j = 0; j < kPiece / 16; ++j, add = true) {
-                            const int col = x == 0 ? (j / 4) * 64 + (j % 4) * 8 : Lay::c_p + (x - 1) * 64 + j * 8;
-                            mma_ts(tmem + Lay::c_i, tmem + col, tile_desc(base16 + ((Lay::v + y * kTileBytes + j * 2048) >> 4), kTileBytes),
-                                   instr_desc<bf16>(64, false, true), add, lead);
-                        }
-                mma_commit(bar(kO1), lead);
-                if (i + 1 < pieces) {
-                    ok = warp_wait(bar(kO1), ph, failed);
-                    if (!ok) break;
-                    load_v(i + 1);
-                    ++loaded_v;
-                }
-            }
-            if (*failed) {
-                // let what is in flight land before the block gives its memory back
-                warp_wait(bar(kRaw), (loaded - 1) & 1, failed + 1);
-                warp_wait(bar(kRawV), (loaded_v - 1) & 1, failed + 1);
-            }
-        }
-        __syncwarp();
-    } else if (warp == 9) {
-        const float *g = static_cast<const float *>(a.decay) + b * a.decay_stride[0] + h * a.decay_stride[2];
-        sum_decays<REV>(g, a.decay_stride[1], n, pieces, tables, bar(kDecFull0), bar(kDecFree0), failed);
-    } else {
-        // ------------------------------------------------------------------ compute
-        const int quarter = warp & 3, half = warp >> 2;
-        const int row = quarter * 32 + lane;                       // time step in the piece
-        const int srow = (quarter & 1) * 32 + lane;                // row of a half of the state
+    if (warp < 8) {
+        // ------------------------------------------------------------------ terms of R, K, V and V'; the state
+        const int srow = (quarter & 1) * 32 + lane;                // row of a half of the state (they stand twice in the 128 lanes)
         const int sc0 = (quarter >> 1) * 32 + half * 16;           // first of 16 columns of the state
         const int gcol0 = vt * 64 + sc0;
-        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const long long state0 = bh * a.d1 * a.d2;
         float S[PANELS][16];
+        auto all_state = [&](bool transposed, auto fn) {   // fn(value, its position), (d1, d2) or (d2, d1)
+            const int step = transposed ? a.d1 : 1;
+#pragma unroll
+            for (int p = 0; p < PANELS; ++p) {
+                const int r1 = p * 64 + srow;
+                long long at = state0 + (transposed ? (long long)gcol0 * a.d1 + r1 : (long long)r1 * a.d2 + gcol0);
+#pragma unroll
+                for (int j = 0; j < 16; ++j, at += step)
+                    if (r1 < a.d1 && gcol0 + j < a.d2) fn(S[p][j], at);
+            }
+        };
 #pragma unroll
         for (int p = 0; p < PANELS; ++p)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int r1 = p * 64 + srow;
-                S[p][j] = 0.f;
-                if (a.init != nullptr && r1 < a.d1 && gcol0 + j < a.d2)
-                    S[p][j] = static_cast<const float *>(a.init)[state0 + (a.init_transposed ? (long long)(gcol0 + j) * a.d1 + r1
-                                                                                             : (long long)r1 * a.d2 + gcol0 + j)];
-            }
-        auto all_state = [&](auto fn) {   // fn(value, position in a (d1, d2) state, transposed position)
-#pragma unroll
-            for (int p = 0; p < PANELS; ++p)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int r1 = p * 64 + srow;
-                    if (r1 < a.d1 && gcol0 + j < a.d2) fn(S[p][j], (long long)r1 * a.d2 + gcol0 + j, (long long)(gcol0 + j) * a.d1 + r1);
-                }
-        };
-        T *out_t = static_cast<T *>(a.out);
-        float *out_f = static_cast<float *>(a.out);
-        const T *dot_row = static_cast<const T *>(a.dot.data);
-        if (dot_row != nullptr) dot_row += b * a.dot.stride[0] + (h / a.dot.share) * a.dot.stride[2];
-        const int ocol0 = vt * 64 + half * 32;
-        constexpr int G = 16 / (int)sizeof(T);   // values of an access of an output row
+            for (int j = 0; j < 16; ++j) S[p][j] = 0.f;
+        if (a.init != nullptr)
+            all_state(a.init_transposed, [&](float &v, long long at) { v = static_cast<const float *>(a.init)[at]; });
         const float kv_scale = (float)a.kv_scale;
         uint32_t swaps = 0;
         // float32: the terms of a row's one half overwrite the raw values of its other half, which another thread holds
@@ -302,10 +208,17 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
             warp_arrive(bar(kSwap));
             return warp_wait(bar(kSwap), swaps++ & 1, failed);
         };
+        auto convert = [&](int at, int m) {
+            float x[32];
+            read_raw<T>(smem + at, row, half, row < m, x);
+            if (!swap()) return false;
+            write_terms<NI>(smem + at, kTileBytes, row, half * 4, x);
+            return true;
+        };
         bool ok = true;
-        for (int i = 0; i < pieces; ++i) {
-            const uint32_t ph = i & 1;
-            const long long t0 = (long long)(REV ? pieces - 1 - i : i) * kPiece;
+#pragma unroll 1
+        for (int i = 0; i < pieces && ok; ++i) {
+            const long long t0 = piece_start(i);
             const int m = (int)(n - t0 < kPiece ? n - t0 : kPiece);
             const long long end = t0 + m;
             const bool boundary = end == n || end % kSegment == 0;
@@ -316,87 +229,132 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
 #pragma unroll
                 for (int p = 0; p < PANELS; ++p)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) dot = fmaf(S[p][j], anchor[(p * 16 + j) * kCompute], dot);
+                    for (int j = 0; j < 16; ++j) dot = fmaf(S[p][j], anchor[(p * 16 + j) * kStateThreads], dot);
                 for (int s = 16; s >= 1; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
                 if (lane == 0) static_cast<float *>(a.anchor_dots)[((bh * segments + segment) * tiles + vt) * 8 + warp] = dot;
             }
             const DecayTables &d = tables[i & 1];
             ok = warp_wait(bar(kDecFull0 + (i & 1)), (i >> 1) & 1, failed);
+            if (!ok) break;
+            const float keep = d.keep, w = d.tail[row];
+            warp_arrive(bar(kDecFree0 + (i & 1)));
 #pragma unroll
             for (int p = 0; p < PANELS; ++p) {
                 const int idx = i * PANELS + p;
-                ok = ok && warp_wait(bar(kRaw), idx & 1, failed);   // all products of the half before are done, too
-                if (p == 0) ok = ok && warp_wait(bar(kRawV), ph, failed);
+                // the products of the half before are done, so its tiles and the state's operand are free
+                ok = warp_wait(bar(kRaw), idx & 1, failed);
                 if (!ok) break;
-                {   // the state's half as an operand
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float x[8];
+                for (int c = 0; c < 2; ++c) {   // the state's half as an operand
+                    float x[8];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) x[j] = S[p][c * 8 + j];
+                    for (int j = 0; j < 8; ++j) x[j] = S[p][c * 8 + j];
 #pragma unroll
-                        for (int term = 0; term < Lay::NS; ++term) {
-                            uint4 w;
-                            w.x = next_term<bf16>(x[0], x[1], term == Lay::NS - 1);
-                            w.y = next_term<bf16>(x[2], x[3], term == Lay::NS - 1);
-                            w.z = next_term<bf16>(x[4], x[5], term == Lay::NS - 1);
-                            w.w = next_term<bf16>(x[6], x[7], term == Lay::NS - 1);
-                            *reinterpret_cast<uint4 *>(smem + Lay::s + term * 8192 + swizzled(srow, sc0 / 8 + c)) = w;
-                        }
+                    for (int term = 0; term < Lay::NS; ++term) {
+                        uint4 o;
+                        o.x = next_term<bf16>(x[0], x[1], term == Lay::NS - 1);
+                        o.y = next_term<bf16>(x[2], x[3], term == Lay::NS - 1);
+                        o.z = next_term<bf16>(x[4], x[5], term == Lay::NS - 1);
+                        o.w = next_term<bf16>(x[6], x[7], term == Lay::NS - 1);
+                        *reinterpret_cast<uint4 *>(smem + Lay::s + term * 8192 + swizzled(srow, sc0 / 8 + c)) = o;
                     }
                 }
-                // R, K and, with the first half, V and V'.  One loop for all: the code has to stay in the instruction cache
 #pragma unroll 1
-                for (int tile = 0; tile < (p == 0 ? 3 : 2); ++tile) {
-                    unsigned char *at = smem + tile * NI * kTileBytes;   // R, K, V stand one behind the other
-                    float x[32];
-                    read_raw<T>(at, row, half, row < m, x);
-                    ok = swap();
-                    if (!ok) break;
-                    if (tile == 2) {
-                        float y[32];
-                        const float w = d.tail[row];
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) y[j] = x[j] * w;
-                        write_terms<Lay::NV>(smem + Lay::vw, kTileBytes, row, half * 4, y);
-                    }
-                    write_terms<NI>(at, kTileBytes, row, half * 4, x);
-                }
+                for (int tile = 0; tile < 2 && ok; ++tile) ok = convert(tile == 0 ? Lay::r : Lay::k, m);
                 if (!ok) break;
                 fence_async();
                 warp_arrive(bar(kReady));
+                if (p == 0) {
+                    ok = warp_wait(bar(kRawV), i & 1, failed);
+                    if (!ok) break;
+                    float x[32], y[32];
+                    read_raw<T>(smem + Lay::v, row, half, row < m, x);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) y[j] = x[j] * w;
+                    ok = swap();
+                    if (!ok) break;
+                    write_terms<Lay::NV>(smem + Lay::vw, kTileBytes, row, half * 4, y);
+                    write_terms<NI>(smem + Lay::v, kTileBytes, row, half * 4, x);
+                    fence_async();
+                    warp_arrive(bar(kReadyV));
+                }
+                ok = warp_wait(bar(kInc), idx & 1, failed);
+                if (!ok) break;
+                fence_after();
+                float x[3][16];
+#pragma unroll
+                for (int o = 0; o < 3; ++o) tmem_load16(tmem + lanes + Lay::c_i + o * 64 + sc0, x[o]);
+                tmem_loaded();
+                fence_before();
+                warp_arrive(bar(kIncRead));
+#pragma unroll
+                for (int j = 0; j < 16; ++j) S[p][j] = fmaf(S[p][j], keep, (x[0][j] + (x[1][j] + x[2][j])) * kv_scale);
             }
             if (!ok) break;
-            // P = scores, weighted
-            ok = warp_wait(bar(kScores), ph, failed);
-            if (!ok) break;
-            fence_after();
+            if (!REV && a.anchors != nullptr && boundary) {
+                // in the threads' own order: the sweep that reads them has the same threads
+                float *anchor = static_cast<float *>(a.anchors) + ((bh * segments + (end - 1) / kSegment) * tiles + vt) * PANELS * 4096 + tid;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int s0 = half * 64 + q * 16;
-                const int block = half * 2 + q / 2;
-                const uint32_t own = tmem + lanes + half * 64;
-                uint32_t p0[8], p1[8], p2[8];
+                for (int p = 0; p < PANELS; ++p)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) anchor[(p * 16 + j) * kStateThreads] = S[p][j];
+            }
+        }
+        if (a.final != nullptr)
+            all_state(a.final_transposed, [&](float &v, long long at) { static_cast<float *>(a.final)[at] = v; });
+    } else if (warp < 16) {
+        // ------------------------------------------------------------------ P = scores, weighted; out
+        const uint32_t own = tmem + lanes + half * 64;      // this thread's columns of the scores
+        T *out_t = static_cast<T *>(a.out);
+        float *out_f = static_cast<float *>(a.out);
+        const T *dot_row = static_cast<const T *>(a.dot.data);
+        if (dot_row != nullptr) dot_row += b * a.dot.stride[0] + (h / a.dot.share) * a.dot.stride[2];
+        const int ocol0 = vt * 64 + half * 32;
+        constexpr int G = 16 / (int)sizeof(T);              // values of an access of an output row
+        const int tid_out = tid - kStateThreads;
+#pragma unroll 1
+        for (int i = 0; i < pieces; ++i) {
+            const uint32_t ph = i & 1;
+            const long long t0 = piece_start(i), t = t0 + row;
+            const int m = (int)(n - t0 < kPiece ? n - t0 : kPiece);
+            const DecayTables &d = tables[i & 1];
+            if (!warp_wait(bar(kDecFull0 + (i & 1)), (i >> 1) & 1, failed)) break;
+            const float la = d.la[row], head = d.head[row];
+            float f[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) f[q] = exp_two((float)(d.a[row] - d.a[(half * 2 + q) * 32 + (REV ? 0 : 31)]));
+            if (!warp_wait(bar(kScores), ph, failed)) break;
+            fence_after();
+#pragma unroll 1
+            for (int q = 0; q < 4; ++q) {   // 16 columns each
+                const int block = half * 2 + q / 2, s0 = half * 64 + q * 16;
                 float x[16];
                 if (REV ? block >= quarter : block <= quarter) {
                     tmem_load16(own + q * 16, x);
-                    tmem_loaded();
-                    if (block == quarter) {
-                        const float la = d.la[row];
+                    const float4 *table = reinterpret_cast<const float4 *>((block == quarter ? d.la : d.cf) + s0);
+                    float w[16];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const int s = s0 + j;
-                            x[j] = (REV ? s >= row : s <= row) ? x[j] * exp_two(la - d.la[s]) : 0.f;
-                        }
-                    } else {
-                        const float f = exp_two((float)(d.a[row] - d.a[REV ? block * 32 : block * 32 + 31]));
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) x[j] *= f * d.cf[s0 + j];
+                    for (int j = 0; j < 4; ++j) {
+                        const float4 v = table[j];
+                        w[4 * j] = v.x, w[4 * j + 1] = v.y, w[4 * j + 2] = v.z, w[4 * j + 3] = v.w;
                     }
+                    if (block == quarter) {
+                        const int j0 = row - s0;   // the step's own column
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) w[j] = (REV ? j >= j0 : j <= j0) ? exp_two(la - w[j]) : 0.f;
+                    } else {
+                        const float fq = q < 2 ? f[0] : f[1];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) w[j] *= fq;
+                    }
+                    tmem_loaded();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) x[j] *= w[j];
                 } else {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) x[j] = 0.f;
                 }
+                uint32_t p0[8], p1[8], p2[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     p0[j] = next_term<bf16>(x[2 * j], x[2 * j + 1], false);
@@ -408,44 +366,23 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                 if (Lay::NP > 2) tmem_store8(tmem + lanes + Lay::c_p + 64 + half * 32 + q * 8, p2);
             }
             tmem_stored();
-            // the state behind the piece
-            ok = warp_wait(bar(kInc), (i * PANELS + PANELS - 1) & 1, failed);
-            if (!ok) break;
-            fence_after();
-#pragma unroll
-            for (int p = 0; p < PANELS; ++p) {
-                float x[16];
-                tmem_load16(tmem + lanes + Lay::c_i + p * 64 + sc0, x);
-                tmem_loaded();
-#pragma unroll
-                for (int j = 0; j < 16; ++j) S[p][j] = fmaf(S[p][j], d.keep, x[j] * kv_scale);
-            }
             fence_before();
             warp_arrive(bar(kP));
-            if (!REV && a.anchors != nullptr && boundary) {
-                // in the threads' own order: the sweep that reads them has the same threads
-                float *anchor = static_cast<float *>(a.anchors) + ((bh * segments + (end - 1) / kSegment) * tiles + vt) * PANELS * 4096 + tid;
-#pragma unroll
-                for (int p = 0; p < PANELS; ++p)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) anchor[(p * 16 + j) * kCompute] = S[p][j];
-            }
-            // out
-            const float head = d.head[row];
-            ok = warp_wait(bar(kO1), ph, failed);
-            if (!ok) break;
+            warp_arrive(bar(kDecFree0 + (i & 1)));
+            if (!warp_wait(bar(kO1), ph, failed)) break;
             fence_after();
-            const long long t = t0 + row;
             float dot = 0.f;
-#pragma unroll
+            const float f1 = (float)(a.out_scale * a.kv_scale), f2 = (float)a.out_scale * head;
+#pragma unroll 1
             for (int c = 0; c < 2; ++c) {
-                float x[16], y[16];
+                float x[16], y[16], z[16], o2[16];
                 tmem_load16(tmem + lanes + Lay::c_i + half * 32 + c * 16, x);
-                tmem_load16(tmem + lanes + Lay::c_o2 + half * 32 + c * 16, y);
+                tmem_load16(tmem + lanes + Lay::c_i + 64 + half * 32 + c * 16, y);
+                if (LEVEL > 1) tmem_load16(tmem + lanes + Lay::c_i + 128 + half * 32 + c * 16, z);
+                tmem_load16(tmem + lanes + Lay::c_o2 + half * 32 + c * 16, o2);
                 tmem_loaded();
-                const float f1 = (float)(a.out_scale * a.kv_scale), f2 = (float)a.out_scale * head;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] = row < m ? fmaf(x[j], f1, y[j] * f2) : 0.f;
+                for (int j = 0; j < 16; ++j) x[j] = row < m ? fmaf(x[j] + (LEVEL > 1 ? y[j] + z[j] : y[j]), f1, o2[j] * f2) : 0.f;
                 if (t >= a.L) continue;
 #pragma unroll
                 for (int e = 0; e < 16; e += G) {
@@ -482,12 +419,11 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
             }
             fence_before();
             warp_arrive(bar(kEpi));
-            warp_arrive(bar(kDecFree0 + (i & 1)));
             if (dot_row != nullptr && t < a.L) a.dots[((long long)(vt * 2 + half) * a.B * a.L + b * a.L + t) * a.H + h] = dot;
         }
-        // rows behind the last piece, and the last state
+        // rows behind the last piece
         const long long first = (long long)pieces * kPiece;
-        for (long long e = tid; e < (a.L - first) * 16; e += kCompute) {
+        for (long long e = tid_out; e < (a.L - first) * 16; e += kOutThreads) {
             const long long t = first + e / 16;
             const int col = vt * 64 + (int)(e % 16) * 4;
             if (col >= a.d2) continue;
@@ -496,16 +432,137 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
             else *reinterpret_cast<uint2 *>(out_t + at) = make_uint2(0u, 0u);
         }
         if (dot_row != nullptr)
-            for (long long e = tid; e < (a.L - first) * 2; e += kCompute)
+            for (long long e = tid_out; e < (a.L - first) * 2; e += kOutThreads)
                 a.dots[((vt * 2 + e % 2) * a.B * a.L + b * a.L + first + e / 2) * a.H + h] = 0.f;
-        if (a.final != nullptr)
-            all_state([&](float v, long long at, long long transposed) {
-                static_cast<float *>(a.final)[state0 + (a.final_transposed ? transposed : at)] = v;
-            });
+    } else if (warp == 16) {
+        // ------------------------------------------------------------------ products
+        const uint32_t lead = lane == 0, base16 = base >> 4;
+        bool ok = true;
+#pragma unroll 1
+        for (int i = 0; i < pieces && ok; ++i) {
+            const uint32_t ph = i & 1;
+#pragma unroll 1
+            for (int p = 0; p < PANELS; ++p) {
+                const int idx = i * PANELS + p;
+                ok = warp_wait(bar(kReady), idx & 1, failed);
+                if (ok && p == 0 && i > 0) ok = warp_wait(bar(kO1), ph ^ 1, failed);   // P of the piece before has been used
+                if (!ok) break;
+                fence_after();
+                // scores += R K^T
+#pragma unroll 1
+                for (int pair = 0; pair < pair_count(NI, NI, LEVEL); ++pair) {
+                    const int x = (int)(pair_list(NI, NI, LEVEL) >> (4 * pair)) & 3, y = (int)(pair_list(NI, NI, LEVEL) >> (4 * pair + 2)) & 3;
+                    const uint32_t r16 = base16 + ((Lay::r + x * kTileBytes) >> 4), k16 = base16 + ((Lay::k + y * kTileBytes) >> 4);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        mma_ss(tmem, tile_desc(r16 + j * 2, 16), tile_desc(k16 + j * 2, 16), instr_desc<bf16>(128, false, false),
+                               p > 0 || pair > 0 || j > 0, lead);
+                }
+                if (p == PANELS - 1) mma_commit(bar(kScores), lead);
+                if (p == 0 && i > 0) ok = warp_wait(bar(kEpi), ph ^ 1, failed);        // O2 and O1 of the piece before have been read
+                if (!ok) break;
+                fence_after();
+                // O2 += R S
+#pragma unroll 1
+                for (int pair = 0; pair < pair_count(NI, Lay::NS, LEVEL); ++pair) {
+                    const int x = (int)(pair_list(NI, Lay::NS, LEVEL) >> (4 * pair)) & 3, y = (int)(pair_list(NI, Lay::NS, LEVEL) >> (4 * pair + 2)) & 3;
+                    const uint32_t r16 = base16 + ((Lay::r + x * kTileBytes) >> 4), s16 = base16 + ((Lay::s + y * 8192) >> 4);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        mma_ss(tmem + Lay::c_o2, tile_desc(r16 + j * 2, 16), tile_desc(s16 + j * 128, kTileBytes), instr_desc<bf16>(64, false, true),
+                               p > 0 || pair > 0 || j > 0, lead);
+                }
+                if (p == 0) ok = warp_wait(bar(kReadyV), ph, failed);
+                else ok = warp_wait(bar(kIncRead), (idx - 1) & 1, failed);
+                if (!ok) break;
+                fence_after();
+                // I = K^T V', term x of K with the terms 0 .. 2 - x of V'; the state's 64 rows twice (the distance of the second
+                // block is 0), so that all lanes hold some
+#pragma unroll 1
+                for (int j = 0; j < kPiece / 16; ++j) {
+                    const uint32_t k16 = base16 + (Lay::k >> 4) + j * 128, w16 = base16 + (Lay::vw >> 4) + j * 128;
+                    mma_ss(tmem + Lay::c_i, tile_desc(k16, 0), tile_desc(w16, kTileBytes), instr_desc<bf16>(192, true, true), j > 0, lead);
+                    mma_ss(tmem + Lay::c_i + 64, tile_desc(k16 + (kTileBytes >> 4), 0), tile_desc(w16, kTileBytes), instr_desc<bf16>(128, true, true), true, lead);
+                    if (NI > 2)
+                        mma_ss(tmem + Lay::c_i + 128, tile_desc(k16 + (2 * kTileBytes >> 4), 0), tile_desc(w16, kTileBytes), instr_desc<bf16>(64, true, true), true, lead);
+                }
+                mma_commit(bar(kInc), lead);
+            }
+            if (!ok) break;
+            ok = warp_wait(bar(kP), ph, failed) && warp_wait(bar(kIncRead), (i * PANELS + PANELS - 1) & 1, failed);
+            if (!ok) break;
+            fence_after();
+            // O1 = P V, term x of P with the terms 0 .. LEVEL - x of V (as many as there are)
+#pragma unroll 1
+            for (int j = 0; j < kPiece / 16; ++j) {
+                const uint32_t v16 = base16 + (Lay::v >> 4) + j * 128, p0 = tmem + (j / 4) * 64 + (j % 4) * 8, p1 = tmem + Lay::c_p + j * 8;
+                constexpr int first = LEVEL + 1 < NI ? LEVEL + 1 : NI;
+                // orders that term 0 does not reach (float16 at LEVEL 2) start with term 1
+                mma_ts(tmem + Lay::c_i, p0, tile_desc(v16, kTileBytes), instr_desc<bf16>(first * 64, false, true), j > 0, lead);
+                if constexpr (LEVEL == 2 && NI == 2) {
+                    mma_ts(tmem + Lay::c_i + 64, p1, tile_desc(v16, kTileBytes), instr_desc<bf16>(64, false, true), true, lead);
+                    mma_ts(tmem + Lay::c_i + 128, p1, tile_desc(v16 + (kTileBytes >> 4), kTileBytes), instr_desc<bf16>(64, false, true), j > 0, lead);
+                } else {
+                    mma_ts(tmem + Lay::c_i + 64, p1, tile_desc(v16, kTileBytes), instr_desc<bf16>(LEVEL * 64, false, true), true, lead);
+                }
+                if constexpr (LEVEL == 2)
+                    mma_ts(tmem + Lay::c_i + 128, p1 + 64, tile_desc(v16, kTileBytes), instr_desc<bf16>(64, false, true), true, lead);
+            }
+            mma_commit(bar(kO1), lead);
+        }
+    } else if (warp == 17) {
+        // ------------------------------------------------------------------ copies
+        if (pieces > 0) {
+            const uint32_t lead = lane == 0;
+            const int rh = h / a.r.share, kh = h / a.k.share, vh = h / a.v.share;
+            constexpr int per_box = 128 / (int)sizeof(T);
+            auto load_rk = [&](int idx) {
+                if (!lead) return;
+                const int t0 = (int)piece_start(idx / PANELS), x0 = idx % PANELS * 64;
+                bar_expect(bar(kRaw), 2 * RAW_BOXES * kTileBytes);
+#pragma unroll
+                for (int p = 0; p < RAW_BOXES; ++p) {
+                    tma_load(base + Lay::r + p * kTileBytes, &map_r, bar(kRaw), x0 + p * per_box, rh, t0, (int)b);
+                    tma_load(base + Lay::k + p * kTileBytes, &map_k, bar(kRaw), x0 + p * per_box, kh, t0, (int)b);
+                }
+            };
+            auto load_v = [&](int piece) {
+                if (!lead) return;
+                bar_expect(bar(kRawV), RAW_BOXES * kTileBytes);
+#pragma unroll
+                for (int p = 0; p < RAW_BOXES; ++p)
+                    tma_load(base + Lay::v + p * kTileBytes, &map_v, bar(kRawV), vt * 64 + p * per_box, vh, (int)piece_start(piece), (int)b);
+            };
+            load_rk(0);
+            load_v(0);
+            int loaded = 1, loaded_v = 1;
+            bool ok = true;
+#pragma unroll 1
+            for (int idx = 0; idx + 1 < pieces * PANELS && ok; ++idx) {
+                ok = warp_wait(bar(kInc), idx & 1, failed);        // the last product that reads this half of R and K
+                if (!ok) break;
+                load_rk(idx + 1);
+                ++loaded;
+                const int i = idx / PANELS;
+                if (idx % PANELS != PANELS - 1) continue;
+                ok = warp_wait(bar(kO1), i & 1, failed);           // the last product that reads V
+                if (!ok) break;
+                load_v(i + 1);
+                ++loaded_v;
+            }
+            if (*failed) {
+                // let what is in flight land before the block gives its memory back
+                warp_wait(bar(kRaw), (loaded - 1) & 1, failed + 1);
+                warp_wait(bar(kRawV), (loaded_v - 1) & 1, failed + 1);
+            }
+        }
+    } else {
+        const float *g = static_cast<const float *>(a.decay) + b * a.decay_stride[0] + h * a.decay_stride[2];
+        sum_decays<REV>(g, a.decay_stride[1], n, pieces, tables, bar(kDecFull0), bar(kDecFree0), failed);
     }
     fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 16) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(Lay::columns));
     }
@@ -522,7 +579,7 @@ int launch_split(const Sweep &a, int dtype, cudaStream_t stream)
     auto kernel = attn_sweep_split_terms<T, PANELS, LEVEL, REV>;
     if (!prepare_kernel(kernel, Lay::alloc, true)) return PSIG_ERR_CUDA;
     const long long blocks = a.B * a.H * ((a.d2 + 63) / 64);
-    kernel<<<(unsigned)blocks, kTileThreads, Lay::alloc, stream>>>(r, k, v, a);
+    kernel<<<(unsigned)blocks, kSplitThreads, Lay::alloc, stream>>>(r, k, v, a);
     return check_launch();
 }
 
