@@ -426,6 +426,7 @@ Sweep sweep_of(const PsigAttnDesc &d, const void *decay)
     s.H = d.H;
     s.out_scale = 1.0;
     s.kv_scale = 1.0;
+    s.splits = 1;
     return s;
 }
 
@@ -491,10 +492,24 @@ struct Call {
     }
 };
 
+// Scratch for the parts of long sequences in a sweep over heads of d1 and d2 (bytes, a multiple of 256; 0: one part).
+long long split_bytes(const PsigAttnDesc &d, int d1, int d2)
+{
+    if (d.dtype == PSIG_F64 || d.dk > 128 || d.dv > 128) return 0;
+    const int splits = split_plan(d.B, d.L, d.H, d2);
+    return splits == 1 ? 0 : (4 * d.B * d.H * splits * (split_state_size(d1, d2) + 1) + 255) / 256 * 256;
+}
+void set_splits(Sweep &s, void *scratch)
+{
+    s.splits = split_plan(s.B, s.L, s.H, s.d2);
+    s.split_states = static_cast<float *>(scratch);
+    s.split_decays = s.split_states + s.B * s.H * s.splits * split_state_size(s.d1, s.d2);
+}
+
 // Scratch of the backward pass, in the order it is laid out (256-byte aligned pieces).  It does not depend on which
 // form of the sweeps serves the call, which the operands' addresses decide too.
 struct BackwardScratch {
-    long long gq, gk, gv, pairs, anchors, dots, totals, bytes;
+    long long gq, gk, gv, pairs, anchors, dots, totals, parts, bytes;
 };
 
 int anchor_parts(const PsigAttnDesc &d)
@@ -522,18 +537,22 @@ BackwardScratch backward_scratch(const PsigAttnDesc &d)
     s.anchors = take(acc * bh * seg * ((d.dk + 63) / 64 * 64) * ((d.dv + 63) / 64 * 64));
     s.dots = take(acc * bh * seg * anchor_parts(d));
     s.totals = take(8 * bh * seg);
+    const long long one = split_bytes(d, d.dv, d.dk), two = split_bytes(d, d.dk, d.dv);
+    s.parts = take(one > two ? one : two);
     s.bytes = at;
     return s;
 }
 
 template <typename T>
-int run_forward(const Call &c, const void *init, void *out, void *final, cudaStream_t stream)
+int run_forward(const Call &c, const void *init, void *out, void *final, void *ws, cudaStream_t stream)
 {
     Sweep s = c.forward();
     s.init = init;
     s.final = final;
     s.out = out;
-    return c.tiles(out) ? attn_sweep_on_tiles(s, false, c.d.dtype, stream) : sweep_rows<T>(s, stream);
+    if (!c.tiles(out)) return sweep_rows<T>(s, stream);
+    set_splits(s, ws);
+    return attn_sweep_on_tiles(s, false, c.d.dtype, stream);
 }
 
 unsigned blocks_for(long long items, int per_block)
@@ -598,16 +617,19 @@ int run_backward_tiles(const Call &c, const void *init, const void *gs, void *gr
     s.init = init;
     s.out = grad_q;
     if (grad_decay != nullptr) s.anchors = ws + at.anchors, s.dot = c.q, s.dots = x;
+    set_splits(s, ws + at.parts);
     if ((rc = attn_sweep_on_tiles(s, grad_decay != nullptr, d.dtype, stream)) != PSIG_OK) return rc;
     s = c.grad_k();
     s.init = gs;
     s.out = shared ? ws + at.gk : grad_k, s.out_acc = shared;
     if (grad_decay != nullptr) s.anchors = ws + at.anchors, s.anchor_dots = ws + at.dots, s.dot = c.k, s.dots = y;
+    set_splits(s, ws + at.parts);
     if ((rc = attn_sweep_on_tiles(s, grad_decay != nullptr, d.dtype, stream)) != PSIG_OK) return rc;
     s = c.grad_v();
     s.init = gs;
     s.final = grad_init;
     s.out = shared ? ws + at.gv : grad_v, s.out_acc = shared;
+    set_splits(s, ws + at.parts);
     if ((rc = attn_sweep_on_tiles(s, false, d.dtype, stream)) != PSIG_OK) return rc;
     if (shared) {
         if ((rc = sum_heads<T>(ws + at.gk, grad_k, kv_rows, c.share, d.dk, stream)) != PSIG_OK) return rc;
@@ -663,7 +685,11 @@ int run_backward(const Call &c, const void *init, const void *gs, void *grad_q, 
 
 using namespace psig;
 
-extern "C" int64_t psig_attn_forward_workspace(const PsigAttnDesc *desc) { return check_attn(desc); }
+extern "C" int64_t psig_attn_forward_workspace(const PsigAttnDesc *desc)
+{
+    const int rc = check_attn(desc);
+    return rc != PSIG_OK ? rc : split_bytes(*desc, desc->dk, desc->dv);
+}
 
 extern "C" int64_t psig_attn_backward_workspace(const PsigAttnDesc *desc)
 {
@@ -677,13 +703,14 @@ extern "C" int psig_attn_forward(const PsigAttnDesc *desc, const void *q, const 
 {
     const int rc = check_attn(desc);
     if (rc != PSIG_OK) return rc;
-    (void)workspace, (void)workspace_bytes;
     if (desc->B == 0) return PSIG_OK;
     if (desc->L > 0 && (!q || !k || !v || !log_decay || !out)) return PSIG_ERR_NULL;
     if (desc->L == 0 && final_state == nullptr) return PSIG_OK;
+    const int64_t need = split_bytes(*desc, desc->dk, desc->dv);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return PSIG_ERR_WORKSPACE;
     return with_dtype(desc->dtype, [&](auto t) {
         return run_forward<decltype(t)>(Call(*desc, q, k, v, log_decay, nullptr), initial_state, out, final_state,
-                                        static_cast<cudaStream_t>(stream));
+                                        workspace, static_cast<cudaStream_t>(stream));
     });
 }
 

@@ -114,7 +114,7 @@ __device__ __forceinline__ void write_terms(unsigned char *tile, int stride, int
         }
 }
 
-template <typename T, int PANELS, int LEVEL, bool REV>
+template <typename T, int PANELS, int LEVEL, bool REV, bool STATE>
 __global__ void __launch_bounds__(kSplitThreads, 1)
 attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const Sweep a)
@@ -139,9 +139,11 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
         n = a.lengths[b];
         n = n < 0 ? 0 : n > a.L ? a.L : n;
     }
-    const int pieces = (int)((n + kPiece - 1) / kPiece);
+    const int all = (int)((n + kPiece - 1) / kPiece);                 // pieces of the sequence
+    const int part = blockIdx.y;
+    const int first = (int)((long long)all * part / a.splits), pieces = (int)((long long)all * (part + 1) / a.splits) - first;
     const long long segments = (a.L + kSegment - 1) / kSegment;
-    auto piece_start = [&](int i) { return (long long)(REV ? pieces - 1 - i : i) * kPiece; };
+    auto piece_start = [&](int i) { return (long long)(REV ? all - 1 - first - i : first + i) * kPiece; };
 
     if (tid == 0) {
         const int warps_state = kStateThreads / 32, warps_out = kOutThreads / 32;
@@ -158,7 +160,7 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
         bar_init(bar(kSwap), warps_state);
         for (int i = 0; i < 2; ++i) {
             bar_init(bar(kDecFull0 + i), 1);
-            bar_init(bar(kDecFree0 + i), warps_state + warps_out);
+            bar_init(bar(kDecFree0 + i), warps_state + (STATE ? 0 : warps_out));
         }
         failed[0] = failed[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -198,7 +200,14 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
         for (int p = 0; p < PANELS; ++p)
 #pragma unroll
             for (int j = 0; j < 16; ++j) S[p][j] = 0.f;
-        if (a.init != nullptr)
+        float *parts = a.split_states + ((bh * a.splits + part) * tiles + vt) * PANELS * 4096 + tid;   // this part's, in the threads' order
+        if (part > 0 && !STATE) {
+            parts -= (long long)tiles * PANELS * 4096;
+#pragma unroll
+            for (int p = 0; p < PANELS; ++p)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) S[p][j] = parts[(p * 16 + j) * kStateThreads];
+        } else if (part == 0 && a.init != nullptr)
             all_state(a.init_transposed, [&](float &v, long long at) { v = static_cast<const float *>(a.init)[at]; });
         const float kv_scale = (float)a.kv_scale;
         uint32_t swaps = 0;
@@ -222,7 +231,7 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
             const int m = (int)(n - t0 < kPiece ? n - t0 : kPiece);
             const long long end = t0 + m;
             const bool boundary = end == n || end % kSegment == 0;
-            if (REV && a.anchor_dots != nullptr && boundary) {
+            if (REV && !STATE && a.anchor_dots != nullptr && boundary) {
                 const long long segment = (end - 1) / kSegment;
                 const float *anchor = static_cast<const float *>(a.anchors) + ((bh * segments + segment) * tiles + vt) * PANELS * 4096 + tid;
                 float dot = 0.f;
@@ -245,7 +254,7 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                 ok = warp_wait(bar(kRaw), idx & 1, failed);
                 if (!ok) break;
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {   // the state's half as an operand
+                for (int c = 0; c < (STATE ? 0 : 2); ++c) {   // the state's half as an operand
                     float x[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) x[j] = S[p][c * 8 + j];
@@ -260,7 +269,7 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                     }
                 }
 #pragma unroll 1
-                for (int tile = 0; tile < 2 && ok; ++tile) ok = convert(tile == 0 ? Lay::r : Lay::k, m);
+                for (int tile = STATE ? 1 : 0; tile < 2 && ok; ++tile) ok = convert(tile == 0 ? Lay::r : Lay::k, m);
                 if (!ok) break;
                 fence_async();
                 warp_arrive(bar(kReady));
@@ -274,7 +283,7 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                     ok = swap();
                     if (!ok) break;
                     write_terms<Lay::NV>(smem + Lay::vw, kTileBytes, row, half * 4, y);
-                    write_terms<NI>(smem + Lay::v, kTileBytes, row, half * 4, x);
+                    if (!STATE) write_terms<NI>(smem + Lay::v, kTileBytes, row, half * 4, x);
                     fence_async();
                     warp_arrive(bar(kReadyV));
                 }
@@ -291,7 +300,7 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                 for (int j = 0; j < 16; ++j) S[p][j] = fmaf(S[p][j], keep, (x[0][j] + (x[1][j] + x[2][j])) * kv_scale);
             }
             if (!ok) break;
-            if (!REV && a.anchors != nullptr && boundary) {
+            if (!REV && !STATE && a.anchors != nullptr && boundary) {
                 // in the threads' own order: the sweep that reads them has the same threads
                 float *anchor = static_cast<float *>(a.anchors) + ((bh * segments + (end - 1) / kSegment) * tiles + vt) * PANELS * 4096 + tid;
 #pragma unroll
@@ -300,7 +309,12 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                     for (int j = 0; j < 16; ++j) anchor[(p * 16 + j) * kStateThreads] = S[p][j];
             }
         }
-        if (a.final != nullptr)
+        if (STATE) {
+#pragma unroll
+            for (int p = 0; p < PANELS; ++p)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) parts[(p * 16 + j) * kStateThreads] = S[p][j];
+        } else if (a.final != nullptr && part == a.splits - 1)
             all_state(a.final_transposed, [&](float &v, long long at) { static_cast<float *>(a.final)[at] = v; });
     } else if (warp < 16) {
         // ------------------------------------------------------------------ P = scores, weighted; out
@@ -313,7 +327,7 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
         constexpr int G = 16 / (int)sizeof(T);              // values of an access of an output row
         const int tid_out = tid - kStateThreads;
 #pragma unroll 1
-        for (int i = 0; i < pieces; ++i) {
+        for (int i = 0; i < (STATE ? 0 : pieces); ++i) {
             const uint32_t ph = i & 1;
             const long long t0 = piece_start(i), t = t0 + row;
             const int m = (int)(n - t0 < kPiece ? n - t0 : kPiece);
@@ -422,9 +436,9 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
             if (dot_row != nullptr && t < a.L) a.dots[((long long)(vt * 2 + half) * a.B * a.L + b * a.L + t) * a.H + h] = dot;
         }
         // rows behind the last piece
-        const long long first = (long long)pieces * kPiece;
-        for (long long e = tid_out; e < (a.L - first) * 16; e += kOutThreads) {
-            const long long t = first + e / 16;
+        const long long end = STATE || part < a.splits - 1 ? a.L : (long long)all * kPiece;
+        for (long long e = tid_out; e < (a.L - end) * 16; e += kOutThreads) {
+            const long long t = end + e / 16;
             const int col = vt * 64 + (int)(e % 16) * 4;
             if (col >= a.d2) continue;
             const long long at = ((b * a.L + t) * a.H + h) * a.d2 + col;
@@ -432,8 +446,8 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
             else *reinterpret_cast<uint2 *>(out_t + at) = make_uint2(0u, 0u);
         }
         if (dot_row != nullptr)
-            for (long long e = tid_out; e < (a.L - first) * 2; e += kOutThreads)
-                a.dots[((vt * 2 + e % 2) * a.B * a.L + b * a.L + first + e / 2) * a.H + h] = 0.f;
+            for (long long e = tid_out; e < (a.L - end) * 2; e += kOutThreads)
+                a.dots[((vt * 2 + e % 2) * a.B * a.L + b * a.L + end + e / 2) * a.H + h] = 0.f;
     } else if (warp == 16) {
         // ------------------------------------------------------------------ products
         const uint32_t lead = lane == 0, base16 = base >> 4;
@@ -445,12 +459,12 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
             for (int p = 0; p < PANELS; ++p) {
                 const int idx = i * PANELS + p;
                 ok = warp_wait(bar(kReady), idx & 1, failed);
-                if (ok && p == 0 && i > 0) ok = warp_wait(bar(kO1), ph ^ 1, failed);   // P of the piece before has been used
+                if (!STATE && ok && p == 0 && i > 0) ok = warp_wait(bar(kO1), ph ^ 1, failed);   // P of the piece before has been used
                 if (!ok) break;
                 fence_after();
                 // scores += R K^T
 #pragma unroll 1
-                for (int pair = 0; pair < pair_count(NI, NI, LEVEL); ++pair) {
+                for (int pair = 0; pair < (STATE ? 0 : pair_count(NI, NI, LEVEL)); ++pair) {
                     const int x = (int)(pair_list(NI, NI, LEVEL) >> (4 * pair)) & 3, y = (int)(pair_list(NI, NI, LEVEL) >> (4 * pair + 2)) & 3;
                     const uint32_t r16 = base16 + ((Lay::r + x * kTileBytes) >> 4), k16 = base16 + ((Lay::k + y * kTileBytes) >> 4);
 #pragma unroll
@@ -458,13 +472,13 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                         mma_ss(tmem, tile_desc(r16 + j * 2, 16), tile_desc(k16 + j * 2, 16), instr_desc<bf16>(128, false, false),
                                p > 0 || pair > 0 || j > 0, lead);
                 }
-                if (p == PANELS - 1) mma_commit(bar(kScores), lead);
-                if (p == 0 && i > 0) ok = warp_wait(bar(kEpi), ph ^ 1, failed);        // O2 and O1 of the piece before have been read
+                if (p == PANELS - 1 && !STATE) mma_commit(bar(kScores), lead);
+                if (!STATE && p == 0 && i > 0) ok = warp_wait(bar(kEpi), ph ^ 1, failed);        // O2 and O1 of the piece before have been read
                 if (!ok) break;
                 fence_after();
                 // O2 += R S
 #pragma unroll 1
-                for (int pair = 0; pair < pair_count(NI, Lay::NS, LEVEL); ++pair) {
+                for (int pair = 0; pair < (STATE ? 0 : pair_count(NI, Lay::NS, LEVEL)); ++pair) {
                     const int x = (int)(pair_list(NI, Lay::NS, LEVEL) >> (4 * pair)) & 3, y = (int)(pair_list(NI, Lay::NS, LEVEL) >> (4 * pair + 2)) & 3;
                     const uint32_t r16 = base16 + ((Lay::r + x * kTileBytes) >> 4), s16 = base16 + ((Lay::s + y * 8192) >> 4);
 #pragma unroll
@@ -473,7 +487,7 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                                p > 0 || pair > 0 || j > 0, lead);
                 }
                 if (p == 0) ok = warp_wait(bar(kReadyV), ph, failed);
-                else ok = warp_wait(bar(kIncRead), (idx - 1) & 1, failed);
+                if (STATE ? idx > 0 : p > 0) ok = ok && warp_wait(bar(kIncRead), (idx - 1) & 1, failed);
                 if (!ok) break;
                 fence_after();
                 // I = K^T V', term x of K with the terms 0 .. 2 - x of V'; the state's 64 rows twice (the distance of the second
@@ -489,6 +503,7 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                 mma_commit(bar(kInc), lead);
             }
             if (!ok) break;
+            if constexpr (STATE) continue;
             ok = warp_wait(bar(kP), ph, failed) && warp_wait(bar(kIncRead), (i * PANELS + PANELS - 1) & 1, failed);
             if (!ok) break;
             fence_after();
@@ -519,10 +534,10 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
             auto load_rk = [&](int idx) {
                 if (!lead) return;
                 const int t0 = (int)piece_start(idx / PANELS), x0 = idx % PANELS * 64;
-                bar_expect(bar(kRaw), 2 * RAW_BOXES * kTileBytes);
+                bar_expect(bar(kRaw), (STATE ? 1 : 2) * RAW_BOXES * kTileBytes);
 #pragma unroll
                 for (int p = 0; p < RAW_BOXES; ++p) {
-                    tma_load(base + Lay::r + p * kTileBytes, &map_r, bar(kRaw), x0 + p * per_box, rh, t0, (int)b);
+                    if (!STATE) tma_load(base + Lay::r + p * kTileBytes, &map_r, bar(kRaw), x0 + p * per_box, rh, t0, (int)b);
                     tma_load(base + Lay::k + p * kTileBytes, &map_k, bar(kRaw), x0 + p * per_box, kh, t0, (int)b);
                 }
             };
@@ -545,7 +560,7 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                 ++loaded;
                 const int i = idx / PANELS;
                 if (idx % PANELS != PANELS - 1) continue;
-                ok = warp_wait(bar(kO1), i & 1, failed);           // the last product that reads V
+                if (!STATE) ok = warp_wait(bar(kO1), i & 1, failed);           // the last product that reads V
                 if (!ok) break;
                 load_v(i + 1);
                 ++loaded_v;
@@ -558,7 +573,8 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
         }
     } else {
         const float *g = static_cast<const float *>(a.decay) + b * a.decay_stride[0] + h * a.decay_stride[2];
-        sum_decays<REV>(g, a.decay_stride[1], n, pieces, tables, bar(kDecFull0), bar(kDecFree0), failed);
+        const double whole = sum_decays<REV>(g, a.decay_stride[1], n, first, pieces, tables, bar(kDecFull0), bar(kDecFree0), failed);
+        if (STATE && vt == 0 && lane == 0) a.split_decays[bh * a.splits + part] = (float)whole;
     }
     fence_before();
     __syncthreads();
@@ -576,11 +592,18 @@ int launch_split(const Sweep &a, int dtype, cudaStream_t stream)
     if (encoder() == nullptr || !encode(&r, a.r, a, a.d1, dtype) || !encode(&k, a.k, a, a.d1, dtype) ||
         !encode(&v, a.v, a, a.d2, dtype))
         return PSIG_ERR_CUDA;
-    auto kernel = attn_sweep_split_terms<T, PANELS, LEVEL, REV>;
-    if (!prepare_kernel(kernel, Lay::alloc, true)) return PSIG_ERR_CUDA;
-    const long long blocks = a.B * a.H * ((a.d2 + 63) / 64);
-    kernel<<<(unsigned)blocks, kSplitThreads, Lay::alloc, stream>>>(r, k, v, a);
-    return check_launch();
+    const int tiles = tile_columns(a.d2);
+    const unsigned blocks = (unsigned)(a.B * a.H * tiles);
+    auto launch = [&](auto kernel, int parts) {
+        if (!prepare_kernel(kernel, Lay::alloc, true)) return (int)PSIG_ERR_CUDA;
+        kernel<<<dim3(blocks, parts), kSplitThreads, Lay::alloc, stream>>>(r, k, v, a);
+        return check_launch();
+    };
+    if (a.splits > 1) {
+        int rc = launch(attn_sweep_split_terms<T, PANELS, LEVEL, REV, true>, a.splits - 1);
+        if (rc != PSIG_OK || (rc = chain_states(a, 4096LL * PANELS * tiles, stream)) != PSIG_OK) return rc;
+    }
+    return launch(attn_sweep_split_terms<T, PANELS, LEVEL, REV, false>, a.splits);
 }
 
 template <typename T, int LEVEL>

@@ -65,7 +65,7 @@ struct TileLayout {
     static constexpr int columns = 512;
 };
 
-template <typename T, int KP, int NS, int NV, bool DOT, bool REV>
+template <typename T, int KP, int NS, int NV, bool DOT, bool REV, bool STATE>
 __global__ void __launch_bounds__(kTileThreads, 1)
 attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_out,
@@ -90,9 +90,11 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
         n = a.lengths[b];
         n = n < 0 ? 0 : n > a.L ? a.L : n;
     }
-    const int pieces = (int)((n + kPiece - 1) / kPiece);
+    const int all = (int)((n + kPiece - 1) / kPiece);                 // pieces of the sequence
+    const int part = blockIdx.y;
+    const int first = (int)((long long)all * part / a.splits), pieces = (int)((long long)all * (part + 1) / a.splits) - first;
     const long long segments = (a.L + kSegment - 1) / kSegment;
-    auto piece_start = [&](int i) { return (long long)(REV ? pieces - 1 - i : i) * kPiece; };
+    auto piece_start = [&](int i) { return (long long)(REV ? all - 1 - first - i : first + i) * kPiece; };
 
     if (tid == 0) {
         bar_init(bar(kFullRK), 1);
@@ -111,7 +113,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
         bar_init(bar(kDotFree), kOutThreads / 32);
         for (int i = 0; i < 2; ++i) {
             bar_init(bar(kDecFull0 + i), 1);
-            bar_init(bar(kDecFree0 + i), (kStateThreads + kScoreThreads + kOutThreads) / 32);
+            bar_init(bar(kDecFree0 + i), (kStateThreads + (STATE ? 0 : kScoreThreads + kOutThreads)) / 32);
         }
         failed[0] = failed[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -167,9 +169,14 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
         };
 #pragma unroll
         for (int j = 0; j < SC; ++j) S[j] = 0.f;
-        if (a.init != nullptr)
+        float *parts = a.split_states + ((bh * a.splits + part) * tiles + vt) * KP * 64 + tid;   // this part's, in the threads' order
+        if (part > 0 && !STATE) {
+            parts -= (long long)tiles * KP * 64;
+#pragma unroll
+            for (int j = 0; j < SC; ++j) S[j] = parts[j * kStateThreads];
+        } else if (part == 0 && a.init != nullptr)
             all_state(a.init_transposed, state0, [&](float &v, long long at) { v = static_cast<const float *>(a.init)[at]; });
-        store_terms();
+        if (!STATE) store_terms();
         const float kv_scale = (float)a.kv_scale;
 #pragma unroll 1
         for (int i = 0; i < pieces; ++i) {
@@ -220,7 +227,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
             fence_async();
             warp_arrive(bar(kVReady));
             warp_arrive(bar(kDecFree0 + (i & 1)));
-            if (REV && a.anchor_dots != nullptr && boundary) {
+            if (REV && !STATE && a.anchor_dots != nullptr && boundary) {
                 // the state behind this piece against the stored state of the steps up to here
                 const long long segment = (end - 1) / kSegment;
                 const float *anchor = static_cast<const float *>(a.anchors) + ((bh * segments + segment) * tiles + vt) * KP * 64 + tid;
@@ -238,21 +245,25 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
             tmem_loaded();
 #pragma unroll
             for (int j = 0; j < SC; ++j) S[j] = fmaf(S[j], keep, x[j / 16][j % 16] * kv_scale);
-            store_terms();
-            if (!REV && a.anchors != nullptr && boundary) {
+            if (STATE) fence_before();
+            else store_terms();
+            if (!REV && !STATE && a.anchors != nullptr && boundary) {
                 // in the threads' own order: the sweep that reads them has the same threads
                 float *anchor = static_cast<float *>(a.anchors) + ((bh * segments + (end - 1) / kSegment) * tiles + vt) * KP * 64 + tid;
 #pragma unroll
                 for (int j = 0; j < SC; ++j) anchor[j * kStateThreads] = S[j];
             }
         }
-        if (a.final != nullptr)
+        if (STATE) {
+#pragma unroll
+            for (int j = 0; j < SC; ++j) parts[j * kStateThreads] = S[j];
+        } else if (a.final != nullptr && part == a.splits - 1)
             all_state(a.final_transposed, state0, [&](float &v, long long at) { static_cast<float *>(a.final)[at] = v; });
     } else if (warp < 16) {
         // ------------------------------------------------------------------ P = scores, weighted
         const uint32_t own = tmem + lanes + half * 64;   // this thread's columns of the scores
 #pragma unroll 1
-        for (int i = 0; i < pieces; ++i) {
+        for (int i = 0; i < (STATE ? 0 : pieces); ++i) {
             const DecayTables &d = tables[i & 1];
             if (!warp_wait(bar(kDecFull0 + (i & 1)), (i >> 1) & 1, failed)) break;
             const float la = d.la[row];
@@ -315,7 +326,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
         const bool writer = tid == kStateThreads + kScoreThreads;   // starts the copies of the output tiles
         const int col0 = vt * 64;
 #pragma unroll 1
-        for (int i = 0; i < pieces; ++i) {
+        for (int i = 0; i < (STATE ? 0 : pieces); ++i) {
             const long long t0 = piece_start(i), t = t0 + row;
             const int m = (int)(n - t0 < kPiece ? n - t0 : kPiece);
             if (!warp_wait(bar(kDecFull0 + (i & 1)), (i >> 1) & 1, failed)) break;
@@ -393,9 +404,9 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
             }
         }
         // rows behind the last piece
-        const long long first = (long long)pieces * kPiece;
-        for (long long e = tid - (kStateThreads + kScoreThreads); e < (a.L - first) * 8; e += kOutThreads) {
-            const long long t = first + e / 8;
+        const long long end = STATE || part < a.splits - 1 ? a.L : (long long)all * kPiece;
+        for (long long e = tid - (kStateThreads + kScoreThreads); e < (a.L - end) * 8; e += kOutThreads) {
+            const long long t = end + e / 8;
             const int col = col0 + (int)(e % 8) * 8;
             if (col >= a.d2) continue;
             const long long at = ((b * a.L + t) * a.H + h) * a.d2 + col;
@@ -404,18 +415,35 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
             if (a.out_acc) *reinterpret_cast<uint4 *>(out_f + at + 4) = zero;
         }
         if (DOT)
-            for (long long t = first + tid - (kStateThreads + kScoreThreads); t < a.L; t += kOutThreads)
+            for (long long t = end + tid - (kStateThreads + kScoreThreads); t < a.L; t += kOutThreads)
                 a.dots[((long long)vt * a.B * a.L + b * a.L + t) * a.H + h] = 0.f;
         if (writer) tma_store_done();
     } else if (warp == 20) {
         // ------------------------------------------------------------------ TMA and MMA
         if (pieces > 0) {
             const uint32_t lead = lane == 0, base16 = base >> 4;
+            // I = K^T V'; with 64 state rows the second block of 64 is the first once more
+            auto state_product = [&]() {
+#pragma unroll
+                    for (int term = NV - 1; term >= 0; --term)
+#pragma unroll
+                        for (int j = 0; j < kPiece / 16; ++j)
+                            mma_ss(tmem + Lay::c_i, tile_desc(base16 + ((Lay::k + j * 2048) >> 4), KP == 128 ? kTileBytes : 0),
+                                   tile_desc(base16 + ((Lay::vw + term * kTileBytes + j * 2048) >> 4), kTileBytes), instr_desc<T>(64, true, true),
+                                   term < NV - 1 || j > 0, lead);
+                    mma_commit(bar(kInc), lead);
+            };
 #pragma unroll 1
             for (int i = 0; i < pieces; ++i) {
                 const uint32_t ph = i & 1;
                 if (!warp_wait(bar(kFullRK), ph, failed)) break;
                 if (a.lengths != nullptr && n - piece_start(i) < kPiece && !warp_wait(bar(kFix), 0, failed)) break;
+                if constexpr (STATE) {   // I alone
+                    if (!warp_wait(bar(kVReady), ph, failed)) break;
+                    fence_after();
+                    state_product();
+                    continue;
+                }
                 if (i > 0 && !warp_wait(bar(kO1), ph ^ 1, failed)) break;   // P of the piece before has been used
                 if (DOT && !(warp_wait(bar(kDot), ph, failed) && warp_wait(bar(kFullV0), ph, failed))) break;
                 fence_after();
@@ -445,15 +473,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                         mma_ss(tmem + Lay::c_o2, tile_desc(base16 + ((Lay::r + (j / 4) * kTileBytes + (j % 4) * 32) >> 4), 16),
                                tile_desc(base16 + ((Lay::s + term * KP * 128 + j * 2048) >> 4), kTileBytes), instr_desc<T>(64, false, true),
                                term < NS - 1 || j > 0, lead);
-                // I = K^T V'; with 64 state rows the second block of 64 is the first once more
-#pragma unroll
-                for (int term = NV - 1; term >= 0; --term)
-#pragma unroll
-                    for (int j = 0; j < kPiece / 16; ++j)
-                        mma_ss(tmem + Lay::c_i, tile_desc(base16 + ((Lay::k + j * 2048) >> 4), KP == 128 ? kTileBytes : 0),
-                               tile_desc(base16 + ((Lay::vw + term * kTileBytes + j * 2048) >> 4), kTileBytes), instr_desc<T>(64, true, true),
-                               term < NV - 1 || j > 0, lead);
-                mma_commit(bar(kInc), lead);
+                state_product();
                 // O1 = P V
                 const uint32_t v16 = base16 + (Lay::v >> 4) + (VS == 2 ? ph * (kTileBytes >> 4) : 0);
                 if (!warp_wait(bar(kP), ph, failed)) break;
@@ -473,10 +493,10 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
             auto load_rk = [&](int i) {
                 if (!lead) return;
                 const int t0 = (int)piece_start(i);
-                bar_expect(bar(kFullRK), 2 * Lay::panels * kTileBytes);
+                bar_expect(bar(kFullRK), (STATE ? 1 : 2) * Lay::panels * kTileBytes);
 #pragma unroll
                 for (int p = 0; p < Lay::panels; ++p) {
-                    tma_load(base + Lay::r + p * kTileBytes, &map_r, bar(kFullRK), p * 64, rh, t0, (int)b);
+                    if (!STATE) tma_load(base + Lay::r + p * kTileBytes, &map_r, bar(kFullRK), p * 64, rh, t0, (int)b);
                     tma_load(base + Lay::k + p * kTileBytes, &map_k, bar(kFullRK), p * 64, kh, t0, (int)b);
                 }
             };
@@ -506,7 +526,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                 load_rk(i + 1);
                 ++loaded_rk;
                 if (loaded_v == pieces) continue;
-                if (!warp_wait(bar(kO1), i & 1, failed)) break;     // the last product that reads V
+                if (!STATE && !warp_wait(bar(kO1), i & 1, failed)) break;     // the last product that reads V
                 load_v(loaded_v++);
             }
             if (*failed) {
@@ -519,7 +539,8 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
         }
     } else {
         const float *g = static_cast<const float *>(a.decay) + b * a.decay_stride[0] + h * a.decay_stride[2];
-        sum_decays<REV>(g, a.decay_stride[1], n, pieces, tables, bar(kDecFull0), bar(kDecFree0), failed);
+        const double whole = sum_decays<REV>(g, a.decay_stride[1], n, first, pieces, tables, bar(kDecFull0), bar(kDecFree0), failed);
+        if (STATE && vt == 0 && lane == 0) a.split_decays[bh * a.splits + part] = (float)whole;
     }
     fence_before();
     __syncthreads();
@@ -534,17 +555,26 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
 template <typename T, int KP, int NS, int NV, bool DOT, bool REV>
 int launch_tiles(const Sweep &a, int dtype, cudaStream_t stream)
 {
-    using Lay = TileLayout<KP, NS, NV, DOT>;
     CUtensorMap r, k, v, out, dot;
     const SweepOperand o{a.out, {a.L * a.H * a.d2, (long long)a.H * a.d2, a.d2}, 1};
     if (encoder() == nullptr || !encode(&r, a.r, a, a.d1, dtype) || !encode(&k, a.k, a, a.d1, dtype) ||
         !encode(&v, a.v, a, a.d2, dtype) || !encode(&out, o, a, a.d2, dtype) ||
         !encode(&dot, a.dot.data ? a.dot : o, a, a.d2, dtype))
         return PSIG_ERR_CUDA;
-    auto kernel = attn_sweep_tiles<T, KP, NS, NV, DOT, REV>;
+    const int tiles = tile_columns(a.d2);
+    const unsigned blocks = (unsigned)(a.B * a.H * tiles);
+    if (a.splits > 1) {
+        using Lay = TileLayout<KP, 1, 3, false>;
+        auto kernel = attn_sweep_tiles<T, KP, 1, 3, false, REV, true>;
+        if (!prepare_kernel(kernel, Lay::alloc, true)) return PSIG_ERR_CUDA;
+        kernel<<<dim3(blocks, a.splits - 1), kTileThreads, Lay::alloc, stream>>>(r, k, v, out, dot, a);
+        int rc = check_launch();
+        if (rc != PSIG_OK || (rc = chain_states(a, (long long)KP * 64 * tiles, stream)) != PSIG_OK) return rc;
+    }
+    using Lay = TileLayout<KP, NS, NV, DOT>;
+    auto kernel = attn_sweep_tiles<T, KP, NS, NV, DOT, REV, false>;
     if (!prepare_kernel(kernel, Lay::alloc, true)) return PSIG_ERR_CUDA;
-    const long long blocks = a.B * a.H * ((a.d2 + 63) / 64);
-    kernel<<<(unsigned)blocks, kTileThreads, Lay::alloc, stream>>>(r, k, v, out, dot, a);
+    kernel<<<dim3(blocks, a.splits), kTileThreads, Lay::alloc, stream>>>(r, k, v, out, dot, a);
     return check_launch();
 }
 

@@ -78,7 +78,27 @@ struct Sweep {
     // each warp's columns: (attn_tile_dots * column tiles of 64, B, L, H).
     SweepOperand dot;
     float *dots;
+    // Tensor-core sweeps of few long sequences: parts of a sequence (see split_plan), and the scratch for their states
+    // (B, H, splits, tiles of 64 by 64) and decays (B, H, splits).
+    int splits;
+    float *split_states, *split_decays;
 };
+
+inline int tile_columns(int d2) { return (d2 + 63) / 64; }
+inline long long split_state_size(int d1, int d2) { return 4096LL * tile_columns(d1) * tile_columns(d2); }
+
+// Parts to cut each sequence into.  A block sweeps one column tile of one head, so few long sequences leave most of the 148 SMs
+// idle.  The first launch over the parts costs about half a sweep, so parts pay from three on; a part is at least
+// four pieces long.  (16 heads of 128, 16384 steps: 412 us in one part, see launch_tiles for four.)
+inline int split_plan(long long B, long long L, int H, int d2)
+{
+    const long long blocks = B * H * tile_columns(d2), pieces = (L + 127) / 128;
+    if (blocks == 0 || blocks * 2 > 148) return 1;
+    long long splits = 148 / blocks;
+    if (splits > pieces / 4) splits = pieces / 4;
+    if (splits > 64) splits = 64;
+    return splits < 2 ? 1 : (int)splits;
+}
 
 inline long long segments_of(long long L) { return (L + kSegment - 1) / kSegment; }
 
@@ -92,6 +112,5 @@ long long attn_split_timeouts();
 long long norm_timeouts();
 inline int attn_tile_dots(int dtype) { return dtype == PSIG_BF16 ? 1 : 2; }   // at most 2
 constexpr int kTileDots = 8;   // parts of an anchor's sum per column tile of 64
-inline int tile_columns(int d2) { return (d2 + 63) / 64; }
 
 }  // namespace psig

@@ -187,15 +187,18 @@ __device__ __forceinline__ void tma_store_done() { asm volatile("cp.async.bulk.w
 
 __device__ __forceinline__ uint32_t swizzled(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
 
-// One warp: the decay tables of the sweep's pieces, one piece ahead of their use, in two buffers in turn.
+// One warp: the decay tables of `pieces` of the sweep's pieces from number `first` on, one piece ahead of their use, in two
+// buffers in turn.  Returns the sum of all their decays (exponent of 2).
 template <bool REV>
-__device__ __forceinline__ void sum_decays(const float *g, long long stride, long long n, int pieces, DecayTables *tables,
-                                           uint32_t full0, uint32_t free0, volatile int *failed)
+__device__ __forceinline__ double sum_decays(const float *g, long long stride, long long n, int first, int pieces, DecayTables *tables,
+                                             uint32_t full0, uint32_t free0, volatile int *failed)
 {
+    const int all = (int)((n + kPiece - 1) / kPiece);
+    double whole = 0.0;
     const int lane = threadIdx.x & 31;
 #pragma unroll 1
     for (int i = 0; i < pieces; ++i) {
-        const long long t0 = (long long)(REV ? pieces - 1 - i : i) * kPiece;
+        const long long t0 = (long long)(REV ? all - 1 - first - i : first + i) * kPiece;
         const int m = (int)(n - t0 < kPiece ? n - t0 : kPiece);
         double c[4];
         double sum = 0.0;
@@ -215,6 +218,7 @@ __device__ __forceinline__ void sum_decays(const float *g, long long stride, lon
         }
         const double end = __shfl_sync(0xffffffffu, before, 31);
         before -= sum;
+        whole += end;
 #pragma unroll
         for (int j = 0; j < 4; ++j) c[j] = REV ? end - (before + c[j]) : before + c[j];
         // the low end of each block of 32 steps: its last step, or, in reverse, its first
@@ -233,6 +237,24 @@ __device__ __forceinline__ void sum_decays(const float *g, long long stride, lon
         }
         if (lane == 0) d.keep = exp_two((float)end);
             warp_arrive(full0 + 8 * (i & 1));
+    }
+    return whole;
+}
+
+// Parts of a long sequence, each swept by a block of its own: a first launch computes every part's state (all but the last; the
+// first from the initial state), these are chained, and the sweep starts each part from the state before it.
+__global__ void __launch_bounds__(256) chain_split_states(float *__restrict__ states, const float *__restrict__ decays, int splits,
+                                                          long long per_part, long long per_head)
+{
+    // states (heads, splits, per_part), decays (heads, splits); parts of one head are chained in order
+    const long long head = blockIdx.x;
+    const long long e = (long long)blockIdx.y * 256 + threadIdx.x;
+    if (e >= per_part) return;
+    float *s = states + head * splits * per_part + e;
+    float before = s[0];
+    for (int i = 1; i + 1 < splits; ++i) {
+        before = fmaf(before, exp_two(decays[head * per_head + i]), s[i * per_part]);
+        s[i * per_part] = before;
     }
 }
 
@@ -273,6 +295,14 @@ inline bool encode(CUtensorMap *map, const SweepOperand &o, const Sweep &a, int 
     // a thread that has made no runtime call yet (autograd's) has no current context, which the driver call wants
     int device = 0;
     return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess && call() == CUDA_SUCCESS;
+}
+
+inline int chain_states(const Sweep &a, long long per_part, cudaStream_t stream)
+{
+    if (a.splits < 3) return PSIG_OK;
+    chain_split_states<<<dim3((unsigned)(a.B * a.H), (unsigned)((per_part + 255) / 256)), 256, 0, stream>>>(
+        a.split_states, a.split_decays, a.splits, per_part, a.splits);
+    return check_launch();
 }
 
 bool operand_fits(const SweepOperand &o, const Sweep &a, int d, int size)
