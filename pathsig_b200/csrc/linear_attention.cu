@@ -616,7 +616,7 @@ int run_backward_tiles(const Call &c, const void *init, const void *gs, void *gr
     Sweep s = c.grad_q();
     s.init = init;
     s.out = grad_q;
-    if (grad_decay != nullptr) s.anchors = ws + at.anchors, s.dot = c.q, s.dots = x;
+    if (grad_decay != nullptr) s.anchors = ws + at.anchors, s.keep_last = gs != nullptr, s.dot = c.q, s.dots = x;
     set_splits(s, ws + at.parts);
     if ((rc = attn_sweep_on_tiles(s, grad_decay != nullptr, d.dtype, stream)) != PSIG_OK) return rc;
     s = c.grad_k();

@@ -573,7 +573,8 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
         }
     } else {
         const float *g = static_cast<const float *>(a.decay) + b * a.decay_stride[0] + h * a.decay_stride[2];
-        const double whole = sum_decays<REV>(g, a.decay_stride[1], n, first, pieces, tables, bar(kDecFull0), bar(kDecFree0), failed);
+        int count = 0;
+        const double whole = sum_decays<REV>(g, a.decay_stride[1], n, first, pieces, count, tables, bar(kDecFull0), bar(kDecFree0), failed);
         if (STATE && vt == 0 && lane == 0) a.split_decays[bh * a.splits + part] = (float)whole;
     }
     fence_before();

@@ -82,19 +82,8 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int tiles = (a.d2 + 63) / 64;
-    const int vt = blockIdx.x % tiles;
-    const long long bh = blockIdx.x / tiles, b = bh / a.H;
-    const int h = (int)(bh % a.H);
-    long long n = a.L;
-    if (a.lengths != nullptr) {
-        n = a.lengths[b];
-        n = n < 0 ? 0 : n > a.L ? a.L : n;
-    }
-    const int all = (int)((n + kPiece - 1) / kPiece);                 // pieces of the sequence
-    const int part = blockIdx.y;
-    const int first = (int)((long long)all * part / a.splits), pieces = (int)((long long)all * (part + 1) / a.splits) - first;
+    const int part = blockIdx.y, items = (int)(a.B * a.H * tiles);
     const long long segments = (a.L + kSegment - 1) / kSegment;
-    auto piece_start = [&](int i) { return (long long)(REV ? all - 1 - first - i : first + i) * kPiece; };
 
     if (tid == 0) {
         bar_init(bar(kFullRK), 1);
@@ -133,22 +122,18 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
     const int row = quarter * 32 + lane;                 // time step in the piece, or lane of tensor memory
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
 
+    // Pieces that nothing stands before (O2 is 0), and whose state nobody asks for (no V', no I)
+    auto no_past = [&](const Item &it, int i) { return !STATE && it.first + i == 0 && a.init == nullptr; };
+    auto no_future = [&](const Item &it, int i) {
+        return !STATE && it.first + i + 1 == it.all && a.final == nullptr && !(DOT && !REV && a.keep_last);
+    };
+
     if (warp < 8) {
         // ------------------------------------------------------------------ the state, and V' = tail weights times V
         constexpr int SC = KP == 128 ? 32 : 16;   // state columns per thread (64 state rows stand twice in the 128 lanes)
         const int srow = KP == 128 ? row : (quarter & 1) * 32 + lane;
         const int sc0 = KP == 128 ? half * 32 : (quarter >> 1) * 32 + half * 16;
-        const int gcol0 = vt * 64 + sc0;
-        const long long state0 = bh * a.d1 * a.d2;
         float S[SC];
-        auto all_state = [&](bool transposed, long long first, auto fn) {   // fn(value, its position), (d1, d2) or (d2, d1)
-            if (srow >= a.d1) return;
-            const int step = transposed ? a.d1 : 1;
-            long long at = first + (transposed ? (long long)gcol0 * a.d1 + srow : (long long)srow * a.d2 + gcol0);
-#pragma unroll
-            for (int j = 0; j < SC; ++j, at += step)
-                if (gcol0 + j < a.d2) fn(S[j], at);
-        };
         auto store_terms = [&]() {   // S as the B operand of R S: rows = state rows, 64 columns to a row
 #pragma unroll
             for (int c = 0; c < SC / 8; ++c) {
@@ -167,156 +152,181 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
             }
             fence_before();
         };
-#pragma unroll
-        for (int j = 0; j < SC; ++j) S[j] = 0.f;
-        float *parts = a.split_states + ((bh * a.splits + part) * tiles + vt) * KP * 64 + tid;   // this part's, in the threads' order
-        if (part > 0 && !STATE) {
-            parts -= (long long)tiles * KP * 64;
-#pragma unroll
-            for (int j = 0; j < SC; ++j) S[j] = parts[j * kStateThreads];
-        } else if (part == 0 && a.init != nullptr)
-            all_state(a.init_transposed, state0, [&](float &v, long long at) { v = static_cast<const float *>(a.init)[at]; });
-        if (!STATE) store_terms();
         const float kv_scale = (float)a.kv_scale;
+        int g = 0;
+        bool ok = true;
 #pragma unroll 1
-        for (int i = 0; i < pieces; ++i) {
-            const uint32_t ph = i & 1;
-            const long long t0 = piece_start(i);
-            const int m = (int)(n - t0 < kPiece ? n - t0 : kPiece);
-            const long long end = t0 + m;
-            const bool boundary = end == n || end % kSegment == 0;
-            const DecayTables &d = tables[i & 1];
-            if (!warp_wait(bar(kDecFull0 + (i & 1)), (i >> 1) & 1, failed)) break;
-            if (!warp_wait(bar(kFullV0 + i % VS), (i / VS) & 1, failed)) break;
-            const bool fix = a.lengths != nullptr && m < kPiece;
-            unsigned char *v_tile = smem + Lay::v + (i % VS) * kTileBytes;
-            if (fix) {
-                if (!warp_wait(bar(kFullRK), ph, failed)) break;
-                if (row >= m) {
-                    // rows behind the sequence's last step: whatever stands there must not reach a product
-                    const uint4 zero = {0, 0, 0, 0};
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            const Item it(a, item, tiles, part);
+            const int gcol0 = it.vt * 64 + sc0;
+            const long long state0 = it.bh * a.d1 * a.d2;
+            auto all_state = [&](bool transposed, long long first, auto fn) {   // fn(value, its position), (d1, d2) or (d2, d1)
+                if (srow >= a.d1) return;
+                const int step = transposed ? a.d1 : 1;
+                long long at = first + (transposed ? (long long)gcol0 * a.d1 + srow : (long long)srow * a.d2 + gcol0);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4 *>(v_tile + swizzled(row, half * 4 + c)) = zero;
+                for (int j = 0; j < SC; ++j, at += step)
+                    if (gcol0 + j < a.d2) fn(S[j], at);
+            };
 #pragma unroll
-                    for (int p = 0; p < Lay::panels; ++p)
+            for (int j = 0; j < SC; ++j) S[j] = 0.f;
+            float *parts = a.split_states + ((it.bh * a.splits + part) * tiles + it.vt) * KP * 64 + tid;   // this part's, in the threads' order
+            if (part > 0 && !STATE) {
+                parts -= (long long)tiles * KP * 64;
 #pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            *reinterpret_cast<uint4 *>(smem + Lay::k + p * kTileBytes + swizzled(row, half * 4 + c)) = zero;
+                for (int j = 0; j < SC; ++j) S[j] = parts[j * kStateThreads];
+            } else if (part == 0 && a.init != nullptr)
+                all_state(a.init_transposed, state0, [&](float &v, long long at) { v = static_cast<const float *>(a.init)[at]; });
+            if (!STATE) store_terms();
+#pragma unroll 1
+            for (int i = 0; i < it.pieces; ++i, ++g) {
+                const uint32_t ph = g & 1;
+                const long long t0 = it.start<REV>(i);
+                const int m = (int)(it.n - t0 < kPiece ? it.n - t0 : kPiece);
+                const long long end = t0 + m;
+                const bool boundary = end == it.n || end % kSegment == 0;
+                const DecayTables &d = tables[g & 1];
+                if (!(ok = warp_wait(bar(kDecFull0 + (g & 1)), (g >> 1) & 1, failed))) break;
+                if (!(ok = warp_wait(bar(kFullV0 + g % VS), (g / VS) & 1, failed))) break;
+                const bool fix = a.lengths != nullptr && m < kPiece;
+                unsigned char *v_tile = smem + Lay::v + (g % VS) * kTileBytes;
+                if (fix) {
+                    if (!(ok = warp_wait(bar(kFullRK), ph, failed))) break;
+                    if (row >= m) {
+                        // rows behind the sequence's last step: whatever stands there must not reach a product
+                        const uint4 zero = {0, 0, 0, 0};
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4 *>(v_tile + swizzled(row, half * 4 + c)) = zero;
+#pragma unroll
+                        for (int p = 0; p < Lay::panels; ++p)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c)
+                                *reinterpret_cast<uint4 *>(smem + Lay::k + p * kTileBytes + swizzled(row, half * 4 + c)) = zero;
+                    }
+                    fence_async();
+                    warp_arrive(bar(kFix));
+                }
+                const float w = d.tail[row], keep = d.keep;
+                const bool last = no_future(it, i);
+#pragma unroll 2
+                for (int c = 0; c < (last ? 0 : 4); ++c) {   // not wholly unrolled, like the loop over the scores: the roles' code has to stay in the instruction cache
+                    const uint32_t at = swizzled(row, half * 4 + c);
+                    const uint4 in = *reinterpret_cast<const uint4 *>(v_tile + at);
+                    float2 x[4] = {unpack(in.x, T{}), unpack(in.y, T{}), unpack(in.z, T{}), unpack(in.w, T{})};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[j].x *= w, x[j].y *= w;
+#pragma unroll
+                    for (int term = 0; term < NV; ++term) {
+                        uint4 o;
+                        o.x = next_term<T>(x[0].x, x[0].y, term == NV - 1);
+                        o.y = next_term<T>(x[1].x, x[1].y, term == NV - 1);
+                        o.z = next_term<T>(x[2].x, x[2].y, term == NV - 1);
+                        o.w = next_term<T>(x[3].x, x[3].y, term == NV - 1);
+                        *reinterpret_cast<uint4 *>(smem + Lay::vw + term * kTileBytes + at) = o;
+                    }
                 }
                 fence_async();
-                warp_arrive(bar(kFix));
-            }
-            const float w = d.tail[row], keep = d.keep;
-#pragma unroll 2
-            for (int c = 0; c < 4; ++c) {   // not wholly unrolled, like the loop over the scores: the roles' code has to stay in the instruction cache
-                const uint32_t at = swizzled(row, half * 4 + c);
-                const uint4 in = *reinterpret_cast<const uint4 *>(v_tile + at);
-                float2 x[4] = {unpack(in.x, T{}), unpack(in.y, T{}), unpack(in.z, T{}), unpack(in.w, T{})};
+                warp_arrive(bar(kVReady));
+                warp_arrive(bar(kDecFree0 + (g & 1)));
+                if (REV && !STATE && a.anchor_dots != nullptr && boundary) {
+                    // the state behind this piece against the stored state of the steps up to here
+                    const long long segment = (end - 1) / kSegment;
+                    const float *anchor = static_cast<const float *>(a.anchors) + ((it.bh * segments + segment) * tiles + it.vt) * KP * 64 + tid;
+                    float dot = 0.f;
+                    if (end != it.n || a.init != nullptr)   // behind the last step there is nothing else
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[j].x *= w, x[j].y *= w;
+                        for (int j = 0; j < SC; ++j) dot = fmaf(S[j], anchor[j * kStateThreads], dot);
+                    for (int s = 16; s >= 1; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
+                    if (lane == 0) static_cast<float *>(a.anchor_dots)[((it.bh * segments + segment) * tiles + it.vt) * 8 + warp] = dot;
+                }
+                if (!(ok = warp_wait(bar(kInc), ph, failed))) break;
+                if (last) continue;
+                fence_after();
+                float x[SC / 16][16];
 #pragma unroll
-                for (int term = 0; term < NV; ++term) {
-                    uint4 o;
-                    o.x = next_term<T>(x[0].x, x[0].y, term == NV - 1);
-                    o.y = next_term<T>(x[1].x, x[1].y, term == NV - 1);
-                    o.z = next_term<T>(x[2].x, x[2].y, term == NV - 1);
-                    o.w = next_term<T>(x[3].x, x[3].y, term == NV - 1);
-                    *reinterpret_cast<uint4 *>(smem + Lay::vw + term * kTileBytes + at) = o;
+                for (int c = 0; c < SC / 16; ++c) tmem_load16(tmem + lanes + Lay::c_i + sc0 + c * 16, x[c]);
+                tmem_loaded();
+#pragma unroll
+                for (int j = 0; j < SC; ++j) S[j] = fmaf(S[j], keep, x[j / 16][j % 16] * kv_scale);
+                if (STATE || i + 1 == it.pieces) fence_before();
+                else store_terms();
+                if (!REV && !STATE && a.anchors != nullptr && boundary) {
+                    // in the threads' own order: the sweep that reads them has the same threads
+                    float *anchor = static_cast<float *>(a.anchors) + ((it.bh * segments + (end - 1) / kSegment) * tiles + it.vt) * KP * 64 + tid;
+#pragma unroll
+                    for (int j = 0; j < SC; ++j) anchor[j * kStateThreads] = S[j];
                 }
             }
-            fence_async();
-            warp_arrive(bar(kVReady));
-            warp_arrive(bar(kDecFree0 + (i & 1)));
-            if (REV && !STATE && a.anchor_dots != nullptr && boundary) {
-                // the state behind this piece against the stored state of the steps up to here
-                const long long segment = (end - 1) / kSegment;
-                const float *anchor = static_cast<const float *>(a.anchors) + ((bh * segments + segment) * tiles + vt) * KP * 64 + tid;
-                float dot = 0.f;
+            if (STATE) {
 #pragma unroll
-                for (int j = 0; j < SC; ++j) dot = fmaf(S[j], anchor[j * kStateThreads], dot);
-                for (int s = 16; s >= 1; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
-                if (lane == 0) static_cast<float *>(a.anchor_dots)[((bh * segments + segment) * tiles + vt) * 8 + warp] = dot;
-            }
-            if (!warp_wait(bar(kInc), ph, failed)) break;
-            fence_after();
-            float x[SC / 16][16];
-#pragma unroll
-            for (int c = 0; c < SC / 16; ++c) tmem_load16(tmem + lanes + Lay::c_i + sc0 + c * 16, x[c]);
-            tmem_loaded();
-#pragma unroll
-            for (int j = 0; j < SC; ++j) S[j] = fmaf(S[j], keep, x[j / 16][j % 16] * kv_scale);
-            if (STATE) fence_before();
-            else store_terms();
-            if (!REV && !STATE && a.anchors != nullptr && boundary) {
-                // in the threads' own order: the sweep that reads them has the same threads
-                float *anchor = static_cast<float *>(a.anchors) + ((bh * segments + (end - 1) / kSegment) * tiles + vt) * KP * 64 + tid;
-#pragma unroll
-                for (int j = 0; j < SC; ++j) anchor[j * kStateThreads] = S[j];
-            }
+                for (int j = 0; j < SC; ++j) parts[j * kStateThreads] = S[j];
+            } else if (a.final != nullptr && part == a.splits - 1)
+                all_state(a.final_transposed, state0, [&](float &v, long long at) { static_cast<float *>(a.final)[at] = v; });
         }
-        if (STATE) {
-#pragma unroll
-            for (int j = 0; j < SC; ++j) parts[j * kStateThreads] = S[j];
-        } else if (a.final != nullptr && part == a.splits - 1)
-            all_state(a.final_transposed, state0, [&](float &v, long long at) { static_cast<float *>(a.final)[at] = v; });
     } else if (warp < 16) {
         // ------------------------------------------------------------------ P = scores, weighted
         const uint32_t own = tmem + lanes + half * 64;   // this thread's columns of the scores
+        int g = 0;
+        bool ok = !STATE;
 #pragma unroll 1
-        for (int i = 0; i < (STATE ? 0 : pieces); ++i) {
-            const DecayTables &d = tables[i & 1];
-            if (!warp_wait(bar(kDecFull0 + (i & 1)), (i >> 1) & 1, failed)) break;
-            const float la = d.la[row];
-            float f[2];   // 2^(a_t - (a at the low end of the block)) for the two blocks of 32 columns
-#pragma unroll
-            for (int q = 0; q < 2; ++q) f[q] = exp_two((float)(d.a[row] - d.a[(half * 2 + q) * 32 + (REV ? 0 : 31)]));
-            if (!warp_wait(bar(kScores), i & 1, failed)) break;
-            fence_after();
-            float sum = 0.f;
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            const Item it(a, item, tiles, part);
 #pragma unroll 1
-            for (int q = 0; q < 4; ++q) {   // 16 columns each
-                const int block = half * 2 + q / 2, s0 = half * 64 + q * 16;
-                uint32_t p[8];
-                if (REV ? block >= quarter : block <= quarter) {
-                    float x[16], y[16];
-                    tmem_load16(own + q * 16, x);
-                    if (DOT) tmem_load16(own + Lay::c_two + q * 16, y);
-                    const float4 *table = reinterpret_cast<const float4 *>((block == quarter ? d.la : d.cf) + s0);
-                    float t[16];
+            for (int i = 0; i < it.pieces; ++i, ++g) {
+                const DecayTables &d = tables[g & 1];
+                if (!(ok = warp_wait(bar(kDecFull0 + (g & 1)), (g >> 1) & 1, failed))) break;
+                const float la = d.la[row];
+                float f[2];   // 2^(a_t - (a at the low end of the block)) for the two blocks of 32 columns
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float4 v = table[j];
-                        t[4 * j] = v.x, t[4 * j + 1] = v.y, t[4 * j + 2] = v.z, t[4 * j + 3] = v.w;
-                    }
-                    if (block == quarter) {
-                        const int j0 = row - s0;   // the step's own column
+                for (int q = 0; q < 2; ++q) f[q] = exp_two((float)(d.a[row] - d.a[(half * 2 + q) * 32 + (REV ? 0 : 31)]));
+                if (!(ok = warp_wait(bar(kScores), g & 1, failed))) break;
+                fence_after();
+                float sum = 0.f;
+#pragma unroll 1
+                for (int q = 0; q < 4; ++q) {   // 16 columns each
+                    const int block = half * 2 + q / 2, s0 = half * 64 + q * 16;
+                    uint32_t p[8];
+                    if (REV ? block >= quarter : block <= quarter) {
+                        float x[16], y[16];
+                        tmem_load16(own + q * 16, x);
+                        if (DOT) tmem_load16(own + Lay::c_two + q * 16, y);
+                        const float4 *table = reinterpret_cast<const float4 *>((block == quarter ? d.la : d.cf) + s0);
+                        float t[16];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) t[j] = (REV ? j >= j0 : j <= j0) ? exp_two(la - t[j]) : 0.f;
+                        for (int j = 0; j < 4; ++j) {
+                            const float4 v = table[j];
+                            t[4 * j] = v.x, t[4 * j + 1] = v.y, t[4 * j + 2] = v.z, t[4 * j + 3] = v.w;
+                        }
+                        if (block == quarter) {
+                            const int j0 = row - s0;   // the step's own column
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) t[j] = (REV ? j >= j0 : j <= j0) ? exp_two(la - t[j]) : 0.f;
+                        } else {
+                            const float fq = q < 2 ? f[0] : f[1];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) t[j] *= fq;
+                        }
+                        tmem_loaded();
+                        // (weight 0 against a score that is not finite: only in rows behind the end, which nobody reads)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            x[j] *= t[j];
+                            if (DOT) sum = fmaf(x[j], y[j], sum);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) p[j] = pack(x[2 * j], x[2 * j + 1], T{});
                     } else {
-                        const float fq = q < 2 ? f[0] : f[1];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) t[j] *= fq;
+                        for (int j = 0; j < 8; ++j) p[j] = 0;
                     }
-                    tmem_loaded();
-                    // (weight 0 against a score that is not finite: only in rows behind the end, which nobody reads)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        x[j] *= t[j];
-                        if (DOT) sum = fmaf(x[j], y[j], sum);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) p[j] = pack(x[2 * j], x[2 * j + 1], T{});
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) p[j] = 0;
+                    tmem_store8(own + q * 8, p);
                 }
-                tmem_store8(own + q * 8, p);
+                if (DOT) sums[((g & 1) * 2 + half) * kPiece + row] = sum;
+                tmem_stored();
+                fence_before();
+                warp_arrive(bar(kP));
+                warp_arrive(bar(kDecFree0 + (g & 1)));
             }
-            if (DOT) sums[((i & 1) * 2 + half) * kPiece + row] = sum;
-            tmem_stored();
-            fence_before();
-            warp_arrive(bar(kP));
-            warp_arrive(bar(kDecFree0 + (i & 1)));
         }
     } else if (warp < 20) {
         // ------------------------------------------------------------------ out
@@ -324,128 +334,143 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
         float *out_f = static_cast<float *>(a.out);
         const bool staged = !a.out_acc;
         const bool writer = tid == kStateThreads + kScoreThreads;   // starts the copies of the output tiles
-        const int col0 = vt * 64;
+        int g = 0;
+        bool ok = true;
 #pragma unroll 1
-        for (int i = 0; i < (STATE ? 0 : pieces); ++i) {
-            const long long t0 = piece_start(i), t = t0 + row;
-            const int m = (int)(n - t0 < kPiece ? n - t0 : kPiece);
-            if (!warp_wait(bar(kDecFull0 + (i & 1)), (i >> 1) & 1, failed)) break;
-            const float f1 = (float)(a.out_scale * a.kv_scale), f2 = (float)a.out_scale * tables[i & 1].head[row];
-            warp_arrive(bar(kDecFree0 + (i & 1)));
-            uint4 y[DOT ? 8 : 1];
-            if (DOT) {
-                if (!warp_wait(bar(kDot), i & 1, failed)) break;
-#pragma unroll
-                for (int c = 0; c < 8; ++c) y[DOT ? c : 0] = *reinterpret_cast<const uint4 *>(smem + Lay::dot + swizzled(row, c));
-                warp_arrive(bar(kDotFree));
-            }
-            if (staged && i > 0 && !warp_wait(bar(kOutFree), (i - 1) & 1, failed)) break;
-            if (!warp_wait(bar(kO1), i & 1, failed)) break;
-            fence_after();
-            float dot = 0.f;
-            auto columns = [&](int c, const uint4 &p0, const uint4 &p1) {   // 16 of them
-                float u[16], w[16];
-                tmem_load16(tmem + lanes + Lay::c_o1 + c * 16, u);
-                tmem_load16(tmem + lanes + Lay::c_o2 + c * 16, w);
-                tmem_loaded();
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    w[j] = row < m ? w[j] * f2 : 0.f;
-                    u[j] = row < m ? fmaf(u[j], f1, w[j]) : 0.f;
-                }
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            const Item it(a, item, tiles, part);
+            const int col0 = it.vt * 64;
+#pragma unroll 1
+            for (int i = 0; i < (STATE ? 0 : it.pieces); ++i, ++g) {
+                const long long t0 = it.start<REV>(i), t = t0 + row;
+                const int m = (int)(it.n - t0 < kPiece ? it.n - t0 : kPiece);
+                if (!(ok = warp_wait(bar(kDecFull0 + (g & 1)), (g >> 1) & 1, failed))) break;
+                const float f1 = (float)(a.out_scale * a.kv_scale), f2 = (float)a.out_scale * tables[g & 1].head[row];
+                warp_arrive(bar(kDecFree0 + (g & 1)));
+                uint4 y[DOT ? 8 : 1];
                 if (DOT) {
-                    const uint32_t words[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+                    if (!(ok = warp_wait(bar(kDot), g & 1, failed))) break;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float2 two = unpack(words[j], T{});
-                        dot = fmaf(w[2 * j], two.x, fmaf(w[2 * j + 1], two.y, dot));
-                    }
+                    for (int c = 0; c < 8; ++c) y[DOT ? c : 0] = *reinterpret_cast<const uint4 *>(smem + Lay::dot + swizzled(row, c));
+                    warp_arrive(bar(kDotFree));
                 }
+                if (staged && g > 0 && !(ok = warp_wait(bar(kOutFree), (g - 1) & 1, failed))) break;
+                if (!(ok = warp_wait(bar(kO1), g & 1, failed))) break;
+                fence_after();
+                const bool past = !no_past(it, i);
+                float dot = 0.f;
+                auto columns = [&](int c, const uint4 &p0, const uint4 &p1) {   // 16 of them
+                    float u[16], w[16];
+                    tmem_load16(tmem + lanes + Lay::c_o1 + c * 16, u);
+                    if (past) tmem_load16(tmem + lanes + Lay::c_o2 + c * 16, w);
+                    tmem_loaded();
+                    if (!past)
 #pragma unroll
-                for (int e = 0; e < 16; e += 8) {
-                    const int col = col0 + c * 16 + e;
-                    if (staged) {
-                        uint4 o;
-                        o.x = pack(u[e], u[e + 1], T{});
-                        o.y = pack(u[e + 2], u[e + 3], T{});
-                        o.z = pack(u[e + 4], u[e + 5], T{});
-                        o.w = pack(u[e + 6], u[e + 7], T{});
-                        *reinterpret_cast<uint4 *>(smem + Lay::out + swizzled(row, c * 2 + e / 8)) = o;
-                    } else if (t < a.L && col < a.d2) {
-                        float *at = out_f + ((b * a.L + t) * a.H + h) * a.d2 + col;
-                        *reinterpret_cast<float4 *>(at) = make_float4(u[e], u[e + 1], u[e + 2], u[e + 3]);
-                        *reinterpret_cast<float4 *>(at + 4) = make_float4(u[e + 4], u[e + 5], u[e + 6], u[e + 7]);
+                        for (int j = 0; j < 16; ++j) w[j] = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        w[j] = row < m ? w[j] * f2 : 0.f;
+                        u[j] = row < m ? fmaf(u[j], f1, w[j]) : 0.f;
                     }
-                }
-            };
-            if constexpr (DOT) {
+                    if (DOT) {
+                        const uint32_t words[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
 #pragma unroll
-                for (int c = 0; c < 4; ++c) columns(c, y[2 * c], y[2 * c + 1]);
-            } else {
+                        for (int j = 0; j < 8; ++j) {
+                            const float2 two = unpack(words[j], T{});
+                            dot = fmaf(w[2 * j], two.x, fmaf(w[2 * j + 1], two.y, dot));
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; e += 8) {
+                        const int col = col0 + c * 16 + e;
+                        if (staged) {
+                            uint4 o;
+                            o.x = pack(u[e], u[e + 1], T{});
+                            o.y = pack(u[e + 2], u[e + 3], T{});
+                            o.z = pack(u[e + 4], u[e + 5], T{});
+                            o.w = pack(u[e + 6], u[e + 7], T{});
+                            *reinterpret_cast<uint4 *>(smem + Lay::out + swizzled(row, c * 2 + e / 8)) = o;
+                        } else if (t < a.L && col < a.d2) {
+                            float *at = out_f + (((long long)it.b * a.L + t) * a.H + it.h) * a.d2 + col;
+                            *reinterpret_cast<float4 *>(at) = make_float4(u[e], u[e + 1], u[e + 2], u[e + 3]);
+                            *reinterpret_cast<float4 *>(at + 4) = make_float4(u[e + 4], u[e + 5], u[e + 6], u[e + 7]);
+                        }
+                    }
+                };
+                if constexpr (DOT) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) columns(c, y[2 * c], y[2 * c + 1]);
+                } else {
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) columns(c, y[0], y[0]);
-            }
-            if (DOT && t < a.L) {
-                const float pairs = sums[((i & 1) * 2) * kPiece + row] + sums[((i & 1) * 2 + 1) * kPiece + row];
-                a.dots[((long long)vt * a.B * a.L + b * a.L + t) * a.H + h] = row < m ? fmaf(pairs, f1, dot) : 0.f;
-            }
-            fence_before();
-            warp_arrive(bar(kEpi));
-            if (staged) {
-                fence_async();
-                warp_arrive(bar(kOutFull));
-                if (writer && bar_wait(bar(kOutFull), i & 1, failed)) {
-                    // steps behind the tensor's end and columns behind its rows are not written
-                    tma_store(base + Lay::out, &map_out, col0, h, (int)t0, (int)b);
-                    tma_store_read();
-                    bar_arrive(bar(kOutFree));
+                    for (int c = 0; c < 4; ++c) columns(c, y[0], y[0]);
                 }
-                __syncwarp();
+                if (DOT && t < a.L) {
+                    const float pairs = sums[((g & 1) * 2) * kPiece + row] + sums[((g & 1) * 2 + 1) * kPiece + row];
+                    a.dots[((long long)it.vt * a.B * a.L + (long long)it.b * a.L + t) * a.H + it.h] = row < m ? fmaf(pairs, f1, dot) : 0.f;
+                }
+                fence_before();
+                warp_arrive(bar(kEpi));
+                if (staged) {
+                    fence_async();
+                    warp_arrive(bar(kOutFull));
+                    if (writer && bar_wait(bar(kOutFull), g & 1, failed)) {
+                        // steps behind the tensor's end and columns behind its rows are not written
+                        tma_store(base + Lay::out, &map_out, col0, it.h, (int)t0, (int)it.b);
+                        tma_store_read();
+                        bar_arrive(bar(kOutFree));
+                    }
+                    __syncwarp();
+                }
             }
+            if (!ok) break;
+            // rows behind the last piece
+            const long long end = STATE || part < a.splits - 1 ? a.L : (long long)it.all * kPiece;
+            for (long long e = tid - (kStateThreads + kScoreThreads); e < (a.L - end) * 8; e += kOutThreads) {
+                const long long t = end + e / 8;
+                const int col = col0 + (int)(e % 8) * 8;
+                if (col >= a.d2) continue;
+                const long long at = (((long long)it.b * a.L + t) * a.H + it.h) * a.d2 + col;
+                const uint4 zero = {0, 0, 0, 0};
+                *reinterpret_cast<uint4 *>(a.out_acc ? (void *)(out_f + at) : (void *)(out_t + at)) = zero;
+                if (a.out_acc) *reinterpret_cast<uint4 *>(out_f + at + 4) = zero;
+            }
+            if (DOT)
+                for (long long t = end + tid - (kStateThreads + kScoreThreads); t < a.L; t += kOutThreads)
+                    a.dots[((long long)it.vt * a.B * a.L + (long long)it.b * a.L + t) * a.H + it.h] = 0.f;
         }
-        // rows behind the last piece
-        const long long end = STATE || part < a.splits - 1 ? a.L : (long long)all * kPiece;
-        for (long long e = tid - (kStateThreads + kScoreThreads); e < (a.L - end) * 8; e += kOutThreads) {
-            const long long t = end + e / 8;
-            const int col = col0 + (int)(e % 8) * 8;
-            if (col >= a.d2) continue;
-            const long long at = ((b * a.L + t) * a.H + h) * a.d2 + col;
-            const uint4 zero = {0, 0, 0, 0};
-            *reinterpret_cast<uint4 *>(a.out_acc ? (void *)(out_f + at) : (void *)(out_t + at)) = zero;
-            if (a.out_acc) *reinterpret_cast<uint4 *>(out_f + at + 4) = zero;
-        }
-        if (DOT)
-            for (long long t = end + tid - (kStateThreads + kScoreThreads); t < a.L; t += kOutThreads)
-                a.dots[((long long)vt * a.B * a.L + b * a.L + t) * a.H + h] = 0.f;
         if (writer) tma_store_done();
     } else if (warp == 20) {
         // ------------------------------------------------------------------ TMA and MMA
-        if (pieces > 0) {
-            const uint32_t lead = lane == 0, base16 = base >> 4;
-            // I = K^T V'; with 64 state rows the second block of 64 is the first once more
-            auto state_product = [&]() {
+        const uint32_t lead = lane == 0, base16 = base >> 4;
+        // I = K^T V'; with 64 state rows the second block of 64 is the first once more
+        auto state_product = [&]() {
 #pragma unroll
-                    for (int term = NV - 1; term >= 0; --term)
+                for (int term = NV - 1; term >= 0; --term)
 #pragma unroll
-                        for (int j = 0; j < kPiece / 16; ++j)
-                            mma_ss(tmem + Lay::c_i, tile_desc(base16 + ((Lay::k + j * 2048) >> 4), KP == 128 ? kTileBytes : 0),
-                                   tile_desc(base16 + ((Lay::vw + term * kTileBytes + j * 2048) >> 4), kTileBytes), instr_desc<T>(64, true, true),
-                                   term < NV - 1 || j > 0, lead);
-                    mma_commit(bar(kInc), lead);
-            };
+                    for (int j = 0; j < kPiece / 16; ++j)
+                        mma_ss(tmem + Lay::c_i, tile_desc(base16 + ((Lay::k + j * 2048) >> 4), KP == 128 ? kTileBytes : 0),
+                               tile_desc(base16 + ((Lay::vw + term * kTileBytes + j * 2048) >> 4), kTileBytes), instr_desc<T>(64, true, true),
+                               term < NV - 1 || j > 0, lead);
+                mma_commit(bar(kInc), lead);
+        };
+        int g = 0, fixes = 0;
+        bool ok = true;
 #pragma unroll 1
-            for (int i = 0; i < pieces; ++i) {
-                const uint32_t ph = i & 1;
-                if (!warp_wait(bar(kFullRK), ph, failed)) break;
-                if (a.lengths != nullptr && n - piece_start(i) < kPiece && !warp_wait(bar(kFix), 0, failed)) break;
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            const Item it(a, item, tiles, part);
+#pragma unroll 1
+            for (int i = 0; i < it.pieces; ++i, ++g) {
+                const uint32_t ph = g & 1;
+                if (!(ok = warp_wait(bar(kFullRK), ph, failed))) break;
+                if (a.lengths != nullptr && it.n - it.start<REV>(i) < kPiece && !(ok = warp_wait(bar(kFix), fixes++ & 1, failed))) break;
                 if constexpr (STATE) {   // I alone
-                    if (!warp_wait(bar(kVReady), ph, failed)) break;
+                    if (!(ok = warp_wait(bar(kVReady), ph, failed))) break;
                     fence_after();
                     state_product();
                     continue;
                 }
-                if (i > 0 && !warp_wait(bar(kO1), ph ^ 1, failed)) break;   // P of the piece before has been used
-                if (DOT && !(warp_wait(bar(kDot), ph, failed) && warp_wait(bar(kFullV0), ph, failed))) break;
+                if (g > 0 && !(ok = warp_wait(bar(kO1), ph ^ 1, failed))) break;   // P of the piece before has been used
+                if (DOT && !(ok = warp_wait(bar(kDot), ph, failed) && warp_wait(bar(kFullV0), ph, failed))) break;
                 fence_after();
                 // scores = R K^T
 #pragma unroll
@@ -463,9 +488,11 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                 // O2 = R S, when O2 of the piece before has been read and the state's operand is there (it was written before
                 // V').  Small terms first here and below: the accumulator drops what does not fit its 24 bits at every step,
                 // towards zero.
-                if (i > 0 && !warp_wait(bar(kEpi), ph ^ 1, failed)) break;
-                if (!warp_wait(bar(kVReady), ph, failed)) break;
+                if (g > 0 && !(ok = warp_wait(bar(kEpi), ph ^ 1, failed))) break;
+                if (!(ok = warp_wait(bar(kVReady), ph, failed))) break;
                 fence_after();
+                const bool past = !no_past(it, i), future = !no_future(it, i);
+                if (past)
 #pragma unroll
                 for (int term = NS - 1; term >= 0; --term)
 #pragma unroll
@@ -473,10 +500,11 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                         mma_ss(tmem + Lay::c_o2, tile_desc(base16 + ((Lay::r + (j / 4) * kTileBytes + (j % 4) * 32) >> 4), 16),
                                tile_desc(base16 + ((Lay::s + term * KP * 128 + j * 2048) >> 4), kTileBytes), instr_desc<T>(64, false, true),
                                term < NS - 1 || j > 0, lead);
-                state_product();
+                if (future) state_product();
+                else mma_commit(bar(kInc), lead);
                 // O1 = P V
                 const uint32_t v16 = base16 + (Lay::v >> 4) + (VS == 2 ? ph * (kTileBytes >> 4) : 0);
-                if (!warp_wait(bar(kP), ph, failed)) break;
+                if (!(ok = warp_wait(bar(kP), ph, failed))) break;
                 fence_after();
 #pragma unroll
                 for (int j = 0; j < kPiece / 16; ++j)
@@ -487,60 +515,55 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
         }
     } else if (warp == 21) {
         // ------------------------------------------------------------------ TMA
-        if (pieces > 0) {
-            const uint32_t lead = lane == 0;
-            const int rh = h / a.r.share, kh = h / a.k.share, vh = h / a.v.share;
-            auto load_rk = [&](int i) {
-                if (!lead) return;
-                const int t0 = (int)piece_start(i);
-                bar_expect(bar(kFullRK), (STATE ? 1 : 2) * Lay::panels * kTileBytes);
-#pragma unroll
-                for (int p = 0; p < Lay::panels; ++p) {
-                    if (!STATE) tma_load(base + Lay::r + p * kTileBytes, &map_r, bar(kFullRK), p * 64, rh, t0, (int)b);
-                    tma_load(base + Lay::k + p * kTileBytes, &map_k, bar(kFullRK), p * 64, kh, t0, (int)b);
-                }
-            };
-            auto load_v = [&](int i) {
-                if (!lead) return;
-                bar_expect(bar(kFullV0 + i % VS), kTileBytes);
-                tma_load(base + Lay::v + (i % VS) * kTileBytes, &map_v, bar(kFullV0 + i % VS), vt * 64, vh, (int)piece_start(i), (int)b);
-            };
-            auto load_dot = [&](int i) {
-                if (!lead) return;
-                bar_expect(bar(kDot), kTileBytes);
-                tma_load(base + Lay::dot, &map_dot, bar(kDot), vt * 64, h / a.dot.share, (int)piece_start(i), (int)b);
-            };
-            load_rk(0);
-            load_v(0);
-            if (DOT) load_dot(0);
-            if (VS == 2 && pieces > 1) load_v(1);
-            int loaded_rk = 1, loaded_dot = 1, loaded_v = VS == 2 && pieces > 1 ? 2 : 1;
+        if (lane == 0) {   // one thread; the piece's copies in the order in which their places become free
+            int g = 0, stop = 0;
 #pragma unroll 1
-            for (int i = 0; i + 1 < pieces; ++i) {
-                if (DOT) {
-                    if (!warp_wait(bar(kScores), i & 1, failed) || !warp_wait(bar(kDotFree), i & 1, failed)) break;
-                    load_dot(i + 1);
-                    ++loaded_dot;
+            for (int item = blockIdx.x; item < items && !stop; item += gridDim.x) {
+                const Item it(a, item, tiles, part);
+                const int rh = it.h / a.r.share, kh = it.h / a.k.share, vh = it.h / a.v.share, dh = DOT ? it.h / a.dot.share : 0;
+#pragma unroll 1
+                for (int i = 0; i < it.pieces; ++i, ++g) {
+                    const int t0 = (int)it.start<REV>(i), b = (int)it.b;
+                    auto load_v = [&]() {   // behind the last product that reads the V in its place
+                        if (g >= VS && !bar_wait(bar(STATE ? kInc : kO1), (g - VS) & 1, failed)) return false;
+                        bar_expect(bar(kFullV0 + g % VS), kTileBytes);
+                        tma_load(base + Lay::v + (g % VS) * kTileBytes, &map_v, bar(kFullV0 + g % VS), it.vt * 64, vh, t0, b);
+                        return true;
+                    };
+                    if (VS == 2 && !load_v()) { stop = 1; break; }
+                    if (DOT) {
+                        if (g > 0 && !(bar_wait(bar(kScores), (g - 1) & 1, failed) && bar_wait(bar(kDotFree), (g - 1) & 1, failed))) { stop = 2; break; }
+                        bar_expect(bar(kDot), kTileBytes);
+                        tma_load(base + Lay::dot, &map_dot, bar(kDot), it.vt * 64, dh, t0, b);
+                    }
+                    if (g > 0 && !bar_wait(bar(kInc), (g - 1) & 1, failed)) { stop = 3; break; }   // the last product that reads R and K
+                    bar_expect(bar(kFullRK), (STATE ? 1 : 2) * Lay::panels * kTileBytes);
+#pragma unroll
+                    for (int p = 0; p < Lay::panels; ++p) {
+                        if (!STATE) tma_load(base + Lay::r + p * kTileBytes, &map_r, bar(kFullRK), p * 64, rh, t0, b);
+                        tma_load(base + Lay::k + p * kTileBytes, &map_k, bar(kFullRK), p * 64, kh, t0, b);
+                    }
+                    if (VS == 1 && !load_v()) { stop = 4; break; }
                 }
-                if (!warp_wait(bar(kInc), i & 1, failed)) break;    // the last product that reads R and K
-                load_rk(i + 1);
-                ++loaded_rk;
-                if (loaded_v == pieces) continue;
-                if (!STATE && !warp_wait(bar(kO1), i & 1, failed)) break;     // the last product that reads V
-                load_v(loaded_v++);
             }
             if (*failed) {
-                // let what is in flight land before the block gives its memory back
-                warp_wait(bar(kFullRK), (loaded_rk - 1) & 1, failed + 1);
-                if (DOT) warp_wait(bar(kDot), (loaded_dot - 1) & 1, failed + 1);
-                for (int i = loaded_v > VS ? loaded_v - VS : 0; i < loaded_v; ++i)
-                    warp_wait(bar(kFullV0 + i % VS), (i / VS) & 1, failed + 1);
+                // let what is in flight land before the block gives its memory back: g whole pieces, and what the last one got
+                const int v = g + (stop > 1 && VS == 2), dots = g + (stop > 2), rk = g + (stop > 3);
+                if (rk > 0) bar_wait(bar(kFullRK), (rk - 1) & 1, failed + 1);
+                if (DOT && dots > 0) bar_wait(bar(kDot), (dots - 1) & 1, failed + 1);
+                for (int i = v > VS ? v - VS : 0; i < v; ++i) bar_wait(bar(kFullV0 + i % VS), (i / VS) & 1, failed + 1);
             }
         }
+        __syncwarp();
     } else {
-        const float *g = static_cast<const float *>(a.decay) + b * a.decay_stride[0] + h * a.decay_stride[2];
-        const double whole = sum_decays<REV>(g, a.decay_stride[1], n, first, pieces, tables, bar(kDecFull0), bar(kDecFree0), failed);
-        if (STATE && vt == 0 && lane == 0) a.split_decays[bh * a.splits + part] = (float)whole;
+        int count = 0;
+#pragma unroll 1
+        for (int item = blockIdx.x; item < items && !*failed; item += gridDim.x) {
+            const Item it(a, item, tiles, part);
+            const float *g = static_cast<const float *>(a.decay) + (long long)it.b * a.decay_stride[0] + it.h * a.decay_stride[2];
+            const double whole = sum_decays<REV>(g, a.decay_stride[1], it.n, it.first, it.pieces, count, tables, bar(kDecFull0), bar(kDecFree0), failed);
+            if (STATE && it.vt == 0 && lane == 0) a.split_decays[it.bh * a.splits + part] = (float)whole;
+        }
     }
     fence_before();
     __syncthreads();
@@ -562,7 +585,9 @@ int launch_tiles(const Sweep &a, int dtype, cudaStream_t stream)
         !encode(&dot, a.dot.data ? a.dot : o, a, a.d2, dtype))
         return PSIG_ERR_CUDA;
     const int tiles = tile_columns(a.d2);
-    const unsigned blocks = (unsigned)(a.B * a.H * tiles);
+    // an SM holds one block: no more than that, each takes every so many items
+    const long long items = a.B * a.H * tiles;
+    const unsigned blocks = (unsigned)(items < 148 ? items : 148);
     if (a.splits > 1) {
         using Lay = TileLayout<KP, 1, 3, false>;
         auto kernel = attn_sweep_tiles<T, KP, 1, 3, false, REV, true>;
@@ -596,7 +621,7 @@ int select_tiles(const Sweep &a, int dtype, cudaStream_t stream)
 bool attn_tiles_supported(const Sweep &a, int dtype)
 {
     const int size = dtype == PSIG_F32 ? 4 : 2;
-    return dtype != PSIG_F64 && a.d1 <= 128 && a.d2 <= 128 && a.L < (1LL << 31) && a.B < (1LL << 31) && a.B * a.H < (1LL << 30) &&
+    return dtype != PSIG_F64 && a.d1 <= 128 && a.d2 <= 128 && a.L < (1LL << 31) - kPiece && a.B < (1LL << 31) && a.B * a.H < (1LL << 30) &&
            operand_fits(a.r, a, a.d1, size) && operand_fits(a.k, a, a.d1, size) && operand_fits(a.v, a, a.d2, size);
 }
 

@@ -73,6 +73,7 @@ struct Sweep {
     // Decay gradient (see attn_decay_grad): the grad_q sweep stores the state at the end of every kSegment steps,
     // the grad_k sweep multiplies its own state into it and leaves one number per segment and column tile.
     void *anchors;        // (B, H, segments, d1, d2); the tensor-core forms keep them in an order of their own
+    bool keep_last;       // whether the state behind the last step counts (there is a grad_state)
     void *anchor_dots;    // (B, H, segments, parts of the sum)
     // Tensor-core sweeps only: the unrounded output row times the row of a third operand, summed over each block's and
     // each warp's columns: (attn_tile_dots * column tiles of 64, B, L, H).

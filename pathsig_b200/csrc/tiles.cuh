@@ -187,17 +187,48 @@ __device__ __forceinline__ void tma_store_done() { asm volatile("cp.async.bulk.w
 
 __device__ __forceinline__ uint32_t swizzled(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
 
+// A block's work: one column tile of one head of one sequence, or a part of it.  Blocks take items one after the other; the
+// pieces of all of them are counted through (`g` below), so that a piece's stages overlap across the items, too: with
+// sequences of one piece (61 steps, 2048 of them) a block each, 82 us a sweep went to starting blocks up.
+struct Item {
+    int vt, h, b, all, first, pieces;   // column tile, head, sequence; pieces of the sequence; this part's first and number
+    long long bh, n;                    // n: steps of the sequence
+    __device__ __forceinline__ Item(const Sweep &a, int item, int tiles, int part)
+    {
+        // fewer than 2^31 items (attn_tiles_supported), one or two column tiles
+        const unsigned head = tiles == 1 ? item : (unsigned)item >> 1;
+        vt = tiles == 1 ? 0 : item & 1;
+        b = (int)(head / (unsigned)a.H);
+        h = (int)(head - (unsigned)b * a.H);
+        bh = head;
+        int steps = (int)a.L;
+        if (a.lengths != nullptr) {
+            const int len = a.lengths[b];
+            steps = len < 0 ? 0 : len > steps ? steps : len;
+        }
+        n = steps;
+        all = (steps + (kPiece - 1)) / kPiece;
+        first = 0, pieces = all;
+        if (a.splits > 1) {   // at most 64 parts of at most 2^24 pieces
+            first = (int)((unsigned)all * part / (unsigned)a.splits);
+            pieces = (int)((unsigned)all * (part + 1) / (unsigned)a.splits) - first;
+        }
+    }
+    template <bool REV>
+    __device__ __forceinline__ long long start(int i) const { return (long long)(REV ? all - 1 - first - i : first + i) * kPiece; }
+};
+
 // One warp: the decay tables of `pieces` of the sweep's pieces from number `first` on, one piece ahead of their use, in two
-// buffers in turn.  Returns the sum of all their decays (exponent of 2).
+// buffers in turn (`count` counts the pieces over all items).  Returns the sum of all their decays (exponent of 2).
 template <bool REV>
-__device__ __forceinline__ double sum_decays(const float *g, long long stride, long long n, int first, int pieces, DecayTables *tables,
+__device__ __forceinline__ double sum_decays(const float *g, long long stride, long long n, int first, int pieces, int &count, DecayTables *tables,
                                              uint32_t full0, uint32_t free0, volatile int *failed)
 {
     const int all = (int)((n + kPiece - 1) / kPiece);
     double whole = 0.0;
     const int lane = threadIdx.x & 31;
 #pragma unroll 1
-    for (int i = 0; i < pieces; ++i) {
+    for (int i = 0; i < pieces; ++i, ++count) {
         const long long t0 = (long long)(REV ? all - 1 - first - i : first + i) * kPiece;
         const int m = (int)(n - t0 < kPiece ? n - t0 : kPiece);
         double c[4];
@@ -223,8 +254,8 @@ __device__ __forceinline__ double sum_decays(const float *g, long long stride, l
         for (int j = 0; j < 4; ++j) c[j] = REV ? end - (before + c[j]) : before + c[j];
         // the low end of each block of 32 steps: its last step, or, in reverse, its first
         const double low = __shfl_sync(0xffffffffu, REV ? c[0] : c[3], REV ? (lane & ~7) : (lane | 7));
-        if (i >= 2 && !warp_wait(free0 + 8 * (i & 1), ((i >> 1) & 1) ^ 1, failed)) break;
-        DecayTables &d = tables[i & 1];
+        if (count >= 2 && !warp_wait(free0 + 8 * (count & 1), ((count >> 1) & 1) ^ 1, failed)) break;
+        DecayTables &d = tables[count & 1];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int t = lane * 4 + j;
@@ -236,7 +267,7 @@ __device__ __forceinline__ double sum_decays(const float *g, long long stride, l
             d.head[t] = exp_two((float)c[j]);
         }
         if (lane == 0) d.keep = exp_two((float)end);
-            warp_arrive(full0 + 8 * (i & 1));
+            warp_arrive(full0 + 8 * (count & 1));
     }
     return whole;
 }
