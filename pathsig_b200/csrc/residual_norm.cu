@@ -29,9 +29,16 @@ struct NormArgs {
     void *grad_x, *grad_gate, *grad_residual;
     void *partial;   // (blocks, 3, D) sums for weight, scale, next_weight
     long long rows, D;
-    double eps;
+    double mean, eps;      // 1 / D
+    float mean_f, eps_f;   // the same: converting costs a thread as much as some values of its row
     int activation;
 };
+
+template <typename A> __device__ __forceinline__ A scalar(double wide, float narrow)
+{
+    if constexpr (sizeof(A) == 8) return wide;
+    else return narrow;
+}
 
 template <int BYTES> struct Raw;
 template <> struct Raw<16> { using type = uint4; };
@@ -217,7 +224,7 @@ __global__ void __launch_bounds__(kTeamMax) norm_forward_team(const NormArgs a, 
     extern __shared__ __align__(128) unsigned char dynamic[];
     const int teams = team_log2 < 5 ? blockDim.x >> team_log2 : 1;
     const int team = team_log2 < 5 ? threadIdx.x >> team_log2 : 0, j = team_log2 < 5 ? threadIdx.x & (threads - 1) : threadIdx.x;
-    const A mean = A(1) / A((int)a.D), eps = (A)a.eps;
+    const A mean = scalar<A>(a.mean, a.mean_f), eps = scalar<A>(a.eps, a.eps_f);
     const long long step = (long long)gridDim.x * teams;
     const RingState rs{dynamic + 128, norm_shared(dynamic), ring};
     if (RING) {
@@ -338,7 +345,7 @@ __global__ void __launch_bounds__(kTeamMax) norm_backward_team(const NormArgs a,
     const int team = team_log2 < 5 ? threadIdx.x >> team_log2 : 0, j = team_log2 < 5 ? threadIdx.x & (threads - 1) : threadIdx.x;
     constexpr bool KEEP = NV * E == 8;       // column constants and the next row fit in registers
     constexpr bool PREFETCH = KEEP && !RING;
-    const A mean = A(1) / A((int)a.D), eps = (A)a.eps;
+    const A mean = scalar<A>(a.mean, a.mean_f), eps = scalar<A>(a.eps, a.eps_f);
     const int D = (int)a.D;
     const long long step = (long long)gridDim.x * teams;
     A q[NV * E], qn[NEXT ? NV * E : 1], wc_kept[KEEP ? NV * E : 1], w2_kept[KEEP && NEXT ? NV * E : 1];
@@ -630,7 +637,7 @@ __global__ void __launch_bounds__(kWideThreads) norm_forward_wide(const NormArgs
 {
     using A = typename Acc<T>::type;
     __shared__ A shared[4 * (kTeamMax / 32)];
-    const A mean = A(1) / A(a.D), eps = (A)a.eps;
+    const A mean = scalar<A>(a.mean, a.mean_f), eps = scalar<A>(a.eps, a.eps_f);
     int round = 0;
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const long long base = row * a.D;
@@ -677,7 +684,7 @@ __global__ void __launch_bounds__(kWideThreads) norm_backward_wide(const NormArg
 {
     using A = typename Acc<T>::type;
     __shared__ A shared[4 * (kTeamMax / 32)];
-    const A mean = A(1) / A(a.D), eps = (A)a.eps;
+    const A mean = scalar<A>(a.mean, a.mean_f), eps = scalar<A>(a.eps, a.eps_f);
     A *part = static_cast<A *>(a.partial) + (long long)blockIdx.x * 3 * a.D;
     int round = 0;
     bool fresh = true;
@@ -799,6 +806,13 @@ int check_norm(const PsigNormDesc *d)
     return PSIG_OK;
 }
 
+void set_sizes(NormArgs &a, const PsigNormDesc &d)
+{
+    a.rows = d.rows, a.D = d.D, a.activation = d.activation;
+    a.mean = 1.0 / (double)d.D, a.eps = d.eps;
+    a.mean_f = (float)a.mean, a.eps_f = (float)a.eps;
+}
+
 // How a row is dealt to threads: 8 values to a thread, 16 where the row would need more than 256 threads (a block with
 // more of them waits longer at its barriers than the larger number of values costs: 4680 values, see norm_forward_team).
 struct TeamPlan {
@@ -821,12 +835,14 @@ TeamPlan team_plan(long long D)
     return p;
 }
 
-// Blocks of the backward pass: about as many as are resident together (each keeps its column sums over all its rows).
+// Blocks of the backward pass: about as many as are resident together (each keeps its column sums over all its rows).  Measured
+// with 1 to 12 to an SM: 15616 x 1024 tokens 103 us with 4 (118 with 8), 15616 x 4680 signatures 169 us with 2 (284 with 3, where no
+// ring of two stages fits), 262144 x 128 heads 81 us with 2 (91 with 4).
 int backward_blocks(const PsigNormDesc &d)
 {
     if (d.D > kNormWidest) return (int)(d.rows < 148 * 2 ? d.rows : 148 * 2);
     const TeamPlan p = team_plan(d.D);
-    const long long need = (d.rows + p.teams() - 1) / p.teams(), per_sm = p.block <= 128 ? 8 : p.block <= 256 ? 4 : p.block <= 320 ? 3 : 2;
+    const long long need = (d.rows + p.teams() - 1) / p.teams(), per_sm = p.team_log2 == 5 && p.block <= 128 ? 4 : p.team_log2 == 5 && p.block <= 256 ? 3 : 2;
     return (int)(need < 148 * per_sm ? need : 148 * per_sm);
 }
 
@@ -912,7 +928,7 @@ extern "C" int psig_norm_forward(const PsigNormDesc *desc, const void *x, const 
     NormArgs a{};
     a.x = x, a.weight = weight, a.gate = gate, a.residual = residual, a.scale = residual_scale;
     a.next_weight = next_weight, a.h = h, a.n = n;
-    a.rows = desc->rows, a.D = desc->D, a.eps = desc->eps, a.activation = desc->activation;
+    set_sizes(a, *desc);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return with_dtype(desc->dtype, [&](auto t) {
         using T = decltype(t);
@@ -925,11 +941,12 @@ extern "C" int psig_norm_forward(const PsigNormDesc *desc, const void *x, const 
         }
         const TeamPlan p = team_plan(a.D);
         const long long blocks = (a.rows + p.teams() - 1) / p.teams();
-        if (blocks > 0x7fffffffLL) return (int)PSIG_ERR_TOO_LARGE;
-        const int per_sm = p.block <= 128 ? 12 : p.block <= 256 ? 6 : 4;
+        const unsigned grid = (unsigned)(blocks < 148 * 32 ? blocks : 148 * 32);
+        // Wide rows: a ring of rows and 3 blocks to an SM (15616 x 4680 signatures 115 us, 143 with 2).  Shorter ones are faster without,
+        // on many small blocks (15616 x 1024 tokens 43 us, with a ring 47 to 54).
+        const int per_sm = 3;
         Ring ring;
-        // a ring pays when a block walks several rows
-        const int smem = a.rows >= 148LL * per_sm * 4 ? plan_ring<T>(a, p, false, a.next_weight != nullptr, per_sm, &ring) : 0;
+        const int smem = p.block > 256 && a.rows >= 148LL * per_sm * 4 ? plan_ring<T>(a, p, false, a.next_weight != nullptr, per_sm, &ring) : 0;
         return with_shape<T>(access_width<T>(a), p.values, [&](auto e, auto nv) {
             constexpr int E = decltype(e)::value, NV = decltype(nv)::value;
             auto launch = [&](auto kernel, unsigned grid, int bytes) {
@@ -941,8 +958,8 @@ extern "C" int psig_norm_forward(const PsigNormDesc *desc, const void *x, const 
                 if (smem > 0)
                     return a.next_weight ? launch(norm_forward_team<T, E, NV, true, true>, 148 * per_sm, smem)
                                          : launch(norm_forward_team<T, E, NV, false, true>, 148 * per_sm, smem);
-            return a.next_weight ? launch(norm_forward_team<T, E, NV, true, false>, (unsigned)blocks, 0)
-                                 : launch(norm_forward_team<T, E, NV, false, false>, (unsigned)blocks, 0);
+            return a.next_weight ? launch(norm_forward_team<T, E, NV, true, false>, grid, 0)
+                                 : launch(norm_forward_team<T, E, NV, false, false>, grid, 0);
         });
     });
 }
@@ -970,7 +987,7 @@ extern "C" int psig_norm_backward(const PsigNormDesc *desc, const void *x, const
     a.next_weight = next_weight, a.grad_h = grad_h, a.grad_n = grad_n;
     a.grad_x = grad_x, a.grad_gate = gate ? grad_gate : nullptr, a.grad_residual = residual ? grad_residual : nullptr;
     a.partial = workspace;
-    a.rows = desc->rows, a.D = desc->D, a.eps = desc->eps, a.activation = desc->activation;
+    set_sizes(a, *desc);
     const int blocks = backward_blocks(*desc);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return with_dtype(desc->dtype, [&](auto t) {
