@@ -277,7 +277,7 @@ __global__ void attn_decay_grad(const PairSums pairs, const A *__restrict__ dots
         __syncthreads();
         if (threadIdx.x == 0) {
             double v = 0.0;
-            for (int i = 0; i < kSegment / 32; ++i) v += total_s[i];
+            for (int i = 0; i < blockDim.x >> 5; ++i) v += total_s[i];
             totals[bh * segments + segment] = v;
         }
     }
@@ -572,12 +572,13 @@ int decay_gradient(const Call &c, PairSums pairs, const typename Acc<T>::type *d
     int rc;
     // the grid's second dimension is limited to 65535
     const long long per_launch = 65535 / d.H > 0 ? 65535 / d.H : 1;
+    const int threads = d.L < kSegment ? (int)(d.L + 31) / 32 * 32 : kSegment;   // a thread per step of a segment
     for (long long b0 = 0; b0 < d.B; b0 += per_launch) {
         const long long nb = d.B - b0 < per_launch ? d.B - b0 : per_launch;
         PairSums p = pairs;
         p.plus = static_cast<const P *>(pairs.plus) + b0 * d.L * d.H;
         p.minus = static_cast<const P *>(pairs.minus) + b0 * d.L * d.H;
-        attn_decay_grad<A, P><<<dim3((unsigned)segments, (unsigned)(nb * d.H)), kSegment, 0, stream>>>(
+        attn_decay_grad<A, P><<<dim3((unsigned)segments, (unsigned)(nb * d.H)), threads, 0, stream>>>(
             p, dots + b0 * d.H * segments * parts, parts,
             static_cast<const A *>(c.decay) + b0 * d.decay_strides[0], d.decay_strides[0], d.decay_strides[1],
             d.decay_strides[2], d.lengths == nullptr ? nullptr : d.lengths + b0, d.L, d.H,

@@ -2,7 +2,7 @@
 //
 // With the decays summed inside a piece, a_t (towards the end of the sweep), r_t, k_s, v_s the rows of the sweep
 // (sequence.cuh) and S the state (d1, 64 columns) at the piece's beginning,
-//     out_t = out_scale ( sum_{s to t} exp(a_t - a_s) (r_t . k_s) kv_scale v_s + exp(a_t) r_t^T S )
+//     out_t = out_scale ( sum_{s to t} exp(a_t - a_s) kv_scale (r_t . k_s) v_s + exp(a_t) r_t^T S )
 //     S    <- exp(a_end) S + sum_s k_s ( exp(a_end - a_s) kv_scale v_s )^T
 // that is four matrix products a piece: scores = R K^T, O2 = R S, I = K^T V', O1 = P V with P the weighted scores.
 // All run as tcgen05.mma with M = 128 and fp32 accumulators in tensor memory; R, K, V come by TMA into 128-byte
@@ -37,14 +37,14 @@ constexpr int kStateThreads = 256, kScoreThreads = 256, kOutThreads = 128;
 constexpr int kTileThreads = kStateThreads + kScoreThreads + kOutThreads + 96;
 
 enum Barrier {
-    kFullRK, kFullV0, kFullV1, kVReady, kScores, kInc, kP, kO1, kEpi, kFix, kOutFull, kOutFree, kDot, kDotFree,
+    kFullRK, kFullV0, kFullV1, kVReady, kScores, kInc, kP, kO2, kO1, kFix, kOutFull, kOutFree, kDot, kDotFree,
     kDecFull0, kDecFull1, kDecFree0, kDecFree1, kBarriers
 };
 
 template <int KP, int NS, int NV, bool DOT>
 struct TileLayout {
     static constexpr int panels = KP / 64;
-    static constexpr int VS = DOT ? 1 : 2;                  // pieces of V in turn (shared memory is full with DOT)
+    static constexpr int VS = DOT && KP == 128 ? 1 : 2;     // pieces of V in turn (else shared memory is full)
     static constexpr int r = 0;
     static constexpr int k = r + panels * kTileBytes;
     static constexpr int v = k + panels * kTileBytes;
@@ -94,7 +94,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
         bar_init(bar(kInc), 1);
         bar_init(bar(kP), kScoreThreads / 32);
         bar_init(bar(kO1), 1);
-        bar_init(bar(kEpi), kOutThreads / 32);
+        bar_init(bar(kO2), kOutThreads / 32);
         bar_init(bar(kFix), kStateThreads / 32);
         bar_init(bar(kOutFull), kOutThreads / 32);
         bar_init(bar(kOutFree), 1);
@@ -266,6 +266,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
     } else if (warp < 16) {
         // ------------------------------------------------------------------ P = scores, weighted
         const uint32_t own = tmem + lanes + half * 64;   // this thread's columns of the scores
+        const float kv_scale = (float)a.kv_scale;
         int g = 0;
         bool ok = !STATE;
 #pragma unroll 1
@@ -278,7 +279,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                 const float la = d.la[row];
                 float f[2];   // 2^(a_t - (a at the low end of the block)) for the two blocks of 32 columns
 #pragma unroll
-                for (int q = 0; q < 2; ++q) f[q] = exp_two((float)(d.a[row] - d.a[(half * 2 + q) * 32 + (REV ? 0 : 31)]));
+                for (int q = 0; q < 2; ++q) f[q] = kv_scale * exp_two((float)(d.a[row] - d.a[(half * 2 + q) * 32 + (REV ? 0 : 31)]));
                 if (!(ok = warp_wait(bar(kScores), g & 1, failed))) break;
                 fence_after();
                 float sum = 0.f;
@@ -300,7 +301,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                         if (block == quarter) {
                             const int j0 = row - s0;   // the step's own column
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) t[j] = (REV ? j >= j0 : j <= j0) ? exp_two(la - t[j]) : 0.f;
+                            for (int j = 0; j < 16; ++j) t[j] = (REV ? j >= j0 : j <= j0) ? kv_scale * exp_two(la - t[j]) : 0.f;
                         } else {
                             const float fq = q < 2 ? f[0] : f[1];
 #pragma unroll
@@ -345,41 +346,47 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                 const long long t0 = it.start<REV>(i), t = t0 + row;
                 const int m = (int)(it.n - t0 < kPiece ? it.n - t0 : kPiece);
                 if (!(ok = warp_wait(bar(kDecFull0 + (g & 1)), (g >> 1) & 1, failed))) break;
-                const float f1 = (float)(a.out_scale * a.kv_scale), f2 = (float)a.out_scale * tables[g & 1].head[row];
+                const float out_scale = (float)a.out_scale, head = tables[g & 1].head[row];
                 warp_arrive(bar(kDecFree0 + (g & 1)));
-                uint4 y[DOT ? 8 : 1];
-                if (DOT) {
-                    if (!(ok = warp_wait(bar(kDot), g & 1, failed))) break;
+                // the state's part first, into O1's columns: it is there before P, and O2's columns are free at once
+                const bool past = !no_past(it, i);
+                float dot = 0.f;
+                if (DOT && !(ok = warp_wait(bar(kDot), g & 1, failed))) break;
+                if (past) {
+                    if (!(ok = warp_wait(bar(kInc), g & 1, failed))) break;
+                    fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {   // 16 columns each
+                        float u[16];
+                        tmem_load16(tmem + lanes + Lay::c_o2 + c * 16, u);
+                        tmem_loaded();
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) y[DOT ? c : 0] = *reinterpret_cast<const uint4 *>(smem + Lay::dot + swizzled(row, c));
-                    warp_arrive(bar(kDotFree));
+                        for (int j = 0; j < 16; ++j) u[j] *= head;
+                        tmem_store16(tmem + lanes + Lay::c_o1 + c * 16, u);
+                        if (DOT && row < m)
+#pragma unroll
+                            for (int e = 0; e < 16; e += 8) {
+                                const uint4 p = *reinterpret_cast<const uint4 *>(smem + Lay::dot + swizzled(row, c * 2 + e / 8));
+                                const float2 two[4] = {unpack(p.x, T{}), unpack(p.y, T{}), unpack(p.z, T{}), unpack(p.w, T{})};
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) dot = fmaf(u[e + 2 * j], two[j].x, fmaf(u[e + 2 * j + 1], two[j].y, dot));
+                            }
+                    }
+                    tmem_stored();
+                    fence_before();
                 }
+                warp_arrive(bar(kO2));
+                if (DOT) warp_arrive(bar(kDotFree));
                 if (staged && g > 0 && !(ok = warp_wait(bar(kOutFree), (g - 1) & 1, failed))) break;
                 if (!(ok = warp_wait(bar(kO1), g & 1, failed))) break;
                 fence_after();
-                const bool past = !no_past(it, i);
-                float dot = 0.f;
-                auto columns = [&](int c, const uint4 &p0, const uint4 &p1) {   // 16 of them
-                    float u[16], w[16];
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    float u[16];
                     tmem_load16(tmem + lanes + Lay::c_o1 + c * 16, u);
-                    if (past) tmem_load16(tmem + lanes + Lay::c_o2 + c * 16, w);
                     tmem_loaded();
-                    if (!past)
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) w[j] = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        w[j] = row < m ? w[j] * f2 : 0.f;
-                        u[j] = row < m ? fmaf(u[j], f1, w[j]) : 0.f;
-                    }
-                    if (DOT) {
-                        const uint32_t words[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float2 two = unpack(words[j], T{});
-                            dot = fmaf(w[2 * j], two.x, fmaf(w[2 * j + 1], two.y, dot));
-                        }
-                    }
+                    for (int j = 0; j < 16; ++j) u[j] = row < m ? u[j] * out_scale : 0.f;
 #pragma unroll
                     for (int e = 0; e < 16; e += 8) {
                         const int col = col0 + c * 16 + e;
@@ -396,20 +403,12 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                             *reinterpret_cast<float4 *>(at + 4) = make_float4(u[e + 4], u[e + 5], u[e + 6], u[e + 7]);
                         }
                     }
-                };
-                if constexpr (DOT) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) columns(c, y[2 * c], y[2 * c + 1]);
-                } else {
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) columns(c, y[0], y[0]);
                 }
                 if (DOT && t < a.L) {
                     const float pairs = sums[((g & 1) * 2) * kPiece + row] + sums[((g & 1) * 2 + 1) * kPiece + row];
-                    a.dots[((long long)it.vt * a.B * a.L + (long long)it.b * a.L + t) * a.H + it.h] = row < m ? fmaf(pairs, f1, dot) : 0.f;
+                    a.dots[((long long)it.vt * a.B * a.L + (long long)it.b * a.L + t) * a.H + it.h] = row < m ? (pairs + dot) * out_scale : 0.f;
                 }
                 fence_before();
-                warp_arrive(bar(kEpi));
                 if (staged) {
                     fence_async();
                     warp_arrive(bar(kOutFull));
@@ -470,8 +469,9 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                     continue;
                 }
                 if (g > 0 && !(ok = warp_wait(bar(kO1), ph ^ 1, failed))) break;   // P of the piece before has been used
-                if (DOT && !(ok = warp_wait(bar(kDot), ph, failed) && warp_wait(bar(kFullV0), ph, failed))) break;
+                if (DOT && !(ok = warp_wait(bar(kDot), ph, failed) && warp_wait(bar(kFullV0 + g % VS), (g / VS) & 1, failed))) break;
                 fence_after();
+                const uint32_t v16 = base16 + (Lay::v >> 4) + (VS == 2 ? ph * (kTileBytes >> 4) : 0);
                 // scores = R K^T
 #pragma unroll
                 for (int j = 0; j < KP / 16; ++j) {
@@ -482,13 +482,11 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                 if (DOT)   // Y V^T
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        mma_ss(tmem + Lay::c_two, tile_desc(base16 + ((Lay::dot + j * 32) >> 4), 16), tile_desc(base16 + ((Lay::v + j * 32) >> 4), 16),
+                        mma_ss(tmem + Lay::c_two, tile_desc(base16 + ((Lay::dot + j * 32) >> 4), 16), tile_desc(v16 + j * 2, 16),
                                instr_desc<T>(128, false, false), j > 0, lead);
                 mma_commit(bar(kScores), lead);
-                // O2 = R S, when O2 of the piece before has been read and the state's operand is there (it was written before
-                // V').  Small terms first here and below: the accumulator drops what does not fit its 24 bits at every step,
+                // O2 = R S, when the state's operand is there (it was written before V').  Small terms first here and below: the accumulator drops what does not fit its 24 bits at every step,
                 // towards zero.
-                if (g > 0 && !(ok = warp_wait(bar(kEpi), ph ^ 1, failed))) break;
                 if (!(ok = warp_wait(bar(kVReady), ph, failed))) break;
                 fence_after();
                 const bool past = !no_past(it, i), future = !no_future(it, i);
@@ -502,14 +500,13 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                                term < NS - 1 || j > 0, lead);
                 if (future) state_product();
                 else mma_commit(bar(kInc), lead);
-                // O1 = P V
-                const uint32_t v16 = base16 + (Lay::v >> 4) + (VS == 2 ? ph * (kTileBytes >> 4) : 0);
-                if (!(ok = warp_wait(bar(kP), ph, failed))) break;
+                // O1 += P V, on top of the state's part, which the output warps put there
+                if (!(ok = warp_wait(bar(kP), ph, failed) && warp_wait(bar(kO2), ph, failed))) break;
                 fence_after();
 #pragma unroll
                 for (int j = 0; j < kPiece / 16; ++j)
                     mma_ts(tmem + Lay::c_o1, tmem + (j / 4) * 64 + (j % 4) * 8, tile_desc(v16 + (j * 2048 >> 4), kTileBytes),
-                           instr_desc<T>(64, false, true), j > 0, lead);
+                           instr_desc<T>(64, false, true), past || j > 0, lead);
                 mma_commit(bar(kO1), lead);
             }
         }
