@@ -39,7 +39,8 @@ def make(seed, B, L, H, Hkv, Dk, Dv, dtype, *, decay="step", state=False, length
 
 def absolute(c):
     """The same case with absolute values: every sum below then is the sum of the absolute values of its terms."""
-    return {n: t.abs() if isinstance(t, torch.Tensor) and n not in ("log_decay", "lengths") else t for n, t in c.items()}
+    return {n: t.abs() if isinstance(t, torch.Tensor) and n not in ("log_decay", "lengths") else abs(t) if n == "scale" else t
+            for n, t in c.items()}
 
 
 def attention(c, sign=-1.0):

@@ -317,6 +317,115 @@ def test_many_sequences_and_heads(ps):
     _check(_run(ps, _on_gpu(c, torch.float32)), *so.attention_bounds(c, torch.float32))
 
 
+LONG = [  # few long sequences are swept in parts, many short ones several to a block
+    ((1, 1200, 2, 1, 64, 64), None),
+    ((2, 1100, 2, 2, 128, 96), [1100, 700]),
+    ((1, 1700, 1, 1, 40, 128), None),
+    ((3, 1030, 1, 1, 64, 64), [0, 1030, 130]),
+    ((1, 1153, 1, 1, 128, 128), [1]),
+    ((50, 150, 4, 2, 64, 32), "random"),
+    ((70, 61, 4, 4, 32, 64), None),
+    ((40, 300, 4, 1, 96, 128), "random"),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("shape,lengths", LONG)
+@pytest.mark.parametrize("state", [False, True])
+def test_sequences_in_parts_and_several_to_a_block(ps, shape, lengths, state, dtype):
+    if lengths is not None:
+        gen = torch.Generator().manual_seed(shape[1])
+        lengths = torch.randint(0, shape[1] + 1, (shape[0],), generator=gen) if lengths == "random" else torch.tensor(lengths)
+    c = so.make(sum(shape), *shape, dtype, state=state, lengths=lengths, rate=0.02)
+    _check(_run(ps, _on_gpu(c, dtype)), *so.attention_bounds(c, dtype))
+    _no_timeouts()
+
+
+def _no_timeouts():
+    from pathsig_b200 import _load
+    assert _load.ensure_loaded().psig_sequence_wait_timeouts() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("shape", [(2, 61, 8, 8, 64, 64), (1, 300, 4, 2, 128, 72)])
+def test_kernels_of_every_size_at_the_sizes_of_the_others(ps, shape, dtype):
+    c = so.make(17, *shape, dtype, state=True)
+    ps.ops.set_algorithm("generic")
+    try:
+        got = _run(ps, _on_gpu(c, dtype))
+    finally:
+        ps.ops.set_algorithm("auto")
+    _check(got, *so.attention_bounds(c, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [0.0, 1.0, -2.5])
+def test_scales(ps, dtype, scale):
+    c = so.make(23, 2, 140, 2, 1, 64, 64, dtype, state=True) | {"scale": scale}
+    got = _run(ps, _on_gpu(c, dtype), scale=scale)
+    _check(got, *so.attention_bounds(c, dtype))
+    if scale == 0.0:
+        assert not got["out"].any() and not got["grad_q"].any()
+
+
+def test_float16_scores_and_states_beyond_its_range(ps):
+    """Scores of 128 * 300 * 300 and sums of 200 such products do not fit float16; the results do."""
+    c = so.make(29, 1, 200, 1, 1, 128, 64, torch.float16, decay="none")
+    for n, size in (("q", 300.0), ("k", 300.0), ("v", 2.0 ** -14), ("grad_out", 2.0 ** -14)):
+        c[n] = (c[n].sign() * size * (1 + c[n].abs() / 64)).to(torch.float16).double()
+    c["q"], c["k"] = c["q"].abs(), c["k"].abs()
+    exact, bounds = so.attention_bounds(c, torch.float16)
+    got = _run(ps, _on_gpu(c, torch.float16))
+    assert float(exact["out"].abs().max()) < 65504
+    _check({n: got[n] for n in ("out", "state")}, exact, bounds)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_offsets_beyond_32_bits(ps, dtype):
+    """Operands of more than 2^31 elements: the last heads of the last steps against a call on those heads alone."""
+    L, H, D = 65664, 256, 128
+    gen = torch.Generator(DEV).manual_seed(3)
+    big = torch.randn(1, L, H, D, device=DEV, generator=gen, dtype=dtype)
+    assert big.numel() > 2 ** 31
+    decay = -torch.rand(H, device=DEV, generator=gen)
+    out, state = ps.linear_attention(big, big, big, decay, return_state=True)
+    few = big[:, :, -2:].contiguous()
+    want, want_state = ps.linear_attention(few, few, few, decay[-2:], return_state=True)
+    # the few heads are swept in parts, so sums run in another order: one rounding of the storage type, and of sums
+    apart = 2 * so.half_step(dtype) if dtype == torch.bfloat16 else 3e-6
+    assert util.rel_error(out[:, -3000:, -2:], want[:, -3000:]) < apart
+    assert util.rel_error(state[:, -2:], want_state) < 3e-6
+    del out, big
+    torch.cuda.empty_cache()
+
+
+def test_concurrent_host_threads_and_streams(ps):
+    import threading
+    c = so.make(31, 3, 300, 4, 2, 64, 64, torch.bfloat16, state=True)
+    g = _on_gpu(c, torch.bfloat16)
+    want = _run(ps, g)
+    torch.cuda.synchronize()
+    results, errors = {}, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    results[i] = _run(ps, g)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:   # noqa: BLE001 - reported below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors
+    for got in results.values():
+        for name in want:
+            assert torch.equal(got[name], want[name]), name
+    _no_timeouts()
+
+
 def test_refusals_on_the_gpu(ps):
     f = lambda *s, t=torch.float32: torch.zeros(*s, dtype=t, device=DEV)
     q, k, v, d = f(2, 5, 4, 8), f(2, 5, 2, 8), f(2, 5, 2, 6), f(4)

@@ -58,6 +58,20 @@ def test_missing_pointers_and_workspaces_are_refused():
     assert lib.psig_norm_backward_workspace(ctypes.byref(n)) == -2
 
 
+def test_parts_of_long_sequences_need_a_workspace():
+    lib = _load.ensure_loaded()
+    one = ctypes.c_void_p(256)
+    short, long = _attn(B=1, H=2, L=500), _attn(B=1, H=2, L=16384)
+    assert lib.psig_attn_forward_workspace(ctypes.byref(short)) == 0
+    need = lib.psig_attn_forward_workspace(ctypes.byref(long))
+    assert need >= 2 * 2 * 4 * 64 * 64          # two heads, two parts or more, a tile of states each
+    assert lib.psig_attn_forward(ctypes.byref(long), one, one, one, one, None, one, None, None, 0, None) == -6
+    assert lib.psig_attn_forward(ctypes.byref(long), one, one, one, one, None, one, None, one, need - 1, None) == -6
+    assert lib.psig_attn_backward_workspace(ctypes.byref(long)) > need
+    many = _attn(B=64, H=16, L=16384)           # enough blocks without
+    assert lib.psig_attn_forward_workspace(ctypes.byref(many)) == 0
+
+
 def test_nothing_to_do_is_no_error():
     lib = _load.ensure_loaded()
     d = ctypes.byref(_attn(B=0))
