@@ -260,7 +260,10 @@ int psig_chen_backward(const PsigChenDesc *desc, const void *a, const void *b, c
  *     float64 when dtype is PSIG_F64.  Meant to be <= 0; -inf forgets everything before the step.
  *   initial_state, final_state and their gradients (B, H, dk, dv): contiguous, type of log_decay.
  *   out, grad_out (B, L, H, dv), grad_q, grad_k, grad_v: contiguous, dtype.
- * dk and dv are at most 256; sums and states are held in 32 bits (64 for PSIG_F64). */
+ * dk and dv are at most 256; sums and states are held in 32 bits (64 for PSIG_F64).
+ * Head sizes up to 128 whose rows are whole 16-byte pieces run on the tensor cores when the operands start on 16-byte boundaries
+ * and their strides are multiples of 16 bytes.  For operands that do not start on such boundaries set algo to
+ * PSIG_ALGO_GENERIC, for the workspace query as for the call (it returns PSIG_ERR_WORKSPACE otherwise). */
 typedef struct PsigAttnDesc {
     int32_t dtype;            /* PsigDtype */
     int32_t dk, dv;           /* head sizes, 1..256 */

@@ -406,7 +406,7 @@ int check_attn(const PsigAttnDesc *d)
     if (d->B < 0 || d->L < 0 || d->dk < 1 || d->dv < 1 || d->H < 1 || d->Hkv < 1 || d->H % d->Hkv != 0)
         return PSIG_ERR_SHAPE;
     if (d->dk > 256 || d->dv > 256) return PSIG_ERR_TOO_LARGE;
-    if (d->B * d->H > 0x7fffffffLL) return PSIG_ERR_TOO_LARGE;
+    if (d->H > 65535 || d->B > 0x7fffffffLL / d->H) return PSIG_ERR_TOO_LARGE;   // a block's index, a grid's second dimension
     return PSIG_OK;
 }
 
@@ -484,11 +484,12 @@ struct Call {
         s.kv_scale = d.scale;
         return s;
     }
-    bool tiles(const void *o1, const void *o2 = nullptr, const void *o3 = nullptr) const
+    // By sizes and strides; with null pointers for the operands this is what the workspace queries go by.
+    bool tiles(const void *o1 = nullptr, const void *o2 = nullptr, const void *o3 = nullptr) const
     {
         for (const void *o : {o1, o2, o3})
             if (reinterpret_cast<uintptr_t>(o) % 16 != 0) return false;
-        return d.algo != PSIG_ALGO_GENERIC && attn_tiles_supported(forward(), d.dtype);
+        return d.algo != PSIG_ALGO_GENERIC && attn_tiles_supported(forward(), d.dtype) && attn_tiles_supported(grad_q(), d.dtype);
     }
 };
 
@@ -506,8 +507,8 @@ void set_splits(Sweep &s, void *scratch)
     s.split_decays = s.split_states + s.B * s.H * s.splits * split_state_size(s.d1, s.d2);
 }
 
-// Scratch of the backward pass, in the order it is laid out (256-byte aligned pieces).  It does not depend on which
-// form of the sweeps serves the call, which the operands' addresses decide too.
+// Scratch of the backward pass, in the order it is laid out (256-byte aligned pieces).  The tensor-core sweeps write
+// gradients to their place, but for heads that share a key/value head; the others keep them unrounded first.
 struct BackwardScratch {
     long long gq, gk, gv, pairs, anchors, dots, totals, parts, bytes;
 };
@@ -518,7 +519,7 @@ int anchor_parts(const PsigAttnDesc &d)
     return rows > tiles ? rows : tiles;
 }
 
-BackwardScratch backward_scratch(const PsigAttnDesc &d)
+BackwardScratch backward_scratch(const PsigAttnDesc &d, bool tiles)
 {
     const long long acc = d.dtype == PSIG_F64 ? 8 : 4, rows = d.B * d.L * d.H, bh = d.B * d.H, seg = segments_of(d.L);
     BackwardScratch s{};
@@ -528,11 +529,12 @@ BackwardScratch backward_scratch(const PsigAttnDesc &d)
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    s.gq = take(acc * rows * d.dk);
-    s.gk = take(acc * rows * d.dk);
-    s.gv = take(acc * rows * d.dv);
-    const long long pair_bytes = 4 * 4 * tile_columns(d.dk);   // the tiles' two sets of two float arrays per column tile
-    s.pairs = take((pair_bytes > 8 ? pair_bytes : 8) * rows);
+    const bool shared = d.H != d.Hkv;
+    s.gq = take(tiles ? 0 : acc * rows * d.dk);
+    s.gk = take(tiles && !shared ? 0 : acc * rows * d.dk);
+    s.gv = take(tiles && !shared ? 0 : acc * rows * d.dv);
+    // the tiles' two sets of float arrays, one array or two per column tile
+    s.pairs = take((tiles ? 2 * 4 * attn_tile_dots(d.dtype) * tile_columns(d.dk) : 8) * rows);
     // the tensor-core sweeps store whole tiles of 64 by 64
     s.anchors = take(acc * bh * seg * ((d.dk + 63) / 64 * 64) * ((d.dv + 63) / 64 * 64));
     s.dots = take(acc * bh * seg * anchor_parts(d));
@@ -608,11 +610,11 @@ int run_backward_tiles(const Call &c, const void *init, const void *gs, void *gr
                        void *grad_decay, void *grad_init, char *ws, cudaStream_t stream)
 {
     const PsigAttnDesc &d = c.d;
-    const BackwardScratch at = backward_scratch(d);
+    const BackwardScratch at = backward_scratch(d, true);
     const long long rows = d.B * d.L * d.H, kv_rows = d.B * d.L * d.Hkv;
     const int tiles = tile_columns(d.dk);
     const bool shared = c.share > 1;
-    float *x = reinterpret_cast<float *>(ws + at.pairs), *y = x + 2 * tiles * rows;
+    float *x = reinterpret_cast<float *>(ws + at.pairs), *y = x + attn_tile_dots(d.dtype) * tiles * rows;
     int rc;
     Sweep s = c.grad_q();
     s.init = init;
@@ -645,13 +647,16 @@ int run_backward_tiles(const Call &c, const void *init, const void *gs, void *gr
 
 template <typename T>
 int run_backward(const Call &c, const void *init, const void *gs, void *grad_q, void *grad_k, void *grad_v,
-                 void *grad_decay, void *grad_init, char *ws, cudaStream_t stream)
+                 void *grad_decay, void *grad_init, char *ws, long long ws_bytes, cudaStream_t stream)
 {
     using A = typename Acc<T>::type;
-    if (c.tiles(grad_q, grad_k, grad_v) && attn_tiles_supported(c.grad_q(), c.d.dtype))
+    const bool tiles = c.tiles(grad_q, grad_k, grad_v);
+    const long long need = backward_scratch(c.d, tiles).bytes;
+    if (need > 0 && (ws == nullptr || ws_bytes < need)) return PSIG_ERR_WORKSPACE;
+    if (tiles)
         return run_backward_tiles<T>(c, init, gs, grad_q, grad_k, grad_v, grad_decay, grad_init, ws, stream);
     const PsigAttnDesc &d = c.d;
-    const BackwardScratch at = backward_scratch(d);
+    const BackwardScratch at = backward_scratch(d, false);
     const long long rows = d.B * d.L * d.H, kv_rows = d.B * d.L * d.Hkv;
     A *gq = reinterpret_cast<A *>(ws + at.gq), *gk = reinterpret_cast<A *>(ws + at.gk);
     double *pairs = reinterpret_cast<double *>(ws + at.pairs);
@@ -695,7 +700,7 @@ extern "C" int64_t psig_attn_forward_workspace(const PsigAttnDesc *desc)
 extern "C" int64_t psig_attn_backward_workspace(const PsigAttnDesc *desc)
 {
     const int rc = check_attn(desc);
-    return rc != PSIG_OK ? rc : backward_scratch(*desc).bytes;
+    return rc != PSIG_OK ? rc : backward_scratch(*desc, Call(*desc, nullptr, nullptr, nullptr, nullptr, nullptr).tiles()).bytes;
 }
 
 extern "C" int psig_attn_forward(const PsigAttnDesc *desc, const void *q, const void *k, const void *v,
@@ -725,12 +730,10 @@ extern "C" int psig_attn_backward(const PsigAttnDesc *desc, const void *q, const
     if (rc != PSIG_OK) return rc;
     if (desc->B == 0 || desc->L == 0) return PSIG_OK;   // nothing depends on the operands
     if (!q || !k || !v || !log_decay || !grad_out || !grad_q || !grad_k || !grad_v) return PSIG_ERR_NULL;
-    const int64_t need = backward_scratch(*desc).bytes;
-    if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return PSIG_ERR_WORKSPACE;
     return with_dtype(desc->dtype, [&](auto t) {
         return run_backward<decltype(t)>(Call(*desc, q, k, v, log_decay, grad_out), initial_state, grad_state, grad_q, grad_k,
                                          grad_v, grad_log_decay, grad_initial_state, static_cast<char *>(workspace),
-                                         static_cast<cudaStream_t>(stream));
+                                         workspace_bytes, static_cast<cudaStream_t>(stream));
     });
 }
 

@@ -17,17 +17,18 @@
 // DOT: the sweep also gives x_t = out_t . y_t for the rows y of a third operand, to 32 bits (the decay gradient needs
 // q . grad_q and k . grad_k).  The part of the piece's own pairs is sum_s exp(a_t - a_s) (r_t . k_s) (y_t . v_s), the
 // weighted scores times a second product Y V^T, entry by entry before anything is rounded; the state's part is
-// exp(a_t) (r_t^T S) . y_t.  (With the output row itself, P would have to enter as three terms: 380 us against
-// the time in launch_tiles.)
+// exp(a_t) (r_t^T S) . y_t.  (With the output row itself, P would have to enter as three terms.)
 //
 // Warps, so that a piece's stages overlap with the neighbouring pieces': 8 hold the state and weigh V (thread = state
 // row, and = time step), 8 weigh the scores, 4 write the output, one each issues the products, starts the copies, and sums the next piece's decays.
 // A thread reads the 32 lanes of tensor memory that its warp's number allows; two warps share 32 rows and split the
 // columns.  They meet at mbarriers; every wait is bounded (psig_sequence_wait_timeouts).
 //
-// Measured (one 16384-step sequence of 16 heads of 128, 32 blocks): 3.9 us a piece when the same 8 warps did all stages
-// one after the other and a branch of one thread issued the products (of 7000 cycles: 2150 scores to P, 1400 output, 1000
-// V', 1100 issue); see launch_tiles for this form.
+// Measured, 8 sequences of 4096 steps of 16 heads of 128 (the bytes alone: 82 us forward): 382 us forward when the same 8 warps
+// did all stages one after the other (of 7000 cycles a piece: 2150 scores to P, 1400 output, 1000 V', 1100 issue); 200 us
+// in this form, 355 us with DOT (one and two 24-bit operands more).  Tensor pipe 28 % busy: the products of 64 columns are limited
+// by reading their operands from shared memory, and a piece's chain of scores, weights and product by latency.  Code size matters:
+// with all loops unrolled the six roles miss the instruction cache (63 % hits, 290 us).
 #include "tiles.cuh"
 
 namespace psig {

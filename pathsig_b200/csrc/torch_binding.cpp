@@ -432,8 +432,18 @@ void check_operand(const at::Tensor &anchor, const at::Tensor &t, const char *na
     TORCH_CHECK(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
 }
 
-// The kernels read operands through their strides; only the last dimension has to be dense.
-at::Tensor dense_last(const at::Tensor &t) { return t.size(-1) > 1 && t.stride(-1) != 1 ? t.contiguous() : t; }
+// The kernels read operands through their strides; only the last dimension has to be dense.  Rows of whole 16-byte pieces are
+// copied where they do not start on 16-byte boundaries (an odd offset, a broadcast dimension): that costs less than what the
+// tensor-core kernels, which want this, save.
+at::Tensor readable(const at::Tensor &t)
+{
+    if (t.size(-1) > 1 && t.stride(-1) != 1) return t.contiguous();
+    const int64_t unit = 16 / t.element_size();
+    if (t.size(-1) % unit != 0 || t.size(-1) > 128) return t;
+    bool fits = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    for (int64_t i = 0; i + 1 < t.dim(); ++i) fits = fits && (t.size(i) <= 1 || (t.stride(i) > 0 && t.stride(i) % unit == 0));
+    return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
 
 void set_strides(int64_t *to, const at::Tensor &t, bool has_time)
 {
@@ -470,7 +480,7 @@ PsigAttnDesc attn_desc(at::Tensor &q, at::Tensor &k, at::Tensor &v, at::Tensor &
     desc.dv = (int32_t)v.size(-1);
     desc.scale = scale;
     desc.algo = g_algo.load() == PSIG_ALGO_GENERIC ? PSIG_ALGO_GENERIC : PSIG_ALGO_AUTO;
-    q = dense_last(q), k = dense_last(k), v = dense_last(v);
+    q = readable(q), k = readable(k), v = readable(v);
     set_strides(desc.q_strides, q, has_time);
     set_strides(desc.k_strides, k, has_time);
     set_strides(desc.v_strides, v, has_time);
@@ -558,7 +568,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_at
         check_operand(q, *grad_out, "grad_out", q.scalar_type());
         TORCH_CHECK(grad_out->dim() == 4 && grad_out->size(0) == desc.B && grad_out->size(1) == desc.L &&
                     grad_out->size(2) == desc.H && grad_out->size(3) == desc.dv, "grad_out must have the shape of the output");
-        go = grad_out->contiguous();
+        go = readable(grad_out->contiguous());
     } else {
         go = at::zeros({desc.B, desc.L, desc.H, desc.dv}, q.options());
     }
