@@ -37,8 +37,10 @@ namespace {
 constexpr int kStateThreads = 256, kScoreThreads = 256, kOutThreads = 128;
 constexpr int kTileThreads = kStateThreads + kScoreThreads + kOutThreads + 96;
 
+// A wait names the parity of a phase, so nobody may be two phases behind: what a place of V waits for (I or O1 of two pieces
+// before) is counted by that place.
 enum Barrier {
-    kFullRK, kFullV0, kFullV1, kVReady, kScores, kInc, kP, kO2, kO1, kFix, kOutFull, kOutFree, kDot, kDotFree,
+    kFullRK, kFullV0, kFullV1, kVReady, kScores, kInc0, kInc1, kP, kO2, kO1_0, kO1_1, kFix, kOutFull, kOutFree, kDot, kDotFree,
     kDecFull0, kDecFull1, kDecFree0, kDecFree1, kBarriers
 };
 
@@ -92,9 +94,11 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
         bar_init(bar(kFullV1), 1);
         bar_init(bar(kVReady), kStateThreads / 32);
         bar_init(bar(kScores), 1);
-        bar_init(bar(kInc), 1);
+        bar_init(bar(kInc0), 1);
+        bar_init(bar(kInc1), 1);
         bar_init(bar(kP), kScoreThreads / 32);
-        bar_init(bar(kO1), 1);
+        bar_init(bar(kO1_0), 1);
+        bar_init(bar(kO1_1), 1);
         bar_init(bar(kO2), kOutThreads / 32);
         bar_init(bar(kFix), kStateThreads / 32);
         bar_init(bar(kOutFull), kOutThreads / 32);
@@ -240,7 +244,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                     for (int s = 16; s >= 1; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
                     if (lane == 0) static_cast<float *>(a.anchor_dots)[((it.bh * segments + segment) * tiles + it.vt) * 8 + warp] = dot;
                 }
-                if (!(ok = warp_wait(bar(kInc), ph, failed))) break;
+                if (!(ok = warp_wait(bar(kInc0 + (g & 1)), (g >> 1) & 1, failed))) break;
                 if (last) continue;
                 fence_after();
                 float x[SC / 16][16];
@@ -353,9 +357,9 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                 const bool past = !no_past(it, i);
                 float dot = 0.f;
                 if (DOT && !(ok = warp_wait(bar(kDot), g & 1, failed))) break;
+                if (!(ok = warp_wait(bar(kInc0 + (g & 1)), (g >> 1) & 1, failed))) break;   // without a past too: no phase is left out
+                fence_after();
                 if (past) {
-                    if (!(ok = warp_wait(bar(kInc), g & 1, failed))) break;
-                    fence_after();
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {   // 16 columns each
                         float u[16];
@@ -379,7 +383,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                 warp_arrive(bar(kO2));
                 if (DOT) warp_arrive(bar(kDotFree));
                 if (staged && g > 0 && !(ok = warp_wait(bar(kOutFree), (g - 1) & 1, failed))) break;
-                if (!(ok = warp_wait(bar(kO1), g & 1, failed))) break;
+                if (!(ok = warp_wait(bar(kO1_0 + (g & 1)), (g >> 1) & 1, failed))) break;
                 fence_after();
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
@@ -443,7 +447,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
         // ------------------------------------------------------------------ TMA and MMA
         const uint32_t lead = lane == 0, base16 = base >> 4;
         // I = K^T V'; with 64 state rows the second block of 64 is the first once more
-        auto state_product = [&]() {
+        auto state_product = [&](int g) {
 #pragma unroll
                 for (int term = NV - 1; term >= 0; --term)
 #pragma unroll
@@ -451,7 +455,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                         mma_ss(tmem + Lay::c_i, tile_desc(base16 + ((Lay::k + j * 2048) >> 4), KP == 128 ? kTileBytes : 0),
                                tile_desc(base16 + ((Lay::vw + term * kTileBytes + j * 2048) >> 4), kTileBytes), instr_desc<T>(64, true, true),
                                term < NV - 1 || j > 0, lead);
-                mma_commit(bar(kInc), lead);
+                mma_commit(bar(kInc0 + (g & 1)), lead);
         };
         int g = 0, fixes = 0;
         bool ok = true;
@@ -466,10 +470,10 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                 if constexpr (STATE) {   // I alone
                     if (!(ok = warp_wait(bar(kVReady), ph, failed))) break;
                     fence_after();
-                    state_product();
+                    state_product(g);
                     continue;
                 }
-                if (g > 0 && !(ok = warp_wait(bar(kO1), ph ^ 1, failed))) break;   // P of the piece before has been used
+                if (g > 0 && !(ok = warp_wait(bar(kO1_0 + (ph ^ 1)), ((g - 1) >> 1) & 1, failed))) break;   // P of the piece before has been used
                 if (DOT && !(ok = warp_wait(bar(kDot), ph, failed) && warp_wait(bar(kFullV0 + g % VS), (g / VS) & 1, failed))) break;
                 fence_after();
                 const uint32_t v16 = base16 + (Lay::v >> 4) + (VS == 2 ? ph * (kTileBytes >> 4) : 0);
@@ -499,8 +503,8 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                         mma_ss(tmem + Lay::c_o2, tile_desc(base16 + ((Lay::r + (j / 4) * kTileBytes + (j % 4) * 32) >> 4), 16),
                                tile_desc(base16 + ((Lay::s + term * KP * 128 + j * 2048) >> 4), kTileBytes), instr_desc<T>(64, false, true),
                                term < NS - 1 || j > 0, lead);
-                if (future) state_product();
-                else mma_commit(bar(kInc), lead);
+                if (future) state_product(g);
+                else mma_commit(bar(kInc0 + (g & 1)), lead);
                 // O1 += P V, on top of the state's part, which the output warps put there
                 if (!(ok = warp_wait(bar(kP), ph, failed) && warp_wait(bar(kO2), ph, failed))) break;
                 fence_after();
@@ -508,7 +512,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                 for (int j = 0; j < kPiece / 16; ++j)
                     mma_ts(tmem + Lay::c_o1, tmem + (j / 4) * 64 + (j % 4) * 8, tile_desc(v16 + (j * 2048 >> 4), kTileBytes),
                            instr_desc<T>(64, false, true), past || j > 0, lead);
-                mma_commit(bar(kO1), lead);
+                mma_commit(bar(kO1_0 + (g & 1)), lead);
             }
         }
     } else if (warp == 21) {
@@ -523,7 +527,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                 for (int i = 0; i < it.pieces; ++i, ++g) {
                     const int t0 = (int)it.start<REV>(i), b = (int)it.b;
                     auto load_v = [&]() {   // behind the last product that reads the V in its place
-                        if (g >= VS && !bar_wait(bar(STATE ? kInc : kO1), (g - VS) & 1, failed)) return false;
+                        if (g >= VS && !bar_wait(bar((STATE ? kInc0 : kO1_0) + ((g - VS) & 1)), ((g - VS) >> 1) & 1, failed)) return false;
                         bar_expect(bar(kFullV0 + g % VS), kTileBytes);
                         tma_load(base + Lay::v + (g % VS) * kTileBytes, &map_v, bar(kFullV0 + g % VS), it.vt * 64, vh, t0, b);
                         return true;
@@ -534,7 +538,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                         bar_expect(bar(kDot), kTileBytes);
                         tma_load(base + Lay::dot, &map_dot, bar(kDot), it.vt * 64, dh, t0, b);
                     }
-                    if (g > 0 && !bar_wait(bar(kInc), (g - 1) & 1, failed)) { stop = 3; break; }   // the last product that reads R and K
+                    if (g > 0 && !bar_wait(bar(kInc0 + ((g - 1) & 1)), ((g - 1) >> 1) & 1, failed)) { stop = 3; break; }   // the last product that reads R and K
                     bar_expect(bar(kFullRK), (STATE ? 1 : 2) * Lay::panels * kTileBytes);
 #pragma unroll
                     for (int p = 0; p < Lay::panels; ++p) {
