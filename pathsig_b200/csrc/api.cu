@@ -159,7 +159,7 @@ const char *psig_status_string(int status)
     switch (status) {
         case PSIG_OK: return "ok";
         case PSIG_ERR_NULL: return "a required pointer is NULL";
-        case PSIG_ERR_DTYPE: return "dtype must be float32 or float64";
+        case PSIG_ERR_DTYPE: return "dtype is not one that this entry point takes";
         case PSIG_ERR_DEPTH: return "depth must be in [1,12]";
         case PSIG_ERR_SHAPE: return "invalid shape (need B >= 0, L >= 2, d >= 1, W >= 0, consistent level sizes)";
         case PSIG_ERR_PACKING: return "d^depth does not fit a 64-bit word code";

@@ -618,12 +618,12 @@ int select_tiles(const Sweep &a, int dtype, cudaStream_t stream)
 
 }  // namespace
 
-// Head sizes up to 128, in whole 16-byte pieces (TMA).  Both forms take the same sizes: a call's forward pass and its
+// Head sizes up to 128, in whole 16-byte pieces (TMA); as many items (two tiles a head) as an int counts in steps of a grid.  Both forms take the same sizes: a call's forward pass and its
 // three gradients go the same way.
 bool attn_tiles_supported(const Sweep &a, int dtype)
 {
     const int size = dtype == PSIG_F32 ? 4 : 2;
-    return dtype != PSIG_F64 && a.d1 <= 128 && a.d2 <= 128 && a.L < (1LL << 31) - kPiece && a.B < (1LL << 31) && a.B * a.H < (1LL << 30) &&
+    return dtype != PSIG_F64 && a.d1 <= 128 && a.d2 <= 128 && a.L < (1LL << 31) - kPiece && a.B < (1LL << 31) && a.B * a.H < (1LL << 30) - 148 &&
            operand_fits(a.r, a, a.d1, size) && operand_fits(a.k, a, a.d1, size) && operand_fits(a.v, a, a.d2, size);
 }
 

@@ -813,8 +813,7 @@ void set_sizes(NormArgs &a, const PsigNormDesc &d)
     a.mean_f = (float)a.mean, a.eps_f = (float)a.eps;
 }
 
-// How a row is dealt to threads: 8 values to a thread, 16 where the row would need more than 256 threads (a block with
-// more of them waits longer at its barriers than the larger number of values costs: 4680 values, see norm_forward_team).
+// How a row is dealt to threads: 8 values to a thread, 16 where the row would need more than 256 threads.
 struct TeamPlan {
     int team_log2, threads, block;   // log2 of the team inside a warp (5: the block is the team); threads per row; block size
     int values;                      // per thread

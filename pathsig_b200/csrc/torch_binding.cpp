@@ -471,6 +471,7 @@ PsigAttnDesc attn_desc(at::Tensor &q, at::Tensor &k, at::Tensor &v, at::Tensor &
     TORCH_CHECK(q.size(-2) >= 1 && k.size(-2) >= 1 && q.size(-2) % k.size(-2) == 0, "the number of heads of q (", q.size(-2),
                 ") must be a multiple of that of k and v (", k.size(-2), ")");
     TORCH_CHECK(q.size(-1) >= 1 && q.size(-1) <= 256 && v.size(-1) >= 1 && v.size(-1) <= 256, "head sizes must be in [1,256]");
+    TORCH_CHECK(q.size(-2) <= 65535, "there may be at most 65535 heads");   // before they are narrowed
     TORCH_CHECK(std::isfinite(scale), "scale must be finite");
     desc.B = q.size(0);
     desc.L = has_time ? q.size(1) : 1;
@@ -744,6 +745,44 @@ std::tuple<at::Tensor, at::Tensor> attention_below(const at::Tensor &q, const at
     return op.call(q, k, v, decay, init, lengths, scale, return_state);
 }
 
+// The gradients' own gradients are refused (torch would warn and leave them out).
+using AttentionGrads = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+
+AttentionGrads attention_backward_below(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &decay,
+                                        const OptionalTensor &init, const OptionalTensor &lengths, const OptionalTensor &go,
+                                        const OptionalTensor &gs, double scale, bool decay_grad)
+{
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = handle<decltype(linear_attention_backward)>("pathsig_b200::linear_attention_backward");
+    return op.call(q, k, v, decay, init, lengths, go, gs, scale, decay_grad);
+}
+
+struct AttentionGradsFunction : torch::autograd::Function<AttentionGradsFunction> {
+    static variable_list forward(AutogradContext *, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
+                                 const at::Tensor &decay, const OptionalTensor &init, const OptionalTensor &lengths,
+                                 const OptionalTensor &go, const OptionalTensor &gs, double scale, bool decay_grad)
+    {
+        auto [gq, gk, gv, gd, gi] = attention_backward_below(q, k, v, decay, init, lengths, go, gs, scale, decay_grad);
+        return {gq, gk, gv, gd, gi};
+    }
+    static variable_list backward(AutogradContext *, variable_list)
+    {
+        TORCH_CHECK(false, "linear_attention is differentiable once: its gradients have no gradient");
+    }
+};
+
+AttentionGrads linear_attention_backward_autograd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
+                                                  const at::Tensor &decay, const OptionalTensor &init,
+                                                  const OptionalTensor &lengths, const OptionalTensor &go,
+                                                  const OptionalTensor &gs, double scale, bool decay_grad)
+{
+    if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad() || decay.requires_grad() ||
+                                         tracked(init) || tracked(go) || tracked(gs)))
+        return attention_backward_below(q, k, v, decay, init, lengths, go, gs, scale, decay_grad);
+    variable_list g = AttentionGradsFunction::apply(q, k, v, decay, init, lengths, go, gs, scale, decay_grad);
+    return std::make_tuple(g[0], g[1], g[2], g[3], g[4]);
+}
+
 struct AttentionFunction : torch::autograd::Function<AttentionFunction> {
     static variable_list forward(AutogradContext *ctx, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
                                  const at::Tensor &decay, const OptionalTensor &init, const OptionalTensor &lengths, double scale,
@@ -792,6 +831,47 @@ std::tuple<at::Tensor, at::Tensor> norm_below(const at::Tensor &x, const Optiona
     at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = handle<decltype(gated_residual_norm)>("pathsig_b200::gated_residual_norm");
     return op.call(x, weight, gate, residual, residual_scale, next_weight, activation, eps);
+}
+
+using NormGrads = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+
+NormGrads norm_backward_below(const at::Tensor &x, const OptionalTensor &weight, const OptionalTensor &gate,
+                              const OptionalTensor &residual, const OptionalTensor &residual_scale,
+                              const OptionalTensor &next_weight, const OptionalTensor &grad_h, const OptionalTensor &grad_n,
+                              int64_t activation, double eps)
+{
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = handle<decltype(gated_residual_norm_backward)>("pathsig_b200::gated_residual_norm_backward");
+    return op.call(x, weight, gate, residual, residual_scale, next_weight, grad_h, grad_n, activation, eps);
+}
+
+struct NormGradsFunction : torch::autograd::Function<NormGradsFunction> {
+    static variable_list forward(AutogradContext *, const at::Tensor &x, const OptionalTensor &weight, const OptionalTensor &gate,
+                                 const OptionalTensor &residual, const OptionalTensor &residual_scale,
+                                 const OptionalTensor &next_weight, const OptionalTensor &grad_h, const OptionalTensor &grad_n,
+                                 int64_t activation, double eps)
+    {
+        auto [gx, gw, gg, gr, gs, gn] =
+            norm_backward_below(x, weight, gate, residual, residual_scale, next_weight, grad_h, grad_n, activation, eps);
+        return {gx, gw, gg, gr, gs, gn};
+    }
+    static variable_list backward(AutogradContext *, variable_list)
+    {
+        TORCH_CHECK(false, "gated_residual_norm is differentiable once: its gradients have no gradient");
+    }
+};
+
+NormGrads gated_residual_norm_backward_autograd(const at::Tensor &x, const OptionalTensor &weight, const OptionalTensor &gate,
+                                                const OptionalTensor &residual, const OptionalTensor &residual_scale,
+                                                const OptionalTensor &next_weight, const OptionalTensor &grad_h,
+                                                const OptionalTensor &grad_n, int64_t activation, double eps)
+{
+    if (!at::GradMode::is_enabled() || !(x.requires_grad() || tracked(weight) || tracked(gate) || tracked(residual) ||
+                                         tracked(residual_scale) || tracked(next_weight) || tracked(grad_h) || tracked(grad_n)))
+        return norm_backward_below(x, weight, gate, residual, residual_scale, next_weight, grad_h, grad_n, activation, eps);
+    variable_list g =
+        NormGradsFunction::apply(x, weight, gate, residual, residual_scale, next_weight, grad_h, grad_n, activation, eps);
+    return std::make_tuple(g[0], g[1], g[2], g[3], g[4], g[5]);
 }
 
 struct NormFunction : torch::autograd::Function<NormFunction> {
@@ -891,5 +971,7 @@ TORCH_LIBRARY_IMPL(pathsig_b200, CUDA, m)
 TORCH_LIBRARY_IMPL(pathsig_b200, Autograd, m)
 {
     m.impl("linear_attention", &linear_attention_autograd);
+    m.impl("linear_attention_backward", &linear_attention_backward_autograd);
     m.impl("gated_residual_norm", &gated_residual_norm_autograd);
+    m.impl("gated_residual_norm_backward", &gated_residual_norm_backward_autograd);
 }

@@ -46,7 +46,9 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *, init
     [0, L] are clamped).  ``scale`` defaults to ``Dk ** -0.5``.
 
     Returns the output (B, L, H, Dv) in the type of ``q``; with ``return_state`` also the state after the last step
-    (B, H, Dk, Dv).  Differentiable (once) wrt all floating operands; gradients are the same bits on every run.
+    (B, H, Dk, Dv).  Differentiable once wrt all floating operands (a second derivative is refused); gradients
+    are the same bits on every run.  Under CUDA graph capture, capture forward and backward together, with no graph of an
+    eager call on the same leaves alive.
     """
     out, state = ops.linear_attention(q, k, v, log_decay, initial_state, lengths, _scale(q, scale), bool(return_state))
     return (out, state) if return_state else out
@@ -81,8 +83,8 @@ def gated_residual_norm(x: Tensor, weight: Optional[Tensor] = None, *, gate: Opt
     ``weight``, ``residual_scale`` and ``next_weight`` (D) are float32 (float64 next to float64), or in the type of
     ``x``.  ``n`` is the norm of h before h is rounded.
 
-    Returns ``h``, or ``(h, n)`` when ``next_weight`` is given, in the type of ``x``.  Differentiable (once) wrt all
-    operands; gradients are the same bits on every run.
+    Returns ``h``, or ``(h, n)`` when ``next_weight`` is given, in the type of ``x``.  Differentiable once wrt all
+    operands (a second derivative is refused); gradients are the same bits on every run.
     """
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}")

@@ -458,3 +458,20 @@ def test_refusals_on_the_gpu(ps):
         ps.linear_attention_step(q[:, 0].clone().requires_grad_(True), *step[1:], state)
     with pytest.raises(RuntimeError, match="state"):
         ps.linear_attention_step(*step, f(1, 4, 8, 6))
+    many = torch.zeros(1, 1, 1, 1, device=DEV)
+    for heads in (65536, 2 ** 32 + 1):   # would be 1 in 32 bits
+        with pytest.raises(RuntimeError, match="65535 heads"):
+            ps.linear_attention(many.expand(1, 1, heads, 1), many, many, f(1))
+
+
+def test_second_derivatives_are_refused(ps):
+    """A gradient with a graph of its own is the plain gradient; its gradient is refused, not left out."""
+    q, k, v = (torch.randn(1, 6, 2, 8, device=DEV, requires_grad=True) for _ in range(3))
+    d = torch.full((2,), -0.1, device=DEV, requires_grad=True)
+    leaves = (q, k, v, d)
+    plain = torch.autograd.grad(ps.linear_attention(*leaves).square().sum(), leaves)
+    graph = torch.autograd.grad(ps.linear_attention(*leaves).square().sum(), leaves, create_graph=True)
+    for a, b in zip(plain, graph):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        graph[0].sum().backward()

@@ -254,3 +254,15 @@ def test_refusals_on_the_gpu(ps):
         ps.gated_residual_norm(x.int())
     with pytest.raises(RuntimeError, match="D >= 1"):
         ps.gated_residual_norm(torch.zeros(3, 0, device=DEV))
+
+
+def test_second_derivatives_are_refused(ps):
+    """A gradient with a graph of its own is the plain gradient; its gradient is refused, not left out."""
+    x = torch.randn(5, 24, device=DEV, requires_grad=True)
+    w = torch.randn(24, device=DEV, requires_grad=True)
+    plain = torch.autograd.grad(ps.gated_residual_norm(x, w).square().sum(), (x, w))
+    graph = torch.autograd.grad(ps.gated_residual_norm(x, w).square().sum(), (x, w), create_graph=True)
+    for a, b in zip(plain, graph):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        graph[0].sum().backward()
