@@ -485,8 +485,14 @@ struct Call {
         return s;
     }
     // By sizes and strides; with null pointers for the operands this is what the workspace queries go by.
-    bool tiles(const void *o1 = nullptr, const void *o2 = nullptr, const void *o3 = nullptr) const
+    // A tile is computed whole, 128 steps, however few are there; the row kernel's time grows with the steps.  Rows / tiles, us:
+    // float16, 720 heads of 64: forward 20 / 41 at 8 steps, 32 / 41 at 16, 45 / 41 at 24; backward 125 / 150 and 171 / 152.
+    // float32: 31 / 54 at 16 steps, 45 / 54 at 24, but backward of 1024 heads of 128 753 / 749.  bfloat16 tiles are quicker and
+    // leave out the products of empty states: 1024 heads of 128 45 / 48 at 2 steps, 57 / 48 at 4; carrying a state from call
+    // to call 174 / 208 at 16 steps, 302 / 208 at 32.
+    bool tiles(bool carries, const void *o1 = nullptr, const void *o2 = nullptr, const void *o3 = nullptr) const
     {
+        if (d.L <= (d.dtype == PSIG_BF16 && !carries ? 2 : 16)) return false;
         for (const void *o : {o1, o2, o3})
             if (reinterpret_cast<uintptr_t>(o) % 16 != 0) return false;
         return d.algo != PSIG_ALGO_GENERIC && attn_tiles_supported(forward(), d.dtype) && attn_tiles_supported(grad_q(), d.dtype);
@@ -552,7 +558,7 @@ int run_forward(const Call &c, const void *init, void *out, void *final, void *w
     s.init = init;
     s.final = final;
     s.out = out;
-    if (!c.tiles(out)) return sweep_rows<T>(s, stream);
+    if (!c.tiles(init != nullptr && final != nullptr, out)) return sweep_rows<T>(s, stream);
     set_splits(s, ws);
     return attn_sweep_on_tiles(s, false, c.d.dtype, stream);
 }
@@ -650,7 +656,7 @@ int run_backward(const Call &c, const void *init, const void *gs, void *grad_q, 
                  void *grad_decay, void *grad_init, char *ws, long long ws_bytes, cudaStream_t stream)
 {
     using A = typename Acc<T>::type;
-    const bool tiles = c.tiles(grad_q, grad_k, grad_v);
+    const bool tiles = c.tiles(false, grad_q, grad_k, grad_v);
     const long long need = backward_scratch(c.d, tiles).bytes;
     if (need > 0 && (ws == nullptr || ws_bytes < need)) return PSIG_ERR_WORKSPACE;
     if (tiles)
@@ -700,7 +706,7 @@ extern "C" int64_t psig_attn_forward_workspace(const PsigAttnDesc *desc)
 extern "C" int64_t psig_attn_backward_workspace(const PsigAttnDesc *desc)
 {
     const int rc = check_attn(desc);
-    return rc != PSIG_OK ? rc : backward_scratch(*desc, Call(*desc, nullptr, nullptr, nullptr, nullptr, nullptr).tiles()).bytes;
+    return rc != PSIG_OK ? rc : backward_scratch(*desc, Call(*desc, nullptr, nullptr, nullptr, nullptr, nullptr).tiles(false)).bytes;
 }
 
 extern "C" int psig_attn_forward(const PsigAttnDesc *desc, const void *q, const void *k, const void *v,

@@ -618,8 +618,8 @@ int select_tiles(const Sweep &a, int dtype, cudaStream_t stream)
 
 }  // namespace
 
-// Head sizes up to 128, in whole 16-byte pieces (TMA); as many items (two tiles a head) as an int counts in steps of a grid.  Both forms take the same sizes: a call's forward pass and its
-// three gradients go the same way.
+// Head sizes up to 128, in whole 16-byte pieces (TMA); as many items (two tiles a head) as an int counts in steps of a
+// grid.  Both forms take the same sizes; a backward pass's three sweeps go the same way.
 bool attn_tiles_supported(const Sweep &a, int dtype)
 {
     const int size = dtype == PSIG_F32 ? 4 : 2;

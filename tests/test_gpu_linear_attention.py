@@ -475,3 +475,15 @@ def test_second_derivatives_are_refused(ps):
         assert torch.equal(a, b)
     with pytest.raises(RuntimeError, match="differentiable once"):
         graph[0].sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("state", [False, True])
+@pytest.mark.parametrize("steps", [1, 2, 3, 16, 17])
+def test_short_sequences_on_both_sides_of_the_kernels_limits(ps, steps, state, dtype):
+    c = so.make(steps + 40, 2, steps, 4, 2, 40, 72, dtype, state=state)
+    g = _on_gpu(c, dtype)
+    exact, bounds = so.attention_bounds(c, dtype)
+    _check(_run(ps, g), exact, bounds)
+    out = ps.linear_attention(*(g[n] for n in NAMES[:4]), initial_state=g["initial_state"])   # no state asked for
+    _check({"out": out}, exact, bounds)
