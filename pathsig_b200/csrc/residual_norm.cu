@@ -776,25 +776,29 @@ __global__ void __launch_bounds__(kWideThreads) norm_backward_wide(const NormArg
     }
 }
 
-// Sums of the blocks' partial rows, in a fixed order: 32 columns to a block, its warps take every 8th partial row.
+// Sums of the blocks' partial rows, in a fixed order: 32 columns to a block, its warps take the partial rows in turn, then the
+// columns.  Few columns are few blocks, so the loads in flight count: 32 warps (17909 x 376 8.8 -> 4.8 us, 15616 x 1024 9.3 -> 5.2);
+// where the columns fill the SMs 8 are quicker (12794 x 8192 9.8 us, 12.2 with 32).
 template <typename A>
-__global__ void __launch_bounds__(256) norm_sum_partials(const A *__restrict__ partial, int blocks, long long D,
+__global__ void __launch_bounds__(1024) norm_sum_partials(const A *__restrict__ partial, int blocks, long long D,
                                                          A *__restrict__ out_w, A *__restrict__ out_c, A *__restrict__ out_w2)
 {
-    __shared__ A shared[8][33];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ A shared[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const long long col = (long long)blockIdx.x * 32 + lane;
     A *out = blockIdx.y == 0 ? out_w : blockIdx.y == 1 ? out_c : out_w2;
     if (out == nullptr) return;
     A sum = A(0);
     if (col < D)
 #pragma unroll 4
-        for (int b = warp; b < blocks; b += 8) sum += partial[((long long)b * 3 + blockIdx.y) * D + col];
+        for (int b = warp; b < blocks; b += warps) sum += partial[((long long)b * 3 + blockIdx.y) * D + col];
     shared[warp][lane] = sum;
     __syncthreads();
-    if (warp == 0 && col < D) {
-        for (int i = 1; i < 8; ++i) sum += shared[i][lane];
-        out[col] = sum;
+    for (int c = warp; c < 32; c += warps) {
+        sum = lane < warps ? shared[lane][c] : A(0);
+        for (int i = 16; i >= 1; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+        const long long own = (long long)blockIdx.x * 32 + c;
+        if (lane == 0 && own < D) out[own] = sum;
     }
 }
 
@@ -1020,7 +1024,7 @@ extern "C" int psig_norm_backward(const PsigNormDesc *desc, const void *x, const
             });
         }
         if (status != PSIG_OK || (!grad_weight && !grad_residual_scale && !grad_next_weight)) return status;
-        norm_sum_partials<A><<<dim3((unsigned)((a.D + 31) / 32), 3), 256, 0, s>>>(
+        norm_sum_partials<A><<<dim3((unsigned)((a.D + 31) / 32), 3), a.D >= 32 * 128 ? 256 : 1024, 0, s>>>(
             static_cast<const A *>(workspace), blocks, a.D, static_cast<A *>(grad_weight),
             static_cast<A *>(grad_residual_scale), static_cast<A *>(grad_next_weight));
         return check_launch();
