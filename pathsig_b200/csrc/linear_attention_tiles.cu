@@ -8,11 +8,12 @@
 // All run as tcgen05.mma with M = 128 and fp32 accumulators in tensor memory; R, K, V come by TMA into 128-byte
 // swizzled tiles, in which K and V serve both as they are and transposed (the descriptor's major bit).
 //
-// Rounding.  The products take 16-bit operands, exact for R, K and V.  P, S and V' are computed in 32 bits.  P enters
-// rounded once: only the 16-bit output depends on it.  S and V' enter as a sum of NS and NV 16-bit terms (the value, what
-// its rounding left, what that left): three (24 bits) where a 32-bit result depends on them, the state itself or the decay
-// gradient.  The state lives in registers in 32 bits and is never rounded but for its copy as an operand.  Sums of
-// decays are in 64 bits, so that a weight exp(a_t - a_s) does not lose the difference of two long sums.
+// Rounding.  The products take 16-bit operands, exact for R, K and V.  P, S and V' are computed in 32 bits and enter as sums of
+// 16-bit terms (the value, what its rounding left, what that left): P as two, S as NS and V' as NV, two (16 bits) where only
+// a 16-bit output depends on them, so that its one rounding is all that counts (error of the outputs 1.66e-3 of their size;
+// with P and S as one term each 2.35e-3, in seven eighths of the time), three (24 bits) where a 32-bit result does, the
+// state itself or the decay gradient.  The state lives in registers in 32 bits and is never rounded but for its copy as an
+// operand.  Sums of decays are in 64 bits, so that a weight exp(a_t - a_s) does not lose the difference of two long sums.
 //
 // DOT: the sweep also gives x_t = out_t . y_t for the rows y of a third operand, to 32 bits (the decay gradient needs
 // q . grad_q and k . grad_k).  The part of the piece's own pairs is sum_s exp(a_t - a_s) (r_t . k_s) (y_t . v_s), the
@@ -65,7 +66,9 @@ struct TileLayout {
     static constexpr int c_o2 = DOT ? 256 : 128;
     static constexpr int c_i = c_o2 + 64;
     static constexpr int c_o1 = c_i + 64;
+    static constexpr int c_p = c_o1 + 64;   // what P's rounding to its first term left
     static constexpr int columns = 512;
+    static_assert(c_p + 64 <= columns, "tensor memory");
 };
 
 template <typename T, int KP, int NS, int NV, bool DOT, bool REV, bool STATE>
@@ -291,7 +294,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
 #pragma unroll 1
                 for (int q = 0; q < 4; ++q) {   // 16 columns each
                     const int block = half * 2 + q / 2, s0 = half * 64 + q * 16;
-                    uint32_t p[8];
+                    uint32_t p[8], left[8];   // P's two terms
                     if (REV ? block >= quarter : block <= quarter) {
                         float x[16], y[16];
                         tmem_load16(own + q * 16, x);
@@ -320,12 +323,16 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                             if (DOT) sum = fmaf(x[j], y[j], sum);
                         }
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) p[j] = pack(x[2 * j], x[2 * j + 1], T{});
+                        for (int j = 0; j < 8; ++j) {
+                            p[j] = next_term<T>(x[2 * j], x[2 * j + 1], false);
+                            left[j] = next_term<T>(x[2 * j], x[2 * j + 1], true);
+                        }
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) p[j] = 0;
+                        for (int j = 0; j < 8; ++j) p[j] = left[j] = 0;
                     }
                     tmem_store8(own + q * 8, p);
+                    tmem_store8(tmem + lanes + Lay::c_p + half * 32 + q * 8, left);
                 }
                 if (DOT) sums[((g & 1) * 2 + half) * kPiece + row] = sum;
                 tmem_stored();
@@ -510,8 +517,12 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                 fence_after();
 #pragma unroll
                 for (int j = 0; j < kPiece / 16; ++j)
-                    mma_ts(tmem + Lay::c_o1, tmem + (j / 4) * 64 + (j % 4) * 8, tile_desc(v16 + (j * 2048 >> 4), kTileBytes),
+                    mma_ts(tmem + Lay::c_o1, tmem + Lay::c_p + j * 8, tile_desc(v16 + (j * 2048 >> 4), kTileBytes),
                            instr_desc<T>(64, false, true), past || j > 0, lead);
+#pragma unroll
+                for (int j = 0; j < kPiece / 16; ++j)
+                    mma_ts(tmem + Lay::c_o1, tmem + (j / 4) * 64 + (j % 4) * 8, tile_desc(v16 + (j * 2048 >> 4), kTileBytes),
+                           instr_desc<T>(64, false, true), true, lead);
                 mma_commit(bar(kO1_0 + (g & 1)), lead);
             }
         }
@@ -612,8 +623,8 @@ int select_tiles(const Sweep &a, int dtype, cudaStream_t stream)
         return a.d1 <= 64 ? launch_tiles<T, 64, 3, 3, true, REV>(a, dtype, stream) : launch_tiles<T, 128, 3, 3, true, REV>(a, dtype, stream);
     // two terms of V' (16 bits) are plenty for a state that nobody sees but through a 16-bit output
     if (a.final == nullptr)
-        return a.d1 <= 64 ? launch_tiles<T, 64, 1, 2, false, REV>(a, dtype, stream) : launch_tiles<T, 128, 1, 2, false, REV>(a, dtype, stream);
-    return a.d1 <= 64 ? launch_tiles<T, 64, 1, 3, false, REV>(a, dtype, stream) : launch_tiles<T, 128, 1, 3, false, REV>(a, dtype, stream);
+        return a.d1 <= 64 ? launch_tiles<T, 64, 2, 2, false, REV>(a, dtype, stream) : launch_tiles<T, 128, 2, 2, false, REV>(a, dtype, stream);
+    return a.d1 <= 64 ? launch_tiles<T, 64, 2, 3, false, REV>(a, dtype, stream) : launch_tiles<T, 128, 2, 3, false, REV>(a, dtype, stream);
 }
 
 }  // namespace

@@ -97,7 +97,7 @@ def lost_below(dtype):
     return 2.0 ** -996 if dtype == torch.float64 else 2.0 ** -100
 
 
-def attention_bounds(c, dtype):
+def attention_bounds(c, dtype, terms=1):
     """How far each output may be from its exact value, element by element.
 
     Every output is a sum of products; with all terms replaced by their absolute values it is some T.  A chain of m
@@ -106,7 +106,11 @@ def attention_bounds(c, dtype):
     piece, plus the sums over a head, the exponentials (2 units each, the argument a sum over a piece) and a few
     products: m = 2 L + Dk + Dv + 64.  Operands of the matrix products in 16 bits are rounded at most twice on the
     way of a term (the state's part or the pair's weight, and the weighted row): 3 half steps of the storage type cover
-    both and their products; results in the storage type add a half step of themselves."""
+    both and their products; results in the storage type add a half step of themselves.
+
+    ``terms`` = 2: what enters the products is the value's rounding to bfloat16 and the rounding of what that left, so
+    off by a half step of bfloat16 squared (2^-16), three times at most as above: the result is rounded to its type
+    once, and nothing before it to so few bits."""
     T = attention(absolute(c), sign=1.0)
     B, L, H, Dk = c["q"].shape
     u = half_step(torch.float64 if dtype == torch.float64 else torch.float32)
@@ -131,6 +135,7 @@ def attention_bounds(c, dtype):
             bounds[name] = m * u * t + lost_below(dtype)
         else:
             inner = 3 * stored if dtype in (torch.bfloat16, torch.float16) else 0.0
+            inner = 3 * half_step(torch.bfloat16) ** 2 if inner and terms == 2 else inner
             bounds[name] = (m * u + inner) * t + stored * exact[name].abs() * 1.01 + lost_below(dtype)
             if dtype == torch.float16:
                 bounds[name] = bounds[name] + 2.0 ** -25 * (1 + t.amax())   # below the smallest normal number

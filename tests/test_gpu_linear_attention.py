@@ -487,3 +487,24 @@ def test_short_sequences_on_both_sides_of_the_kernels_limits(ps, steps, state, d
     _check(_run(ps, g), exact, bounds)
     out = ps.linear_attention(*(g[n] for n in NAMES[:4]), initial_state=g["initial_state"])   # no state asked for
     _check({"out": out}, exact, bounds)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("state", [False, True])
+@pytest.mark.parametrize("shape", [(2, 61, 8, 8, 64, 64), (2, 127, 2, 1, 48, 80), (1, 300, 2, 1, 128, 128), (1, 640, 1, 1, 128, 72),
+                                   (1, 1200, 2, 1, 64, 64)])
+def test_16_bit_results_are_rounded_once(ps, shape, state, dtype):
+    """Weights of pairs and states enter the products as two 16-bit terms: outputs and gradients are as near as 32-bit
+    arithmetic and one rounding bring them."""
+    c = so.make(sum(shape) + 1, *shape, dtype, state=state, rate=0.05)
+    g = _on_gpu(c, dtype)
+    exact, bounds = so.attention_bounds(c, dtype, terms=2)
+    _check(_run(ps, g), exact, bounds)
+    out = ps.linear_attention(*(g[n] for n in NAMES[:4]), initial_state=g["initial_state"])   # no state asked for
+    _check({"out": out}, exact, bounds)
+    leaves = [g[n].detach().requires_grad_(True) for n in NAMES[:3]]                          # no decay gradient
+    out, last = ps.linear_attention(*leaves, g["log_decay"], initial_state=g["initial_state"], return_state=True)
+    heads, grads = ([out, last], [g["grad_out"], g["grad_state"]]) if state else ([out], [g["grad_out"]])
+    got = torch.autograd.grad(heads, leaves, grads)
+    _check({"grad_" + n: t for n, t in zip(NAMES, got)}, exact, bounds)
+    _no_timeouts()
