@@ -23,7 +23,10 @@ bool prepare_kernel_once(const void *kernel, size_t dynamic_smem, bool prefer_sh
     std::lock_guard<std::mutex> lock(mutex);
     size_t &have = granted[std::make_pair(kernel, device)];
     if (have > dynamic_smem) return true;
-    if (dynamic_smem > 48 * 1024 &&
+    // the default limit of 48 KB holds for the kernel's static shared memory and the dynamic together
+    cudaFuncAttributes attributes;
+    if (dynamic_smem > 0 && cudaFuncGetAttributes(&attributes, kernel) != cudaSuccess) return false;
+    if (dynamic_smem > 0 && attributes.sharedSizeBytes + dynamic_smem > 48 * 1024 &&
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dynamic_smem) != cudaSuccess)
         return false;
     if (prefer_shared_carveout && have == 0)

@@ -92,7 +92,7 @@ long long closure_source(const PsigSigDesc &desc, const LevelTable &lt, int targ
 int closure_compile_only(const char *text, const char *arch, char *log, long long log_capacity);
 bool closure_compiler_available();
 
-// Launch attributes of a kernel (opt-in dynamic shared memory above 48 KB, preference for the largest
+// Launch attributes of a kernel (opt-in dynamic shared memory above 48 KB with the kernel's static, preference for the largest
 // shared-memory carveout) are properties of the function on a device: they are set the first time a
 // kernel is launched on a device, and again only when a launch needs more dynamic shared memory than
 // any launch before it -- not on every call.  Returns false when the runtime refuses.

@@ -1,11 +1,15 @@
 """The norm around a block (gate, residual, next norm) on the GPU against 64-bit formulas and their autograd gradients."""
 from __future__ import annotations
 
+import subprocess
+import sys
+
 import pytest
 import torch
 
 from . import sequence_oracle as so
 from . import util
+from .conftest import ROOT
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -266,3 +270,15 @@ def test_second_derivatives_are_refused(ps):
         assert torch.equal(a, b)
     with pytest.raises(RuntimeError, match="differentiable once"):
         graph[0].sum().backward()
+
+
+@pytest.mark.parametrize("rows,D,dtype,form", [
+    (2400, 612, "float32", 4), (2400, 764, "float32", 5), (2400, 1020, "float32", 2), (2400, 1528, "float32", 1),
+    (2400, 3056, "bfloat16", 1), (2400, 6104, "bfloat16", 0)])
+def test_rings_that_just_fit_the_default_shared_memory(rows, D, dtype, form):
+    """Rings of rows that, with the kernel's own 256 bytes, are just above the 48 KB that need no consent.  Each in a
+    process of its own, where no wider ring has been launched before."""
+    code = (f"import torch, pathsig_b200 as ps; from tests import test_gpu_residual_norm as t; "
+            f"t._check(ps, t._make(1, {rows}, {D}, torch.{dtype}, t.FORMS[{form}]), torch.{dtype})")
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
