@@ -506,7 +506,8 @@ __global__ void __launch_bounds__(kTeamMax) norm_backward_team(const NormArgs a,
                     const int i = v * E + e;
                     const A dn = d[e] * r2;
                     dh[i] += w2[e] * dn - h[i] * m2;
-                    qn[NEXT ? i : 0] += dn * h[i];
+                    // a team without a row holds zeros, whose root with eps = 0 is infinite
+                    if (live_row) qn[NEXT ? i : 0] += dn * h[i];
                     one[0] += dh[i] * f[i] * t[e];
                 }
             }

@@ -282,3 +282,12 @@ def test_rings_that_just_fit_the_default_shared_memory(rows, D, dtype, form):
             f"t._check(ps, t._make(1, {rows}, {D}, torch.{dtype}, t.FORMS[{form}]), torch.{dtype})")
     done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("form", FORMS[3:])
+@pytest.mark.parametrize("rows,D", [(1, 8), (1, 128), (17, 64), (33, 100), (3, 1001)])
+def test_no_eps(ps, rows, D, form, dtype):
+    """eps = 0, with row counts that leave some of a block's teams without a row (or none, where a block holds one)."""
+    c = _make(rows * D, rows, D, dtype, form, eps=0.0)
+    _check(ps, c, dtype)
