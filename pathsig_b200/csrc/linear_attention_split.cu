@@ -334,7 +334,7 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
             const int m = (int)(n - t0 < kPiece ? n - t0 : kPiece);
             const DecayTables &d = tables[i & 1];
             if (!warp_wait(bar(kDecFull0 + (i & 1)), (i >> 1) & 1, failed)) break;
-            const float la = d.la[row], head = d.head[row];
+            const float la = d.la[row], lb = d.lb[row], head = d.head[row];
             float f[2];
 #pragma unroll
             for (int q = 0; q < 2; ++q) f[q] = exp_two((float)(d.a[row] - d.a[(half * 2 + q) * 32 + (REV ? 0 : 31)]));
@@ -354,9 +354,16 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                         w[4 * j] = v.x, w[4 * j + 1] = v.y, w[4 * j + 2] = v.z, w[4 * j + 3] = v.w;
                     }
                     if (block == quarter) {
+                        const float4 *rest = reinterpret_cast<const float4 *>(d.lb + s0);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {   // a_t - a_s to 24 bits of its own size, not of the two's
+                            const float4 v = rest[j];
+                            w[4 * j] = (la - w[4 * j]) + (lb - v.x), w[4 * j + 1] = (la - w[4 * j + 1]) + (lb - v.y);
+                            w[4 * j + 2] = (la - w[4 * j + 2]) + (lb - v.z), w[4 * j + 3] = (la - w[4 * j + 3]) + (lb - v.w);
+                        }
                         const int j0 = row - s0;   // the step's own column
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) w[j] = (REV ? j >= j0 : j <= j0) ? exp_two(la - w[j]) : 0.f;
+                        for (int j = 0; j < 16; ++j) w[j] = (REV ? j >= j0 : j <= j0) ? exp_two(w[j]) : 0.f;
                     } else {
                         const float fq = q < 2 ? f[0] : f[1];
 #pragma unroll

@@ -284,7 +284,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
             for (int i = 0; i < it.pieces; ++i, ++g) {
                 const DecayTables &d = tables[g & 1];
                 if (!(ok = warp_wait(bar(kDecFull0 + (g & 1)), (g >> 1) & 1, failed))) break;
-                const float la = d.la[row];
+                const float la = d.la[row], lb = d.lb[row];
                 float f[2];   // 2^(a_t - (a at the low end of the block)) for the two blocks of 32 columns
 #pragma unroll
                 for (int q = 0; q < 2; ++q) f[q] = kv_scale * exp_two((float)(d.a[row] - d.a[(half * 2 + q) * 32 + (REV ? 0 : 31)]));
@@ -307,9 +307,16 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                             t[4 * j] = v.x, t[4 * j + 1] = v.y, t[4 * j + 2] = v.z, t[4 * j + 3] = v.w;
                         }
                         if (block == quarter) {
+                            const float4 *rest = reinterpret_cast<const float4 *>(d.lb + s0);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {   // a_t - a_s to 24 bits of its own size, not of the two's
+                                const float4 v = rest[j];
+                                t[4 * j] = (la - t[4 * j]) + (lb - v.x), t[4 * j + 1] = (la - t[4 * j + 1]) + (lb - v.y);
+                                t[4 * j + 2] = (la - t[4 * j + 2]) + (lb - v.z), t[4 * j + 3] = (la - t[4 * j + 3]) + (lb - v.w);
+                            }
                             const int j0 = row - s0;   // the step's own column
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) t[j] = (REV ? j >= j0 : j <= j0) ? kv_scale * exp_two(la - t[j]) : 0.f;
+                            for (int j = 0; j < 16; ++j) t[j] = (REV ? j >= j0 : j <= j0) ? kv_scale * exp_two(t[j]) : 0.f;
                         } else {
                             const float fq = q < 2 ? f[0] : f[1];
 #pragma unroll

@@ -31,6 +31,7 @@ constexpr unsigned kPollTime = 10000;         // ns a poll may sleep; warps that
 struct DecayTables {       // of one piece; all exponents are of 2
     double a[kPiece];      // a_t
     float la[kPiece];      // a_s - (a at the low end of s's block of 32)
+    float lb[kPiece];      // what rounding that to la left
     float cf[kPiece];      // 2^-la
     float tail[kPiece];    // 2^(a_end - a_s)
     float head[kPiece];    // 2^a_t
@@ -269,12 +270,13 @@ __device__ __forceinline__ double sum_decays(const float *g, long long stride, l
             const float la = (float)(c[j] - low);
             d.a[t] = c[j];
             d.la[t] = la;
+            d.lb[t] = (float)((c[j] - low) - (double)la);
             d.cf[t] = exp_two(-la);
             d.tail[t] = exp_two((float)(end - c[j]));
             d.head[t] = exp_two((float)c[j]);
         }
         if (lane == 0) d.keep = exp_two((float)end);
-            warp_arrive(full0 + 8 * (count & 1));
+        warp_arrive(full0 + 8 * (count & 1));
     }
     return whole;
 }

@@ -97,7 +97,7 @@ def lost_below(dtype):
     return 2.0 ** -996 if dtype == torch.float64 else 2.0 ** -100
 
 
-def attention_bounds(c, dtype, terms=1):
+def attention_bounds(c, dtype, terms=1, chain=None):
     """How far each output may be from its exact value, element by element.
 
     Every output is a sum of products; with all terms replaced by their absolute values it is some T.  A chain of m
@@ -110,11 +110,11 @@ def attention_bounds(c, dtype, terms=1):
 
     ``terms`` = 2: what enters the products is the value's rounding to bfloat16 and the rounding of what that left, so
     off by a half step of bfloat16 squared (2^-16), three times at most as above: the result is rounded to its type
-    once, and nothing before it to so few bits."""
+    once, and nothing before it to so few bits.  ``chain``: m, for operands that are nearly all zero."""
     T = attention(absolute(c), sign=1.0)
     B, L, H, Dk = c["q"].shape
     u = half_step(torch.float64 if dtype == torch.float64 else torch.float32)
-    m = 2 * L + Dk + c["v"].shape[-1] + 64
+    m = chain or 2 * L + Dk + c["v"].shape[-1] + 64
     exact = attention(c)
     bounds = {}
     stored = half_step(dtype)

@@ -508,3 +508,28 @@ def test_16_bit_results_are_rounded_once(ps, shape, state, dtype):
     got = torch.autograd.grad(heads, leaves, grads)
     _check({"grad_" + n: t for n, t in zip(NAMES, got)}, exact, bounds)
     _no_timeouts()
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("Dk,Dv", [(64, 64), (128, 72)])
+def test_weights_next_to_steps_that_forget(ps, Dk, Dv, dtype):
+    """Pairs of steps on one side of steps that forget everything (or nearly: exp(-60)), with small decays between the two.
+    One entry of one row in 32 is not zero, so a sum has at most ten terms here and its error is that of their weights: four
+    exponentials on the way of a term (4 units each: 2^-22), their arguments (below 4, or the weight does not count), the sum
+    of ten and two dozen products and splits: 64 units of 2^-24 cover them."""
+    B, L, H = 2, 300, 4
+    c = so.make(41, B, L, H, H, Dk, Dv, dtype, state=True, rate=0.01)
+    gen = torch.Generator().manual_seed(9)
+    for h, resets in enumerate((0, 1, 5, 15)):
+        for b in range(B):
+            for t0 in range(0, L, 32):
+                at = t0 + torch.randperm(32, generator=gen)[:resets]
+                c["log_decay"][b, at[at < L], h] = -float("inf") if b == 0 else -60.0
+    for name, at in (("q", 23), ("k", 3), ("v", 3), ("grad_out", 23)):
+        few = torch.zeros_like(c[name])
+        for t in range(L):
+            if t % 32 == at or name in ("q", "k") and t % 32 in (3, 4, 23, 24):
+                few[:, t, :, 5] = c[name][:, t, :, 5]
+        c[name] = few
+    _check(_run(ps, _on_gpu(c, dtype)), *so.attention_bounds(c, dtype, terms=2, chain=64))
+    _no_timeouts()
