@@ -296,8 +296,11 @@ int psig_attn_step(const PsigAttnDesc *desc, const void *q, const void *k, const
 
 /* Diagnostic: waits inside the kernels of psig_attn_* and psig_norm_* that ran out on the current device since the last call
  * (read and cleared; synchronises).  Every wait for a copy, a matrix product or another warp is bounded; one that runs
- * out ends its block early, and the call's results are then not valid.  0 in normal operation. */
+ * out ends its block early, and the call's results are then not valid.  0 in normal operation.
+ * psig_set_norm_wait_polls sets how often the norms' kernels of later calls look for a row that they stream through shared
+ * memory (negative: the default, 2^22; 0: never, so that every such wait runs out), for tests. */
 int64_t psig_sequence_wait_timeouts(void);
+int psig_set_norm_wait_polls(int polls);
 
 /* Norm around a block, fused with the block's gate, the residual sum and the norm before the next block; no
  * counterpart in the reference.  Per row of D features, rms(x) = x / sqrt(mean(x^2) + eps):

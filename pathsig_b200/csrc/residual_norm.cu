@@ -14,6 +14,8 @@
 // pieces and read again, mostly from L2.
 #include "sequence.cuh"
 
+#include <atomic>
+
 namespace psig {
 namespace {
 
@@ -150,7 +152,11 @@ __device__ __forceinline__ void team_sum(A (&v)[N], int team_log2, A *shared, in
     for (int s = 0; s < team_log2; ++s)
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 1 << s);
-    if (team_log2 < 5 || blockDim.x == 32) return;
+    if (team_log2 < 5) return;
+    if (blockDim.x == 32) {
+        __syncwarp();
+        return;
+    }
     A *mine = shared + (round & 1) * 2 * (kTeamMax / 32);
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
@@ -168,15 +174,21 @@ __device__ __forceinline__ void team_sum(A (&v)[N], int team_log2, A *shared, in
 // RING: the rows of one block are streamed into shared memory ahead of their use (one thread, cp.async.bulk, an mbarrier
 // for each of the stages), so that the memory system is busy while a row waits at its barriers; every pass
 // reads its operands from there.  Needs rows that are whole 16-byte pieces.  Otherwise a thread loads its part of a row itself.
+// Waits for a row are bounded.  When one runs out the block leaves its loop -- all threads at once: the flag is set before
+// the row's first barrier, read behind it, and not set for the next row before another barrier -- writes nothing from that row
+// on, and waits (bounded again) for the copies in flight before it gives its shared memory back.
 
 __device__ __forceinline__ uint32_t norm_shared(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 constexpr int kNormOperands = 5;
 constexpr unsigned kNormPolls = 1u << 22;
+// Polls of a row's wait; a test lowers it to make the wait run out.  The wait for the copies in flight keeps its own limit.
+std::atomic<unsigned> g_row_polls{kNormPolls};
 __device__ unsigned long long g_norm_timeouts;
 
 struct Ring {
     int stages;
+    unsigned polls;                      // of the wait for a row
     int row_bytes;                       // of one operand
     int count;                           // operands per stage
     const void *data[kNormOperands];     // in the order of their slots
@@ -186,9 +198,11 @@ struct RingState {
     unsigned char *buffer;
     uint32_t bars;
     const Ring &ring;
+    volatile int *failed;   // of the block
     __device__ __forceinline__ uint32_t bar(int stage) const { return bars + 8 * stage; }
     __device__ __forceinline__ void init() const
     {
+        *failed = 0;
         for (int i = 0; i < ring.stages; ++i)
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar(i)) : "memory");
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -203,16 +217,29 @@ struct RingState {
                            "l"(static_cast<const unsigned char *>(ring.data[i]) + row * ring.row_bytes), "r"(ring.row_bytes), "r"(bar(stage))
                          : "memory");
     }
-    __device__ __forceinline__ bool wait(int stage, uint32_t parity) const
+    __device__ __forceinline__ bool arrived(int stage, uint32_t parity, unsigned polls) const
     {
-        for (unsigned i = 0; i < kNormPolls; ++i) {
+        for (unsigned i = 0; i < polls; ++i) {
             uint32_t ok;
             asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
                          : "=r"(ok) : "r"(bar(stage)), "r"(parity) : "memory");
             if (ok) return true;
         }
-        atomicAdd(&g_norm_timeouts, 1ull);
         return false;
+    }
+    __device__ __forceinline__ void wait(int stage, uint32_t parity) const
+    {
+        if (!arrived(stage, parity, ring.polls)) *failed = 1;
+    }
+    // one thread, behind a wait that ran out for row `row` in `stage`: the copies of that row and of the rows behind it, as many
+    // as there are stages, have been started
+    __device__ __forceinline__ void drain(int stage, uint32_t parity, long long row, long long step, long long rows) const
+    {
+        atomicAdd(&g_norm_timeouts, 1ull);
+        for (int i = 0; i < ring.stages && row + i * step < rows; ++i) {
+            const int s = stage + i;
+            arrived(s < ring.stages ? s : s - ring.stages, s < ring.stages ? parity : parity ^ 1, kNormPolls);
+        }
     }
 };
 
@@ -226,7 +253,7 @@ __global__ void __launch_bounds__(kTeamMax) norm_forward_team(const NormArgs a, 
     const int team = team_log2 < 5 ? threadIdx.x >> team_log2 : 0, j = team_log2 < 5 ? threadIdx.x & (threads - 1) : threadIdx.x;
     const A mean = scalar<A>(a.mean, a.mean_f), eps = scalar<A>(a.eps, a.eps_f);
     const long long step = (long long)gridDim.x * teams;
-    const RingState rs{dynamic + 128, norm_shared(dynamic), ring};
+    const RingState rs{dynamic + 128, norm_shared(dynamic), ring, reinterpret_cast<int *>(dynamic + 64)};
     if (RING) {
         if (threadIdx.x == 0) {
             rs.init();
@@ -264,6 +291,10 @@ __global__ void __launch_bounds__(kTeamMax) norm_forward_team(const NormArgs a, 
             for (int e = 0; e < E; ++e) sum[0] += t[e] * t[e];
         }
         team_sum(sum, team_log2, shared, round++);
+        if (RING && *rs.failed) {
+            if (threadIdx.x == 0) rs.drain(stage, phase, first, step, a.rows);
+            break;
+        }
         const A r = inverse_root(sum[0] * mean + eps);
         A h[NEXT ? NV * E : 1];
         sum[0] = A(0);
@@ -392,7 +423,7 @@ __global__ void __launch_bounds__(kTeamMax) norm_backward_team(const NormArgs a,
             }
         }
     };
-    const RingState rs{dynamic + 128, norm_shared(dynamic), ring};
+    const RingState rs{dynamic + 128, norm_shared(dynamic), ring, reinterpret_cast<int *>(dynamic + 64)};
     if (RING) {
         if (threadIdx.x == 0) {
             rs.init();
@@ -457,11 +488,18 @@ __global__ void __launch_bounds__(kTeamMax) norm_backward_team(const NormArgs a,
         }
         if (!NEXT) {   // the gradient of h is there: both sums in one exchange
             team_sum(two, team_log2, shared, round++);
-            r = inverse_root(two[0] * mean + eps);
-            m = two[1] * mean * r * r * r;
         } else {
             one[0] = two[0];
             team_sum(one, team_log2, shared, round++);
+        }
+        if (RING && *rs.failed) {
+            if (threadIdx.x == 0) rs.drain(stage, phase, first, step, a.rows);
+            break;
+        }
+        if (!NEXT) {
+            r = inverse_root(two[0] * mean + eps);
+            m = two[1] * mean * r * r * r;
+        } else {
             r = inverse_root(one[0] * mean + eps);
             two[0] = two[1] = A(0);
             A h[NV * E];
@@ -866,6 +904,7 @@ int plan_ring(const NormArgs &a, const TeamPlan &p, bool backward, bool next, in
     const long long bytes = a.D * (long long)sizeof(T);
     if (p.team_log2 < 5 || bytes % 16 != 0 || sizeof(T) == 8) return 0;
     ring->row_bytes = (int)bytes;
+    ring->polls = g_row_polls.load(std::memory_order_relaxed);
     const long long room = 220 * 1024 / per_sm - 1024 - 128, stage = bytes * ring->count;
     ring->stages = (int)(room / stage < 4 ? room / stage : 4);
     return ring->stages < 2 ? 0 : 128 + (int)(stage * ring->stages);
@@ -920,6 +959,12 @@ long long norm_timeouts()
 }  // namespace psig
 
 using namespace psig;
+
+extern "C" int psig_set_norm_wait_polls(int polls)
+{
+    g_row_polls.store(polls < 0 ? kNormPolls : (unsigned)polls, std::memory_order_relaxed);
+    return PSIG_OK;
+}
 
 extern "C" int psig_norm_forward(const PsigNormDesc *desc, const void *x, const void *weight, const void *gate,
                                  const void *residual, const void *residual_scale, const void *next_weight, void *h,

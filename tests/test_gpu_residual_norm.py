@@ -291,3 +291,32 @@ def test_no_eps(ps, rows, D, form, dtype):
     """eps = 0, with row counts that leave some of a block's teams without a row (or none, where a block holds one)."""
     c = _make(rows * D, rows, D, dtype, form, eps=0.0)
     _check(ps, c, dtype)
+
+
+@pytest.mark.parametrize("rows,D,dtype,form", [(2400, 1528, "float32", 1), (2400, 1024, "bfloat16", 4), (3000, 200, "bfloat16", 6)])
+def test_a_wait_for_a_row_that_runs_out_ends_its_block(ps, rows, D, dtype, form):
+    """With no poll allowed the blocks that stream rows leave at the first, count that, and wait for the copies in flight;
+    later calls are as ever."""
+    from pathsig_b200 import _load
+    lib = _load.ensure_loaded()
+    dtype = getattr(torch, dtype)
+    c = _gpu(_make(2, rows, D, dtype, FORMS[form]), dtype)
+    args = [c[n] for n in NAMES]
+
+    def backward():
+        got = torch.ops.pathsig_b200.gated_residual_norm_backward(*args, c["grad_h"], c["grad_n"], 0, 1e-6)
+        torch.cuda.synchronize()
+        return got
+
+    want = backward()
+    assert lib.psig_sequence_wait_timeouts() == 0
+    try:
+        assert lib.psig_set_norm_wait_polls(0) == 0
+        backward()
+        assert lib.psig_sequence_wait_timeouts() > 0
+        assert lib.psig_sequence_wait_timeouts() == 0      # read and cleared
+    finally:
+        assert lib.psig_set_norm_wait_polls(-1) == 0
+    for a, b in zip(backward(), want):
+        assert torch.equal(a, b)
+    assert lib.psig_sequence_wait_timeouts() == 0
