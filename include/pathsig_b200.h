@@ -295,8 +295,8 @@ int psig_attn_step(const PsigAttnDesc *desc, const void *q, const void *k, const
                    void *state, void *out, void *stream);
 
 /* Diagnostic: waits inside the kernels of psig_attn_* and psig_norm_* that ran out on the current device since the last call
- * (read and cleared; synchronises).  Every wait for a copy, a matrix product or another warp is bounded; one that runs
- * out ends its block early, and the call's results are then not valid.  0 in normal operation.
+ * (read and cleared; synchronises).  Every wait for a copy, a matrix product or another warp is bounded (2^22 polls, and two
+ * seconds); one that runs out ends its block early, and the call's results are then not valid.  0 in normal operation.
  * psig_set_norm_wait_polls sets how often the norms' kernels of later calls look for a row that they stream through shared
  * memory (negative: the default, 2^22; 0: never, so that every such wait runs out), for tests. */
 int64_t psig_sequence_wait_timeouts(void);

@@ -181,9 +181,8 @@ __device__ __forceinline__ void team_sum(A (&v)[N], int team_log2, A *shared, in
 __device__ __forceinline__ uint32_t norm_shared(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 constexpr int kNormOperands = 5;
-constexpr unsigned kNormPolls = 1u << 22;
 // Polls of a row's wait; a test lowers it to make the wait run out.  The wait for the copies in flight keeps its own limit.
-std::atomic<unsigned> g_row_polls{kNormPolls};
+std::atomic<unsigned> g_row_polls{kWaitPolls};
 __device__ unsigned long long g_norm_timeouts;
 
 struct Ring {
@@ -219,11 +218,13 @@ struct RingState {
     }
     __device__ __forceinline__ bool arrived(int stage, uint32_t parity, unsigned polls) const
     {
+        unsigned long long start = 0;
         for (unsigned i = 0; i < polls; ++i) {
             uint32_t ok;
             asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
                          : "=r"(ok) : "r"(bar(stage)), "r"(parity) : "memory");
             if (ok) return true;
+            if (wait_expired(i, start)) break;
         }
         return false;
     }
@@ -238,7 +239,7 @@ struct RingState {
         atomicAdd(&g_norm_timeouts, 1ull);
         for (int i = 0; i < ring.stages && row + i * step < rows; ++i) {
             const int s = stage + i;
-            arrived(s < ring.stages ? s : s - ring.stages, s < ring.stages ? parity : parity ^ 1, kNormPolls);
+            arrived(s < ring.stages ? s : s - ring.stages, s < ring.stages ? parity : parity ^ 1, kWaitPolls);
         }
     }
 };
@@ -962,7 +963,7 @@ using namespace psig;
 
 extern "C" int psig_set_norm_wait_polls(int polls)
 {
-    g_row_polls.store(polls < 0 ? kNormPolls : (unsigned)polls, std::memory_order_relaxed);
+    g_row_polls.store(polls < 0 ? kWaitPolls : (unsigned)polls, std::memory_order_relaxed);
     return PSIG_OK;
 }
 

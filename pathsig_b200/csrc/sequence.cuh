@@ -26,6 +26,19 @@ template <> __device__ __forceinline__ __half from_acc<__half>(float v) { return
 __device__ __forceinline__ float exp_acc(float v) { return expf(v); }
 __device__ __forceinline__ double exp_acc(double v) { return exp(v); }
 
+// Limits of a wait for an mbarrier: this many polls (each of which may sleep for a time that the hardware sets), and about this
+// many nanoseconds, looked at every 64 polls.
+constexpr unsigned kWaitPolls = 1u << 22;
+constexpr unsigned long long kWaitTime = 2000000000ull;
+__device__ __forceinline__ bool wait_expired(unsigned poll, unsigned long long &start)
+{
+    if ((poll & 63) != 63) return false;
+    unsigned long long now;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+    if (start == 0) start = now;
+    return now - start > kWaitTime;
+}
+
 // Calls fn.template operator()<T>() with the storage type of a PsigDtype.
 template <typename Fn>
 int with_dtype(int dtype, Fn fn)

@@ -25,8 +25,6 @@ __device__ unsigned long long g_tile_timeouts;   // of the translation unit
 
 constexpr int kPiece = 128;
 constexpr int kTileBytes = kPiece * 128;      // 128 rows of 64 16-bit values
-constexpr unsigned kWaitPolls = 1u << 22;     // of at most kPollTime each: two to three seconds
-constexpr unsigned kPollTime = 10000;         // ns a poll may sleep; warps that spin take issue slots and instruction cache from others
 
 struct DecayTables {       // of one piece; all exponents are of 2
     double a[kPiece];      // a_t
@@ -62,11 +60,13 @@ __device__ __forceinline__ bool bar_passed(uint32_t bar, uint32_t parity)
 // Out of line: the code of all roles has to fit the instruction cache.
 __device__ __noinline__ bool bar_wait_on(uint32_t bar, uint32_t parity, volatile int *failed)
 {
+    unsigned long long start = 0;
 #pragma unroll 1
     for (unsigned i = 0; i < kWaitPolls; ++i) {
         if (bar_passed(bar, parity)) return true;
-        if (*failed) return false;
+        if (*failed || wait_expired(i, start)) break;
     }
+    if (*failed) return false;
     if (atomicExch(const_cast<int *>(failed), 1) == 0) atomicAdd(&g_tile_timeouts, 1ull);
     return false;
 }
