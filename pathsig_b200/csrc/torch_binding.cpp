@@ -16,6 +16,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 #include <nvtx3/nvToolsExt.h>
@@ -824,6 +825,21 @@ std::tuple<at::Tensor, at::Tensor> linear_attention_autograd(const at::Tensor &q
     return std::make_tuple(got[0], got[1]);
 }
 
+// The step changes its state in place: the state's version says so to graphs that have saved it, which then refuse to run
+// (the schema alone does not).  Tensors made in inference mode have no version.
+at::Tensor linear_attention_step_in_place(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &decay,
+                                          at::Tensor &state, double scale)
+{
+    at::Tensor out;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        static const auto op = handle<decltype(linear_attention_step)>("pathsig_b200::linear_attention_step");
+        out = op.call(q, k, v, decay, state, scale);
+    }
+    if (!state.is_inference()) torch::autograd::increment_version(state);
+    return out;
+}
+
 std::tuple<at::Tensor, at::Tensor> norm_below(const at::Tensor &x, const OptionalTensor &weight, const OptionalTensor &gate,
                                               const OptionalTensor &residual, const OptionalTensor &residual_scale,
                                               const OptionalTensor &next_weight, int64_t activation, double eps)
@@ -966,6 +982,11 @@ TORCH_LIBRARY_IMPL(pathsig_b200, CUDA, m)
     m.impl("linear_attention_step", &linear_attention_step);
     m.impl("gated_residual_norm", &gated_residual_norm);
     m.impl("gated_residual_norm_backward", &gated_residual_norm_backward);
+}
+
+TORCH_LIBRARY_IMPL(pathsig_b200, ADInplaceOrView, m)
+{
+    m.impl("linear_attention_step", &linear_attention_step_in_place);
 }
 
 TORCH_LIBRARY_IMPL(pathsig_b200, Autograd, m)

@@ -59,7 +59,8 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
     """One time step of :func:`linear_attention` for every sequence, on a kept state.
 
     ``q`` (B, H, Dk), ``k`` (B, Hkv, Dk), ``v`` (B, Hkv, Dv), ``log_decay`` (H) or (B, H); ``state`` (B, H, Dk, Dv),
-    contiguous, in the type of ``log_decay``, is updated in place.  Returns the output (B, H, Dv).  For serving: not
+    contiguous, in the type of ``log_decay``, is updated in place (a graph that has saved it then refuses its backward
+    pass).  Returns the output (B, H, Dv).  For serving: not
     differentiable.
     """
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):

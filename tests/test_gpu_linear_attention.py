@@ -533,3 +533,73 @@ def test_weights_next_to_steps_that_forget(ps, Dk, Dv, dtype):
         c[name] = few
     _check(_run(ps, _on_gpu(c, dtype)), *so.attention_bounds(c, dtype, terms=2, chain=64))
     _no_timeouts()
+
+
+def test_a_state_stepped_while_a_graph_holds_it(ps):
+    c = so.make(47, 2, 6, 4, 2, 16, 24, torch.float32, state=True)
+    g = _on_gpu(c, torch.float32)
+    args = [g[n][:, 0] for n in NAMES[:4]]
+    q = g["q"].clone().requires_grad_(True)
+    out = ps.linear_attention(q, *(g[n] for n in NAMES[1:4]), initial_state=g["initial_state"])
+    with torch.no_grad():
+        ps.linear_attention_step(*args, g["initial_state"])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    out = ps.linear_attention(q, *(g[n] for n in NAMES[1:4]), initial_state=g["initial_state"].clone())
+    with torch.no_grad():
+        ps.linear_attention_step(*args, g["initial_state"])
+    out.sum().backward()
+    assert torch.isfinite(q.grad).all()
+    with torch.inference_mode():                # a state without a version
+        state = c["initial_state"].to(torch.float32).to(DEV)
+        out = ps.linear_attention_step(*args, state)
+    other = c["initial_state"].to(torch.float32).to(DEV)
+    assert torch.equal(out, ps.linear_attention_step(*args, other)) and torch.equal(state, other)
+
+
+def test_operators_by_torchs_own_checks(ps):
+    """Schemas (what is written in place, what aliases what), fake implementations, registration of the formulas."""
+    ops = torch.ops.pathsig_b200
+    c = so.make(53, 2, 20, 4, 2, 16, 24, torch.float32, state=True)
+    g = _on_gpu(c, torch.float32)
+    leaves = [g[n].clone().requires_grad_(True) for n in NAMES]
+    lengths = torch.tensor([20, 7], device=DEV)
+    tests = ("test_schema", "test_faketensor", "test_autograd_registration")
+    torch.library.opcheck(ops.linear_attention.default, (*leaves, lengths, 0.25, True), test_utils=tests)
+    torch.library.opcheck(ops.linear_attention_backward.default, (*(g[n] for n in NAMES), lengths, g["grad_out"], g["grad_state"], 0.25, True),
+                          test_utils=tests[:2])
+    torch.library.opcheck(ops.linear_attention_step.default, (*(g[n][:, 0] for n in NAMES[:4]), g["initial_state"], 0.25), test_utils=tests[:2])
+    x = torch.randn(6, 40, device=DEV)
+    w = [torch.randn(40, device=DEV) for _ in range(3)]
+    leaves = [t.clone().requires_grad_(True) for t in (x, w[0], x, x, w[1], w[2])]
+    torch.library.opcheck(ops.gated_residual_norm.default, (*leaves, 0, 1e-6), test_utils=tests)
+    torch.library.opcheck(ops.gated_residual_norm_backward.default, (x, w[0], x, x, w[1], w[2], x, x, 0, 1e-6), test_utils=tests[:2])
+
+
+def test_step_and_norm_traced_by_torch_compile(ps):
+    c = so.make(59, 2, 3, 2, 2, 16, 16, torch.float32, state=True)
+    g = _on_gpu(c, torch.float32)
+    w = torch.rand(16, device=DEV)
+
+    def f(q, k, v, d, state, w):
+        out = ps.linear_attention_step(q, k, v, d, state)
+        h, n = ps.gated_residual_norm(out, w, gate=q, residual=v, next_weight=w)
+        return h.square().sum() + n.sum() + state.sum()
+
+    step = [g[n][:, 0] for n in NAMES[:4]]
+    one, two = g["initial_state"].clone(), g["initial_state"].clone()
+    with torch.no_grad():
+        want = f(*step, one, w)
+        got = torch.compile(f, backend="aot_eager", fullgraph=True)(*step, two, w)
+    assert torch.equal(got, want) and torch.equal(one, two)
+
+    def norm(x, w, r):
+        h, n = ps.gated_residual_norm(x, w, gate=x, residual=r, residual_scale=w, next_weight=w)
+        return h.square().sum() + n.square().sum()
+
+    leaves = [torch.randn(5, 40, device=DEV), torch.randn(40, device=DEV), torch.randn(5, 40, device=DEV)]
+    a, b = ([t.clone().requires_grad_(True) for t in leaves] for _ in range(2))
+    norm(*a).backward()
+    torch.compile(norm, backend="aot_eager", fullgraph=True)(*b).backward()
+    for x, y in zip(a, b):
+        assert torch.equal(x.grad, y.grad)

@@ -128,3 +128,21 @@ def test_oracle_gradients_against_automatic_differentiation(decay):
     plain = so.attention(c)
     for n, w in zip(names, want):
         assert torch.allclose(plain["grad_" + n], w, rtol=1e-11, atol=1e-12), n
+
+
+def test_the_step_raises_the_version_of_its_state():
+    """By which a graph that has saved the state refuses its backward pass, as with torch's own operators in place."""
+    with FakeTensorMode():
+        q, k, v = (torch.empty(2, 4, 8, device="cuda") for _ in range(3))
+        decay, state = torch.empty(4, device="cuda"), torch.empty(2, 4, 8, 8, device="cuda")
+        view = state[0]
+        for n in range(1, 4):
+            ps.linear_attention_step(q, k, v, decay, state)
+            assert state._version == n and view._version == n
+        assert q._version == k._version == v._version == decay._version == 0
+        with torch.no_grad():
+            ps.linear_attention_step(q, k, v, decay, state)
+        assert state._version == 4
+        with torch.inference_mode():
+            ps.linear_attention_step(q, k, v, decay, state)
+            ps.linear_attention_step(q, k, v, decay, torch.empty(2, 4, 8, 8, device="cuda"))   # has no version
