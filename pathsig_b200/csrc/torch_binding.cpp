@@ -27,6 +27,7 @@
 #include <mutex>
 #include <optional>
 #include <tuple>
+#include <type_traits>
 #include <vector>
 
 #include "../../include/pathsig_b200.h"
@@ -731,6 +732,18 @@ OptionalTensor given(const Variable &t) { return t.defined() ? OptionalTensor(t)
 Variable plain(const OptionalTensor &t) { return t.has_value() ? *t : Variable(); }
 bool tracked(const OptionalTensor &t) { return t.has_value() && t->defined() && t->requires_grad(); }
 
+// Forward-mode tangents are refused: an operand that has one may not require a gradient, and would pass by the functions below.
+template <typename... Operands>
+void refuse_tangents(const char *name, const Operands &...operands)
+{
+    auto has = [](const at::Tensor &t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); };
+    auto any = [&](const auto &t) {
+        if constexpr (std::is_same_v<std::decay_t<decltype(t)>, OptionalTensor>) return t.has_value() && has(*t);
+        else return has(t);
+    };
+    TORCH_CHECK(!(any(operands) || ...), name, " has no forward-mode derivative: an operand has a tangent");
+}
+
 template <typename Fn>
 c10::TypedOperatorHandle<Fn> handle(const char *name)
 {
@@ -777,6 +790,7 @@ AttentionGrads linear_attention_backward_autograd(const at::Tensor &q, const at:
                                                   const OptionalTensor &lengths, const OptionalTensor &go,
                                                   const OptionalTensor &gs, double scale, bool decay_grad)
 {
+    refuse_tangents("linear_attention_backward", q, k, v, decay, init, go, gs);
     if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad() || decay.requires_grad() ||
                                          tracked(init) || tracked(go) || tracked(gs)))
         return attention_backward_below(q, k, v, decay, init, lengths, go, gs, scale, decay_grad);
@@ -818,6 +832,7 @@ std::tuple<at::Tensor, at::Tensor> linear_attention_autograd(const at::Tensor &q
                                                              const at::Tensor &decay, const OptionalTensor &init,
                                                              const OptionalTensor &lengths, double scale, bool return_state)
 {
+    refuse_tangents("linear_attention", q, k, v, decay, init);
     if (!at::GradMode::is_enabled() ||
         !(q.requires_grad() || k.requires_grad() || v.requires_grad() || decay.requires_grad() || tracked(init)))
         return attention_below(q, k, v, decay, init, lengths, scale, return_state);
@@ -830,6 +845,7 @@ std::tuple<at::Tensor, at::Tensor> linear_attention_autograd(const at::Tensor &q
 at::Tensor linear_attention_step_in_place(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &decay,
                                           at::Tensor &state, double scale)
 {
+    refuse_tangents("linear_attention_step", q, k, v, decay, state);
     at::Tensor out;
     {
         at::AutoDispatchBelowADInplaceOrView below;
@@ -882,6 +898,7 @@ NormGrads gated_residual_norm_backward_autograd(const at::Tensor &x, const Optio
                                                 const OptionalTensor &next_weight, const OptionalTensor &grad_h,
                                                 const OptionalTensor &grad_n, int64_t activation, double eps)
 {
+    refuse_tangents("gated_residual_norm_backward", x, weight, gate, residual, residual_scale, next_weight, grad_h, grad_n);
     if (!at::GradMode::is_enabled() || !(x.requires_grad() || tracked(weight) || tracked(gate) || tracked(residual) ||
                                          tracked(residual_scale) || tracked(next_weight) || tracked(grad_h) || tracked(grad_n)))
         return norm_backward_below(x, weight, gate, residual, residual_scale, next_weight, grad_h, grad_n, activation, eps);
@@ -924,6 +941,7 @@ std::tuple<at::Tensor, at::Tensor> gated_residual_norm_autograd(const at::Tensor
                                                                 const OptionalTensor &residual_scale, const OptionalTensor &next_weight,
                                                                 int64_t activation, double eps)
 {
+    refuse_tangents("gated_residual_norm", x, weight, gate, residual, residual_scale, next_weight);
     if (!at::GradMode::is_enabled() || !(x.requires_grad() || tracked(weight) || tracked(gate) || tracked(residual) ||
                                          tracked(residual_scale) || tracked(next_weight)))
         return norm_below(x, weight, gate, residual, residual_scale, next_weight, activation, eps);

@@ -322,6 +322,8 @@ _FAKES = {
     "gated_residual_norm": _fake_gated_residual_norm,
     "gated_residual_norm_backward": _fake_gated_residual_norm_backward,
 }
+_SEQUENCE_OPERATORS = ("linear_attention", "linear_attention_backward", "linear_attention_step", "gated_residual_norm",
+                       "gated_residual_norm_backward")
 _libraries = {}  # namespace -> torch.library.Library or True (kept alive for the life of the process)
 
 
@@ -351,6 +353,9 @@ def register_namespace(ns: str) -> None:
         lib = torch.library.Library(ns, "FRAGMENT")
         for name, schema in _SCHEMAS.items():
             lib.define(name + schema, tags=(torch.Tag.pt2_compliant_tag,))
+            if name in _SEQUENCE_OPERATORS:   # whole: with the compiled library's formulas, refusals and versions
+                lib.impl(name, _forward_to_compiled(name), "CompositeImplicitAutograd")
+                continue
             lib.impl(name, _forward_to_compiled(name), "CUDA")
             torch.library.register_fake(f"{ns}::{name}", _FAKES[name], lib=lib)
 
@@ -434,39 +439,6 @@ def register_namespace(ns: str) -> None:
             ga = op.chen_product_backward.default(zero, ggb, grad_out, ctx.depth, ctx.d)[0] - grad_out
         return ga, gb, gg, None, None
 
-    def setup_attn(ctx, inputs, output):
-        q, k, v, log_decay, initial_state, lengths, scale, return_state = inputs
-        ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths)
-        ctx.scale, ctx.return_state = scale, bool(return_state)
-        ctx.set_materialize_grads(False)
-
-    def backward_attn(ctx, grad_out, grad_state):
-        q, k, v, log_decay, initial_state, lengths = ctx.saved_tensors
-        if (grad_out is None and grad_state is None) or not any(ctx.needs_input_grad[:5]):
-            return (None,) * 8
-        grads = getattr(torch.ops, ns).linear_attention_backward.default(
-            q, k, v, log_decay, initial_state, lengths, grad_out, grad_state if ctx.return_state else None, ctx.scale,
-            ctx.needs_input_grad[3])
-        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad[:5])) + (None, None, None)
-
-    def setup_norm(ctx, inputs, output):
-        ctx.save_for_backward(*inputs[:6])
-        ctx.activation, ctx.eps = int(inputs[6]), float(inputs[7])
-        ctx.set_materialize_grads(False)
-
-    def backward_norm(ctx, grad_h, grad_n):
-        saved = ctx.saved_tensors
-        if saved[5] is None:
-            grad_n = None
-        if (grad_h is None and grad_n is None) or not any(ctx.needs_input_grad[:6]):
-            return (None,) * 8
-        grads = getattr(torch.ops, ns).gated_residual_norm_backward.default(*saved, grad_h, grad_n, ctx.activation,
-                                                                            ctx.eps)
-        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad[:6])) + (None, None)
-
-    if lib is not None:   # those of this package's own namespace are part of the compiled library
-        torch.library.register_autograd(f"{ns}::linear_attention", backward_attn, setup_context=setup_attn, lib=lib)
-        torch.library.register_autograd(f"{ns}::gated_residual_norm", backward_norm, setup_context=setup_norm, lib=lib)
     torch.library.register_autograd(f"{ns}::chen_product", backward_chen, setup_context=setup_chen, lib=lib)
     torch.library.register_autograd(f"{ns}::chen_product_backward", backward_chen_bwd,
                                     setup_context=setup_chen_bwd, lib=lib)

@@ -46,8 +46,8 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *, init
     [0, L] are clamped).  ``scale`` defaults to ``Dk ** -0.5``.
 
     Returns the output (B, L, H, Dv) in the type of ``q``; with ``return_state`` also the state after the last step
-    (B, H, Dk, Dv).  Differentiable once wrt all floating operands (a second derivative is refused); gradients
-    are the same bits on every run.  Under CUDA graph capture, capture forward and backward together, with no graph of an
+    (B, H, Dk, Dv).  Differentiable once wrt all floating operands (second derivatives and forward mode are
+    refused); gradients are the same bits on every run.  Under CUDA graph capture, capture forward and backward together, with no graph of an
     eager call on the same leaves alive.
     """
     out, state = ops.linear_attention(q, k, v, log_decay, initial_state, lengths, _scale(q, scale), bool(return_state))
@@ -85,7 +85,7 @@ def gated_residual_norm(x: Tensor, weight: Optional[Tensor] = None, *, gate: Opt
     ``x``.  ``n`` is the norm of h before h is rounded.
 
     Returns ``h``, or ``(h, n)`` when ``next_weight`` is given, in the type of ``x``.  Differentiable once wrt all
-    operands (a second derivative is refused); gradients are the same bits on every run.
+    operands (second derivatives and forward mode are refused); gradients are the same bits on every run.
     """
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}")

@@ -6,6 +6,7 @@ import ctypes
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 import pathsig_b200 as ps
@@ -146,3 +147,47 @@ def test_the_step_raises_the_version_of_its_state():
         with torch.inference_mode():
             ps.linear_attention_step(q, k, v, decay, state)
             ps.linear_attention_step(q, k, v, decay, torch.empty(2, 4, 8, 8, device="cuda"))   # has no version
+
+
+@pytest.mark.parametrize("namespace", ["pathsig_b200", "pathsig"])
+def test_forward_mode_is_refused(namespace):
+    """An operand with a tangent, whether or not another requires a gradient; by the compiled operators, so under both names."""
+    ps.ops.register_namespace("pathsig")
+    op = getattr(torch.ops, namespace)
+    with FakeTensorMode(), forward_ad.dual_level():
+        z = lambda *s: torch.empty(*s, device="cuda")
+        attention = (z(2, 5, 4, 8), z(2, 5, 2, 8), z(2, 5, 2, 6), z(4), z(2, 4, 8, 6))
+        norm = (z(3, 8), z(8), z(3, 8), z(3, 8), z(8), z(8))
+        step = (z(2, 4, 8), z(2, 2, 8), z(2, 2, 6), z(4), z(2, 4, 8, 6))
+        out, state = z(2, 5, 4, 6), z(2, 4, 8, 6)
+        calls = {
+            "linear_attention": (attention, lambda a: op.linear_attention(*a, None, 1.0, True)),
+            "linear_attention_backward": (attention + (out, state),
+                                          lambda a: op.linear_attention_backward(*a[:5], None, *a[5:], 1.0, True)),
+            "linear_attention_step": (step, lambda a: op.linear_attention_step(*a, 1.0)),
+            "gated_residual_norm": (norm, lambda a: op.gated_residual_norm(*a, 0, 1e-6)),
+            "gated_residual_norm_backward": (norm + (norm[0], norm[0]), lambda a: op.gated_residual_norm_backward(*a, 0, 1e-6)),
+        }
+        for name, (operands, call) in calls.items():
+            call(operands)
+            for i, t in enumerate(operands):
+                dual = list(operands)
+                dual[i] = forward_ad.make_dual(t, torch.empty_like(t))
+                with pytest.raises(RuntimeError, match=name + " has no forward-mode"):
+                    call(dual)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                    call(dual)
+
+
+def test_the_other_namespace_runs_the_same_operators():
+    ps.ops.register_namespace("pathsig")
+    with FakeTensorMode():
+        q, k, v = (torch.empty(2, 9, h, d, device="cuda") for h, d in ((4, 16), (2, 16), (2, 24)))
+        decay = torch.empty(4, device="cuda", requires_grad=True)
+        out, state = torch.ops.pathsig.linear_attention(q, k, v, decay, None, None, 1.0, True)
+        assert out.shape == (2, 9, 4, 24) and state.shape == (2, 4, 16, 24) and out.requires_grad and state.requires_grad
+        state = state.detach()
+        torch.ops.pathsig.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], decay.detach(), state, 1.0)
+        assert state._version == 1
+    with pytest.raises(NotImplementedError):
+        torch.ops.pathsig.gated_residual_norm(torch.zeros(2, 4), None, None, None, None, None, 0, 1e-6)
