@@ -24,7 +24,7 @@
 namespace psig {
 namespace {
 
-enum Barrier { kRaw, kRawV, kReady, kReadyV, kScores, kInc, kIncRead, kP, kO1, kEpi, kDecFull0, kDecFull1, kDecFree0, kDecFree1, kSwap, kBarriers };
+enum Barrier { kRaw, kRawV, kReady, kReadyV, kScores, kInc, kIncRead, kP, kO1, kEpi, kDecFull0, kDecFull1, kDecFree0, kDecFree1, kSwap, kFinish, kBarriers };
 
 using bf16 = __nv_bfloat16;
 
@@ -159,6 +159,7 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
         bar_init(bar(kO1), 1);
         bar_init(bar(kEpi), warps_out);
         bar_init(bar(kSwap), warps_state);
+        bar_init(bar(kFinish), 1);
         for (int i = 0; i < 2; ++i) {
             bar_init(bar(kDecFull0 + i), 1);
             bar_init(bar(kDecFree0 + i), warps_state + (STATE ? 0 : warps_out));
@@ -573,11 +574,9 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
                 load_v(i + 1);
                 ++loaded_v;
             }
-            if (*failed) {
-                // let what is in flight land before the block gives its memory back
-                warp_wait(bar(kRaw), (loaded - 1) & 1, failed + 1);
-                warp_wait(bar(kRawV), (loaded_v - 1) & 1, failed + 1);
-            }
+            // let what is in flight land before the block gives its memory back, whoever else fails from here on
+            warp_wait(bar(kRaw), (loaded - 1) & 1, failed + 1);
+            warp_wait(bar(kRawV), (loaded_v - 1) & 1, failed + 1);
         }
     } else {
         const float *g = static_cast<const float *>(a.decay) + b * a.decay_stride[0] + h * a.decay_stride[2];
@@ -589,6 +588,10 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
     __syncthreads();
     if (warp == 16) {
         fence_after();
+        if (*failed) {   // products in flight read shared and tensor memory
+            mma_commit(bar(kFinish), lane == 0);
+            warp_wait(bar(kFinish), 0, failed + 1);
+        }
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(Lay::columns));
     }
 }

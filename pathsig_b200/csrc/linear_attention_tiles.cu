@@ -42,7 +42,7 @@ constexpr int kTileThreads = kStateThreads + kScoreThreads + kOutThreads + 96;
 // before) is counted by that place.
 enum Barrier {
     kFullRK, kFullV0, kFullV1, kVReady, kScores, kInc0, kInc1, kP, kO2, kO1_0, kO1_1, kFix, kOutFull, kOutFree, kDot, kDotFree,
-    kDecFull0, kDecFull1, kDecFree0, kDecFree1, kBarriers
+    kDecFull0, kDecFull1, kDecFree0, kDecFree1, kFinish, kBarriers
 };
 
 template <int KP, int NS, int NV, bool DOT>
@@ -107,6 +107,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
         bar_init(bar(kOutFull), kOutThreads / 32);
         bar_init(bar(kOutFree), 1);
         bar_init(bar(kDot), 1);
+        bar_init(bar(kFinish), 1);
         bar_init(bar(kDotFree), kOutThreads / 32);
         for (int i = 0; i < 2; ++i) {
             bar_init(bar(kDecFull0 + i), 1);
@@ -566,13 +567,12 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                     if (VS == 1 && !load_v()) { stop = 4; break; }
                 }
             }
-            if (*failed) {
-                // let what is in flight land before the block gives its memory back: g whole pieces, and what the last one got
-                const int v = g + (stop > 1 && VS == 2), dots = g + (stop > 2), rk = g + (stop > 3);
-                if (rk > 0) bar_wait(bar(kFullRK), (rk - 1) & 1, failed + 1);
-                if (DOT && dots > 0) bar_wait(bar(kDot), (dots - 1) & 1, failed + 1);
-                for (int i = v > VS ? v - VS : 0; i < v; ++i) bar_wait(bar(kFullV0 + i % VS), (i / VS) & 1, failed + 1);
-            }
+            // let what is in flight land before the block gives its memory back, whoever else fails from here on: g whole pieces,
+            // and what the last one got
+            const int v = g + (stop > 1 && VS == 2), dots = g + (stop > 2), rk = g + (stop > 3);
+            if (rk > 0) bar_wait(bar(kFullRK), (rk - 1) & 1, failed + 1);
+            if (DOT && dots > 0) bar_wait(bar(kDot), (dots - 1) & 1, failed + 1);
+            for (int i = v > VS ? v - VS : 0; i < v; ++i) bar_wait(bar(kFullV0 + i % VS), (i / VS) & 1, failed + 1);
         }
         __syncwarp();
     } else {
@@ -589,6 +589,10 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
     __syncthreads();
     if (warp == 20) {
         fence_after();
+        if (*failed) {   // products in flight read shared and tensor memory
+            mma_commit(bar(kFinish), lane == 0);
+            warp_wait(bar(kFinish), 0, failed + 1);
+        }
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(Lay::columns));
     }
 }
