@@ -297,9 +297,12 @@ int psig_attn_step(const PsigAttnDesc *desc, const void *q, const void *k, const
 /* Diagnostic: waits inside the kernels of psig_attn_* and psig_norm_* that ran out on the current device since the last call
  * (read and cleared; synchronises).  Every wait for a copy, a matrix product or another warp is bounded (2^22 polls, and two
  * seconds); one that runs out ends its block early, and the call's results are then not valid.  0 in normal operation.
+ * psig_set_sequence_failure_flag: kernels of later calls store 1 in *flag (host memory that the devices can write, at the address
+ * given; NULL: nowhere) when one of their waits runs out, so that a host need not synchronise to hear of it; the host clears it.
  * psig_set_norm_wait_polls sets how often the norms' kernels of later calls look for a row that they stream through shared
  * memory (negative: the default, 2^22; 0: never, so that every such wait runs out), for tests. */
 int64_t psig_sequence_wait_timeouts(void);
+int psig_set_sequence_failure_flag(int32_t *flag);
 int psig_set_norm_wait_polls(int polls);
 
 /* Norm around a block, fused with the block's gate, the residual sum and the norm before the next block; no

@@ -140,6 +140,7 @@ EXPORTS = {
     "psig_attn_backward": (_int, [_AttnP] + [_vp] * 13 + [_i64, _vp]),
     "psig_attn_step": (_int, [_AttnP] + [_vp] * 7),
     "psig_sequence_wait_timeouts": (_i64, []),
+    "psig_set_sequence_failure_flag": (_int, [_vp]),
     "psig_set_norm_wait_polls": (_int, [_int]),
     "psig_norm_forward": (_int, [_NormP] + [_vp] * 9),
     "psig_norm_backward_workspace": (_i64, [_NormP]),

@@ -11,6 +11,8 @@
 // the difference of the two sums never runs over more than a segment, however long the sequence is.
 #include "sequence.cuh"
 
+#include <atomic>
+
 namespace psig {
 namespace {
 
@@ -427,8 +429,11 @@ Sweep sweep_of(const PsigAttnDesc &d, const void *decay)
     s.out_scale = 1.0;
     s.kv_scale = 1.0;
     s.splits = 1;
+    s.failure = failure_flag();
     return s;
 }
+
+std::atomic<int *> g_failure_flag{nullptr};
 
 bool per_head(const PsigAttnDesc &d) { return d.decay_strides[0] == 0 && d.decay_strides[1] == 0; }
 
@@ -693,6 +698,9 @@ int run_backward(const Call &c, const void *init, const void *gs, void *grad_q, 
 }
 
 }  // namespace
+
+int *failure_flag() { return g_failure_flag.load(std::memory_order_acquire); }
+
 }  // namespace psig
 
 using namespace psig;
@@ -744,6 +752,12 @@ extern "C" int psig_attn_backward(const PsigAttnDesc *desc, const void *q, const
 }
 
 extern "C" int64_t psig_sequence_wait_timeouts(void) { return attn_tile_timeouts() + attn_split_timeouts() + norm_timeouts(); }
+
+extern "C" int psig_set_sequence_failure_flag(int32_t *flag)
+{
+    g_failure_flag.store(flag, std::memory_order_release);
+    return PSIG_OK;
+}
 
 extern "C" int psig_attn_step(const PsigAttnDesc *desc, const void *q, const void *k, const void *v,
                               const void *log_decay, void *state, void *out, void *stream)

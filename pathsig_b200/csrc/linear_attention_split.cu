@@ -589,6 +589,7 @@ attn_sweep_split_terms(const __grid_constant__ CUtensorMap map_r, const __grid_c
     if (warp == 16) {
         fence_after();
         if (*failed) {   // products in flight read shared and tensor memory
+            if (lane == 0) report_failure(a.failure);
             mma_commit(bar(kFinish), lane == 0);
             warp_wait(bar(kFinish), 0, failed + 1);
         }

@@ -34,6 +34,7 @@ struct NormArgs {
     double mean, eps;      // 1 / D
     float mean_f, eps_f;   // the same: converting costs a thread as much as some values of its row
     int activation;
+    int *failure;          // see failure_flag
 };
 
 template <typename A> __device__ __forceinline__ A scalar(double wide, float narrow)
@@ -234,9 +235,10 @@ struct RingState {
     }
     // one thread, behind a wait that ran out for row `row` in `stage`: the copies of that row and of the rows behind it, as many
     // as there are stages, have been started
-    __device__ __forceinline__ void drain(int stage, uint32_t parity, long long row, long long step, long long rows) const
+    __device__ __forceinline__ void drain(int stage, uint32_t parity, long long row, long long step, long long rows, int *failure) const
     {
         atomicAdd(&g_norm_timeouts, 1ull);
+        report_failure(failure);
         for (int i = 0; i < ring.stages && row + i * step < rows; ++i) {
             const int s = stage + i;
             arrived(s < ring.stages ? s : s - ring.stages, s < ring.stages ? parity : parity ^ 1, kWaitPolls);
@@ -293,7 +295,7 @@ __global__ void __launch_bounds__(kTeamMax) norm_forward_team(const NormArgs a, 
         }
         team_sum(sum, team_log2, shared, round++);
         if (RING && *rs.failed) {
-            if (threadIdx.x == 0) rs.drain(stage, phase, first, step, a.rows);
+            if (threadIdx.x == 0) rs.drain(stage, phase, first, step, a.rows, a.failure);
             break;
         }
         const A r = inverse_root(sum[0] * mean + eps);
@@ -494,7 +496,7 @@ __global__ void __launch_bounds__(kTeamMax) norm_backward_team(const NormArgs a,
             team_sum(one, team_log2, shared, round++);
         }
         if (RING && *rs.failed) {
-            if (threadIdx.x == 0) rs.drain(stage, phase, first, step, a.rows);
+            if (threadIdx.x == 0) rs.drain(stage, phase, first, step, a.rows, a.failure);
             break;
         }
         if (!NEXT) {
@@ -855,6 +857,7 @@ void set_sizes(NormArgs &a, const PsigNormDesc &d)
     a.rows = d.rows, a.D = d.D, a.activation = d.activation;
     a.mean = 1.0 / (double)d.D, a.eps = d.eps;
     a.mean_f = (float)a.mean, a.eps_f = (float)a.eps;
+    a.failure = failure_flag();
 }
 
 // How a row is dealt to threads: 8 values to a thread, 16 where the row would need more than 256 threads.

@@ -39,6 +39,15 @@ __device__ __forceinline__ bool wait_expired(unsigned poll, unsigned long long &
     return now - start > kWaitTime;
 }
 
+// Where the host sees that a wait ran out (psig_set_sequence_failure_flag), or NULL.
+int *failure_flag();
+__device__ __forceinline__ void report_failure(int *flag)
+{
+    if (flag == nullptr) return;
+    *reinterpret_cast<volatile int *>(flag) = 1;
+    __threadfence_system();
+}
+
 // Calls fn.template operator()<T>() with the storage type of a PsigDtype.
 template <typename Fn>
 int with_dtype(int dtype, Fn fn)
@@ -96,6 +105,7 @@ struct Sweep {
     // (B, H, splits, tiles of 64 by 64) and decays (B, H, splits).
     int splits;
     float *split_states, *split_decays;
+    int *failure;         // see failure_flag
 };
 
 inline int tile_columns(int d2) { return (d2 + 63) / 64; }

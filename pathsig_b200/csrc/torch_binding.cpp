@@ -412,6 +412,31 @@ std::tuple<at::Tensor, at::Tensor> chen_product_backward(const at::Tensor &sig_a
 
 // ---- decayed linear attention and the norm around a block (no counterpart in the reference) ----
 
+// A wait inside a kernel that ran out leaves wrong results behind and a mark in a word of host memory; the next call of a
+// sequence operator raises for it, once.  (The word is written by the devices: one page-locked integer for the process.)
+void refuse_after_failure()
+{
+    static volatile int32_t *const flag = []() -> volatile int32_t * {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;   // the first call may stand in a capture
+        if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+        void *host = nullptr, *device = nullptr;
+        if (cudaHostAlloc(&host, sizeof(int32_t), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess ||
+            cudaHostGetDevicePointer(&device, host, 0) != cudaSuccess) {
+            cudaGetLastError();
+            host = nullptr;
+        }
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (host == nullptr) return nullptr;
+        *static_cast<volatile int32_t *>(host) = 0;
+        psig_set_sequence_failure_flag(static_cast<int32_t *>(device));
+        return static_cast<volatile int32_t *>(host);
+    }();
+    if (flag == nullptr || *flag == 0) return;
+    *flag = 0;
+    TORCH_CHECK(false, "a wait inside an earlier linear_attention or gated_residual_norm kernel ran out: results since then are not "
+                       "valid (psig_sequence_wait_timeouts counts such waits)");
+}
+
 int sequence_dtype(const at::Tensor &t, const char *name)
 {
     switch (t.scalar_type()) {
@@ -525,6 +550,7 @@ std::tuple<at::Tensor, at::Tensor> linear_attention(const at::Tensor &q_in, cons
     Range range("pathsig_b200::linear_attention");
     TORCH_CHECK(q_in.is_cuda(), "q must be a CUDA tensor");
     c10::cuda::CUDAGuard guard(q_in.device());
+    refuse_after_failure();
     at::Tensor q = q_in, k = k_in, v = v_in, decay = log_decay_in;
     PsigAttnDesc desc = attn_desc(q, k, v, decay, scale, true);
     at::Tensor init;
@@ -560,6 +586,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_at
     Range range("pathsig_b200::linear_attention_backward");
     TORCH_CHECK(q_in.is_cuda(), "q must be a CUDA tensor");
     c10::cuda::CUDAGuard guard(q_in.device());
+    refuse_after_failure();
     at::Tensor q = q_in, k = k_in, v = v_in, decay = log_decay_in;
     PsigAttnDesc desc = attn_desc(q, k, v, decay, scale, true);
     at::Tensor init, go, gs;
@@ -606,6 +633,7 @@ at::Tensor linear_attention_step(const at::Tensor &q_in, const at::Tensor &k_in,
     Range range("pathsig_b200::linear_attention_step");
     TORCH_CHECK(q_in.is_cuda(), "q must be a CUDA tensor");
     c10::cuda::CUDAGuard guard(q_in.device());
+    refuse_after_failure();
     at::Tensor q = q_in, k = k_in, v = v_in, decay = log_decay_in;
     PsigAttnDesc desc = attn_desc(q, k, v, decay, scale, false);
     check_state(desc, q, state, "state");
@@ -670,6 +698,7 @@ std::tuple<at::Tensor, at::Tensor> gated_residual_norm(const at::Tensor &x, cons
     Range range("pathsig_b200::gated_residual_norm");
     TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
     c10::cuda::CUDAGuard guard(x.device());
+    refuse_after_failure();
     NormOperands o = norm_operands(x, weight, gate, residual, residual_scale, next_weight, activation, eps);
     at::Tensor h = at::empty(x.sizes(), x.options());
     at::Tensor n = o.next.defined() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
@@ -690,6 +719,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
     Range range("pathsig_b200::gated_residual_norm_backward");
     TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
     c10::cuda::CUDAGuard guard(x.device());
+    refuse_after_failure();
     NormOperands o = norm_operands(x, weight, gate, residual, residual_scale, next_weight, activation, eps);
     at::Tensor grad_h, grad_n;
     for (auto [t, name, to] : {std::make_tuple(&grad_h_in, "grad_h", &grad_h), std::make_tuple(&grad_n_in, "grad_n", &grad_n)}) {

@@ -317,6 +317,34 @@ def test_a_wait_for_a_row_that_runs_out_ends_its_block(ps, rows, D, dtype, form)
         assert lib.psig_sequence_wait_timeouts() == 0      # read and cleared
     finally:
         assert lib.psig_set_norm_wait_polls(-1) == 0
+    with pytest.raises(RuntimeError, match="ran out"):
+        backward()
     for a, b in zip(backward(), want):
         assert torch.equal(a, b)
     assert lib.psig_sequence_wait_timeouts() == 0
+
+
+def test_a_wait_that_ran_out_is_an_error_of_the_next_call(ps):
+    """The call itself has been enqueued and has returned by then; the one after it raises, once, whichever operator it is."""
+    from pathsig_b200 import _load
+    lib = _load.ensure_loaded()
+    c = _gpu(_make(3, 2400, 1024, torch.bfloat16, FORMS[4]), torch.bfloat16)
+    args = [c[n] for n in NAMES]
+    backward = torch.ops.pathsig_b200.gated_residual_norm_backward
+    want = backward(*args, c["grad_h"], c["grad_n"], 0, 1e-6)
+    q, d = torch.randn(1, 3, 2, 8, device=DEV), torch.zeros(2, device=DEV)
+    for following in (lambda: backward(*args, c["grad_h"], c["grad_n"], 0, 1e-6), lambda: ps.gated_residual_norm(c["x"]),
+                      lambda: ps.linear_attention(q, q, q, d),
+                      lambda: ps.linear_attention_step(q[:, 0], q[:, 0], q[:, 0], d, torch.zeros(1, 2, 8, 8, device=DEV))):
+        try:
+            assert lib.psig_set_norm_wait_polls(0) == 0
+            backward(*args, c["grad_h"], c["grad_n"], 0, 1e-6)
+            torch.cuda.synchronize()
+        finally:
+            assert lib.psig_set_norm_wait_polls(-1) == 0
+        with pytest.raises(RuntimeError, match="ran out"):
+            following()
+        following()
+        assert lib.psig_sequence_wait_timeouts() > 0
+    for a, b in zip(backward(*args, c["grad_h"], c["grad_n"], 0, 1e-6), want):
+        assert torch.equal(a, b)
