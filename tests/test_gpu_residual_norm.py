@@ -348,3 +348,24 @@ def test_a_wait_that_ran_out_is_an_error_of_the_next_call(ps):
         assert lib.psig_sequence_wait_timeouts() > 0
     for a, b in zip(backward(*args, c["grad_h"], c["grad_n"], 0, 1e-6), want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32])
+@pytest.mark.parametrize("activation", ["silu", "sigmoid"])
+@pytest.mark.parametrize("D", [8, 16384])
+def test_gates_far_out_are_good_to_the_types_last_bits(ps, D, activation, dtype):
+    """Gates of -85 to 85, each value relative to itself.  Units of half a step: the root 9 (eight squares and their sum, halved by
+    the root: 4; mean and eps 1; the root 4; for the long row its sums run over 32 lanes and 16 warps or more, 1024 / 32 + 20 more
+    at most), the exponential 4, the sum, quotient and product 3, three more products: below 24, and 80 for the long row.  The slope
+    of the gate, s (1 + g (1 - s)), is looked at below -3, where neither difference cancels by more than half.  The gate's value
+    and slope are normal numbers (above exp(-85)), but their product with a small x or gradient, the last on its way, may lie below
+    2^-126: it is then a multiple of 2^-149, off by half of that."""
+    c = _make(D, 3, D, dtype, (False, activation, False, False, False))
+    c["gate"] = torch.linspace(-85, 85, 3 * D, dtype=torch.float64).to(dtype).double().reshape(3, D)
+    c["activation"] = activation
+    got = _run(lambda t: _ours(ps, c["eps"])(dict(t, activation=activation)), _gpu(c, dtype))
+    exact, _ = so.norm_bounds(c, dtype)
+    units = (24 if D == 8 else 80) * so.half_step(dtype)
+    for name, where in (("h", c["gate"] == c["gate"]), ("grad_gate", c["gate"] < -3)):
+        off = (got[name].double().cpu() - exact[name]).abs()[where]
+        assert not (off > units * exact[name].abs()[where] + 2.0 ** -150).any(), (name, float((off / exact[name].abs()[where]).max() / so.half_step(dtype)))
