@@ -61,14 +61,15 @@ struct TileLayout {
     static constexpr int bars = sums + (DOT ? 4 * kPiece * 4 : 0);
     static constexpr int tmem = bars + kBarriers * 8;
     static constexpr int alloc = tmem + 16;
-    // tensor memory columns: scores (P takes the columns its own thread has read), the second scores, O2, I and O1
+    // tensor memory columns: scores (P's two terms for 16 steps take the columns that those steps' scores were read from), the
+    // second scores, O2 and I with the terms of S and V' side by side as far as there is room, O1
+    static constexpr int o2_blocks = NS > 1 ? 2 : 1, i_blocks = DOT ? 1 : NV;   // of 64 columns
     static constexpr int c_two = 128;
     static constexpr int c_o2 = DOT ? 256 : 128;
-    static constexpr int c_i = c_o2 + 64;
-    static constexpr int c_o1 = c_i + 64;
-    static constexpr int c_p = c_o1 + 64;   // what P's rounding to its first term left
+    static constexpr int c_i = c_o2 + 128;
+    static constexpr int c_o1 = c_i + 64 * i_blocks;
     static constexpr int columns = 512;
-    static_assert(c_p + 64 <= columns, "tensor memory");
+    static_assert(c_o1 + 64 <= columns, "tensor memory");
 };
 
 template <typename T, int KP, int NS, int NV, bool DOT, bool REV, bool STATE>
@@ -152,10 +153,14 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
 #pragma unroll
                 for (int term = 0; term < NS; ++term) {
                     uint4 w;
-                    w.x = next_term<T>(x[0], x[1], term == NS - 1);
-                    w.y = next_term<T>(x[2], x[3], term == NS - 1);
-                    w.z = next_term<T>(x[4], x[5], term == NS - 1);
-                    w.w = next_term<T>(x[6], x[7], term == NS - 1);
+                    if (NS == 2 && term == 0) {
+                        w.x = cut_term(x[0], x[1]), w.y = cut_term(x[2], x[3]), w.z = cut_term(x[4], x[5]), w.w = cut_term(x[6], x[7]);
+                    } else {
+                        w.x = next_term<T>(x[0], x[1], term == NS - 1);
+                        w.y = next_term<T>(x[2], x[3], term == NS - 1);
+                        w.z = next_term<T>(x[4], x[5], term == NS - 1);
+                        w.w = next_term<T>(x[6], x[7], term == NS - 1);
+                    }
                     *reinterpret_cast<uint4 *>(smem + Lay::s + term * KP * 128 + swizzled(srow, sc0 / 8 + c)) = w;
                 }
             }
@@ -186,7 +191,7 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                 for (int j = 0; j < SC; ++j) S[j] = parts[j * kStateThreads];
             } else if (part == 0 && a.init != nullptr)
                 all_state(a.init_transposed, state0, [&](float &v, long long at) { v = static_cast<const float *>(a.init)[at]; });
-            if (!STATE) store_terms();
+            if (!STATE && (part > 0 || a.init != nullptr)) store_terms();   // nothing stands before the first piece else
 #pragma unroll 1
             for (int i = 0; i < it.pieces; ++i, ++g) {
                 const uint32_t ph = g & 1;
@@ -251,12 +256,22 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                 if (!(ok = warp_wait(bar(kInc0 + (g & 1)), (g >> 1) & 1, failed))) break;
                 if (last) continue;
                 fence_after();
-                float x[SC / 16][16];
 #pragma unroll
-                for (int c = 0; c < SC / 16; ++c) tmem_load16(tmem + lanes + Lay::c_i + sc0 + c * 16, x[c]);
-                tmem_loaded();
+                for (int c = 0; c < SC; c += 16) {
+                    float x[16];
+                    tmem_load16(tmem + lanes + Lay::c_i + (Lay::i_blocks - 1) * 64 + sc0 + c, x);
+                    tmem_loaded();
 #pragma unroll
-                for (int j = 0; j < SC; ++j) S[j] = fmaf(S[j], keep, x[j / 16][j % 16] * kv_scale);
+                    for (int b = Lay::i_blocks - 2; b >= 0; --b) {
+                        float y[16];
+                        tmem_load16(tmem + lanes + Lay::c_i + b * 64 + sc0 + c, y);
+                        tmem_loaded();
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) add_two(x[j], x[j + 1], y[j], y[j + 1]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) S[c + j] = fmaf(S[c + j], keep, x[j] * kv_scale);
+                }
                 if (STATE || i + 1 == it.pieces) fence_before();
                 else store_terms();
                 if (!REV && !STATE && a.anchors != nullptr && boundary) {
@@ -292,8 +307,11 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                 if (!(ok = warp_wait(bar(kScores), g & 1, failed))) break;
                 fence_after();
                 float sum = 0.f;
+                // rows behind the last step are nobody's, and the product leaves out a second half of 64 columns without any
+                const int m = (int)(it.n - it.start<REV>(i));
+                const int chunks = quarter * 32 < m && half * 64 < m ? 4 : 0;
 #pragma unroll 1
-                for (int q = 0; q < 4; ++q) {   // 16 columns each
+                for (int q = 0; q < chunks; ++q) {   // 16 columns each
                     const int block = half * 2 + q / 2, s0 = half * 64 + q * 16;
                     uint32_t p[8], left[8];   // P's two terms
                     if (REV ? block >= quarter : block <= quarter) {
@@ -321,26 +339,26 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                         } else {
                             const float fq = q < 2 ? f[0] : f[1];
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) t[j] *= fq;
+                            for (int j = 0; j < 16; j += 2) mul_two(t[j], t[j + 1], fq, fq);
                         }
                         tmem_loaded();
                         // (weight 0 against a score that is not finite: only in rows behind the end, which nobody reads)
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            x[j] *= t[j];
-                            if (DOT) sum = fmaf(x[j], y[j], sum);
+                        for (int j = 0; j < 16; j += 2) {
+                            mul_two(x[j], x[j + 1], t[j], t[j + 1]);
+                            if (DOT) sum = fmaf(x[j + 1], y[j + 1], fmaf(x[j], y[j], sum));
                         }
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            p[j] = next_term<T>(x[2 * j], x[2 * j + 1], false);
+                            p[j] = cut_term(x[2 * j], x[2 * j + 1]);
                             left[j] = next_term<T>(x[2 * j], x[2 * j + 1], true);
                         }
                     } else {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) p[j] = left[j] = 0;
                     }
-                    tmem_store8(own + q * 8, p);
-                    tmem_store8(tmem + lanes + Lay::c_p + half * 32 + q * 8, left);
+                    tmem_store8(own + q * 16, p);
+                    tmem_store8(own + q * 16 + 8, left);
                 }
                 if (DOT) sums[((g & 1) * 2 + half) * kPiece + row] = sum;
                 tmem_stored();
@@ -379,9 +397,17 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                     for (int c = 0; c < 4; ++c) {   // 16 columns each
                         float u[16];
                         tmem_load16(tmem + lanes + Lay::c_o2 + c * 16, u);
-                        tmem_loaded();
+                        if constexpr (Lay::o2_blocks > 1) {
+                            float w[16];
+                            tmem_load16(tmem + lanes + Lay::c_o2 + 64 + c * 16, w);
+                            tmem_loaded();
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) u[j] *= head;
+                            for (int j = 0; j < 16; j += 2) add_two(u[j], u[j + 1], w[j], w[j + 1]);
+                        } else {
+                            tmem_loaded();
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) mul_two(u[j], u[j + 1], head, head);
                         tmem_store16(tmem + lanes + Lay::c_o1 + c * 16, u);
                         if (DOT && row < m)
 #pragma unroll
@@ -461,16 +487,17 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
     } else if (warp == 20) {
         // ------------------------------------------------------------------ TMA and MMA
         const uint32_t lead = lane == 0, base16 = base >> 4;
-        // I = K^T V'; with 64 state rows the second block of 64 is the first once more
+        // I = K^T V' (all terms of V' in one product where they have columns of their own: K is read once); with 64 state rows the
+        // second block of 64 is the first once more
         auto state_product = [&](int g) {
 #pragma unroll
-                for (int term = NV - 1; term >= 0; --term)
+            for (int term = NV - Lay::i_blocks; term >= 0; --term)
 #pragma unroll
-                    for (int j = 0; j < kPiece / 16; ++j)
-                        mma_ss(tmem + Lay::c_i, tile_desc(base16 + ((Lay::k + j * 2048) >> 4), KP == 128 ? kTileBytes : 0),
-                               tile_desc(base16 + ((Lay::vw + term * kTileBytes + j * 2048) >> 4), kTileBytes), instr_desc<T>(64, true, true),
-                               term < NV - 1 || j > 0, lead);
-                mma_commit(bar(kInc0 + (g & 1)), lead);
+                for (int j = 0; j < kPiece / 16; ++j)
+                    mma_ss(tmem + Lay::c_i, tile_desc(base16 + ((Lay::k + j * 2048) >> 4), KP == 128 ? kTileBytes : 0),
+                           tile_desc(base16 + ((Lay::vw + term * kTileBytes + j * 2048) >> 4), kTileBytes),
+                           instr_desc<T>(Lay::i_blocks * 64, true, true), term < NV - Lay::i_blocks || j > 0, lead);
+            mma_commit(bar(kInc0 + (g & 1)), lead);
         };
         int g = 0, fixes = 0;
         bool ok = true;
@@ -512,25 +539,27 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                 const bool past = !no_past(it, i), future = !no_future(it, i);
                 if (past)
 #pragma unroll
-                for (int term = NS - 1; term >= 0; --term)
+                for (int term = 0; term < NS; term += 2)   // the first two terms in one product, the third added to the second
 #pragma unroll
                     for (int j = 0; j < KP / 16; ++j)
-                        mma_ss(tmem + Lay::c_o2, tile_desc(base16 + ((Lay::r + (j / 4) * kTileBytes + (j % 4) * 32) >> 4), 16),
-                               tile_desc(base16 + ((Lay::s + term * KP * 128 + j * 2048) >> 4), kTileBytes), instr_desc<T>(64, false, true),
-                               term < NS - 1 || j > 0, lead);
+                        mma_ss(tmem + Lay::c_o2 + term / 2 * 64, tile_desc(base16 + ((Lay::r + (j / 4) * kTileBytes + (j % 4) * 32) >> 4), 16),
+                               tile_desc(base16 + ((Lay::s + term * KP * 128 + j * 2048) >> 4), KP * 128),
+                               instr_desc<T>(term == 0 ? Lay::o2_blocks * 64 : 64, false, true), term > 0 || j > 0, lead);
                 if (future) state_product(g);
                 else mma_commit(bar(kInc0 + (g & 1)), lead);
                 // O1 += P V, on top of the state's part, which the output warps put there
                 if (!(ok = warp_wait(bar(kP), ph, failed) && warp_wait(bar(kO2), ph, failed))) break;
                 fence_after();
+                auto half_product = [&](int j0, bool add) {   // of 64 steps; P's second term, then its first
 #pragma unroll
-                for (int j = 0; j < kPiece / 16; ++j)
-                    mma_ts(tmem + Lay::c_o1, tmem + Lay::c_p + j * 8, tile_desc(v16 + (j * 2048 >> 4), kTileBytes),
-                           instr_desc<T>(64, false, true), past || j > 0, lead);
+                    for (int left = 8; left >= 0; left -= 8)
 #pragma unroll
-                for (int j = 0; j < kPiece / 16; ++j)
-                    mma_ts(tmem + Lay::c_o1, tmem + (j / 4) * 64 + (j % 4) * 8, tile_desc(v16 + (j * 2048 >> 4), kTileBytes),
-                           instr_desc<T>(64, false, true), true, lead);
+                        for (int j = j0; j < j0 + 4; ++j)
+                            mma_ts(tmem + Lay::c_o1, tmem + j * 16 + left, tile_desc(v16 + (j * 2048 >> 4), kTileBytes),
+                                   instr_desc<T>(64, false, true), add || left == 0 || j > j0, lead);
+                };
+                half_product(0, past);
+                if (it.n - it.start<REV>(i) > kPiece / 2) half_product(4, true);
                 mma_commit(bar(kO1_0 + (g & 1)), lead);
             }
         }

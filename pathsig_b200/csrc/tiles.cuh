@@ -171,6 +171,24 @@ __device__ __forceinline__ uint32_t pack(float x, float y, __half) { __half2 p =
 __device__ __forceinline__ float2 unpack(uint32_t v, __nv_bfloat16) { return float2{__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)}; }
 __device__ __forceinline__ float2 unpack(uint32_t v, __half) { return __half22float2(*reinterpret_cast<__half2 *>(&v)); }
 
+// Two additions, subtractions or products in one instruction.
+__device__ __forceinline__ void add_two(float &x, float &y, float a, float b)
+{
+    asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tadd.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}" : "+f"(x), "+f"(y) : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void mul_two(float &x, float &y, float a, float b)
+{
+    asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmul.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}" : "+f"(x), "+f"(y) : "f"(a), "f"(b));
+}
+
+// The first of two bfloat16 terms of a pair, cut instead of rounded (one instruction for both); leaves the rest, which the second
+// term rounds: together within 2^-15, where two rounded terms are within 2^-16.
+__device__ __forceinline__ uint32_t cut_term(float &x, float &y)
+{
+    const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+    add_two(x, y, -__uint_as_float(a & 0xFFFF0000u), -__uint_as_float(b & 0xFFFF0000u));
+    return __byte_perm(a, b, 0x7632);
+}
 // The next 16-bit term of a pair; leaves what the rounding left.
 template <typename T>
 __device__ __forceinline__ uint32_t next_term(float &x, float &y, bool last)
