@@ -378,8 +378,11 @@ __global__ void __launch_bounds__(kTeamMax) norm_forward_team(const NormArgs a, 
 // Blocks walk the rows; a thread keeps the sums over rows for its own columns in registers: q = sum dh act x r, which
 // is the gradient of weight but for the factor residual_scale of the column, and the other way round, and sum dn h r2.
 // NEXT: with the norm before the next block (three exchanges a row instead of one).
+// Registers: where float32 rows are streamed without the next norm, so many that an SM holds two blocks of 320 threads (15616 x 4680
+// signatures 170 us, 220 with two registers more and one block); else what a block of 512 threads can have (a bound on the
+// block's size instead made the compiler stop at 64 for eight values to a thread: 15616 x 1528 81 us, in this form 64).
 template <typename T, int E, int NV, bool NEXT, bool RING>
-__global__ void __launch_bounds__(kTeamMax) norm_backward_team(const NormArgs a, int team_log2, int threads, const Ring ring)
+__global__ void __maxnreg__(RING && !NEXT && NV * E == 16 && sizeof(T) == 4 ? 96 : 128) norm_backward_team(const NormArgs a, int team_log2, int threads, const Ring ring)
 {
     using A = typename Acc<T>::type;
     __shared__ A shared[4 * (kTeamMax / 32)];
