@@ -490,14 +490,16 @@ struct Call {
         return s;
     }
     // By sizes and strides; with null pointers for the operands this is what the workspace queries go by.
-    // A tile is computed whole, 128 steps, however few are there; the row kernel's time grows with the steps.  Rows / tiles, us:
-    // float16, 720 heads of 64: forward 20 / 41 at 8 steps, 32 / 41 at 16, 45 / 41 at 24; backward 125 / 150 and 171 / 152.
-    // float32: 31 / 54 at 16 steps, 45 / 54 at 24, but backward of 1024 heads of 128 753 / 749.  bfloat16 tiles are quicker and
-    // leave out the products of empty states: 1024 heads of 128 45 / 48 at 2 steps, 57 / 48 at 4; carrying a state from call
-    // to call 174 / 208 at 16 steps, 302 / 208 at 32.
+    // A tile is computed whole, 128 steps, however few are there; the row kernel's time grows with the steps and with the heads'
+    // sizes.  Tiles / rows, us, bfloat16: 1024 heads of 128 forward 53 / 45 at 2 steps, 53 / 57 at 4, backward 197 / 185 and 197 / 228;
+    // 720 heads of 64 forward 19 / 15 at 4 steps, 19 / 21 at 8, backward 76 / 65 and 76 / 85; 4096 heads of 32 forward 94 / 47 at 8
+    // steps, 94 / 105 at 24, backward 363 / 188 and 363 / 400.  So 800 / (dk + dv) steps, at most 16; 16 where a state is carried
+    // from call to call (1024 heads of 128: 206 / 174 at 16 steps, 207 / 245 at 24) and in the other types: 720 heads of 64, float16
+    // forward 41 / 32 at 16 steps, 41 / 45 at 24, backward 150 / 125 and 152 / 171, float32 forward 54 / 31 and 54 / 45.  (Heads of 32
+    // and less would gain from a higher limit there: 4096 of them, 24 steps, float16 218 / 105, float32 290 / 105.)
     bool tiles(bool carries, const void *o1 = nullptr, const void *o2 = nullptr, const void *o3 = nullptr) const
     {
-        if (d.L <= (d.dtype == PSIG_BF16 && !carries ? 2 : 16)) return false;
+        if (d.L <= 16 && (d.dtype != PSIG_BF16 || carries || d.L * (d.dk + d.dv) <= 800)) return false;
         for (const void *o : {o1, o2, o3})
             if (reinterpret_cast<uintptr_t>(o) % 16 != 0) return false;
         return d.algo != PSIG_ALGO_GENERIC && attn_tiles_supported(forward(), d.dtype) && attn_tiles_supported(grad_q(), d.dtype);

@@ -603,3 +603,16 @@ def test_step_and_norm_traced_by_torch_compile(ps):
     torch.compile(norm, backend="aot_eager", fullgraph=True)(*b).backward()
     for x, y in zip(a, b):
         assert torch.equal(x.grad, y.grad)
+
+
+@pytest.mark.parametrize("state", [False, True])
+@pytest.mark.parametrize("steps,D", [(3, 128), (4, 128), (6, 64), (7, 64), (12, 32), (13, 32), (16, 24), (17, 24)])
+def test_short_bfloat16_sequences_by_head_size(ps, steps, D, state):
+    """Either side of the limit of steps by head size; both kernels give results that are rounded once."""
+    c = so.make(steps + D, 3, steps, 4, 2, D, D, torch.bfloat16, state=state)
+    g = _on_gpu(c, torch.bfloat16)
+    exact, bounds = so.attention_bounds(c, torch.bfloat16, terms=2)
+    _check(_run(ps, g), exact, bounds)
+    out = ps.linear_attention(*(g[n] for n in NAMES[:4]), initial_state=g["initial_state"])
+    _check({"out": out}, exact, bounds)
+    _no_timeouts()
