@@ -257,7 +257,10 @@ int psig_chen_backward(const PsigChenDesc *desc, const void *a, const void *b, c
  *   q (B, L, H, dk), k (B, L, Hkv, dk), v (B, L, Hkv, dv): dtype; strides in elements for (b, t, head), the last
  *     dimension has stride 1.
  *   log_decay: element (b, t, h) at b*ds[0] + t*ds[1] + h*ds[2] (strides 0 where it does not vary); float32, or
- *     float64 when dtype is PSIG_F64.  Meant to be <= 0; -inf forgets everything before the step.
+ *     float64 when dtype is PSIG_F64.  Meant to be <= 0 (growth beyond 2^127 within 32 steps may overflow where the results
+ *     do not); -inf forgets everything before the step.
+ *   Rows t < n are meant to be finite: an infinity or NaN there may reach every step of its sequence and head, those up to 127
+ *   steps before it too.
  *   initial_state, final_state and their gradients (B, H, dk, dv): contiguous, type of log_decay.
  *   out, grad_out (B, L, H, dv), grad_q, grad_k, grad_v: contiguous, dtype.
  * dk and dv are at most 256; sums and states are held in 32 bits (64 for PSIG_F64).

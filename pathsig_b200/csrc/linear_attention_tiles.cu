@@ -9,11 +9,13 @@
 // swizzled tiles, in which K and V serve both as they are and transposed (the descriptor's major bit).
 //
 // Rounding.  The products take 16-bit operands, exact for R, K and V.  P, S and V' are computed in 32 bits and enter as sums of
-// 16-bit terms (the value, what its rounding left, what that left): P as two, S as NS and V' as NV, two (16 bits) where only
-// a 16-bit output depends on them, so that its one rounding is all that counts (error of the outputs 1.66e-3 of their size;
-// with P and S as one term each 2.35e-3, in seven eighths of the time), three (24 bits) where a 32-bit result does, the
-// state itself or the decay gradient.  The state lives in registers in 32 bits and is never rounded but for its copy as an
-// operand.  Sums of decays are in 64 bits, so that a weight exp(a_t - a_s) does not lose the difference of two long sums.
+// 16-bit terms (the value, what its rounding left, what that left): P as two, S as NS and V' as NV, two (15 or 16 bits) where
+// only a 16-bit output depends on them, so that its one rounding is all that counts (error of the outputs 1.66e-3 of their size;
+// 2.35e-3 with P and S as one term each), three (24 bits) where a 32-bit result does, the state itself or the decay gradient.
+// Terms of S and of V' stand side by side in one product where tensor memory has room, so that R and K are read once; the rest of
+// them, and P's second term, are products of their own, the small ones first into a common accumulator.  The state lives in
+// registers in 32 bits and is never rounded but for its copy as an operand.  Sums of decays are in 64 bits, and an exponent
+// a_t - a_s has 24 bits of its own size, so that a weight exp(a_t - a_s) does not lose the difference of two long sums.
 //
 // DOT: the sweep also gives x_t = out_t . y_t for the rows y of a third operand, to 32 bits (the decay gradient needs
 // q . grad_q and k . grad_k).  The part of the piece's own pairs is sum_s exp(a_t - a_s) (r_t . k_s) (y_t . v_s), the
@@ -25,11 +27,12 @@
 // A thread reads the 32 lanes of tensor memory that its warp's number allows; two warps share 32 rows and split the
 // columns.  They meet at mbarriers; every wait is bounded (psig_sequence_wait_timeouts).
 //
-// Measured, 8 sequences of 4096 steps of 16 heads of 128 (the bytes alone: 82 us forward): 382 us forward when the same 8 warps
-// did all stages one after the other (of 7000 cycles a piece: 2150 scores to P, 1400 output, 1000 V', 1100 issue); 200 us
-// in this form, 355 us with DOT (one and two 24-bit operands more).  Tensor pipe 28 % busy: the products of 64 columns are limited
-// by reading their operands from shared memory, and a piece's chain of scores, weights and product by latency.  Code size matters:
-// with all loops unrolled the six roles miss the instruction cache (63 % hits, 290 us).
+// Measured, 8 sequences of 4096 steps of 16 heads of 128 (the bytes alone: 82 us forward), with one term of P and S: 382 us forward
+// when the same 8 warps did all stages one after the other (of 7000 cycles a piece: 2150 scores to P, 1400 output, 1000 V', 1100
+// issue), 197 us in this form; with two terms 240 us (263 with a product for each term of S and V' and rounded first terms), 372 us
+// with DOT.  Tensor pipe 32 % busy: the products of 64 columns are limited by reading their operands from shared memory, and a
+// piece's chain of scores, weights and products by latency.  Code size matters: with all loops unrolled the six roles miss the
+// instruction cache (63 % hits, 290 us with one term).
 #include "tiles.cuh"
 
 namespace psig {
@@ -342,7 +345,8 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                             for (int j = 0; j < 16; j += 2) mul_two(t[j], t[j + 1], fq, fq);
                         }
                         tmem_loaded();
-                        // (weight 0 against a score that is not finite: only in rows behind the end, which nobody reads)
+                        // (a score that is not finite gives NaN against a weight of 0, too: in rows behind the end nobody reads it,
+                        // in others the operands have to be finite)
 #pragma unroll
                         for (int j = 0; j < 16; j += 2) {
                             mul_two(x[j], x[j + 1], t[j], t[j + 1]);
@@ -532,8 +536,8 @@ attn_sweep_tiles(const __grid_constant__ CUtensorMap map_r, const __grid_constan
                         mma_ss(tmem + Lay::c_two, tile_desc(base16 + ((Lay::dot + j * 32) >> 4), 16), tile_desc(v16 + j * 2, 16),
                                instr_desc<T>(128, false, false), j > 0, lead);
                 mma_commit(bar(kScores), lead);
-                // O2 = R S, when the state's operand is there (it was written before V').  Small terms first here and below: the accumulator drops what does not fit its 24 bits at every step,
-                // towards zero.
+                // O2 = R S, when the state's operand is there (it was written before V').  Small terms go first into a common accumulator
+                // here and below, or into one that holds small ones only: it drops what does not fit its 24 bits at every step, towards zero.
                 if (!(ok = warp_wait(bar(kVReady), ph, failed))) break;
                 fence_after();
                 const bool past = !no_past(it, i), future = !no_future(it, i);

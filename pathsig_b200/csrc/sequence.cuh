@@ -113,7 +113,7 @@ inline long long split_state_size(int d1, int d2) { return 4096LL * tile_columns
 
 // Parts to cut each sequence into.  A block sweeps one column tile of one head, so few long sequences leave most of the 148 SMs
 // idle.  The first launch over the parts costs about half a sweep, so two parts pay already (32-bit sequences 132 -> 105 us); a
-// part is at least four pieces long.  (16 heads of 128, 16384 steps: 412 us in one part, 77 + 3 + 113 us in four.)
+// part is at least four pieces long.  (16 heads of 128, 16384 steps: 412 us in one part, 62 + 3 + 123 us in four.)
 inline int split_plan(long long B, long long L, int H, int d2)
 {
     const long long blocks = B * H * tile_columns(d2), pieces = (L + 127) / 128;

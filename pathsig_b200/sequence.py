@@ -5,8 +5,8 @@ A signature folds a time-ordered sequence into iterated outer products; the laye
 (for example the ``(B, W, D)`` windows of :class:`Signature`) over time.  The state of :func:`linear_attention` is the
 degree-2 tensor of its keys and values with a fading memory -- without decay, with ``k_t = x_{t-1} - x_0 + dx_t / 2``
 and ``v_t = dx_t``, it is the second degree of the signature of ``x`` -- and :func:`linear_attention_step` updates it by
-one time step, as :func:`chen_product` extends a signature.  :func:`gated_residual_norm` brings features of different
-scale (signature words shrink with 1/degree!) to one scale around a block.  The reference package has no counterpart.
+one time step, as :func:`chen_product` extends a signature.  :func:`gated_residual_norm` brings rows to one scale around a
+block; its weight lets features of different size (signature words shrink with 1/degree!) count as the model learns.  The reference package has no counterpart.
 """
 from __future__ import annotations
 
@@ -40,10 +40,11 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *, init
     ``q`` (B, L, H, Dk), ``k`` (B, L, Hkv, Dk), ``v`` (B, L, Hkv, Dv): float32, float64, bfloat16 or float16, any
     strides; H is a multiple of Hkv and consecutive heads of ``q`` share a head of ``k`` and ``v``.  Head sizes are at
     most 256.  ``log_decay``: float32 (float64 for float64 operands), (H) -- a constant per head -- or (B, L, H), for
-    example ``-rate * dt`` for irregularly spaced observations.  It is meant to be at most 0; ``-inf`` forgets all that
-    was before the step.  ``initial_state`` (B, H, Dk, Dv): the type of ``log_decay``.  ``lengths`` (B), int32 or int64
+    example ``-rate * dt`` for irregularly spaced observations.  It is meant to be at most 0 (growth beyond 2^127 within 32
+    steps may overflow where the results do not); ``-inf`` forgets all that was before the step.  ``initial_state`` (B, H, Dk, Dv): the type of ``log_decay``.  ``lengths`` (B), int32 or int64
     on the GPU: later rows of a sequence are not read, their output is 0, and the state stops there (values outside
-    [0, L] are clamped).  ``scale`` defaults to ``Dk ** -0.5``.
+    [0, L] are clamped).  Rows up to the lengths are meant to be finite: an infinity or NaN there may reach every step of its
+    sequence and head, steps up to 127 before it too.  ``scale`` defaults to ``Dk ** -0.5``.
 
     Returns the output (B, L, H, Dv) in the type of ``q``; with ``return_state`` also the state after the last step
     (B, H, Dk, Dv).  Differentiable once wrt all floating operands (second derivatives and forward mode are
