@@ -369,3 +369,30 @@ def test_gates_far_out_are_good_to_the_types_last_bits(ps, D, activation, dtype)
     for name, where in (("h", c["gate"] == c["gate"]), ("grad_gate", c["gate"] < -3)):
         off = (got[name].double().cpu() - exact[name]).abs()[where]
         assert not (off > units * exact[name].abs()[where] + 2.0 ** -150).any(), (name, float((off / exact[name].abs()[where]).max() / so.half_step(dtype)))
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    """Nothing is set up at a first call that a capture forbids: attributes of kernels, the word that tells of failures, tensor maps."""
+    code = """
+import torch, pathsig_b200 as ps
+x = torch.randn(2400, 1528, device="cuda")
+w = torch.ones(1528, device="cuda")
+q = torch.randn(2, 300, 4, 64, device="cuda")
+d = torch.full((4,), -0.1, device="cuda")
+s = torch.zeros(2, 4, 64, 64, device="cuda")
+torch.cuda.synchronize()
+op = torch.ops.pathsig_b200
+def calls(s):
+    return (ps.gated_residual_norm(x, w), *op.gated_residual_norm_backward(x, w, None, None, None, None, x, None, 0, 1e-6)[:2],
+            ps.linear_attention(q, q, q, d), ps.linear_attention(q.half(), q.half(), q.half(), d), ps.linear_attention(*(3 * [q.bfloat16()]), d),
+            *op.linear_attention_backward(q, q, q, d, None, None, q, None, 0.1, True)[:4], ps.linear_attention_step(q[:, 0], q[:, 0], q[:, 0], d, s), s)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = calls(s)
+graph.replay()
+torch.cuda.synchronize()
+for a, b in zip(got, calls(torch.zeros_like(s))):
+    assert torch.equal(a, b)
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
